@@ -55,6 +55,25 @@ class DecodeState(C.Structure):
                 ("vshift", c_vp), ("scores", c_vp), ("pos", c_vp), ("tokens", c_vp), ("history", c_vp)]
 
 
+class PagedCache(C.Structure):
+    _fields_ = [("k", c_vp), ("v", c_vp)] + [(n, c_i64) for n in (
+        "k_stride_page", "k_stride_head", "k_stride_row", "v_stride_page", "v_stride_head", "v_stride_row")] + [
+        (n, C.c_int32) for n in ("num_pages", "page_size", "n_kv_heads", "head_dim", "dtype")]
+
+
+class QkNormRopeArgs(C.Structure):
+    _fields_ = [(n, c_vp) for n in ("q", "k", "v", "q_out", "k_out", "slots", "positions", "cos", "sin", "q_weight", "k_weight")] + [
+        (n, c_i64 * 3) for n in ("q_stride", "k_stride", "v_stride", "q_out_stride", "k_out_stride")] + [
+        (n, c_i64) for n in ("positions_stride", "table_rows", "table_ld")] + [
+        (n, C.c_int32) for n in ("positions_64", "B", "S", "Hq", "Hkv", "hd", "rot", "layout", "norm", "dtype")] + [
+        (n, c_f32) for n in ("eps", "q_scale", "k_scale")]
+
+
+ROPE_LAYOUTS = {"interleaved": 0, "half": 1}                                    # HB200_ROPE_*
+QK_NORMS = {None: 0, "rms": 1, "l2": 2}                                         # HB200_NORM_*
+PLAN_OUT_OF_PAGES, PLAN_TABLE_FULL, PLAN_OUT_OF_ROOM, PLAN_BAD_LENGTH = 1, 2, 4, 8   # HB200_PLAN_*
+
+
 # name -> (restype, argtypes); mirrors include/hydra_b200.h one to one
 SIGNATURES = {
     "hb200_version": (c_i32, []),
@@ -96,6 +115,13 @@ SIGNATURES = {
                                            c_vp]),
     "hb200_ccgqa_forward_static_max_bytes": (c_sz, []),
     "hb200_ccgqa_forward_static": (c_i32, [C.POINTER(Model), c_i32, c_vp, c_vp, c_i32, c_i32, c_vp, c_vp]),
+    "hb200_paged_plan": (c_i32, [c_vp, c_vp, c_i32, c_vp, c_i64, c_i32, c_i32, c_vp, c_i64, c_vp, c_vp, c_vp, c_vp, c_vp, c_i32,
+                                 c_vp, c_vp, c_vp]),
+    "hb200_qk_norm_rope": (c_i32, [C.POINTER(QkNormRopeArgs), C.POINTER(PagedCache), c_vp]),
+    "hb200_paged_attention_workspace_bytes": (c_sz, [c_i32, c_i32, c_i32, c_i32]),
+    "hb200_paged_decode_attention": (c_i32, [C.POINTER(PagedCache), c_vp, c_i64, c_i64, c_vp, c_vp, c_vp, c_i64, c_i32, c_vp,
+                                             c_i32, c_i32, c_f32, c_vp, c_sz, c_vp]),
+    "hb200_token_logprobs": (c_i32, [c_vp, c_vp, c_i64, c_i32, c_i64, c_i64, c_f32, c_i32, c_vp, c_vp, c_vp, c_vp, c_i32, c_vp]),
     "hb200_profile_create": (c_vp, [c_i32]),
     "hb200_profile_destroy": (None, [c_vp]),
     "hb200_profile_reset": (c_i32, [c_vp]),

@@ -1,0 +1,377 @@
+// Log probabilities of given tokens, entropy and the top alternatives of logit rows, from one pass over the logits.
+//
+//   z = x / T, m = max z, Z = sum e^{z-m};  log p(t) = z_t - m - ln Z;  H = ln Z - sum (z-m) e^{z-m} / Z
+//
+// Bound: HBM for many rows (each logit read once), latency for few.  Every thread keeps a running maximum with the two
+// sums relative to it in 32 bits (new maxima are rare after the first pieces, so the rescaling hardly ever runs).
+//
+// Top alternatives without a second pass over the row: the maxima of the threads, taken over 64 groups of threads, give a
+// bound that at least `top` logits reach (the top-th largest group maximum); only threads whose own maximum reaches it
+// re-read their pieces (a warp together, out of L2), and the few logits found are ranked by (value, index).  Of
+// equal logits the lowest index comes first; ties at the bound beyond the candidate list's size are collected in index
+// order.  Rows that hold NaN or +inf, or more than kCand logits above the bound, take `top` exact selection rounds instead.
+//
+// Few rows are split over a cluster of CTAs, whose partial results the first CTA merges through distributed shared memory.
+#include <cooperative_groups.h>
+
+#include "common.cuh"
+
+namespace hb200 {
+namespace {
+
+namespace cg = cooperative_groups;
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr int kCand = 512;       // candidate list of a CTA
+constexpr int kMaxTop = 32;
+constexpr int kGroups = 64;
+constexpr int kUnroll = 4;
+constexpr float kLowest = -3.402823466e38f;
+
+struct LogprobParams {
+  const void* x;
+  const int64_t* tokens;
+  float *logprobs, *entropy, *top_lp;
+  int64_t* top_id;
+  int64_t ld, ignore;
+  int cols, top, slice;   // slice: columns per CTA of a cluster
+  float inv_t;
+};
+
+__device__ __forceinline__ float ex2f(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {   // NaN if either is
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
+
+// Order of logits as whole numbers: larger value, larger key; -0 as +0; NaN above +inf.
+__device__ __forceinline__ uint32_t order_key(float v) {
+  if (v != v) return 0xffffffffu;
+  const uint32_t b = __float_as_uint(v + 0.f);
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float key_value(uint32_t k) {
+  if (k == 0xffffffffu) return __int_as_float(0x7fc00000);
+  return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
+}
+__device__ __forceinline__ uint64_t entry(float v, int i) { return ((uint64_t)order_key(v) << 32) | (uint32_t)~i; }
+__device__ __forceinline__ int entry_index(uint64_t e) { return (int)~(uint32_t)e; }
+
+// Running statistics of the logits a thread (a row) has seen: maximum, sum 2^t and sum t 2^t, t = (x - max) c.
+struct Stat {
+  float m, s, u;
+  __device__ float base() const { return fmaxf(m, kLowest); }   // finite while only -inf was seen
+};
+__device__ __forceinline__ void rebase(Stat& a, float to, float c) {   // to >= a.base()
+  const float d = fmaxf((a.base() - to) * c, -200.f), f = ex2f(d);
+  a.u = f * fmaf(d, a.s, a.u);
+  a.s *= f;
+}
+__device__ __forceinline__ Stat merge(Stat a, Stat b, float c) {
+  const float m = fmaxf(a.m, b.m), to = fmaxf(m, kLowest);
+  rebase(a, to, c);
+  rebase(b, to, c);
+  return {m, a.s + b.s, a.u + b.u};
+}
+
+template <typename T, int N>
+__device__ __forceinline__ void take(Stat& a, const float (&f)[N], float c) {
+  float mx = f[0];
+#pragma unroll
+  for (int i = 1; i < N; ++i) mx = fmaxf(mx, f[i]);
+  if (mx > a.m) {
+    rebase(a, fmaxf(mx, kLowest), c);
+    a.m = mx;
+  }
+  const float base = a.base();
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    // -inf (and anything far below) counts as 2^-200 = 0 times a finite distance; NaN and +inf stay NaN
+    const float t = max_nan((f[i] - base) * c, -200.f), e = ex2f(t);
+    a.s += e;
+    a.u = fmaf(t, e, a.u);
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void unpack(const uint4& raw, float (&f)[16 / sizeof(T)]) {
+  const T* e = reinterpret_cast<const T*>(&raw);
+#pragma unroll
+  for (int i = 0; i < (int)(16 / sizeof(T)); ++i) f[i] = Cvt<T>::to_f(e[i]);
+}
+
+// What a CTA of a cluster leaves for the first one.
+struct Partial {
+  Stat stat;
+  int n;                       // entries
+  uint64_t best[kMaxTop];      // in order
+};
+
+template <typename T, int NT, bool TOP>
+__global__ void __launch_bounds__(NT) token_logprobs_kernel(const LogprobParams p) {
+  constexpr int V = 16 / sizeof(T), NW = NT / 32, LPG = NT / kGroups;   // lanes per group of threads
+  __shared__ Partial s_part;
+  __shared__ Stat s_stat[NW];
+  __shared__ float s_group[kGroups];
+  __shared__ uint64_t s_cand[kCand];
+  __shared__ uint64_t s_best[NW + 1];
+  __shared__ float s_bound;
+  __shared__ int s_count, s_scan[NW];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+  const int64_t r = blockIdx.x / C;
+  const T* row = static_cast<const T*>(p.x) + r * p.ld;
+  const int c0 = min(p.cols, rank * p.slice), c1 = min(p.cols, c0 + p.slice), n = c1 - c0;
+  const T* x = row + c0;
+  const float c = p.inv_t * kLog2e;
+  const int64_t tgt = rank == 0 ? p.tokens[r] : 0;
+  const bool scored = rank == 0 && tid == 0 && tgt >= 0 && tgt < p.cols;
+  const float x_tgt = scored ? Cvt<T>::to_f(row[tgt]) : 0.f;
+
+  // values before the first 16-byte boundary, 16-byte pieces, values behind the last
+  const int to_boundary = (int)(((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / sizeof(T));
+  const int head = min(n, to_boundary), pieces = (n - head) / V, edge = head + (n - head - pieces * V);
+  const uint4* xv = reinterpret_cast<const uint4*>(x + head);
+  auto edge_at = [&](int i) { return i < head ? i : pieces * V + i; };   // i-th value outside the pieces -> its column
+  Stat a = {-INFINITY, 0.f, 0.f};
+  for (int v0 = tid; v0 < pieces; v0 += NT * kUnroll) {
+    uint4 raw[kUnroll];
+#pragma unroll
+    for (int k = 0; k < kUnroll; ++k)
+      if (v0 + k * NT < pieces) raw[k] = __ldg(xv + v0 + k * NT);
+#pragma unroll
+    for (int k = 0; k < kUnroll; ++k)
+      if (v0 + k * NT < pieces) {
+        float f[V];
+        unpack<T>(raw[k], f);
+        take<T>(a, f, c);
+      }
+  }
+  if (tid < edge) {   // fewer than 2 V <= NT of them
+    const float f[1] = {Cvt<T>::to_f(x[edge_at(tid)])};
+    take<T>(a, f, c);
+  }
+  const float own_max = a.m;
+
+  // the row's (slice's) statistics; on the way the maxima of the 64 groups of threads
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    if (TOP && o == LPG && (lane & (LPG - 1)) == 0) s_group[tid / LPG] = a.m;
+    const Stat b = {__shfl_xor_sync(0xffffffffu, a.m, o), __shfl_xor_sync(0xffffffffu, a.s, o), __shfl_xor_sync(0xffffffffu, a.u, o)};
+    a = merge(a, b, c);
+  }
+  if (lane == 0) s_stat[warp] = a;
+  if (tid == 0) s_count = 0;
+  __syncthreads();
+  a = s_stat[0];
+#pragma unroll
+  for (int w = 1; w < NW; ++w) a = merge(a, s_stat[w], c);
+  const int want = TOP ? min(p.top, n) : 0;
+
+  if (TOP && want > 0) {
+    // the bound: the want-th largest group maximum (at least `want` logits reach it)
+    if (tid < kGroups) {
+      const float mine = s_group[tid];
+      int above = 0;
+      for (int i = 0; i < kGroups; ++i) {
+        const float o = s_group[i];
+        above += (o > mine || (o == mine && i < tid)) ? 1 : 0;
+      }
+      if (above == want - 1) s_bound = mine;
+    }
+    __syncthreads();
+    const float bound = s_bound;
+    const bool sane = a.s == a.s;         // NaN or +inf somewhere: the maxima above say nothing
+    // every logit above the bound (`equal`: or at it) into the list; the number of them, also where it overflows
+    auto collect = [&](bool equal) {
+      auto offer = [&](float v, int col) {
+        if (v > bound || (equal && v == bound)) {
+          const int at = atomicAdd(&s_count, 1);
+          if (at < kCand) s_cand[at] = entry(v, c0 + col);
+        }
+      };
+      unsigned flagged = __ballot_sync(0xffffffffu, own_max > bound || (equal && own_max == bound));
+      while (flagged) {                    // a thread's pieces, looked through by its whole warp
+        const int l = __ffs(flagged) - 1;
+        flagged &= flagged - 1;
+        for (int v = warp * 32 + l + lane * NT; v < pieces; v += 32 * NT) {
+          float f[V];
+          unpack<T>(__ldg(xv + v), f);
+#pragma unroll
+          for (int i = 0; i < V; ++i) offer(f[i], head + v * V + i);
+        }
+      }
+      if (tid < edge) {
+        const int col = edge_at(tid);
+        offer(Cvt<T>::to_f(x[col]), col);
+      }
+      __syncthreads();
+      return s_count;
+    };
+    int found = kCand + 1;
+    if (sane && bound > -INFINITY) found = collect(true);
+    if (sane && found > kCand) {           // many ties at the bound: those above it, then the first that equal it
+      __syncthreads();
+      if (tid == 0) s_count = 0;
+      __syncthreads();
+      found = collect(false);
+      if (found > kCand - kMaxTop) found = kCand + 1;
+      for (int i0 = 0; found < want && i0 < n; i0 += NT) {   // uniform over the CTA
+        const int i = i0 + tid;
+        const bool eq = i < n && Cvt<T>::to_f(x[i]) == bound;
+        const unsigned vote = __ballot_sync(0xffffffffu, eq);
+        if (lane == 0) s_scan[warp] = __popc(vote);
+        __syncthreads();
+        int at = found + __popc(vote & ((1u << lane) - 1));
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
+          at += w < warp ? s_scan[w] : 0;
+          found += s_scan[w];
+        }
+        if (eq && at < want) s_cand[at] = entry(bound, c0 + i);
+        found = min(found, want);
+        __syncthreads();
+      }
+    }
+    if (sane && found <= kCand) {
+      for (int i = tid; i < found; i += NT) {   // rank by counting
+        const uint64_t mine = s_cand[i];
+        int rk = 0;
+        for (int j = 0; j < found; ++j) rk += s_cand[j] > mine ? 1 : 0;
+        if (rk < want) s_part.best[rk] = mine;
+      }
+    } else {
+      // exact selection rounds: the largest entry below the last one
+      uint64_t last = ~0ull;
+      for (int k = 0; k < want; ++k) {
+        uint64_t best = 0;
+        for (int i = tid; i < n; i += NT) {
+          const uint64_t e = entry(Cvt<T>::to_f(x[i]), c0 + i);
+          if (e < last && e > best) best = e;
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+          const uint64_t e = __shfl_xor_sync(0xffffffffu, best, o);
+          best = e > best ? e : best;
+        }
+        if (lane == 0) s_best[warp] = best;
+        __syncthreads();
+        best = s_best[0];
+#pragma unroll
+        for (int w = 1; w < NW; ++w) best = s_best[w] > best ? s_best[w] : best;
+        if (tid == 0) s_part.best[k] = best;
+        last = best;
+        __syncthreads();
+      }
+    }
+  }
+  if (tid == 0) { s_part.stat = a; s_part.n = want; }
+  __syncthreads();
+
+  const uint64_t* mine_best = s_part.best;
+  int have = want;
+  if (C > 1) {
+    cluster.sync();
+    if (rank == 0) {
+      // the slices' statistics, in order, and their entries ranked together
+      int at = 0;
+      for (int q = 0; q < C; ++q) {
+        const Partial* o = cluster.map_shared_rank(&s_part, q);
+        if (q > 0) a = merge(a, o->stat, c);
+        if (TOP) {
+          const int m = o->n;
+          for (int i = tid; i < m; i += NT) s_cand[at + i] = o->best[i];
+          at += m;
+        }
+      }
+      __syncthreads();
+      if (TOP) {
+        have = min(p.top, at);
+        uint64_t e = 0;
+        int rk = kMaxTop;
+        if (tid < at) {
+          e = s_cand[tid];
+          rk = 0;
+          for (int j = 0; j < at; ++j) rk += s_cand[j] > e ? 1 : 0;
+        }
+        __syncthreads();
+        if (rk < have) s_cand[rk] = e;
+        mine_best = s_cand;
+        __syncthreads();
+      }
+    }
+    cluster.sync();   // no CTA leaves while its shared memory is read
+  }
+  if (rank != 0) return;
+  const float nan = __int_as_float(0x7fc00000);
+  const bool none = !(a.s > 0.f) || a.m == INFINITY;     // no logit above -inf, or NaN / +inf among them
+  const float lz2 = log2f(a.s), base = a.base();
+  if (tid == 0) {
+    float lp = nan;
+    if (tgt == p.ignore) lp = 0.f;
+    else if (scored && !none) lp = fmaf(x_tgt - base, p.inv_t, -kLn2 * lz2);
+    p.logprobs[r] = lp;
+    p.entropy[r] = none ? nan : (lz2 - a.u / a.s) * kLn2;
+  }
+  if (TOP) {
+    for (int i = tid; i < p.top; i += NT) {
+      const uint64_t e = i < have ? mine_best[i] : 0;
+      p.top_id[r * p.top + i] = i < have ? entry_index(e) : -1;
+      p.top_lp[r * p.top + i] = i < have && !none ? fmaf(key_value((uint32_t)(e >> 32)) - base, p.inv_t, -kLn2 * lz2) : nan;
+    }
+  }
+}
+
+template <typename T, int NT, bool TOP>
+int launch_as(const LogprobParams& p, int64_t rows, int cluster, cudaStream_t st) {
+  return launch_chained(token_logprobs_kernel<T, NT, TOP>, dim3((unsigned)(rows * cluster)), dim3(NT), 0, st, false, cluster, p);
+}
+
+template <typename T>
+int launch(LogprobParams p, int64_t rows, cudaStream_t st) {
+  // Few rows: up to eight CTAs per row, so that about two CTAs per SM have work and each still has 4096 columns.
+  int cluster = 1;
+  while (cluster < 8 && rows * cluster * 2 <= 2 * 148 && p.cols / (cluster * 2) >= 4096) cluster *= 2;
+  p.slice = ceil_div(ceil_div(p.cols, cluster), 64) * 64;
+  if (p.top > 0) return launch_as<T, 512, true>(p, rows, cluster, st);
+  return launch_as<T, 512, false>(p, rows, cluster, st);
+}
+
+}  // namespace
+}  // namespace hb200
+
+using namespace hb200;
+
+extern "C" int hb200_token_logprobs(const void* logits, const int64_t* tokens, int64_t rows, int cols, int64_t ld,
+                                    int64_t ignore_index, float temperature, int top, float* logprobs, float* entropy,
+                                    float* top_logprobs, int64_t* top_ids, int dtype, void* stream) {
+  HB_REQUIRE(rows >= 0 && cols >= 1 && (ld >= cols || rows <= 1), HB200_ERR_INVALID, "token_logprobs: bad shape rows=%lld cols=%d ld=%lld",
+             (long long)rows, cols, (long long)ld);
+  HB_REQUIRE(temperature >= 1e-6f && temperature <= 1e6f, HB200_ERR_INVALID,
+             "token_logprobs: temperature %g (1e-6 to 1e6)", temperature);
+  HB_REQUIRE(top >= 0 && top <= kMaxTop, HB200_ERR_UNSUPPORTED, "token_logprobs: %d alternatives (up to %d are built)", top, kMaxTop);
+  HB_REQUIRE(top <= cols, HB200_ERR_INVALID, "token_logprobs: %d alternatives of %d columns", top, cols);
+  if (rows == 0) return 0;
+  HB_REQUIRE(logits && tokens && logprobs && entropy && (top == 0 || (top_logprobs && top_ids)), HB200_ERR_INVALID,
+             "token_logprobs: null pointer");
+  HB_REQUIRE(rows <= 0x7fffffff / 8, HB200_ERR_UNSUPPORTED, "token_logprobs: too many rows");
+  const size_t es = dtype == HB200_F32 ? 4 : 2;
+  HB_REQUIRE(reinterpret_cast<uintptr_t>(logits) % es == 0, HB200_ERR_INVALID, "token_logprobs: misaligned logits");
+  LogprobParams p = {};
+  p.x = logits; p.tokens = tokens; p.logprobs = logprobs; p.entropy = entropy; p.top_lp = top_logprobs; p.top_id = top_ids;
+  p.ld = ld; p.ignore = ignore_index; p.cols = cols; p.top = top;
+  p.inv_t = (float)(1.0 / (double)temperature);
+  cudaStream_t st = (cudaStream_t)stream;
+  if (dtype == HB200_F32) return launch<float>(p, rows, st);
+  if (dtype == HB200_BF16) return launch<__nv_bfloat16>(p, rows, st);
+  if (dtype == HB200_F16) return launch<__half>(p, rows, st);
+  set_error("token_logprobs: unsupported dtype %d", dtype);
+  return HB200_ERR_UNSUPPORTED;
+}

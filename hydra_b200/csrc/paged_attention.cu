@@ -1,0 +1,626 @@
+// Attention of one new token per request over a paged key-value cache, split over the caches' lengths and joined.
+//
+//   s_j = scale * q . k_j  (j < len),   out = sum_j e^{s_j} v_j / sum_j e^{s_j},   lse = ln sum_j e^{s_j}
+//
+// Bound: HBM.  Every K and V row of the valid tokens is read once (4 * hd bytes per token and kv head) for 4 * hd * group
+// operations, so the tensor cores are needed only to keep the arithmetic out of the way: the query heads of one kv head
+// are the 16 rows of an m16n8k16 product.  tcgen05 would want 64 or 128 rows of queries; with 1..16 of them its TMEM
+// round trip buys nothing, so the warp-level instruction is used.
+//
+// Work split: the tiles of all (request, kv head) pairs are laid end to end and dealt out in equal contiguous shares to
+// the warps of a grid that fits the GPU once (one CTA per SM), whatever the lengths are: a batch of one long and many
+// short requests keeps every SM busy to the end.  The lengths live on the device; each CTA scans them itself.  A warp
+// streams its share through a private cp.async ring that runs on across the ends of requests, so no barrier is met after
+// the scan.  A pair that lies within one share is finished by its warp; of the others each share leaves (max, sum,
+// unnormalised output) in 32 bits in the workspace and the join kernel adds them up in a fixed order (no atomics:
+// the same inputs give the same bits).
+#include "common.cuh"
+#include "mma.cuh"
+
+namespace hb200 {
+namespace {
+
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr int kMaxBatch = 4096;
+constexpr int kMinTiles = 4;    // least share of a warp: below this the join's traffic outweighs the parallelism
+
+struct PagedParams {
+  const void *q, *kc, *vc;
+  void* out;
+  float* lse;
+  const int32_t *table, *lens;
+  float* part_o;     // [workers][2][rows][hd]
+  float* part_ml;    // [workers][2][rows][2]
+  int32_t* cum;      // [B + 1] tiles of the requests before each one
+  int64_t q_sb, q_sh, k_sp, k_sh, k_sr, v_sp, v_sh, v_sr, table_ld;
+  int B, Hq, Hkv, hd, group, q_tiles, rows, page_size, width, num_pages, workers;
+  float scale_log2;  // scale * log2(e)
+};
+
+__host__ __device__ constexpr int tile_tokens(int HD) { return HD >= 128 ? 16 : (HD == 64 ? 32 : 64); }
+__host__ __device__ constexpr int warps_of(int HD) { return HD >= 256 ? 4 : 8; }
+constexpr int kStages = 3;
+
+// Cache length of request b as the kernel reads it: what lies outside [0, width * page_size] is marked (`poison`).
+__device__ __forceinline__ int clamp_len(int len, int64_t cap, bool& poison) {
+  poison = (int64_t)len > cap;
+  return len < 0 ? 0 : (poison ? (int)cap : len);
+}
+
+__device__ __forceinline__ void cp_async_16_zfill(uint32_t dst, const void* src, bool there) {
+  const int n = there ? 16 : 0;
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void ldsm_x4(uint32_t (&r)[4], uint32_t a) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];\n"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+}
+__device__ __forceinline__ void ldsm_x4_trans(uint32_t (&r)[4], uint32_t a) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];\n"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+template <typename T>
+__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1);
+template <>
+__device__ __forceinline__ void mma16816<__nv_bfloat16>(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                                        uint32_t b0, uint32_t b1) {
+  mma_bf16_16816(d, a0, a1, a2, a3, b0, b1);
+}
+template <>
+__device__ __forceinline__ void mma16816<__half>(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                                 uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// Two weights in T and what the rounding left of them, in T again: together they carry 16 (bf16) or 22 (f16) bits.
+template <typename T>
+__device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo);
+template <>
+__device__ __forceinline__ void split2<__nv_bfloat16>(float a, float b, uint32_t& hi, uint32_t& lo) {
+  hi = pack_bf16x2(a, b);
+  lo = pack_bf16x2(a - __uint_as_float(hi << 16), b - __uint_as_float(hi & 0xffff0000u));
+}
+template <>
+__device__ __forceinline__ void split2<__half>(float a, float b, uint32_t& hi, uint32_t& lo) {
+  const __half2 h = __floats2half2_rn(a, b);
+  const float2 f = __half22float2(h);
+  const __half2 l = __floats2half2_rn(a - f.x, b - f.y);
+  hi = *reinterpret_cast<const uint32_t*>(&h);
+  lo = *reinterpret_cast<const uint32_t*>(&l);
+}
+
+// 16-byte unit of (row, chunk) in a tile of rows of CH chunks, xor-swizzled so that eight rows of one chunk column lie in
+// eight different bank groups (ldmatrix without conflicts).
+template <int CH>
+__device__ __forceinline__ int unit_of(int row, int c) {
+  if (CH >= 8) return row * CH + (c ^ (row & 7));
+  if (CH == 4) return row * CH + (c ^ ((row >> 1) & 3));
+  return row * CH + (c ^ ((row >> 2) & 1));
+}
+
+// A place in the row of all tiles: request b, head tile h (kv head * q_tiles + tile of its query heads), tile t of n.
+struct Cursor {
+  int b, h, t, n, len;
+  bool poison;
+};
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(warps_of(HD) * 32, 1) paged_attention_kernel(const PagedParams p) {
+  constexpr int NW = warps_of(HD), TT = tile_tokens(HD), CH = HD / 8, ST = kStages;
+  constexpr int KBYTES = TT * HD * 2, STAGE = 2 * KBYTES;
+  constexpr int NT = TT / 8;                 // n tiles of the scores
+  constexpr int LOADS = TT * CH / 32;        // 16-byte copies of K (and of V) per lane and tile
+  constexpr int ROWS_PER = 32 / CH;          // rows one copy instruction of the warp covers (CH <= 32)
+  constexpr int TREG = (TT + 31) / 32;       // token bookkeeping registers per lane
+  constexpr bool Q_IN_SMEM = HD >= 256;      // the query fragments do not fit beside the output's registers
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ int scan_buf[33];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int32_t* s_cum = reinterpret_cast<int32_t*>(smem + NW * (ST * STAGE + (Q_IN_SMEM ? 16 * HD * 2 : 0)));   // [B + 1]
+  int32_t* s_len = s_cum + p.B + 1;                                                                          // [B]
+  chain_release();   // the join kernel may take its place; it waits for this grid's end before it reads anything
+
+  // tiles before each request
+  const int64_t cap = (int64_t)p.width * p.page_size;
+  {
+    const int per = (p.B + NW * 32 - 1) / (NW * 32);
+    const int b0 = threadIdx.x * per;
+    int mine = 0;
+    for (int i = 0; i < per; ++i) {
+      const int b = b0 + i;
+      if (b < p.B) {
+        const int raw = p.lens[b];
+        bool poison;
+        const int len = clamp_len(raw, cap, poison);
+        s_len[b] = poison ? -1 - len : len;
+        mine += (len + TT - 1) / TT;
+      }
+    }
+    int total;
+    int at = block_exclusive_scan(mine, scan_buf, total);
+    for (int i = 0; i < per; ++i) {
+      const int b = b0 + i;
+      if (b < p.B) {
+        s_cum[b] = at;
+        const int v = s_len[b];
+        at += ((v < 0 ? -1 - v : v) + TT - 1) / TT;
+      }
+    }
+    if (threadIdx.x == 0) s_cum[p.B] = total;
+    __syncthreads();
+    if (blockIdx.x == 0)
+      for (int b = threadIdx.x; b <= p.B; b += NW * 32) p.cum[b] = s_cum[b];
+  }
+  const int H = p.Hkv * p.q_tiles;
+  const int64_t total = (int64_t)s_cum[p.B] * H;
+  const int64_t share = max((total + p.workers - 1) / p.workers, (int64_t)kMinTiles);
+  const int w = blockIdx.x * NW + warp;
+  const int64_t begin = (int64_t)w * share;
+  if (begin >= total) return;
+  const int64_t end = begin + share < total ? begin + share : total;
+  int left = (int)(end - begin);   // tiles to compute (a share is far below 2^31: total < 2^31 * H / workers)
+
+  auto enter = [&](Cursor& c) {   // request c.b's length and tiles
+    c.n = s_cum[c.b + 1] - s_cum[c.b];
+    const int v = s_len[c.b];
+    c.poison = v < 0;
+    c.len = v < 0 ? -1 - v : v;
+  };
+  auto advance = [&](Cursor& c) {   // called only while another tile follows
+    if (++c.t == c.n) {
+      c.t = 0;
+      if (++c.h == H) {
+        c.h = 0;
+        do { ++c.b; enter(c); } while (c.n == 0);
+      }
+    }
+  };
+  Cursor cur;
+  {
+    int lo = 0, hi = p.B;   // s_cum[lo] * H <= begin < s_cum[hi] * H
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if ((int64_t)s_cum[mid] * H <= begin) lo = mid; else hi = mid;
+    }
+    cur.b = lo;
+    enter(cur);
+    const int64_t r = begin - (int64_t)s_cum[lo] * H;
+    cur.h = (int)(r / cur.n);
+    cur.t = (int)(r % cur.n);
+  }
+
+  uint8_t* ring = smem + warp * ST * STAGE;
+  const uint32_t ring_u = smem_u32(ring);
+  uint8_t* q_smem = smem + NW * ST * STAGE + warp * 16 * HD * 2;
+  if (p.hd < HD) {   // the padding chunks are never copied to: zero them once (zero times anything the ring held before)
+    for (int u = lane; u < ST * STAGE / 16; u += 32) reinterpret_cast<uint4*>(ring)[u] = make_uint4(0, 0, 0, 0);
+    __syncwarp();
+  }
+
+  // ---- producer: the page of every token of a tile is looked up one tile before its copies are issued
+  Cursor pc = cur;
+  int to_look = left, to_issue = left;
+  int page[TREG], row[TREG], l_kvh = 0;
+  bool bad_seen = false;            // a page outside the cache, in the tile that was looked up
+  uint32_t bad_bits = 0;            // the same per ring slot
+  auto look = [&]() {
+    if (to_look > 0) {
+      --to_look;
+      l_kvh = pc.h / p.q_tiles;
+      bool bad = pc.poison;
+#pragma unroll
+      for (int i = 0; i < TREG; ++i) {
+        const int tok = pc.t * TT + i * 32 + lane;
+        const bool in = tok < pc.len && i * 32 + lane < TT;
+        const int pi = in ? tok / p.page_size : 0;
+        row[i] = tok - pi * p.page_size;
+        const int id = in ? __ldg(p.table + (int64_t)pc.b * p.table_ld + pi) : -1;
+        const bool ok = in && id >= 0 && id < p.num_pages;
+        bad |= in && !ok;
+        page[i] = ok ? id : -1;
+      }
+      bad_seen = bad;
+      if (to_look > 0) advance(pc);
+    }
+  };
+  auto issue = [&](int slot) {
+    if (to_issue > 0) {
+      --to_issue;
+      const uint32_t kdst = ring_u + slot * STAGE, vdst = kdst + KBYTES;
+      const T* kb = static_cast<const T*>(p.kc) + (int64_t)l_kvh * p.k_sh;
+      const T* vb = static_cast<const T*>(p.vc) + (int64_t)l_kvh * p.v_sh;
+      const int c = lane % CH;
+      const bool chunk_in = c * 8 < p.hd;
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) {
+        const int r = i * ROWS_PER + lane / CH;           // r / 32 is the same for all lanes
+        const int pg = __shfl_sync(0xffffffffu, page[(i * ROWS_PER) / 32], r & 31);
+        const int rw = __shfl_sync(0xffffffffu, row[(i * ROWS_PER) / 32], r & 31);
+        const bool there = pg >= 0;
+        const int64_t pp = there ? pg : 0;
+        const int64_t rr = there ? rw : 0;
+        if (chunk_in) {
+          const uint32_t u = unit_of<CH>(r, c) * 16;
+          cp_async_16_zfill(kdst + u, kb + pp * p.k_sp + rr * p.k_sr + c * 8, there);
+          cp_async_16_zfill(vdst + u, vb + pp * p.v_sp + rr * p.v_sr + c * 8, there);
+        }
+      }
+      const bool any_bad = __any_sync(0xffffffffu, bad_seen);
+      bad_bits = any_bad ? bad_bits | (1u << slot) : bad_bits & ~(1u << slot);
+    }
+    cp_async_commit();
+  };
+  look();
+#pragma unroll
+  for (int i = 0; i < ST - 1; ++i) { issue(i); look(); }
+
+  // ---- consumer
+  const int g = lane >> 2, t4 = lane & 3;
+  uint32_t qf[Q_IN_SMEM ? 1 : HD / 16][4];
+  float o[HD / 8][4];
+  float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+  bool poison = false, fresh = true;
+  int first_tile = cur.t;
+  int rows_here = 0, head0 = 0;
+  int slot = 0;
+  while (left > 0) {
+    if (fresh) {   // a new (request, head tile): its queries, empty statistics
+      fresh = false;
+      first_tile = cur.t;
+      const int kvh = cur.h / p.q_tiles, qt = cur.h - kvh * p.q_tiles;
+      head0 = kvh * p.group + qt * 16;
+      rows_here = min(16, p.group - qt * 16);
+      const T* qb = static_cast<const T*>(p.q) + (int64_t)cur.b * p.q_sb + (int64_t)head0 * p.q_sh;
+      if constexpr (Q_IN_SMEM) {
+        __syncwarp();
+        for (int u = lane; u < 16 * CH; u += 32) {
+          const int r = u / CH, c = u % CH;
+          uint4 v = make_uint4(0, 0, 0, 0);
+          if (r < rows_here && c * 8 < p.hd) v = __ldg(reinterpret_cast<const uint4*>(qb + r * p.q_sh + c * 8));
+          reinterpret_cast<uint4*>(q_smem)[unit_of<CH>(r, c)] = v;
+        }
+        __syncwarp();
+      } else {
+#pragma unroll
+        for (int ks = 0; ks < HD / 16; ++ks)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int r = g + (i & 1) * 8, d = ks * 16 + (i >> 1) * 8 + t4 * 2;
+            qf[ks][i] = (r < rows_here && d < p.hd) ? __ldg(reinterpret_cast<const uint32_t*>(qb + r * p.q_sh + d)) : 0u;
+          }
+      }
+#pragma unroll
+      for (int i = 0; i < HD / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+      m0 = m1 = -INFINITY;
+      l0 = l1 = 0.f;
+      poison = false;
+    }
+    cp_async_wait<ST - 2>();
+    __syncwarp();
+    poison |= (bad_bits >> slot) & 1u;
+    const uint32_t kbase = ring_u + slot * STAGE, vbase = kbase + KBYTES;
+
+    // scores of 16 query rows against TT tokens
+    float s[NT][4];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+    const int mi = lane >> 3, mr = lane & 7;
+    if constexpr (HD == 16) {
+#pragma unroll
+      for (int n = 0; n < NT; n += 2) {
+        uint32_t kf[4];
+        ldsm_x4(kf, kbase + unit_of<CH>((n + (mi >> 1)) * 8 + mr, mi & 1) * 16);
+        mma16816<T>(s[n], qf[0][0], qf[0][1], qf[0][2], qf[0][3], kf[0], kf[1]);
+        mma16816<T>(s[n + 1], qf[0][0], qf[0][1], qf[0][2], qf[0][3], kf[2], kf[3]);
+      }
+    } else {
+#pragma unroll
+      for (int ks = 0; ks < HD / 16; ks += 2) {
+        uint32_t qa[4], qb2[4];
+        if constexpr (Q_IN_SMEM) {
+          const uint32_t qs = smem_u32(q_smem);
+          ldsm_x4(qa, qs + unit_of<CH>((mi & 1) * 8 + mr, ks * 2 + (mi >> 1)) * 16);
+          ldsm_x4(qb2, qs + unit_of<CH>((mi & 1) * 8 + mr, ks * 2 + 2 + (mi >> 1)) * 16);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) { qa[i] = qf[ks][i]; qb2[i] = qf[ks + 1][i]; }
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          uint32_t kf[4];
+          ldsm_x4(kf, kbase + unit_of<CH>(n * 8 + mr, ks * 2 + mi) * 16);
+          mma16816<T>(s[n], qa[0], qa[1], qa[2], qa[3], kf[0], kf[1]);
+          mma16816<T>(s[n], qb2[0], qb2[1], qb2[2], qb2[3], kf[2], kf[3]);
+        }
+      }
+    }
+
+    // running maximum and sum, in powers of two
+    const int tok0 = cur.t * TT + t4 * 2;
+    const bool ragged = cur.t * TT + TT > cur.len;
+    float mx0 = -INFINITY, mx1 = -INFINITY;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[n][i] *= p.scale_log2;
+      if (ragged) {
+        if (tok0 + n * 8 >= cur.len) s[n][0] = s[n][2] = -INFINITY;
+        if (tok0 + n * 8 + 1 >= cur.len) s[n][1] = s[n][3] = -INFINITY;
+      }
+      mx0 = fmaxf(mx0, fmaxf(s[n][0], s[n][1]));
+      mx1 = fmaxf(mx1, fmaxf(s[n][2], s[n][3]));
+    }
+    mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 1));
+    mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 2));
+    mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 1));
+    mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 2));
+    if (__any_sync(0xffffffffu, mx0 > m0 || mx1 > m1)) {
+      const float n0 = fmaxf(m0, mx0), n1 = fmaxf(m1, mx1);
+      const float f0 = m0 == n0 ? 1.f : ex2(m0 - n0), f1 = m1 == n1 ? 1.f : ex2(m1 - n1);
+      m0 = n0;
+      m1 = n1;
+      l0 *= f0;
+      l1 *= f1;
+#pragma unroll
+      for (int i = 0; i < HD / 8; ++i) { o[i][0] *= f0; o[i][1] *= f0; o[i][2] *= f1; o[i][3] *= f1; }
+    }
+    const float b0 = m0 == -INFINITY ? 0.f : m0, b1 = m1 == -INFINITY ? 0.f : m1;   // every score -inf: weights 0
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      s[n][0] = ex2(s[n][0] - b0);
+      s[n][1] = ex2(s[n][1] - b0);
+      s[n][2] = ex2(s[n][2] - b1);
+      s[n][3] = ex2(s[n][3] - b1);
+      l0 += s[n][0] + s[n][1];
+      l1 += s[n][2] + s[n][3];
+    }
+
+    // output += weights * V; the weights go in as two summands so that their rounding stays below the output's
+#pragma unroll
+    for (int j = 0; j < TT / 16; ++j) {
+      uint32_t hi[4], lo[4];
+      split2<T>(s[2 * j][0], s[2 * j][1], hi[0], lo[0]);
+      split2<T>(s[2 * j][2], s[2 * j][3], hi[1], lo[1]);
+      split2<T>(s[2 * j + 1][0], s[2 * j + 1][1], hi[2], lo[2]);
+      split2<T>(s[2 * j + 1][2], s[2 * j + 1][3], hi[3], lo[3]);
+#pragma unroll
+      for (int c = 0; c < CH; c += 2) {
+        uint32_t vf[4];
+        ldsm_x4_trans(vf, vbase + unit_of<CH>(j * 16 + (mi & 1) * 8 + mr, c + (mi >> 1)) * 16);
+        mma16816<T>(o[c], hi[0], hi[1], hi[2], hi[3], vf[0], vf[1]);
+        mma16816<T>(o[c + 1], hi[0], hi[1], hi[2], hi[3], vf[2], vf[3]);
+        mma16816<T>(o[c], lo[0], lo[1], lo[2], lo[3], vf[0], vf[1]);
+        mma16816<T>(o[c + 1], lo[0], lo[1], lo[2], lo[3], vf[2], vf[3]);
+      }
+    }
+    __syncwarp();                       // every lane has read the slot before it is filled again
+    const int refill = slot == 0 ? ST - 1 : slot - 1;
+    issue(refill);
+    look();
+    slot = slot + 1 == ST ? 0 : slot + 1;
+    --left;
+
+    if (cur.t + 1 == cur.n || left == 0) {   // the pair's end, or the share's
+      l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
+      l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
+      l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
+      l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
+      if (poison) l0 = l1 = __int_as_float(0x7fc00000);
+      const bool whole = first_tile == 0 && cur.t + 1 == cur.n;
+      if (whole) {
+        const float i0 = 1.f / l0, i1 = 1.f / l1;
+        T* ob = static_cast<T*>(p.out) + ((int64_t)cur.b * p.Hq + head0) * p.hd;
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const int r = g + half * 8;
+          if (r < rows_here) {
+            const float inv = half ? i1 : i0;
+#pragma unroll
+            for (int c = 0; c < CH; ++c) {
+              if (c * 8 < p.hd) {
+                T two[2] = {Cvt<T>::from_f(o[c][half * 2] * inv), Cvt<T>::from_f(o[c][half * 2 + 1] * inv)};
+                *reinterpret_cast<uint32_t*>(ob + (int64_t)r * p.hd + c * 8 + t4 * 2) = *reinterpret_cast<uint32_t*>(two);
+              }
+            }
+            if (p.lse && t4 == 0) p.lse[(int64_t)cur.b * p.Hq + head0 + r] = ((half ? m1 : m0) + log2f(half ? l1 : l0)) * kLn2;
+          }
+        }
+      } else {
+        // slot 0 of the share: the pair that its first tile belongs to; slot 1: the pair that begins inside and goes on
+        const int ps = (cur.t - first_tile + 1 == (int)(end - begin) - left) ? 0 : 1;
+        float* po = p.part_o + ((int64_t)w * 2 + ps) * p.rows * p.hd;
+        float* pm = p.part_ml + ((int64_t)w * 2 + ps) * p.rows * 2;
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const int r = g + half * 8;
+          if (r < rows_here) {
+#pragma unroll
+            for (int c = 0; c < CH; ++c)
+              if (c * 8 < p.hd)
+                *reinterpret_cast<float2*>(po + r * p.hd + c * 8 + t4 * 2) = make_float2(o[c][half * 2], o[c][half * 2 + 1]);
+            if (t4 == 0) *reinterpret_cast<float2*>(pm + r * 2) = make_float2(half ? m1 : m0, half ? l1 : l0);
+          }
+        }
+      }
+      fresh = true;
+    }
+    if (left > 0) advance(cur);
+  }
+  cp_async_wait<0>();
+}
+
+// One CTA per (request, query head): nothing where one share held the whole pair, zeros for an empty request, else the
+// parts' weighted sum.  Thread d holds column d (and d + 128); parts in the order of their shares.
+template <typename T>
+__global__ void __launch_bounds__(128) paged_join_kernel(const PagedParams p) {
+  extern __shared__ float s_w[];    // [parts]
+  __shared__ float s_red[8];
+  const int b = blockIdx.x / p.Hq, hq = blockIdx.x - b * p.Hq;
+  const int kvh = hq / p.group, in_group = hq - kvh * p.group, qt = in_group / 16, r = in_group & 15;
+  const int H = p.Hkv * p.q_tiles, tid = threadIdx.x;
+  T* ob = static_cast<T*>(p.out) + (int64_t)blockIdx.x * p.hd;
+  chain_wait();
+  const int c0 = __ldcg(p.cum + b), c1 = __ldcg(p.cum + b + 1), call = __ldcg(p.cum + p.B);
+  const int n = c1 - c0;
+  if (n == 0) {   // an empty request; one with a length but no table at all is NaN like any that outgrew its table
+    const bool wrong = p.lens[b] > 0;
+    for (int d = tid; d < p.hd; d += 128) ob[d] = Cvt<T>::from_f(wrong ? __int_as_float(0x7fc00000) : 0.f);
+    if (p.lse && tid == 0) p.lse[blockIdx.x] = wrong ? __int_as_float(0x7fc00000) : -INFINITY;
+    return;
+  }
+  const int64_t total = (int64_t)call * H;
+  const int64_t share = max((total + p.workers - 1) / p.workers, (int64_t)kMinTiles);
+  const int64_t t0 = (int64_t)c0 * H + (int64_t)(kvh * p.q_tiles + qt) * n, t1 = t0 + n;
+  const int w0 = (int)(t0 / share), w1 = (int)((t1 - 1) / share);
+  if (w0 == w1) return;
+  const int parts = w1 - w0 + 1;
+  const int64_t first = (int64_t)w0 * 2 + (t0 == (int64_t)w0 * share ? 0 : 1);
+  auto slot = [&](int i) { return i == 0 ? first : (int64_t)(w0 + i) * 2; };
+  float m = -INFINITY;
+  for (int i = tid; i < parts; i += 128) m = fmaxf(m, __ldcg(p.part_ml + (slot(i) * p.rows + r) * 2));
+#pragma unroll
+  for (int s = 16; s > 0; s >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, s));
+  if ((tid & 31) == 0) s_red[tid >> 5] = m;
+  __syncthreads();
+  m = fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3]));
+  const float base = m == -INFINITY ? 0.f : m;
+  float l = 0.f;
+  for (int i = tid; i < parts; i += 128) {
+    const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.part_ml + (slot(i) * p.rows + r) * 2));
+    const float wgt = ex2(ml.x - base);
+    s_w[i] = wgt;
+    l += wgt * ml.y;
+  }
+#pragma unroll
+  for (int s = 16; s > 0; s >>= 1) l += __shfl_xor_sync(0xffffffffu, l, s);
+  if ((tid & 31) == 0) s_red[4 + (tid >> 5)] = l;
+  __syncthreads();
+  l = (s_red[4] + s_red[5]) + (s_red[6] + s_red[7]);
+  const float inv = 1.f / l;
+  for (int d = tid; d < p.hd; d += 128) {
+    float acc = 0.f;
+#pragma unroll 8
+    for (int i = 0; i < parts; ++i) acc += s_w[i] * __ldcg(p.part_o + (slot(i) * p.rows + r) * p.hd + d);
+    ob[d] = Cvt<T>::from_f(acc * inv);
+  }
+  if (p.lse && tid == 0) p.lse[blockIdx.x] = (m + log2f(l)) * kLn2;
+}
+
+int sm_count(int* out) {
+  int dev = 0;
+  HB_CUDA(cudaGetDevice(&dev));
+  HB_CUDA(cudaDeviceGetAttribute(out, cudaDevAttrMultiProcessorCount, dev));
+  return 0;
+}
+
+int padded_hd(int hd) { return hd <= 16 ? 16 : (hd <= 32 ? 32 : (hd <= 64 ? 64 : (hd <= 128 ? 128 : 256))); }
+
+size_t round256(size_t n) { return (n + 255) & ~(size_t)255; }
+
+size_t workspace_for(int B, int Hq, int Hkv, int hd, int sms) {
+  const int group = Hq / Hkv, rows = group < 16 ? group : 16;
+  const size_t slots = (size_t)sms * warps_of(padded_hd(hd)) * 2;
+  return round256(slots * rows * hd * 4) + round256(slots * rows * 8) + round256(((size_t)B + 1) * 4);
+}
+
+template <typename T, int HD>
+int launch(const PagedParams& p, int sms, cudaStream_t st) {
+  constexpr int NW = warps_of(HD);
+  const size_t smem = (size_t)NW * (kStages * 2 * tile_tokens(HD) * HD * 2 + (HD >= 256 ? 16 * HD * 2 : 0)) + (size_t)(2 * p.B + 1) * 4;
+  HB_PROPAGATE(ensure_dynamic_smem((const void*)paged_attention_kernel<T, HD>, smem));
+  HB_PROPAGATE(launch_chained(paged_attention_kernel<T, HD>, dim3((unsigned)sms), dim3(NW * 32), smem, st, false, 1, p));
+  return launch_chained(paged_join_kernel<T>, dim3((unsigned)(p.B * p.Hq)), dim3(128), (size_t)p.workers * 4, st, true, 1, p);
+}
+
+template <typename T>
+int launch_hd(const PagedParams& p, int sms, cudaStream_t st) {
+  switch (padded_hd(p.hd)) {
+    case 16: return launch<T, 16>(p, sms, st);
+    case 32: return launch<T, 32>(p, sms, st);
+    case 64: return launch<T, 64>(p, sms, st);
+    case 128: return launch<T, 128>(p, sms, st);
+    default: return launch<T, 256>(p, sms, st);
+  }
+}
+
+int check_heads(const char* what, int64_t B, int Hq, int Hkv, int hd) {
+  HB_REQUIRE(B >= 0 && Hq >= 1 && Hkv >= 1 && hd >= 1, HB200_ERR_INVALID, "%s: bad shape B=%lld Hq=%d Hkv=%d hd=%d", what,
+             (long long)B, Hq, Hkv, hd);
+  HB_REQUIRE(Hq % Hkv == 0, HB200_ERR_INVALID, "%s: %d query heads are no multiple of %d kv heads", what, Hq, Hkv);
+  HB_REQUIRE(hd % 8 == 0 && hd <= 256, HB200_ERR_UNSUPPORTED, "%s: head_dim %d (a multiple of 8 up to 256 is built)", what, hd);
+  HB_REQUIRE(B <= kMaxBatch, HB200_ERR_UNSUPPORTED, "%s: %lld requests (up to %d in one call)", what, (long long)B, kMaxBatch);
+  HB_REQUIRE(Hq <= 1024, HB200_ERR_UNSUPPORTED, "%s: %d query heads (up to 1024 are built)", what, Hq);
+  return 0;
+}
+
+}  // namespace
+}  // namespace hb200
+
+using namespace hb200;
+
+extern "C" size_t hb200_paged_attention_workspace_bytes(int B, int Hq, int Hkv, int hd) {
+  int sms = 0;
+  if (check_heads("paged_attention_workspace_bytes", B, Hq, Hkv, hd) != 0 || sm_count(&sms) != 0) return 0;
+  return workspace_for(B, Hq, Hkv, hd, sms);
+}
+
+extern "C" int hb200_paged_decode_attention(const hb200_paged_cache* c, const void* q, int64_t q_stride_b, int64_t q_stride_h,
+                                            void* out, float* lse, const int32_t* block_tables, int64_t table_ld, int table_width,
+                                            const int32_t* kv_lens, int B, int Hq, float scale, void* workspace,
+                                            size_t workspace_bytes, void* stream) {
+  HB_REQUIRE(c, HB200_ERR_INVALID, "paged_decode_attention: null pointer");
+  HB_PROPAGATE(check_heads("paged_decode_attention", B, Hq, c->n_kv_heads, c->head_dim));
+  if (B == 0) return 0;
+  HB_REQUIRE(q && out && kv_lens && c->k && c->v && workspace, HB200_ERR_INVALID, "paged_decode_attention: null pointer");
+  HB_REQUIRE(c->num_pages >= 0 && c->page_size >= 1 && table_width >= 0 && table_ld >= table_width && (block_tables || table_width == 0),
+             HB200_ERR_INVALID, "paged_decode_attention: bad cache or table shape");
+  HB_REQUIRE(aligned16(q) && aligned16(out) && aligned16(c->k) && aligned16(c->v) && aligned16(workspace), HB200_ERR_INVALID,
+             "paged_decode_attention: pointers must be 16-byte aligned");
+  const int64_t strides[] = {q_stride_b, q_stride_h, c->k_stride_page, c->k_stride_head, c->k_stride_row,
+                             c->v_stride_page, c->v_stride_head, c->v_stride_row};
+  for (int64_t s : strides)
+    HB_REQUIRE(s % 8 == 0, HB200_ERR_INVALID, "paged_decode_attention: strides must be multiples of 8 elements");
+  HB_REQUIRE(scale == scale, HB200_ERR_INVALID, "paged_decode_attention: scale is NaN");
+  const int group = Hq / c->n_kv_heads;
+  int sms = 0;
+  HB_PROPAGATE(sm_count(&sms));
+  HB_REQUIRE(workspace_bytes >= workspace_for(B, Hq, c->n_kv_heads, c->head_dim, sms), HB200_ERR_WORKSPACE,
+             "paged_decode_attention: workspace of %zu bytes, needs %zu", workspace_bytes,
+             workspace_for(B, Hq, c->n_kv_heads, c->head_dim, sms));
+  // lengths are clamped to the table's reach, so this bounds every tile count in 32 bits
+  const int64_t cap = (int64_t)table_width * c->page_size;
+  HB_REQUIRE(cap <= 0x7fffff00 && (int64_t)B * (cap / 16 + 1) <= 0x7fffffff, HB200_ERR_UNSUPPORTED,
+             "paged_decode_attention: tables of %d pages of %d tokens for %d requests reach too far", table_width, c->page_size, B);
+  PagedParams p = {};
+  p.q = q; p.kc = c->k; p.vc = c->v; p.out = out; p.lse = lse; p.table = block_tables; p.lens = kv_lens;
+  p.q_sb = q_stride_b; p.q_sh = q_stride_h;
+  p.k_sp = c->k_stride_page; p.k_sh = c->k_stride_head; p.k_sr = c->k_stride_row;
+  p.v_sp = c->v_stride_page; p.v_sh = c->v_stride_head; p.v_sr = c->v_stride_row;
+  p.table_ld = table_ld;
+  p.B = B; p.Hq = Hq; p.Hkv = c->n_kv_heads; p.hd = c->head_dim; p.group = group;
+  p.q_tiles = (group + 15) / 16;
+  p.rows = group < 16 ? group : 16;
+  p.page_size = c->page_size; p.width = table_width; p.num_pages = c->num_pages;
+  p.workers = sms * warps_of(padded_hd(c->head_dim));
+  p.scale_log2 = (float)((double)scale * 1.4426950408889634);
+  const size_t slots = (size_t)p.workers * 2;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  p.part_o = reinterpret_cast<float*>(ws);
+  ws += round256(slots * p.rows * p.hd * 4);
+  p.part_ml = reinterpret_cast<float*>(ws);
+  ws += round256(slots * p.rows * 8);
+  p.cum = reinterpret_cast<int32_t*>(ws);
+  cudaStream_t st = (cudaStream_t)stream;
+  if (c->dtype == HB200_BF16) return launch_hd<__nv_bfloat16>(p, sms, st);
+  if (c->dtype == HB200_F16) return launch_hd<__half>(p, sms, st);
+  set_error("paged_decode_attention: unsupported dtype %d (bf16 and f16 are built)", c->dtype);
+  return HB200_ERR_UNSUPPORTED;
+}

@@ -5,6 +5,7 @@ hand-written sm_100a CUDA kernels behind PyTorch-registered custom ops (``torch.
     fused_qk_norm(q, k, scale, temperature=1.0)     hydra/kernels/fused_ops.py:474-493
     fused_swiglu(gate, up)                          hydra/kernels/fused_ops.py:808-883
     fused_rms_norm(x, weight, eps=1e-6)             hydra/kernels/fused_ops.py:1114-1132
+    fused_qk_norm_rope(q, k, cos, sin, ...)         the norm and the rotation in one pass (no counterpart)
     set_use_triton_kernels / get_kernel_status      hydra/kernels/fused_ops.py:123-166
 
 Same argument meaning and result shapes/dtypes as the reference.  Differences, by design: tensors must live on
@@ -13,8 +14,9 @@ a CUDA device (a CPU tensor raises instead of silently taking a PyTorch path), t
 """
 from __future__ import annotations
 
+import ctypes as C
 from contextlib import nullcontext
-from typing import Tuple
+from typing import Optional, Tuple
 
 import torch
 
@@ -202,6 +204,101 @@ def fused_rms_norm(x: Tensor, weight: Tensor, eps: float = 1e-6) -> Tensor:
     return _rms_norm_op(x, weight, float(eps))
 
 
+def _refuse_autograd(what: str, *ts: Optional[Tensor]) -> None:
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
+        raise RuntimeError(f"{what} is inference only: an input requires grad (wrap the call in torch.no_grad())")
+
+
+def _fp32(what: str, t: Optional[Tensor], n: int, dev: torch.device) -> Optional[Tensor]:
+    if t is None:
+        return None
+    if t.device != dev or t.numel() != n:
+        raise ValueError(f"{what} must have {n} elements on {dev}, got {tuple(t.shape)} on {t.device}")
+    return t if t.dtype == torch.float32 and t.is_contiguous() else t.float().contiguous()
+
+
+_Strides = C.c_int64 * 3
+
+
+def _qk_norm_rope(what: str, dev: torch.device, q: Tensor, k: Tensor, cos: Tensor, sin: Tensor, positions: Optional[Tensor],
+                  q_weight: Optional[Tensor], k_weight: Optional[Tensor], norm: Optional[str], eps: float, q_scale: float,
+                  k_scale: float, layout: str, v: Optional[Tensor] = None, slots: Optional[Tensor] = None, cache=None):
+    """The call behind fused_qk_norm_rope and paged_append: q, k (v) [T, H, hd] or [B, H, S, hd]."""
+    _refuse_autograd(what, q, k, v, q_weight, k_weight)
+    if norm not in _lib.QK_NORMS:
+        raise ValueError(f"{what}: norm must be 'rms', 'l2' or None, got {norm!r}")
+    if layout not in _lib.ROPE_LAYOUTS:
+        raise ValueError(f"{what}: layout must be 'interleaved' or 'half', got {layout!r}")
+    hd = q.shape[-1]
+    if cos.dim() == 4:
+        cos, sin = cos[0, 0], sin[0, 0]
+    if cos.dim() != 2 or sin.shape != cos.shape or 2 * cos.shape[1] > hd:
+        raise ValueError(f"{what}: cos and sin must be [rows, rotated / 2] with rotated <= {hd}, got {tuple(cos.shape)} and {tuple(sin.shape)}")
+    if cos.dtype != torch.float32 or sin.dtype != torch.float32 or cos.stride() != sin.stride() or cos.stride(1) != 1 or cos.stride(0) < cos.shape[1]:
+        cos, sin = cos.float().contiguous(), sin.float().contiguous()
+    q = q if q.stride(-1) == 1 else q.contiguous()
+    k = k if k.stride(-1) == 1 else k.contiguous()
+    if q.dim() == 3:
+        B, S = 1, q.shape[0]
+        strides = lambda t: _Strides(0, t.stride(0), t.stride(1))   # noqa: E731
+    else:
+        B, S = q.shape[0], q.shape[2]
+        strides = lambda t: _Strides(t.stride(0), t.stride(2), t.stride(1))   # noqa: E731
+    if positions is not None:
+        if positions.dtype not in (torch.int32, torch.int64):
+            raise TypeError(f"{what}: positions must be int32 or int64, got {positions.dtype}")
+        if positions.shape != (S,) and positions.shape != (B, S):
+            raise ValueError(f"{what}: positions {tuple(positions.shape)} for {B} x {S} tokens")
+        positions = positions if S < 2 or positions.stride(-1) == 1 else positions.contiguous()
+    elif cos.shape[0] < S:
+        raise ValueError(f"{what}: tables {tuple(cos.shape)} do not cover {S} positions")
+    q_weight = _fp32(f"{what}: q_weight", q_weight, hd, dev)
+    k_weight = _fp32(f"{what}: k_weight", k_weight, hd, dev)
+    q_out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    k_out = torch.empty(k.shape, dtype=k.dtype, device=dev) if cache is None else None
+    if q.numel() + k.numel() == 0:
+        return q_out, k_out
+    if v is not None and v.stride(-1) != 1:
+        v = v.contiguous()
+    args = _lib.QkNormRopeArgs(
+        q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr() if v is not None else None, q_out=q_out.data_ptr(),
+        k_out=k_out.data_ptr() if k_out is not None else None, slots=slots.data_ptr() if slots is not None else None,
+        positions=positions.data_ptr() if positions is not None else None, cos=cos.data_ptr(), sin=sin.data_ptr(),
+        q_weight=q_weight.data_ptr() if q_weight is not None else None, k_weight=k_weight.data_ptr() if k_weight is not None else None,
+        q_stride=strides(q), k_stride=strides(k), v_stride=strides(v) if v is not None else _Strides(),
+        q_out_stride=strides(q_out), k_out_stride=strides(k_out) if k_out is not None else _Strides(),
+        positions_stride=positions.stride(0) if positions is not None and positions.dim() == 2 else 0,
+        table_rows=cos.shape[0], table_ld=cos.stride(0) if cos.shape[0] > 1 else cos.shape[1],
+        positions_64=int(positions is not None and positions.dtype == torch.int64), B=B, S=S, Hq=q.shape[1], Hkv=k.shape[1],
+        hd=hd, rot=2 * cos.shape[1], layout=_lib.ROPE_LAYOUTS[layout], norm=_lib.QK_NORMS[norm], dtype=_dtype_code(q),
+        eps=float(eps), q_scale=float(q_scale), k_scale=float(k_scale))
+    with _on(dev):
+        _lib.check(_lib.lib().hb200_qk_norm_rope(C.byref(args), C.byref(cache) if cache is not None else None, _stream(dev)), what)
+    return q_out, k_out
+
+
+def fused_qk_norm_rope(q: Tensor, k: Tensor, cos: Tensor, sin: Tensor, positions: Optional[Tensor] = None, *,
+                       q_weight: Optional[Tensor] = None, k_weight: Optional[Tensor] = None, norm: Optional[str] = "rms",
+                       eps: float = 1e-6, q_scale: float = 1.0, k_scale: float = 1.0,
+                       layout: str = "interleaved") -> Tuple[Tensor, Tensor]:
+    """Norm of every query and key head and the position rotation, in one pass (``hb200_qk_norm_rope``; the reference norms
+    and rotates in two, hydra/attention/backends/ccgqa/attention.py:257-266): 32 bits inside, rounded once.
+
+    q [B, Hq, S, hd] and k [B, Hkv, S, hd], or packed tokens [T, Hq, hd] and [T, Hkv, hd]; strided views are read in place.
+    ``norm``: "rms" (``x * rsqrt(mean(x^2) + eps)``), "l2" (``x * rsqrt(sum(x^2) + eps)``) or None; then times the weight [hd]
+    of q or k (if given) and ``q_scale`` / ``k_scale`` (a softmax scale, CCGQA's key temperature).  cos, sin [rows, rot / 2] (or
+    [1, 1, rows, rot / 2]) turn the first ``rot <= hd`` values of a head, whatever frequencies the tables were built with
+    (scaled ones for long contexts); ``layout`` "interleaved" pairs values (2i, 2i + 1), "half" (i, i + rot / 2).  ``positions``
+    int32 or int64 [S], [B, S] or [T] are table rows (default 0 .. S - 1): a negative one marks padding (zeros), one beyond
+    the tables gives NaN.  hd up to 256.  Returns contiguous q and k."""
+    dev = _require_cuda(q, k, cos, sin, *(() if positions is None else (positions,)))
+    if q.dim() not in (3, 4) or k.dim() != q.dim() or q.dtype != k.dtype or q.shape[-1] != k.shape[-1] or q.shape[0] != k.shape[0] \
+            or (q.dim() == 4 and q.shape[2] != k.shape[2]):
+        raise ValueError("fused_qk_norm_rope: q [B, Hq, S, hd] and k [B, Hkv, S, hd] (or [T, Hq, hd] and [T, Hkv, hd]) of one dtype "
+                         f"are wanted, got {tuple(q.shape)} {q.dtype} and {tuple(k.shape)} {k.dtype}")
+    return _qk_norm_rope("fused_qk_norm_rope", dev, q, k, cos, sin, positions, q_weight, k_weight, norm, eps, q_scale, k_scale, layout)
+
+
 def set_use_triton_kernels(enabled: bool) -> None:
     """Kept for API compatibility (hydra/kernels/fused_ops.py:123-148).  There is exactly one implementation
     here and it has no Triton or PyTorch alternative, so the switch only records the request."""
@@ -229,7 +326,7 @@ def get_kernel_status() -> dict:
 
 
 __all__ = [
-    "fused_rope", "fused_qk_norm", "fused_swiglu", "fused_rms_norm", "set_use_triton_kernels",
+    "fused_rope", "fused_qk_norm", "fused_qk_norm_rope", "fused_swiglu", "fused_rms_norm", "set_use_triton_kernels",
     "get_kernel_status", "TRITON_AVAILABLE", "USE_TRITON_KERNELS", "USE_FUSED_ROPE", "USE_FUSED_QK_NORM",
     "USE_FUSED_SWIGLU", "USE_FUSED_RMS_NORM",
 ]

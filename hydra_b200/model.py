@@ -19,7 +19,7 @@ import torch
 
 from . import _lib, kernels
 from ._pack import PackedBlock, PackedModel, _bf16, _f32
-from .sampling import cross_entropy_rows, sample_rows
+from .sampling import TokenLogprobs, cross_entropy_rows, sample_rows, token_logprobs
 
 Tensor = torch.Tensor
 
@@ -516,6 +516,25 @@ class HydraB200Model:
             return total
         return total / (targets != ignore_index).sum().clamp(min=1).to(total.dtype)
 
+    def token_logprobs(self, ids: Tensor, targets: Optional[Tensor] = None, top: int = 0, temperature: float = 1.0,
+                       ignore_index: int = -100) -> TokenLogprobs:
+        """Log probability of every next token, with the entropy and the ``top`` most likely alternatives of its
+        distribution (:func:`hydra_b200.sampling.token_logprobs`): the model runs on ids [B, S] as in :meth:`eval_loss`
+        and is scored against ``targets`` (default: ``ids[:, 1:]`` after ``ids[:, :-1]``).  Tensors [B, S] and
+        [B, S, top]."""
+        if targets is None:
+            if ids.shape[1] < 2:
+                raise ValueError("token_logprobs needs at least two tokens per sequence")
+            ids, targets = ids[:, :-1], ids[:, 1:]
+        if tuple(targets.shape) != tuple(ids.shape):
+            raise ValueError("targets must have the shape of ids")
+        B, S = ids.shape
+        lg = self.forward(ids)
+        padded = lg.as_strided((B * S, self.ld_logits), (self.ld_logits, 1))      # the rows with their padding columns
+        r = token_logprobs(padded, targets.to(self.device).reshape(-1), top, temperature, vocab=self.vocab_size,
+                           ignore_index=ignore_index)
+        return TokenLogprobs(r.logprobs.view(B, S), r.entropy.view(B, S), r.top_logprobs.view(B, S, top), r.top_ids.view(B, S, top))
+
     def resize_rope_cache(self, new_max_seq_len: int) -> None:
         """HydraModel.resize_rope_cache (model.py:376-392): longer sequences than the model was built for.  The tables
         only ever grow; ``max_seq_len`` takes the new value, as in the reference."""
@@ -808,6 +827,13 @@ class DecodeSession:
                     vocab=self.model.vocab_size, out=self.tokens)
         self.history[:, self.pos] = self.tokens
         return self.tokens
+
+    def token_logprobs(self, top: int = 0, temperature: float = 1.0) -> TokenLogprobs:
+        """Log probabilities of the tokens that the latest ``prefill`` / ``step`` / ``resample`` chose, with the entropy and
+        the ``top`` alternatives of the distributions they were chosen from (rows of ``last_logits``)."""
+        if self.pos < 1:
+            raise RuntimeError("token_logprobs() needs a prefill first")
+        return token_logprobs(self.last_logits, self.tokens, top, temperature, vocab=self.model.vocab_size)
 
     def _launch_step(self) -> None:
         m = self.model

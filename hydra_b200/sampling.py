@@ -4,7 +4,7 @@ with ``torch.multinomial``; here the draw is the inverse CDF at one uniform numb
 from (logits, uniform)."""
 from __future__ import annotations
 
-from typing import Optional
+from typing import NamedTuple, Optional
 
 import torch
 from torch import Tensor
@@ -35,6 +35,55 @@ def cross_entropy_rows(logits: Tensor, targets: Tensor, vocab: Optional[int] = N
             logits.data_ptr(), targets.data_ptr(), N, V, logits.stride(0) if N > 1 else max(logits.stride(0), V),
             int(ignore_index), out.data_ptr(), kernels._stream(logits.device)), "cross_entropy_rows")
     return out
+
+
+class TokenLogprobs(NamedTuple):
+    """What :func:`token_logprobs` returns for N rows."""
+    logprobs: Tensor       # fp32 [N]
+    entropy: Tensor        # fp32 [N], in nats
+    top_logprobs: Tensor   # fp32 [N, top], most likely first
+    top_ids: Tensor        # int64 [N, top]
+
+
+def token_logprobs(logits: Tensor, tokens: Tensor, top: int = 0, temperature: float = 1.0, vocab: Optional[int] = None,
+                   ignore_index: int = -100) -> TokenLogprobs:
+    """Log probability of a given token, entropy and the ``top`` most likely tokens (up to 32) of each logit row
+    (``hb200_token_logprobs``): one pass over the logits, 32 bits inside, nothing read on the host.
+
+    logits [N, ld] bf16, f16 or fp32 on a CUDA device (any row stride, the first ``vocab`` columns count), tokens int64 [N].  The
+    distribution is ``softmax(logits / temperature)``.  A row's log probability is 0 where its token is ``ignore_index`` and NaN
+    where the token lies outside [0, vocab) otherwise (:func:`cross_entropy_rows` checks that on the host instead); entropy and
+    alternatives do not depend on the token.  Of equal logits the lowest id comes first.  -inf logits (a grammar's mask) take
+    no part and come last; a row without any other, or with NaN or +inf, gives NaN."""
+    dev = kernels._require_cuda(logits, tokens)
+    kernels._refuse_autograd("token_logprobs", logits)
+    if logits.dim() != 2 or (logits.stride(1) != 1 and logits.shape[1] > 1):
+        raise ValueError("token_logprobs: logits must be [N, V] with unit column stride")
+    dtype = kernels._dtype_code(logits)
+    N = logits.shape[0]
+    V = int(vocab) if vocab is not None else logits.shape[1]
+    top, temperature = int(top), float(temperature)
+    if not 1 <= V <= logits.shape[1]:
+        raise ValueError(f"token_logprobs: vocab {V} outside the row length {logits.shape[1]}")
+    if tokens.dtype != torch.int64 or tokens.numel() != N:
+        raise ValueError(f"token_logprobs: one int64 token per row, got {tokens.dtype} {tuple(tokens.shape)} for {N} rows")
+    if not 0 <= top <= min(32, V):
+        raise ValueError(f"token_logprobs: top {top} (0 to 32, at most the vocabulary)")
+    if not 1e-6 <= temperature <= 1e6:
+        raise ValueError(f"token_logprobs: temperature {temperature} (1e-6 to 1e6)")
+    if N > 1 and logits.stride(0) < V:
+        logits = logits.contiguous()          # rows that overlap (an expanded row)
+    tokens = tokens if tokens.is_contiguous() else tokens.contiguous()
+    f32 = dict(dtype=torch.float32, device=dev)
+    r = TokenLogprobs(torch.empty(N, **f32), torch.empty(N, **f32), torch.empty((N, top), **f32),
+                      torch.empty((N, top), dtype=torch.int64, device=dev))
+    if N > 0:
+        with kernels._on(dev):
+            _lib.check(_lib.lib().hb200_token_logprobs(
+                logits.data_ptr(), tokens.data_ptr(), N, V, logits.stride(0) if N > 1 else max(logits.stride(0), V), int(ignore_index),
+                temperature, top, r.logprobs.data_ptr(), r.entropy.data_ptr(), r.top_logprobs.data_ptr(), r.top_ids.data_ptr(),
+                dtype, kernels._stream(dev)), "token_logprobs")
+    return r
 
 
 def sample_rows(logits: Tensor, temperature: float = 0.8, top_k: int = 50, top_p: float = 0.9,

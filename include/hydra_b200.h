@@ -399,6 +399,88 @@ int hb200_ccgqa_forward_static(const hb200_model* m, int block_index, const void
                                int32_t* err_flag, void* stream);
 
 /* ---------------------------------------------------------------------------
+ * Serving operators on a paged key-value cache (no counterpart in the reference, which has no cache): the pages and slots
+ * of a step, the norm and rotation of its queries and keys on their way into the cache, the attention of one new token per
+ * request, and the log probabilities of the answer's tokens.  A cache is two tensors of pages, [num_pages, n_kv_heads,
+ * page_size, head_dim] by their strides (in elements; a head row is contiguous), so head-major and token-major pages both
+ * serve.  Slot s of a cache is row s % page_size of page s / page_size.
+ * ------------------------------------------------------------------------- */
+typedef struct hb200_paged_cache {
+  void* k;
+  void* v;
+  int64_t k_stride_page, k_stride_head, k_stride_row;
+  int64_t v_stride_page, v_stride_head, v_stride_row;
+  int32_t num_pages, page_size, n_kv_heads, head_dim, dtype;
+} hb200_paged_cache;
+
+/* Bits of the status that hb200_paged_plan writes. */
+enum { HB200_PLAN_OUT_OF_PAGES = 1,   /* the free list ends before the requests' needs: page -1, slot -1 */
+       HB200_PLAN_TABLE_FULL = 2,     /* a request outgrew its table row: slot -1 behind its end */
+       HB200_PLAN_OUT_OF_ROOM = 4,    /* more new tokens than max_new: the ones behind have no entry */
+       HB200_PLAN_BAD_LENGTH = 8 };   /* a negative length (read as 0) or a sum past 2^31 - 1 (cut) */
+
+/* Block tables, slots and positions of a step from the requests' lengths, on the device, in one launch.
+ * context_lens, new_lens int32 [B]: tokens in the cache, tokens to come.  block_tables int32 [B, table_width] (row stride
+ * table_ld): the pages that each request holds; the entries of the pages it needs beyond them are taken from free_pages
+ * int32 [n_free] in request order, from *free_start on (NULL: 0), and written in place.  Outputs: kv_lens int32 [B] (context
+ * + new), cu_new int32 [B + 1] (new tokens before each request), positions int32 [max_new] and slots int64 [max_new] of the
+ * new tokens, packed request after request (-1 behind the last), free_start_out int32 [1] (where the next call goes on),
+ * status int32 [1].  Nothing overlaps; the inputs other than block_tables are left as they are, so the same call gives
+ * the same result again.  Up to 4096 requests. */
+int hb200_paged_plan(const int32_t* context_lens, const int32_t* new_lens, int B, int32_t* block_tables, int64_t table_ld,
+                     int table_width, int page_size, const int32_t* free_pages, int64_t n_free, const int32_t* free_start,
+                     int32_t* kv_lens, int32_t* cu_new, int32_t* positions, int64_t* slots, int max_new,
+                     int32_t* free_start_out, int32_t* status, void* stream);
+
+enum { HB200_ROPE_INTERLEAVED = 0, HB200_ROPE_HALF = 1 };             /* pairs (2i, 2i + 1) / (i, i + rot / 2) */
+enum { HB200_NORM_NONE = 0, HB200_NORM_RMS = 1, HB200_NORM_L2 = 2 };  /* x rsqrt(mean x^2 + eps) / x rsqrt(sum x^2 + eps) */
+
+typedef struct hb200_qk_norm_rope_args {
+  const void* q;                 /* [B, S, Hq, hd] by strides (batch, token, head), in elements; a head row is contiguous */
+  const void* k;                 /* [B, S, Hkv, hd] */
+  const void* v;                 /* [B, S, Hkv, hd], with a cache */
+  void* q_out;
+  void* k_out;                   /* without a cache */
+  const int64_t* slots;          /* [B * S], with a cache: where k and v go; negative: nowhere */
+  const void* positions;         /* int32 (or int64: positions_64) [B, S], row stride positions_stride; NULL: 0 .. S - 1 */
+  const float* cos;              /* [table_rows, rot / 2], row stride table_ld */
+  const float* sin;
+  const float* q_weight;         /* [hd] or NULL */
+  const float* k_weight;
+  int64_t q_stride[3], k_stride[3], v_stride[3], q_out_stride[3], k_out_stride[3];
+  int64_t positions_stride, table_rows, table_ld;
+  int32_t positions_64, B, S, Hq, Hkv, hd, rot, layout, norm, dtype;
+  float eps, q_scale, k_scale;
+} hb200_qk_norm_rope_args;
+
+/* Per-head norm (times weight and scale) of q and k and rotation of the first `rot` values of each head, in one pass: 32 bits
+ * inside, rounded once.  With `cache`, k and v rows go to their slots instead of k_out (v unchanged; other slots are left as
+ * they are).  A row with a negative position is padding: zeros in q_out / k_out, nothing into the cache.  A position beyond
+ * the tables, or a slot beyond the cache, gives NaN (nothing is written out of range).  head_dim up to 256. */
+int hb200_qk_norm_rope(const hb200_qk_norm_rope_args* args, const hb200_paged_cache* cache, void* stream);
+
+/* Attention of one new token per request over the paged cache: q [B, Hq, hd] by strides, out [B, Hq, hd] contiguous in the
+ * cache's dtype (bf16 or f16), lse fp32 [B, Hq] (ln of the sum of exponentials) or NULL.  block_tables int32 [B,
+ * table_width], kv_lens int32 [B]: request b attends to its first kv_lens[b] tokens.  An empty request gives zeros and -inf;
+ * one whose table names a page outside the cache, or whose length passes its table, gives NaN.  head_dim a multiple of 8 up
+ * to 256; Hq a multiple of the kv heads; up to 4096 requests.  Strides are multiples of 8 elements, pointers 16-byte
+ * aligned.  workspace: hb200_paged_attention_workspace_bytes on the current device, not shared by calls that overlap. */
+size_t hb200_paged_attention_workspace_bytes(int B, int Hq, int Hkv, int hd);
+int hb200_paged_decode_attention(const hb200_paged_cache* cache, const void* q, int64_t q_stride_b, int64_t q_stride_h,
+                                 void* out, float* lse, const int32_t* block_tables, int64_t table_ld, int table_width,
+                                 const int32_t* kv_lens, int B, int Hq, float scale, void* workspace, size_t workspace_bytes,
+                                 void* stream);
+
+/* Log probability of a given token, entropy and the `top` most likely tokens of each logit row at a temperature.  logits
+ * [rows, ld] (any dtype; the first `cols` columns count, rows need no alignment), tokens int64 [rows]: logprobs fp32 [rows]
+ * (0 for ignore_index, NaN for any other token outside [0, cols)), entropy fp32 [rows] in nats, top_logprobs fp32 and
+ * top_ids int64 [rows, top], most likely first, of equal logits the lowest index first.  -inf logits take no part; a row
+ * without any other, or with NaN or +inf, gives NaN (its ids are still in order: NaN above +inf).  top up to 32. */
+int hb200_token_logprobs(const void* logits, const int64_t* tokens, int64_t rows, int cols, int64_t ld, int64_t ignore_index,
+                         float temperature, int top, float* logprobs, float* entropy, float* top_logprobs, int64_t* top_ids,
+                         int dtype, void* stream);
+
+/* ---------------------------------------------------------------------------
  * Measurement aid (no counterpart in the reference): per-launch CUDA-event timing of the kernels that
  * hb200_model_forward / hb200_block_forward / hb200_ccgqa_forward enqueue.  When hb200_model.profile holds a
  * handle, every kernel launch of the executor is bracketed by two events recorded on the launching stream.
