@@ -3,9 +3,10 @@
 //   s_j = scale * q . k_j  (j < len),   out = sum_j e^{s_j} v_j / sum_j e^{s_j},   lse = ln sum_j e^{s_j}
 //
 // Bound: HBM.  Every K and V row of the valid tokens is read once (4 * hd bytes per token and kv head) for 4 * hd * group
-// operations, so the tensor cores are needed only to keep the arithmetic out of the way: the query heads of one kv head
-// are the 16 rows of an m16n8k16 product.  tcgen05 would want 64 or 128 rows of queries; with 1..16 of them its TMEM
-// round trip buys nothing, so the warp-level instruction is used.
+// operations, so the tensor cores are needed only to keep the arithmetic out of the way.  tcgen05 would want 64 or 128 rows
+// on the accumulator's side and a TMEM round trip for the weights; with 1..16 query heads per kv head the warp-level m16n8k16
+// is used, transposed (scores^T = K Q^T, out^T = V^T P^T): the tokens and the head's values are the 16 rows and the query heads
+// the 8 columns, so a group of up to 8 heads costs half of what 16 padded query rows cost, in registers too.
 //
 // Work split: the tiles of all (request, kv head) pairs are laid end to end and dealt out in equal contiguous shares to
 // the warps of a grid that fits the GPU once (one CTA per SM), whatever the lengths are: a batch of one long and many
@@ -32,14 +33,16 @@ struct PagedParams {
   float* part_o;     // [workers][2][rows][hd]
   float* part_ml;    // [workers][2][rows][2]
   int32_t* cum;      // [B + 1] tiles of the requests before each one
-  int64_t q_sb, q_sh, k_sp, k_sh, k_sr, v_sp, v_sh, v_sr, table_ld;
+  int64_t q_sb, q_sh, k_sh, v_sh, table_ld;     // elements
+  int32_t k_sp, k_sr, v_sp, v_sr;               // bytes: page and row of a page
   int B, Hq, Hkv, hd, group, q_tiles, rows, page_size, width, num_pages, workers;
   float scale_log2;  // scale * log2(e)
 };
 
-__host__ __device__ constexpr int tile_tokens(int HD) { return HD >= 128 ? 16 : (HD == 64 ? 32 : 64); }
+// A warp's tile: 8 KB of K and V (16 KB of heads of 256, 4 KB of small ones); its ring keeps 16 KB in flight, a CTA 128 KB.
+__host__ __device__ constexpr int tile_tokens(int HD) { return HD >= 128 ? 16 : (HD == 16 ? 64 : 32); }
 __host__ __device__ constexpr int warps_of(int HD) { return HD >= 256 ? 4 : 8; }
-constexpr int kStages = 3;
+__host__ __device__ constexpr int stages_of(int HD) { return HD <= 32 ? 5 : 3; }
 
 // Cache length of request b as the kernel reads it: what lies outside [0, width * page_size] is marked (`poison`).
 __device__ __forceinline__ int clamp_len(int len, int64_t cap, bool& poison) {
@@ -97,13 +100,18 @@ __device__ __forceinline__ void split2<__half>(float a, float b, uint32_t& hi, u
   lo = *reinterpret_cast<const uint32_t*>(&l);
 }
 
-// 16-byte unit of (row, chunk) in a tile of rows of CH chunks, xor-swizzled so that eight rows of one chunk column lie in
-// eight different bank groups (ldmatrix without conflicts).
+// Transposes an 8x8 matrix of 16-bit values held as in a fragment (thread 4r + c/2 holds (r, c..c+1)).
+__device__ __forceinline__ uint32_t movmatrix_trans(uint32_t a) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(a));
+  return r;
+}
+
+// Swizzle of a tile's 16-byte chunks: chunk c of row r lies at place c ^ swizzle(r), so that eight rows of one chunk column
+// lie in eight different bank groups (ldmatrix without conflicts).  CH: chunks per row.  The same for r and r + 8.
 template <int CH>
-__device__ __forceinline__ int unit_of(int row, int c) {
-  if (CH >= 8) return row * CH + (c ^ (row & 7));
-  if (CH == 4) return row * CH + (c ^ ((row >> 1) & 3));
-  return row * CH + (c ^ ((row >> 2) & 1));
+__device__ __forceinline__ int swizzle(int r) {
+  return CH >= 8 ? (r & 7) : (CH == 4 ? ((r >> 1) & 3) : ((r >> 2) & 1));
 }
 
 // A place in the row of all tiles: request b, head tile h (kv head * q_tiles + tile of its query heads), tile t of n.
@@ -112,20 +120,22 @@ struct Cursor {
   bool poison;
 };
 
-template <typename T, int HD>
+// NQ: columns of eight query heads (group <= 8: 1).
+template <typename T, int HD, int NQ>
 __global__ void __launch_bounds__(warps_of(HD) * 32, 1) paged_attention_kernel(const PagedParams p) {
-  constexpr int NW = warps_of(HD), TT = tile_tokens(HD), CH = HD / 8, ST = kStages;
-  constexpr int KBYTES = TT * HD * 2, STAGE = 2 * KBYTES;
-  constexpr int NT = TT / 8;                 // n tiles of the scores
-  constexpr int LOADS = TT * CH / 32;        // 16-byte copies of K (and of V) per lane and tile
-  constexpr int ROWS_PER = 32 / CH;          // rows one copy instruction of the warp covers (CH <= 32)
-  constexpr int TREG = (TT + 31) / 32;       // token bookkeeping registers per lane
-  constexpr bool Q_IN_SMEM = HD >= 256;      // the query fragments do not fit beside the output's registers
+  constexpr int NW = warps_of(HD), TT = tile_tokens(HD), CH = HD / 8, ST = stages_of(HD);
+  constexpr int ROWB = HD * 2, KBYTES = TT * ROWB, STAGE = 2 * KBYTES;
+  constexpr int MT = TT / 16;                        // 16-token tiles
+  constexpr int KS = HD / 16;                        // 16-value steps of a head
+  constexpr int LPR = CH >= 4 ? 4 : CH;              // copies: lanes per row (64 bytes side by side)
+  constexpr int RPI = 32 / LPR, R = TT / RPI;        // rows per copy instruction, rows per lane
+  constexpr int CI = CH / LPR;                       // copies per row and lane
+  constexpr int NO = KS < 4 ? KS : 4;                // distinct swizzled offsets of the 16-value steps
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int scan_buf[33];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int32_t* s_cum = reinterpret_cast<int32_t*>(smem + NW * (ST * STAGE + (Q_IN_SMEM ? 16 * HD * 2 : 0)));   // [B + 1]
-  int32_t* s_len = s_cum + p.B + 1;                                                                          // [B]
+  int32_t* s_cum = reinterpret_cast<int32_t*>(smem + NW * ST * STAGE);   // [B + 1]
+  int32_t* s_len = s_cum + p.B + 1;                                      // [B]
   chain_release();   // the join kernel may take its place; it waits for this grid's end before it reads anything
 
   // tiles before each request
@@ -162,11 +172,11 @@ __global__ void __launch_bounds__(warps_of(HD) * 32, 1) paged_attention_kernel(c
   const int H = p.Hkv * p.q_tiles;
   const int64_t total = (int64_t)s_cum[p.B] * H;
   const int64_t share = max((total + p.workers - 1) / p.workers, (int64_t)kMinTiles);
-  const int w = blockIdx.x * NW + warp;
+  const int w = warp * gridDim.x + blockIdx.x;       // few shares: one per SM before any SM has two
   const int64_t begin = (int64_t)w * share;
   if (begin >= total) return;
   const int64_t end = begin + share < total ? begin + share : total;
-  int left = (int)(end - begin);   // tiles to compute (a share is far below 2^31: total < 2^31 * H / workers)
+  int left = (int)(end - begin);                     // tiles to compute
 
   auto enter = [&](Cursor& c) {   // request c.b's length and tiles
     c.n = s_cum[c.b + 1] - s_cum[c.b];
@@ -192,65 +202,94 @@ __global__ void __launch_bounds__(warps_of(HD) * 32, 1) paged_attention_kernel(c
     }
     cur.b = lo;
     enter(cur);
-    const int64_t r = begin - (int64_t)s_cum[lo] * H;
-    cur.h = (int)(r / cur.n);
-    cur.t = (int)(r % cur.n);
+    const int r = (int)(begin - (int64_t)s_cum[lo] * H);
+    cur.h = r / cur.n;
+    cur.t = r % cur.n;
   }
 
   uint8_t* ring = smem + warp * ST * STAGE;
   const uint32_t ring_u = smem_u32(ring);
-  uint8_t* q_smem = smem + NW * ST * STAGE + warp * 16 * HD * 2;
   if (p.hd < HD) {   // the padding chunks are never copied to: zero them once (zero times anything the ring held before)
     for (int u = lane; u < ST * STAGE / 16; u += 32) reinterpret_cast<uint4*>(ring)[u] = make_uint4(0, 0, 0, 0);
     __syncwarp();
   }
 
-  // ---- producer: the page of every token of a tile is looked up one tile before its copies are issued
+  // ---- producer: four lanes (two of heads of 16) copy a row, every lane looks up the pages of its own R rows; that is done
+  // one tile before their copies are issued
   Cursor pc = cur;
   int to_look = left, to_issue = left;
-  int page[TREG], row[TREG], l_kvh = 0;
+  int page0 = (int)(((int64_t)pc.t * TT) / p.page_size), off0 = (int)((int64_t)pc.t * TT - (int64_t)page0 * p.page_size);
+  const int32_t* trow = p.table + (int64_t)pc.b * p.table_ld;
+  const char *kb = nullptr, *vb = nullptr;    // the head's rows, of the tile that was looked up
+  int page[R], row[R];
   bool bad_seen = false;            // a page outside the cache, in the tile that was looked up
   uint32_t bad_bits = 0;            // the same per ring slot
+  const int prow = lane / LPR, pch = lane % LPR;
+  uint32_t dst[2];                  // of the lane's even and odd copies of a row
+#pragma unroll
+  for (int i = 0; i < 2; ++i) dst[i] = ring_u + prow * ROWB + (((pch + (CI > 1 ? LPR * i : 0)) ^ swizzle<CH>(prow)) & (CH >= 8 ? 7 : CH - 1)) * 16;
   auto look = [&]() {
     if (to_look > 0) {
       --to_look;
-      l_kvh = pc.h / p.q_tiles;
+      const int kvh = p.q_tiles == 1 ? pc.h : pc.h / p.q_tiles;
+      kb = static_cast<const char*>(p.kc) + (int64_t)kvh * p.k_sh * 2 + pch * 16;
+      vb = static_cast<const char*>(p.vc) + (int64_t)kvh * p.v_sh * 2 + pch * 16;
       bool bad = pc.poison;
+      const int rows_in = pc.len - pc.t * TT;         // > 0
 #pragma unroll
-      for (int i = 0; i < TREG; ++i) {
-        const int tok = pc.t * TT + i * 32 + lane;
-        const bool in = tok < pc.len && i * 32 + lane < TT;
-        const int pi = in ? tok / p.page_size : 0;
-        row[i] = tok - pi * p.page_size;
-        const int id = in ? __ldg(p.table + (int64_t)pc.b * p.table_ld + pi) : -1;
-        const bool ok = in && id >= 0 && id < p.num_pages;
+      for (int j = 0; j < R; ++j) {
+        const int r = prow + j * RPI;
+        int pi = page0, o = off0 + r;
+        if (p.page_size >= TT) {                      // at most one page ends inside the tile
+          if (o >= p.page_size) { o -= p.page_size; ++pi; }
+        } else {
+          const int k = o / p.page_size;
+          pi += k;
+          o -= k * p.page_size;
+        }
+        const bool in = r < rows_in;
+        const int id = in ? __ldg(trow + pi) : -1;
+        const bool ok = (unsigned)id < (unsigned)p.num_pages;
         bad |= in && !ok;
-        page[i] = ok ? id : -1;
+        page[j] = ok ? id : -1;
+        row[j] = o;
       }
       bad_seen = bad;
-      if (to_look > 0) advance(pc);
+      if (to_look > 0) {
+        const int b = pc.b, h = pc.h;
+        advance(pc);
+        if (pc.b != b || pc.h != h) {
+          page0 = off0 = 0;
+          trow = p.table + (int64_t)pc.b * p.table_ld;
+        } else if (p.page_size >= TT) {
+          off0 += TT;
+          if (off0 >= p.page_size) { off0 -= p.page_size; ++page0; }
+        } else {
+          page0 = (int)(((unsigned)pc.t * TT) / (unsigned)p.page_size);
+          off0 = pc.t * TT - page0 * p.page_size;
+        }
+      }
     }
   };
   auto issue = [&](int slot) {
     if (to_issue > 0) {
       --to_issue;
-      const uint32_t kdst = ring_u + slot * STAGE, vdst = kdst + KBYTES;
-      const T* kb = static_cast<const T*>(p.kc) + (int64_t)l_kvh * p.k_sh;
-      const T* vb = static_cast<const T*>(p.vc) + (int64_t)l_kvh * p.v_sh;
-      const int c = lane % CH;
-      const bool chunk_in = c * 8 < p.hd;
+      const uint32_t so = slot * STAGE;
 #pragma unroll
-      for (int i = 0; i < LOADS; ++i) {
-        const int r = i * ROWS_PER + lane / CH;           // r / 32 is the same for all lanes
-        const int pg = __shfl_sync(0xffffffffu, page[(i * ROWS_PER) / 32], r & 31);
-        const int rw = __shfl_sync(0xffffffffu, row[(i * ROWS_PER) / 32], r & 31);
-        const bool there = pg >= 0;
-        const int64_t pp = there ? pg : 0;
-        const int64_t rr = there ? rw : 0;
-        if (chunk_in) {
-          const uint32_t u = unit_of<CH>(r, c) * 16;
-          cp_async_16_zfill(kdst + u, kb + pp * p.k_sp + rr * p.k_sr + c * 8, there);
-          cp_async_16_zfill(vdst + u, vb + pp * p.v_sp + rr * p.v_sr + c * 8, there);
+      for (int j = 0; j < R; ++j) {
+        const bool there = page[j] >= 0;
+        const char *ks = kb, *vs = vb;
+        if (there) {
+          ks += (int64_t)page[j] * p.k_sp + (int64_t)row[j] * p.k_sr;
+          vs += (int64_t)page[j] * p.v_sp + (int64_t)row[j] * p.v_sr;
+        }
+#pragma unroll
+        for (int i = 0; i < CI; ++i) {
+          if (p.hd == HD || (pch + LPR * i) * 8 < p.hd) {
+            const uint32_t d = dst[i & 1] + so + j * RPI * ROWB + (i >> 1) * 128;
+            cp_async_16_zfill(d, ks + i * LPR * 16, there);
+            cp_async_16_zfill(d + KBYTES, vs + i * LPR * 16, there);
+          }
         }
       }
       const bool any_bad = __any_sync(0xffffffffu, bad_seen);
@@ -262,15 +301,20 @@ __global__ void __launch_bounds__(warps_of(HD) * 32, 1) paged_attention_kernel(c
 #pragma unroll
   for (int i = 0; i < ST - 1; ++i) { issue(i); look(); }
 
-  // ---- consumer
-  const int g = lane >> 2, t4 = lane & 3;
-  uint32_t qf[Q_IN_SMEM ? 1 : HD / 16][4];
-  float o[HD / 8][4];
-  float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+  // ---- consumer.  Fragments (g = lane / 4, t4 = lane % 4): scores^T and out^T hold rows g, g + 8 (tokens, values of the
+  // head) and columns 2 t4, 2 t4 + 1 (query heads).
+  const int g = lane >> 2, t4 = lane & 3, mi = lane >> 3, mr = lane & 7;
+  uint32_t kofs[NO], vofs[NO];
+#pragma unroll
+  for (int i = 0; i < NO; ++i) {
+    constexpr int mask = CH >= 8 ? 7 : CH - 1;
+    kofs[i] = ((mi & 1) * 8 + mr) * ROWB + (((2 * i + (mi >> 1)) ^ swizzle<CH>(mr)) & mask) * 16;
+    vofs[i] = KBYTES + ((mi >> 1) * 8 + mr) * ROWB + (((2 * i + (mi & 1)) ^ swizzle<CH>(mr)) & mask) * 16;
+  }
+  uint32_t qf[KS][NQ][2];
+  float o[KS][NQ][4], m[NQ][2], l[NQ][2];
   bool poison = false, fresh = true;
-  int first_tile = cur.t;
-  int rows_here = 0, head0 = 0;
-  int slot = 0;
+  int first_tile = cur.t, rows_here = 0, head0 = 0, slot = 0;
   while (left > 0) {
     if (fresh) {   // a new (request, head tile): its queries, empty statistics
       fresh = false;
@@ -279,177 +323,160 @@ __global__ void __launch_bounds__(warps_of(HD) * 32, 1) paged_attention_kernel(c
       head0 = kvh * p.group + qt * 16;
       rows_here = min(16, p.group - qt * 16);
       const T* qb = static_cast<const T*>(p.q) + (int64_t)cur.b * p.q_sb + (int64_t)head0 * p.q_sh;
-      if constexpr (Q_IN_SMEM) {
-        __syncwarp();
-        for (int u = lane; u < 16 * CH; u += 32) {
-          const int r = u / CH, c = u % CH;
-          uint4 v = make_uint4(0, 0, 0, 0);
-          if (r < rows_here && c * 8 < p.hd) v = __ldg(reinterpret_cast<const uint4*>(qb + r * p.q_sh + c * 8));
-          reinterpret_cast<uint4*>(q_smem)[unit_of<CH>(r, c)] = v;
-        }
-        __syncwarp();
-      } else {
 #pragma unroll
-        for (int ks = 0; ks < HD / 16; ++ks)
+      for (int n = 0; n < NQ; ++n) {
+        const int r = n * 8 + g;
+        const T* qr = qb + (int64_t)r * p.q_sh + t4 * 2;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int r = g + (i & 1) * 8, d = ks * 16 + (i >> 1) * 8 + t4 * 2;
-            qf[ks][i] = (r < rows_here && d < p.hd) ? __ldg(reinterpret_cast<const uint32_t*>(qb + r * p.q_sh + d)) : 0u;
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int d = ks * 16 + i * 8;
+            qf[ks][n][i] = (r < rows_here && d < p.hd) ? __ldg(reinterpret_cast<const uint32_t*>(qr + d)) : 0u;
           }
-      }
+        m[n][0] = m[n][1] = -INFINITY;
+        l[n][0] = l[n][1] = 0.f;
 #pragma unroll
-      for (int i = 0; i < HD / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-      m0 = m1 = -INFINITY;
-      l0 = l1 = 0.f;
+        for (int ks = 0; ks < KS; ++ks) o[ks][n][0] = o[ks][n][1] = o[ks][n][2] = o[ks][n][3] = 0.f;
+      }
       poison = false;
     }
     cp_async_wait<ST - 2>();
     __syncwarp();
     poison |= (bad_bits >> slot) & 1u;
-    const uint32_t kbase = ring_u + slot * STAGE, vbase = kbase + KBYTES;
+    const uint32_t base = ring_u + slot * STAGE;
 
-    // scores of 16 query rows against TT tokens
-    float s[NT][4];
+    // scores
+    float s[MT][NQ][4];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
-    const int mi = lane >> 3, mr = lane & 7;
-    if constexpr (HD == 16) {
+    for (int i = 0; i < MT; ++i)
 #pragma unroll
-      for (int n = 0; n < NT; n += 2) {
-        uint32_t kf[4];
-        ldsm_x4(kf, kbase + unit_of<CH>((n + (mi >> 1)) * 8 + mr, mi & 1) * 16);
-        mma16816<T>(s[n], qf[0][0], qf[0][1], qf[0][2], qf[0][3], kf[0], kf[1]);
-        mma16816<T>(s[n + 1], qf[0][0], qf[0][1], qf[0][2], qf[0][3], kf[2], kf[3]);
+      for (int n = 0; n < NQ; ++n) s[i][n][0] = s[i][n][1] = s[i][n][2] = s[i][n][3] = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        uint32_t a[4];
+        ldsm_x4(a, base + kofs[ks & (NO - 1)] + (ks / 4) * 128 + i * 16 * ROWB);
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) mma16816<T>(s[i][n], a[0], a[1], a[2], a[3], qf[ks][n][0], qf[ks][n][1]);
       }
-    } else {
-#pragma unroll
-      for (int ks = 0; ks < HD / 16; ks += 2) {
-        uint32_t qa[4], qb2[4];
-        if constexpr (Q_IN_SMEM) {
-          const uint32_t qs = smem_u32(q_smem);
-          ldsm_x4(qa, qs + unit_of<CH>((mi & 1) * 8 + mr, ks * 2 + (mi >> 1)) * 16);
-          ldsm_x4(qb2, qs + unit_of<CH>((mi & 1) * 8 + mr, ks * 2 + 2 + (mi >> 1)) * 16);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) { qa[i] = qf[ks][i]; qb2[i] = qf[ks + 1][i]; }
-        }
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          uint32_t kf[4];
-          ldsm_x4(kf, kbase + unit_of<CH>(n * 8 + mr, ks * 2 + mi) * 16);
-          mma16816<T>(s[n], qa[0], qa[1], qa[2], qa[3], kf[0], kf[1]);
-          mma16816<T>(s[n], qb2[0], qb2[1], qb2[2], qb2[3], kf[2], kf[3]);
-        }
-      }
-    }
 
     // running maximum and sum, in powers of two
-    const int tok0 = cur.t * TT + t4 * 2;
-    const bool ragged = cur.t * TT + TT > cur.len;
-    float mx0 = -INFINITY, mx1 = -INFINITY;
+    const int rows_in = cur.len - cur.t * TT;
+    // (the maximum is taken of the scaled scores: a negative scale turns their order)
+    float mx[NQ][2];
+    bool more = false;
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
+    for (int n = 0; n < NQ; ++n) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) s[n][i] *= p.scale_log2;
-      if (ragged) {
-        if (tok0 + n * 8 >= cur.len) s[n][0] = s[n][2] = -INFINITY;
-        if (tok0 + n * 8 + 1 >= cur.len) s[n][1] = s[n][3] = -INFINITY;
+      for (int e = 0; e < 2; ++e) {
+        float v = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+          if (rows_in < TT) {
+            s[i][n][e] = i * 16 + g >= rows_in ? -INFINITY : s[i][n][e] * p.scale_log2;
+            s[i][n][2 + e] = i * 16 + g + 8 >= rows_in ? -INFINITY : s[i][n][2 + e] * p.scale_log2;
+          } else {
+            s[i][n][e] *= p.scale_log2;
+            s[i][n][2 + e] *= p.scale_log2;
+          }
+          v = fmaxf(v, fmaxf(s[i][n][e], s[i][n][2 + e]));
+        }
+        v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
+        v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
+        v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
+        mx[n][e] = fmaxf(v, m[n][e]);
+        more |= mx[n][e] > m[n][e];
       }
-      mx0 = fmaxf(mx0, fmaxf(s[n][0], s[n][1]));
-      mx1 = fmaxf(mx1, fmaxf(s[n][2], s[n][3]));
     }
-    mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 1));
-    mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 2));
-    mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 1));
-    mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 2));
-    if (__any_sync(0xffffffffu, mx0 > m0 || mx1 > m1)) {
-      const float n0 = fmaxf(m0, mx0), n1 = fmaxf(m1, mx1);
-      const float f0 = m0 == n0 ? 1.f : ex2(m0 - n0), f1 = m1 == n1 ? 1.f : ex2(m1 - n1);
-      m0 = n0;
-      m1 = n1;
-      l0 *= f0;
-      l1 *= f1;
+    if (__any_sync(0xffffffffu, more)) {
 #pragma unroll
-      for (int i = 0; i < HD / 8; ++i) { o[i][0] *= f0; o[i][1] *= f0; o[i][2] *= f1; o[i][3] *= f1; }
-    }
-    const float b0 = m0 == -INFINITY ? 0.f : m0, b1 = m1 == -INFINITY ? 0.f : m1;   // every score -inf: weights 0
+      for (int n = 0; n < NQ; ++n) {
+        float f[2];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      s[n][0] = ex2(s[n][0] - b0);
-      s[n][1] = ex2(s[n][1] - b0);
-      s[n][2] = ex2(s[n][2] - b1);
-      s[n][3] = ex2(s[n][3] - b1);
-      l0 += s[n][0] + s[n][1];
-      l1 += s[n][2] + s[n][3];
+        for (int e = 0; e < 2; ++e) {
+          f[e] = m[n][e] == mx[n][e] ? 1.f : ex2(m[n][e] - mx[n][e]);
+          m[n][e] = mx[n][e];
+          l[n][e] *= f[e];
+        }
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) { o[ks][n][0] *= f[0]; o[ks][n][1] *= f[1]; o[ks][n][2] *= f[0]; o[ks][n][3] *= f[1]; }
+      }
     }
-
     // output += weights * V; the weights go in as two summands so that their rounding stays below the output's
 #pragma unroll
-    for (int j = 0; j < TT / 16; ++j) {
-      uint32_t hi[4], lo[4];
-      split2<T>(s[2 * j][0], s[2 * j][1], hi[0], lo[0]);
-      split2<T>(s[2 * j][2], s[2 * j][3], hi[1], lo[1]);
-      split2<T>(s[2 * j + 1][0], s[2 * j + 1][1], hi[2], lo[2]);
-      split2<T>(s[2 * j + 1][2], s[2 * j + 1][3], hi[3], lo[3]);
+    for (int i = 0; i < MT; ++i) {
+      uint32_t hi[NQ][2], lo[NQ][2];
 #pragma unroll
-      for (int c = 0; c < CH; c += 2) {
-        uint32_t vf[4];
-        ldsm_x4_trans(vf, vbase + unit_of<CH>(j * 16 + (mi & 1) * 8 + mr, c + (mi >> 1)) * 16);
-        mma16816<T>(o[c], hi[0], hi[1], hi[2], hi[3], vf[0], vf[1]);
-        mma16816<T>(o[c + 1], hi[0], hi[1], hi[2], hi[3], vf[2], vf[3]);
-        mma16816<T>(o[c], lo[0], lo[1], lo[2], lo[3], vf[0], vf[1]);
-        mma16816<T>(o[c + 1], lo[0], lo[1], lo[2], lo[3], vf[2], vf[3]);
+      for (int n = 0; n < NQ; ++n) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float b = m[n][e] == -INFINITY ? 0.f : m[n][e];   // every score -inf so far: weights 0
+          s[i][n][e] = ex2(s[i][n][e] - b);
+          s[i][n][2 + e] = ex2(s[i][n][2 + e] - b);
+          l[n][e] += s[i][n][e] + s[i][n][2 + e];
+        }
+        split2<T>(s[i][n][0], s[i][n][1], hi[n][0], lo[n][0]);
+        split2<T>(s[i][n][2], s[i][n][3], hi[n][1], lo[n][1]);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          hi[n][e] = movmatrix_trans(hi[n][e]);
+          lo[n][e] = movmatrix_trans(lo[n][e]);
+        }
+      }
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        uint32_t a[4];
+        ldsm_x4_trans(a, base + vofs[ks & (NO - 1)] + (ks / 4) * 128 + i * 16 * ROWB);
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) {
+          mma16816<T>(o[ks][n], a[0], a[1], a[2], a[3], hi[n][0], hi[n][1]);
+          mma16816<T>(o[ks][n], a[0], a[1], a[2], a[3], lo[n][0], lo[n][1]);
+        }
       }
     }
     __syncwarp();                       // every lane has read the slot before it is filled again
-    const int refill = slot == 0 ? ST - 1 : slot - 1;
-    issue(refill);
+    issue(slot == 0 ? ST - 1 : slot - 1);
     look();
     slot = slot + 1 == ST ? 0 : slot + 1;
     --left;
 
     if (cur.t + 1 == cur.n || left == 0) {   // the pair's end, or the share's
-      l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
-      l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
-      l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
-      l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
-      if (poison) l0 = l1 = __int_as_float(0x7fc00000);
       const bool whole = first_tile == 0 && cur.t + 1 == cur.n;
-      if (whole) {
-        const float i0 = 1.f / l0, i1 = 1.f / l1;
-        T* ob = static_cast<T*>(p.out) + ((int64_t)cur.b * p.Hq + head0) * p.hd;
+      // slot 0 of the share: the pair that its first tile belongs to; slot 1: the pair that begins inside and goes on
+      const int ps = (cur.t - first_tile + 1 == (int)(end - begin) - left) ? 0 : 1;
+      float* po = p.part_o + ((int64_t)w * 2 + ps) * p.rows * p.hd;
+      float* pm = p.part_ml + ((int64_t)w * 2 + ps) * p.rows * 2;
+      T* ob = static_cast<T*>(p.out) + ((int64_t)cur.b * p.Hq + head0) * p.hd;
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const int r = g + half * 8;
+      for (int n = 0; n < NQ; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float sum = l[n][e];
+          sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+          sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+          sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+          if (poison) sum = __int_as_float(0x7fc00000);
+          const int r = n * 8 + t4 * 2 + e;
           if (r < rows_here) {
-            const float inv = half ? i1 : i0;
+            const float inv = 1.f / sum;
 #pragma unroll
-            for (int c = 0; c < CH; ++c) {
-              if (c * 8 < p.hd) {
-                T two[2] = {Cvt<T>::from_f(o[c][half * 2] * inv), Cvt<T>::from_f(o[c][half * 2 + 1] * inv)};
-                *reinterpret_cast<uint32_t*>(ob + (int64_t)r * p.hd + c * 8 + t4 * 2) = *reinterpret_cast<uint32_t*>(two);
+            for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                const int d = ks * 16 + i * 8 + g;
+                if (d < p.hd) {
+                  if (whole) ob[r * p.hd + d] = Cvt<T>::from_f(o[ks][n][i * 2 + e] * inv);
+                  else po[r * p.hd + d] = o[ks][n][i * 2 + e];
+                }
               }
+            if (g == 0) {
+              if (!whole) *reinterpret_cast<float2*>(pm + r * 2) = make_float2(m[n][e], sum);
+              else if (p.lse) p.lse[(int64_t)cur.b * p.Hq + head0 + r] = (m[n][e] + log2f(sum)) * kLn2;
             }
-            if (p.lse && t4 == 0) p.lse[(int64_t)cur.b * p.Hq + head0 + r] = ((half ? m1 : m0) + log2f(half ? l1 : l0)) * kLn2;
           }
         }
-      } else {
-        // slot 0 of the share: the pair that its first tile belongs to; slot 1: the pair that begins inside and goes on
-        const int ps = (cur.t - first_tile + 1 == (int)(end - begin) - left) ? 0 : 1;
-        float* po = p.part_o + ((int64_t)w * 2 + ps) * p.rows * p.hd;
-        float* pm = p.part_ml + ((int64_t)w * 2 + ps) * p.rows * 2;
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const int r = g + half * 8;
-          if (r < rows_here) {
-#pragma unroll
-            for (int c = 0; c < CH; ++c)
-              if (c * 8 < p.hd)
-                *reinterpret_cast<float2*>(po + r * p.hd + c * 8 + t4 * 2) = make_float2(o[c][half * 2], o[c][half * 2 + 1]);
-            if (t4 == 0) *reinterpret_cast<float2*>(pm + r * 2) = make_float2(half ? m1 : m0, half ? l1 : l0);
-          }
-        }
-      }
       fresh = true;
     }
     if (left > 0) advance(cur);
@@ -531,24 +558,29 @@ size_t workspace_for(int B, int Hq, int Hkv, int hd, int sms) {
   return round256(slots * rows * hd * 4) + round256(slots * rows * 8) + round256(((size_t)B + 1) * 4);
 }
 
-template <typename T, int HD>
+template <typename T, int HD, int NQ>
 int launch(const PagedParams& p, int sms, cudaStream_t st) {
   constexpr int NW = warps_of(HD);
-  const size_t smem = (size_t)NW * (kStages * 2 * tile_tokens(HD) * HD * 2 + (HD >= 256 ? 16 * HD * 2 : 0)) + (size_t)(2 * p.B + 1) * 4;
-  HB_PROPAGATE(ensure_dynamic_smem((const void*)paged_attention_kernel<T, HD>, smem));
-  HB_PROPAGATE(launch_chained(paged_attention_kernel<T, HD>, dim3((unsigned)sms), dim3(NW * 32), smem, st, false, 1, p));
+  const size_t smem = (size_t)NW * stages_of(HD) * 2 * tile_tokens(HD) * HD * 2 + (size_t)(2 * p.B + 1) * 4;
+  HB_PROPAGATE(ensure_dynamic_smem((const void*)paged_attention_kernel<T, HD, NQ>, smem));
+  HB_PROPAGATE(launch_chained(paged_attention_kernel<T, HD, NQ>, dim3((unsigned)sms), dim3(NW * 32), smem, st, false, 1, p));
   return launch_chained(paged_join_kernel<T>, dim3((unsigned)(p.B * p.Hq)), dim3(128), (size_t)p.workers * 4, st, true, 1, p);
 }
 
-template <typename T>
+template <typename T, int NQ>
 int launch_hd(const PagedParams& p, int sms, cudaStream_t st) {
   switch (padded_hd(p.hd)) {
-    case 16: return launch<T, 16>(p, sms, st);
-    case 32: return launch<T, 32>(p, sms, st);
-    case 64: return launch<T, 64>(p, sms, st);
-    case 128: return launch<T, 128>(p, sms, st);
-    default: return launch<T, 256>(p, sms, st);
+    case 16: return launch<T, 16, NQ>(p, sms, st);
+    case 32: return launch<T, 32, NQ>(p, sms, st);
+    case 64: return launch<T, 64, NQ>(p, sms, st);
+    case 128: return launch<T, 128, NQ>(p, sms, st);
+    default: return launch<T, 256, NQ>(p, sms, st);
   }
+}
+
+template <typename T>
+int launch_group(const PagedParams& p, int sms, cudaStream_t st) {
+  return p.group <= 8 ? launch_hd<T, 1>(p, sms, st) : launch_hd<T, 2>(p, sms, st);
 }
 
 int check_heads(const char* what, int64_t B, int Hq, int Hkv, int hd) {
@@ -602,8 +634,11 @@ extern "C" int hb200_paged_decode_attention(const hb200_paged_cache* c, const vo
   PagedParams p = {};
   p.q = q; p.kc = c->k; p.vc = c->v; p.out = out; p.lse = lse; p.table = block_tables; p.lens = kv_lens;
   p.q_sb = q_stride_b; p.q_sh = q_stride_h;
-  p.k_sp = c->k_stride_page; p.k_sh = c->k_stride_head; p.k_sr = c->k_stride_row;
-  p.v_sp = c->v_stride_page; p.v_sh = c->v_stride_head; p.v_sr = c->v_stride_row;
+  p.k_sh = c->k_stride_head; p.v_sh = c->v_stride_head;
+  const int64_t in_bytes[] = {c->k_stride_page * 2, c->k_stride_row * 2, c->v_stride_page * 2, c->v_stride_row * 2};
+  for (int64_t x : in_bytes)
+    HB_REQUIRE(x >= -0x7fffffffll && x <= 0x7fffffffll, HB200_ERR_UNSUPPORTED, "paged_decode_attention: pages or rows more than 2 GB apart");
+  p.k_sp = (int32_t)in_bytes[0]; p.k_sr = (int32_t)in_bytes[1]; p.v_sp = (int32_t)in_bytes[2]; p.v_sr = (int32_t)in_bytes[3];
   p.table_ld = table_ld;
   p.B = B; p.Hq = Hq; p.Hkv = c->n_kv_heads; p.hd = c->head_dim; p.group = group;
   p.q_tiles = (group + 15) / 16;
@@ -619,8 +654,8 @@ extern "C" int hb200_paged_decode_attention(const hb200_paged_cache* c, const vo
   ws += round256(slots * p.rows * 8);
   p.cum = reinterpret_cast<int32_t*>(ws);
   cudaStream_t st = (cudaStream_t)stream;
-  if (c->dtype == HB200_BF16) return launch_hd<__nv_bfloat16>(p, sms, st);
-  if (c->dtype == HB200_F16) return launch_hd<__half>(p, sms, st);
+  if (c->dtype == HB200_BF16) return launch_group<__nv_bfloat16>(p, sms, st);
+  if (c->dtype == HB200_F16) return launch_group<__half>(p, sms, st);
   set_error("paged_decode_attention: unsupported dtype %d (bf16 and f16 are built)", c->dtype);
   return HB200_ERR_UNSUPPORTED;
 }
