@@ -7,16 +7,15 @@
 // Bound: HBM (each head row read once, written once; 32 bits from the load to the one rounding at the store).  A group of
 // lanes holds one head row, 8 values per lane through 16-byte accesses (or value by value where sizes, strides or
 // pointers are no multiples of 16 bytes).  A lane keeps the same place in the row for all heads of its token, so the
-// token's cosines and sines and the two weight vectors are loaded once into registers.  Four rows are in flight per
-// group.  The half layout fetches the partner value through shared memory (padded by one word in eight: no bank
-// conflicts), which works for every rot.
+// token's cosines and sines are loaded once into registers; the weights sit in shared memory.  Four head rows per group are
+// in flight while four are computed.  The half layout fetches the partner value from its lane where rot / 2 is a multiple of
+// 8 values, else through shared memory (padded by one word in eight: no bank conflicts), which works for every rot.
 #include "common.cuh"
 
 namespace hb200 {
 namespace {
 
 constexpr int kThreads = 128;
-constexpr int kUnroll = 4;
 
 struct RopeParams {
   const void *q, *k, *v;
@@ -33,205 +32,257 @@ struct RopeParams {
   int norm;
 };
 
+// Eight values of a row as they come from memory.
 template <typename T, bool VEC>
-__device__ __forceinline__ void load8(const T* p, int n, float (&f)[8]) {
-  if constexpr (VEC) {
-    constexpr int V = 16 / sizeof(T);
+struct Raw {
+  uint4 v[sizeof(T) / 2];
+  __device__ __forceinline__ void load(const T* p, int) {
 #pragma unroll
-    for (int j = 0; j < 8; j += V) {
-      const uint4 raw = __ldg(reinterpret_cast<const uint4*>(p + j));
-      const T* e = reinterpret_cast<const T*>(&raw);
-#pragma unroll
-      for (int i = 0; i < V; ++i) f[j + i] = Cvt<T>::to_f(e[i]);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = i < n ? Cvt<T>::to_f(p[i]) : 0.f;
+    for (int j = 0; j < (int)sizeof(T) / 2; ++j) v[j] = __ldg(reinterpret_cast<const uint4*>(p) + j);
   }
-}
-template <typename T, bool VEC>
-__device__ __forceinline__ void store8(T* p, int n, const float (&f)[8]) {
-  if constexpr (VEC) {
-    constexpr int V = 16 / sizeof(T);
+  __device__ __forceinline__ void clear() {
 #pragma unroll
-    for (int j = 0; j < 8; j += V) {
-      uint4 raw;
-      T* e = reinterpret_cast<T*>(&raw);
+    for (int j = 0; j < (int)sizeof(T) / 2; ++j) v[j] = make_uint4(0, 0, 0, 0);
+  }
+  __device__ __forceinline__ void get(float (&f)[8]) const {
+    const T* e = reinterpret_cast<const T*>(v);
 #pragma unroll
-      for (int i = 0; i < V; ++i) e[i] = Cvt<T>::from_f(f[j + i]);
-      *reinterpret_cast<uint4*>(p + j) = raw;
-    }
-  } else {
+    for (int i = 0; i < 8; ++i) f[i] = Cvt<T>::to_f(e[i]);
+  }
+  __device__ __forceinline__ void copy(T* p, int) const {
+#pragma unroll
+    for (int j = 0; j < (int)sizeof(T) / 2; ++j) reinterpret_cast<uint4*>(p)[j] = v[j];
+  }
+};
+template <typename T>
+struct Raw<T, false> {
+  T v[8];
+  __device__ __forceinline__ void load(const T* p, int n) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = i < n ? p[i] : Cvt<T>::from_f(0.f);
+  }
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = Cvt<T>::from_f(0.f);
+  }
+  __device__ __forceinline__ void get(float (&f)[8]) const {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = Cvt<T>::to_f(v[i]);
+  }
+  __device__ __forceinline__ void copy(T* p, int n) const {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      if (i < n) p[i] = Cvt<T>::from_f(f[i]);
+      if (i < n) p[i] = v[i];
   }
+};
+template <typename T, bool VEC>
+__device__ __forceinline__ void store8(T* p, int n, const float (&f)[8]) {
+  Raw<T, VEC> r;
+  T* e = reinterpret_cast<T*>(r.v);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) e[i] = Cvt<T>::from_f(f[i]);
+  r.copy(p, n);
 }
 
+// VEC: rows by 16-byte accesses.  TAB: tables by 16-byte loads, a lane's values all turned or all kept, partners in one lane.
 // HALF: pairs (i, i + rot/2); else (2i, 2i + 1).  CACHE: k and v rows go to their slots, else k rows to k_out.
-template <typename T, bool VEC, bool HALF, bool CACHE>
+template <typename T, bool VEC, bool TAB, bool HALF, bool CACHE>
 __global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(const RopeParams p) {
+  constexpr int U = sizeof(T) == 4 ? 2 : 4;                // rows in flight per group, and as many in computation
+  constexpr int NC = HALF || !TAB ? 8 : 4;                 // cosines per lane
   extern __shared__ float s_rows[];
+  __shared__ __align__(16) float s_w[2][256];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int LG = p.group_lanes, groups = 32 / LG;          // lanes per head row (a power of two), rows per warp
   const int gl = lane & (LG - 1), grp = lane / LG;
-  const int64_t item = (int64_t)blockIdx.x * (kThreads / 32) + warp;
-  const int64_t tok = item / p.parts;
-  const int part = (int)(item - tok * p.parts);            // which share of the token's heads
-  if (tok >= p.tokens) return;
-  const int64_t b = tok / p.S, s = tok - b * p.S;
   const int e0 = gl * 8;                                    // first value of this lane
   const int mine = p.hd - e0 < 8 ? (p.hd - e0 > 0 ? p.hd - e0 : 0) : 8;
   const int half = p.rot >> 1;
   float* row = s_rows + (warp * groups + grp) * (LG * 9);
-
-  int64_t pos = s;
-  if (p.positions)
-    pos = p.pos64 ? static_cast<const int64_t*>(p.positions)[b * p.pos_sb + s]
-                  : (int64_t)static_cast<const int32_t*>(p.positions)[b * p.pos_sb + s];
-  int64_t slot = -1;
-  if constexpr (CACHE) slot = p.slots[tok];
-  const bool pad = pos < 0;                                // a row of padding: zeros out, nothing into the cache
-  bool wrong = pos >= p.table_rows;                        // no angle for it: NaN, not a silent clamp
-  if constexpr (CACHE) wrong |= slot >= p.capacity;
-  const int64_t tr = pad || pos >= p.table_rows ? 0 : pos;
-
-  // cosine and (signed) sine of each value
-  float c[8], n[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) { c[i] = 1.f; n[i] = 0.f; }
-  const float* ct = p.cos_t + tr * p.table_ld;
-  const float* st = p.sin_t + tr * p.table_ld;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int e = e0 + i;
-    if (e < p.rot) {
-      const int at = HALF ? (e < half ? e : e - half) : e >> 1;
-      const bool first = HALF ? e < half : (e & 1) == 0;
-      c[i] = __ldg(ct + at);
-      n[i] = first ? -__ldg(st + at) : __ldg(st + at);
-    }
-  }
-  float wq[8], wk[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    wq[i] = p.q_scale * (p.wq && i < mine ? __ldg(p.wq + e0 + i) : 1.f);
-    wk[i] = p.k_scale * (p.wk && i < mine ? __ldg(p.wk + e0 + i) : 1.f);
-  }
-
   const int rows = p.Hq + p.Hkv + (CACHE ? p.Hkv : 0);
-  const T* qb = static_cast<const T*>(p.q) + b * p.q_s[0] + s * p.q_s[1] + e0;
-  const T* kb = static_cast<const T*>(p.k) + b * p.k_s[0] + s * p.k_s[1] + e0;
-  const T* vb = CACHE ? static_cast<const T*>(p.v) + b * p.v_s[0] + s * p.v_s[1] + e0 : nullptr;
-  T* qo = static_cast<T*>(p.q_out) + b * p.qo_s[0] + s * p.qo_s[1] + e0;
-  T *ko = nullptr, *vo = nullptr;
-  int64_t ko_h, vo_h = 0;
-  const bool into_cache = CACHE && !pad && slot >= 0 && slot < p.capacity;
-  if constexpr (CACHE) {
-    const int64_t page = into_cache ? slot / p.page_size : 0, off = into_cache ? slot - page * p.page_size : 0;
-    ko = static_cast<T*>(p.kc) + page * p.kc_s[0] + off * p.kc_s[2] + e0;
-    vo = static_cast<T*>(p.vc) + page * p.vc_s[0] + off * p.vc_s[2] + e0;
-    ko_h = p.kc_s[1];
-    vo_h = p.vc_s[1];
-  } else {
-    ko = static_cast<T*>(p.k_out) + b * p.ko_s[0] + s * p.ko_s[1] + e0;
-    ko_h = p.ko_s[2];
-  }
   const int step = groups * p.parts;
-  for (int r0 = part * groups; r0 < rows; r0 += step * kUnroll) {   // uniform over the warp
-    float x[kUnroll][8];
+  for (int i = threadIdx.x; i < 256; i += kThreads) {
+    s_w[0][i] = p.q_scale * (p.wq && i < p.hd ? __ldg(p.wq + i) : 1.f);
+    s_w[1][i] = p.k_scale * (p.wk && i < p.hd ? __ldg(p.wk + i) : 1.f);
+  }
+  __syncthreads();
+
+  const int64_t items = p.tokens * p.parts, stride = (int64_t)gridDim.x * (kThreads / 32);
+  for (int64_t item = (int64_t)blockIdx.x * (kThreads / 32) + warp; item < items; item += stride) {
+    const int64_t tok = p.parts == 1 ? item : item / p.parts;
+    const int part = (int)(item - tok * p.parts);          // which share of the token's heads
+    const int64_t b = tok < p.S ? 0 : tok / p.S, s = tok - b * p.S;
+    const T* qb = static_cast<const T*>(p.q) + b * p.q_s[0] + s * p.q_s[1] + e0;
+    const T* kb = static_cast<const T*>(p.k) + b * p.k_s[0] + s * p.k_s[1] + e0;
+    const T* vb = CACHE ? static_cast<const T*>(p.v) + b * p.v_s[0] + s * p.v_s[1] + e0 : nullptr;
+    Raw<T, VEC> raw[U], next[U];
+    auto fetch = [&](Raw<T, VEC> (&x)[U], int r0) {
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      const int r = r0 + u * step + grp;
-      const T* src = r < p.Hq ? qb + (int64_t)r * p.q_s[2]
-                              : (r < p.Hq + p.Hkv ? kb + (int64_t)(r - p.Hq) * p.k_s[2]
-                                                  : (CACHE ? vb + (int64_t)(r - p.Hq - p.Hkv) * p.v_s[2] : nullptr));
-      if (r < rows && mine > 0) {
-        load8<T, VEC>(src, mine, x[u]);
-      } else {
+      for (int u = 0; u < U; ++u) {
+        const int r = r0 + u * step + grp;
+        const T* src = r < p.Hq ? qb + (int64_t)r * p.q_s[2]
+                                : (!CACHE || r < p.Hq + p.Hkv ? kb + (int64_t)(r - p.Hq) * p.k_s[2] : vb + (int64_t)(r - p.Hq - p.Hkv) * p.v_s[2]);
+        if (r < rows && mine > 0) x[u].load(src, mine);
+        else x[u].clear();
+      }
+    };
+    fetch(raw, part * groups);
+
+    int64_t pos = s;
+    if (p.positions)
+      pos = p.pos64 ? __ldg(static_cast<const long long*>(p.positions) + b * p.pos_sb + s)
+                    : (int64_t)__ldg(static_cast<const int32_t*>(p.positions) + b * p.pos_sb + s);
+    int64_t slot = -1;
+    if constexpr (CACHE) slot = __ldg(reinterpret_cast<const long long*>(p.slots) + tok);
+    const bool pad = pos < 0;                              // a row of padding: zeros out, nothing into the cache
+    bool wrong = pos >= p.table_rows;                      // no angle for it: NaN, not a silent clamp
+    if constexpr (CACHE) wrong |= slot >= p.capacity;
+    const int64_t tr = pad || pos >= p.table_rows ? 0 : pos;
+
+    // cosines and (signed) sines of the lane's values
+    float c[NC], n[NC];
+    const float* ct = p.cos_t + tr * p.table_ld;
+    const float* st = p.sin_t + tr * p.table_ld;
+    const bool turn = e0 < p.rot;                          // TAB: of all the lane's values
+    if constexpr (TAB) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[u][i] = 0.f;
+      for (int i = 0; i < NC; ++i) c[i] = n[i] = 0.f;
+      if (turn) {
+        const int at = HALF ? (e0 < half ? e0 : e0 - half) : e0 >> 1;
+        const float sign = HALF && e0 < half ? -1.f : 1.f;
+#pragma unroll
+        for (int i = 0; i < NC; i += 4) {
+          const float4 a = __ldg(reinterpret_cast<const float4*>(ct + at + i)), d = __ldg(reinterpret_cast<const float4*>(st + at + i));
+          c[i] = a.x; c[i + 1] = a.y; c[i + 2] = a.z; c[i + 3] = a.w;
+          n[i] = sign * d.x; n[i + 1] = sign * d.y; n[i + 2] = sign * d.z; n[i + 3] = sign * d.w;
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int e = e0 + i;
+        c[i] = 1.f;
+        n[i] = 0.f;
+        if (e < p.rot) {
+          const int at = HALF ? (e < half ? e : e - half) : e >> 1;
+          const bool first = HALF ? e < half : (e & 1) == 0;
+          c[i] = __ldg(ct + at);
+          n[i] = first ? -__ldg(st + at) : __ldg(st + at);
+        }
       }
     }
+
+    T* qo = static_cast<T*>(p.q_out) + b * p.qo_s[0] + s * p.qo_s[1] + e0;
+    T *ko = nullptr, *vo = nullptr;
+    int64_t ko_h, vo_h = 0;
+    const bool into_cache = CACHE && !pad && slot >= 0 && slot < p.capacity;
+    if constexpr (CACHE) {
+      const int64_t page = into_cache ? slot / p.page_size : 0, off = into_cache ? slot - page * p.page_size : 0;
+      ko = static_cast<T*>(p.kc) + page * p.kc_s[0] + off * p.kc_s[2] + e0;
+      vo = static_cast<T*>(p.vc) + page * p.vc_s[0] + off * p.vc_s[2] + e0;
+      ko_h = p.kc_s[1];
+      vo_h = p.vc_s[1];
+    } else {
+      ko = static_cast<T*>(p.k_out) + b * p.ko_s[0] + s * p.ko_s[1] + e0;
+      ko_h = p.ko_s[2];
+    }
+
+    for (int r0 = part * groups; r0 < rows; r0 += step * U) {   // uniform over the warp
+      if (r0 + step * U < rows) fetch(next, r0 + step * U);
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      if (r0 + u * step >= rows) break;                    // uniform over the warp
-      const int r = r0 + u * step + grp;
-      const bool is_q = r < p.Hq, is_v = r >= p.Hq + p.Hkv;
-      float y[8];
-      float inv = 1.f;
-      if (p.norm) {
-        float ss = 0.f;
+      for (int u = 0; u < U; ++u) {
+        if (r0 + u * step >= rows) break;                  // uniform over the warp
+        const int r = r0 + u * step + grp;
+        const bool is_q = r < p.Hq, is_v = CACHE && r >= p.Hq + p.Hkv;
+        float y[8], z[8];
+        raw[u].get(y);
+        float inv = 1.f;
+        if (p.norm) {
+          float ss = 0.f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) ss = fmaf(x[u][i], x[u][i], ss);
-        for (int o = LG >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        inv = rsqrtf(ss * p.norm_c + p.eps);
-      }
-      if (wrong) inv = __int_as_float(0x7fc00000);
+          for (int i = 0; i < 8; ++i) ss = fmaf(y[i], y[i], ss);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] = x[u][i] * inv * (is_q ? wq[i] : wk[i]);
-      float z[8];
-      if constexpr (HALF) {
-        if (u > 0 || r0 > part * groups) __syncwarp();     // the row before this one has been read
-#pragma unroll
-        for (int i = 0; i < 8; ++i) row[gl * 9 + i] = y[i];
-        __syncwarp();
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int e = e0 + i;
-          const int other = e < half ? e + half : e - half;
-          z[i] = e < p.rot ? fmaf(y[i], c[i], row[(other >> 3) * 9 + (other & 7)] * n[i]) : y[i];
+          for (int o = 16; o > 0; o >>= 1)
+            if (o < LG) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+          inv = rsqrtf(ss * p.norm_c + p.eps);
         }
-      } else {
+        if (wrong) inv = __int_as_float(0x7fc00000);
+        const float4* w4 = reinterpret_cast<const float4*>(s_w[is_q ? 0 : 1] + e0);
+        const float4 wa = w4[0], wb = w4[1];
+        const float w[8] = {wa.x, wa.y, wa.z, wa.w, wb.x, wb.y, wb.z, wb.w};
 #pragma unroll
-        for (int i = 0; i < 8; i += 2) {
-          const bool in = e0 + i < p.rot;                  // rot is even: a pair is turned or kept as a whole
-          z[i] = in ? fmaf(y[i], c[i], y[i + 1] * n[i]) : y[i];
-          z[i + 1] = in ? fmaf(y[i + 1], c[i + 1], y[i] * n[i + 1]) : y[i + 1];
-        }
-      }
-      if (r < rows && mine > 0) {
-        if (is_q) {
-          if (pad) {
+        for (int i = 0; i < 8; ++i) y[i] *= inv * w[i];
+        if constexpr (HALF && TAB) {
+          const int away = half >> 3;                      // lanes between partners
+          const int partner = turn ? (e0 < half ? lane + away : lane - away) : lane;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) z[i] = 0.f;
+          for (int i = 0; i < 8; ++i) {
+            const float other = __shfl_sync(0xffffffffu, y[i], partner);
+            z[i] = turn ? fmaf(y[i], c[i], other * n[i]) : y[i];
           }
-          store8<T, VEC>(qo + (int64_t)r * p.qo_s[2], mine, z);
-        } else if (CACHE) {
-          if (into_cache) {
-            if (is_v) store8<T, VEC>(vo + (int64_t)(r - p.Hq - p.Hkv) * vo_h, mine, x[u]);
-            else store8<T, VEC>(ko + (int64_t)(r - p.Hq) * ko_h, mine, z);
+        } else if constexpr (HALF) {
+          __syncwarp();                                    // the row before this one has been read
+#pragma unroll
+          for (int i = 0; i < 8; ++i) row[gl * 9 + i] = y[i];
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int e = e0 + i;
+            const int other = e < half ? e + half : e - half;
+            z[i] = e < p.rot ? fmaf(y[i], c[i], row[(other >> 3) * 9 + (other & 7)] * n[i]) : y[i];
           }
         } else {
+#pragma unroll
+          for (int i = 0; i < 8; i += 2) {
+            const float cc = TAB ? c[i / 2] : c[i], first = TAB ? -n[i / 2] : n[i], second = TAB ? n[i / 2] : n[i + 1];
+            const bool in = TAB ? turn : e0 + i < p.rot;   // rot is even: a pair is turned or kept as a whole
+            z[i] = in ? fmaf(y[i], cc, y[i + 1] * first) : y[i];
+            z[i + 1] = in ? fmaf(y[i + 1], cc, y[i] * second) : y[i + 1];
+          }
+        }
+        if (r < rows && mine > 0) {
           if (pad) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) z[i] = 0.f;
           }
-          store8<T, VEC>(ko + (int64_t)(r - p.Hq) * ko_h, mine, z);
+          if (is_q) {
+            store8<T, VEC>(qo + (int64_t)r * p.qo_s[2], mine, z);
+          } else if (!CACHE) {
+            store8<T, VEC>(ko + (int64_t)(r - p.Hq) * ko_h, mine, z);
+          } else if (into_cache) {
+            if (is_v) raw[u].copy(vo + (int64_t)(r - p.Hq - p.Hkv) * vo_h, mine);
+            else store8<T, VEC>(ko + (int64_t)(r - p.Hq) * ko_h, mine, z);
+          }
         }
       }
+#pragma unroll
+      for (int u = 0; u < U; ++u) raw[u] = next[u];
     }
   }
 }
 
-template <typename T>
-int launch(const RopeParams& p, bool vec, bool half, bool cache, cudaStream_t st) {
-  const int64_t items = p.tokens * p.parts;
-  const dim3 grid((unsigned)ceil_div64(items, kThreads / 32));
-  const size_t smem = half ? (size_t)kThreads * 9 * 4 : 0;
-#define HB_CASE(V, H, C) \
-  if (vec == V && half == H && cache == C) qk_norm_rope_kernel<T, V, H, C><<<grid, kThreads, smem, st>>>(p)
-  HB_CASE(true, true, true);
-  HB_CASE(true, true, false);
-  HB_CASE(true, false, true);
-  HB_CASE(true, false, false);
-  HB_CASE(false, true, true);
-  HB_CASE(false, true, false);
-  HB_CASE(false, false, true);
-  HB_CASE(false, false, false);
-#undef HB_CASE
+template <typename T, bool VEC, bool TAB, bool HALF, bool CACHE>
+int launch_as(const RopeParams& p, cudaStream_t st) {
+  int dev = 0, sms = 0;
+  HB_CUDA(cudaGetDevice(&dev));
+  HB_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+  int64_t grid = ceil_div64(p.tokens * p.parts, kThreads / 32);
+  if (grid > (int64_t)sms * 16) grid = (int64_t)sms * 16;
+  qk_norm_rope_kernel<T, VEC, TAB, HALF, CACHE><<<(unsigned)grid, kThreads, HALF && !TAB ? kThreads * 9 * 4 : 0, st>>>(p);
   HB_LAUNCH_CHECK();
   return 0;
+}
+
+template <typename T, bool HALF, bool CACHE>
+int launch_mode(const RopeParams& p, bool vec, bool tab, cudaStream_t st) {
+  if (!vec) return launch_as<T, false, false, HALF, CACHE>(p, st);
+  return tab ? launch_as<T, true, true, HALF, CACHE>(p, st) : launch_as<T, true, false, HALF, CACHE>(p, st);
+}
+
+template <typename T>
+int launch(const RopeParams& p, bool vec, bool tab, bool half, bool cache, cudaStream_t st) {
+  if (half) return cache ? launch_mode<T, true, true>(p, vec, tab, st) : launch_mode<T, true, false>(p, vec, tab, st);
+  return cache ? launch_mode<T, false, true>(p, vec, tab, st) : launch_mode<T, false, false>(p, vec, tab, st);
 }
 
 }  // namespace
@@ -297,12 +348,12 @@ extern "C" int hb200_qk_norm_rope(const hb200_qk_norm_rope_args* a, const hb200_
   const int rows = a->Hq + a->Hkv * (c ? 2 : 1), groups = 32 / p.group_lanes;
   p.parts = 1;
   while (tokens * p.parts < 148 * 16 && p.parts * groups < rows) p.parts <<= 1;
-  HB_REQUIRE(ceil_div64(tokens * p.parts, kThreads / 32) <= 0x7fffffff, HB200_ERR_UNSUPPORTED, "qk_norm_rope: too many tokens");
+  const bool tab = a->rot % (a->layout == HB200_ROPE_HALF ? 16 : 8) == 0 && a->table_ld % 4 == 0 && aligned16(a->cos) && aligned16(a->sin);
   cudaStream_t st = (cudaStream_t)stream;
   const bool half = a->layout == HB200_ROPE_HALF;
-  if (a->dtype == HB200_F32) return launch<float>(p, vec, half, c != nullptr, st);
-  if (a->dtype == HB200_BF16) return launch<__nv_bfloat16>(p, vec, half, c != nullptr, st);
-  if (a->dtype == HB200_F16) return launch<__half>(p, vec, half, c != nullptr, st);
+  if (a->dtype == HB200_F32) return launch<float>(p, vec, tab, half, c != nullptr, st);
+  if (a->dtype == HB200_BF16) return launch<__nv_bfloat16>(p, vec, tab, half, c != nullptr, st);
+  if (a->dtype == HB200_F16) return launch<__half>(p, vec, tab, half, c != nullptr, st);
   set_error("qk_norm_rope: unsupported dtype %d", a->dtype);
   return HB200_ERR_UNSUPPORTED;
 }
