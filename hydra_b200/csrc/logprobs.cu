@@ -27,7 +27,6 @@ constexpr int kCand = 512;       // candidate list of a CTA
 constexpr int kMaxTop = 32;
 constexpr int kGroups = 64;
 constexpr int kUnroll = 4;
-constexpr float kLowest = -3.402823466e38f;
 
 struct LogprobParams {
   const void* x;
@@ -63,47 +62,106 @@ __device__ __forceinline__ float key_value(uint32_t k) {
 __device__ __forceinline__ uint64_t entry(float v, int i) { return ((uint64_t)order_key(v) << 32) | (uint32_t)~i; }
 __device__ __forceinline__ int entry_index(uint64_t e) { return (int)~(uint32_t)e; }
 
-// Running statistics of the logits a thread (a row) has seen: maximum, sum 2^t and sum t 2^t, t = (x - max) c.
+// Running statistics of the logits a thread (a row) has seen: maximum m, and sum 2^t and sum t 2^t of t = (x - base) c, in
+// powers of two (c = log2(e) / T).  base is m kept finite: a thread may have seen nothing but -inf.  (x - base is formed before
+// the product: x c less a rounded m c would be off by 2^-24 of m c, whatever its size.)
 struct Stat {
   float m, s, u;
-  __device__ float base() const { return fmaxf(m, kLowest); }   // finite while only -inf was seen
 };
-__device__ __forceinline__ void rebase(Stat& a, float to, float c) {   // to >= a.base()
-  const float d = fmaxf((a.base() - to) * c, -200.f), f = ex2f(d);
+__device__ __forceinline__ float base_of(float m) { return fmaxf(m, -3.402823466e38f); }
+__device__ __forceinline__ void rebase(Stat& a, float m, float c) {   // m >= a.m
+  const float d = fmaxf((base_of(a.m) - base_of(m)) * c, -200.f), f = ex2f(d);
   a.u = f * fmaf(d, a.s, a.u);
   a.s *= f;
-}
-__device__ __forceinline__ Stat merge(Stat a, Stat b, float c) {
-  const float m = fmaxf(a.m, b.m), to = fmaxf(m, kLowest);
-  rebase(a, to, c);
-  rebase(b, to, c);
-  return {m, a.s + b.s, a.u + b.u};
+  a.m = m;
 }
 
-template <typename T, int N>
-__device__ __forceinline__ void take(Stat& a, const float (&f)[N], float c) {
-  float mx = f[0];
-#pragma unroll
-  for (int i = 1; i < N; ++i) mx = fmaxf(mx, f[i]);
-  if (mx > a.m) {
-    rebase(a, fmaxf(mx, kLowest), c);
-    a.m = mx;
-  }
-  const float base = a.base();
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    // -inf (and anything far below) counts as 2^-200 = 0 times a finite distance; NaN and +inf stay NaN
-    const float t = max_nan((f[i] - base) * c, -200.f), e = ex2f(t);
-    a.s += e;
-    a.u = fmaf(t, e, a.u);
-  }
+// Two 32-bit values in one operation.
+struct F2 {
+  uint64_t v;
+  __device__ F2() {}
+  __device__ F2(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b)); }
+  __device__ void get(float& a, float& b) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+};
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
 }
 
-template <typename T>
-__device__ __forceinline__ void unpack(const uint4& raw, float (&f)[16 / sizeof(T)]) {
-  const T* e = reinterpret_cast<const T*>(&raw);
+// One 16-byte piece.
+template <typename T> struct Piece;
+template <> struct Piece<float> {
+  float f[4];
+  __device__ explicit Piece(const uint4& r) {
+    f[0] = __uint_as_float(r.x); f[1] = __uint_as_float(r.y); f[2] = __uint_as_float(r.z); f[3] = __uint_as_float(r.w);
+  }
+  __device__ float max() const { return fmaxf(fmaxf(f[0], f[1]), fmaxf(f[2], f[3])); }
+};
+template <> struct Piece<__nv_bfloat16> {
+  float f[8];
+  __nv_bfloat162 top;
+  __device__ explicit Piece(const uint4& r) {
+    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(w);
+    top = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
 #pragma unroll
-  for (int i = 0; i < (int)(16 / sizeof(T)); ++i) f[i] = Cvt<T>::to_f(e[i]);
+    for (int i = 0; i < 4; ++i) { f[2 * i] = __uint_as_float(w[i] << 16); f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
+  }
+  __device__ float max() const { return fmaxf(__low2float(top), __high2float(top)); }
+};
+template <> struct Piece<__half> {
+  float f[8];
+  __half2 top;
+  __device__ explicit Piece(const uint4& r) {
+    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+    const __half2* h = reinterpret_cast<const __half2*>(w);
+    top = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { const float2 t = __half22float2(h[i]); f[2 * i] = t.x; f[2 * i + 1] = t.y; }
+  }
+  __device__ float max() const { return fmaxf(__low2float(top), __high2float(top)); }
+};
+
+// Adds a value, or a piece's values (mx: their maximum, NaN left out), to the statistics.  -inf (and anything far below)
+// counts as 2^-200 = 0 times a finite distance; NaN and +inf stay NaN.
+__device__ __forceinline__ void take1(Stat& a, float v, float c) {
+  if (v > a.m) rebase(a, v, c);
+  const float t = max_nan((v - base_of(a.m)) * c, -200.f), e = ex2f(t);
+  a.s += e;
+  a.u = fmaf(t, e, a.u);
+}
+template <int N>
+__device__ __forceinline__ void take(Stat& a, const float (&f)[N], float mx, float c) {
+  if (mx > a.m) rebase(a, mx, c);
+  const float nb = -base_of(a.m);
+  const F2 nb2(nb, nb), c2(c, c);
+  F2 s(a.s, 0.f), u(a.u, 0.f);
+#pragma unroll
+  for (int i = 0; i < N; i += 2) {
+    float t0, t1;
+    mul2(add2(F2(f[i], f[i + 1]), nb2), c2).get(t0, t1);
+    t0 = max_nan(t0, -200.f);
+    t1 = max_nan(t1, -200.f);
+    const F2 e(ex2f(t0), ex2f(t1));
+    s = add2(s, e);
+    u = fma2(F2(t0, t1), e, u);
+  }
+  float x, y;
+  s.get(x, y);
+  a.s = x + y;
+  u.get(x, y);
+  a.u = x + y;
 }
 
 // What a CTA of a cluster leaves for the first one.
@@ -117,10 +175,10 @@ template <typename T, int NT, bool TOP>
 __global__ void __launch_bounds__(NT) token_logprobs_kernel(const LogprobParams p) {
   constexpr int V = 16 / sizeof(T), NW = NT / 32, LPG = NT / kGroups;   // lanes per group of threads
   __shared__ Partial s_part;
-  __shared__ Stat s_stat[NW];
+  __shared__ float s_max[NW], s_sum[NW][2];
   __shared__ float s_group[kGroups];
   __shared__ uint64_t s_cand[kCand];
-  __shared__ uint64_t s_best[NW + 1];
+  __shared__ uint64_t s_best[NW];
   __shared__ float s_bound;
   __shared__ int s_count, s_scan[NW];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -149,46 +207,61 @@ __global__ void __launch_bounds__(NT) token_logprobs_kernel(const LogprobParams 
 #pragma unroll
     for (int k = 0; k < kUnroll; ++k)
       if (v0 + k * NT < pieces) {
-        float f[V];
-        unpack<T>(raw[k], f);
-        take<T>(a, f, c);
+        const Piece<T> q(raw[k]);
+        take(a, q.f, q.max(), c);
       }
   }
   if (tid < edge) {   // fewer than 2 V <= NT of them
-    const float f[1] = {Cvt<T>::to_f(x[edge_at(tid)])};
-    take<T>(a, f, c);
+    take1(a, Cvt<T>::to_f(x[edge_at(tid)]), c);
   }
   const float own_max = a.m;
 
-  // the row's (slice's) statistics; on the way the maxima of the 64 groups of threads
+  // the slice's maximum (on the way those of the 64 groups of threads), then its sums relative to it
+  float m = a.m;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    if (TOP && o == LPG && (lane & (LPG - 1)) == 0) s_group[tid / LPG] = a.m;
-    const Stat b = {__shfl_xor_sync(0xffffffffu, a.m, o), __shfl_xor_sync(0xffffffffu, a.s, o), __shfl_xor_sync(0xffffffffu, a.u, o)};
-    a = merge(a, b, c);
+    if (TOP && o == LPG && (lane & (LPG - 1)) == 0) s_group[tid / LPG] = m;
+    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
   }
-  if (lane == 0) s_stat[warp] = a;
+  if (lane == 0) s_max[warp] = m;
   if (tid == 0) s_count = 0;
   __syncthreads();
-  a = s_stat[0];
 #pragma unroll
-  for (int w = 1; w < NW; ++w) a = merge(a, s_stat[w], c);
+  for (int w = 0; w < NW; ++w) m = fmaxf(m, s_max[w]);
+  rebase(a, m, c);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    a.s += __shfl_xor_sync(0xffffffffu, a.s, o);
+    a.u += __shfl_xor_sync(0xffffffffu, a.u, o);
+  }
+  if (lane == 0) { s_sum[warp][0] = a.s; s_sum[warp][1] = a.u; }
   const int want = TOP ? min(p.top, n) : 0;
+  if (TOP && want > 0 && tid < kGroups) {
+    // the bound: the want-th largest group maximum (at least `want` logits reach it)
+    const float mine = s_group[tid];
+    int above = 0;
+#pragma unroll 16
+    for (int i = 0; i < kGroups; ++i) {
+      const float o = s_group[i];
+      above += (o > mine || (o == mine && i < tid)) ? 1 : 0;
+    }
+    if (above == want - 1) s_bound = mine;
+  }
+  const bool sane = __syncthreads_or(!(a.s == a.s)) == 0;   // else NaN or +inf somewhere: the maxima say nothing
+  a = {m, 0.f, 0.f};
+  if (warp == 0) {
+    float s = lane < NW ? s_sum[lane][0] : 0.f, u = lane < NW ? s_sum[lane][1] : 0.f;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      s += __shfl_xor_sync(0xffffffffu, s, o);
+      u += __shfl_xor_sync(0xffffffffu, u, o);
+    }
+    a.s = s;
+    a.u = u;
+  }
 
   if (TOP && want > 0) {
-    // the bound: the want-th largest group maximum (at least `want` logits reach it)
-    if (tid < kGroups) {
-      const float mine = s_group[tid];
-      int above = 0;
-      for (int i = 0; i < kGroups; ++i) {
-        const float o = s_group[i];
-        above += (o > mine || (o == mine && i < tid)) ? 1 : 0;
-      }
-      if (above == want - 1) s_bound = mine;
-    }
-    __syncthreads();
     const float bound = s_bound;
-    const bool sane = a.s == a.s;         // NaN or +inf somewhere: the maxima above say nothing
     // every logit above the bound (`equal`: or at it) into the list; the number of them, also where it overflows
     auto collect = [&](bool equal) {
       auto offer = [&](float v, int col) {
@@ -202,10 +275,11 @@ __global__ void __launch_bounds__(NT) token_logprobs_kernel(const LogprobParams 
         const int l = __ffs(flagged) - 1;
         flagged &= flagged - 1;
         for (int v = warp * 32 + l + lane * NT; v < pieces; v += 32 * NT) {
-          float f[V];
-          unpack<T>(__ldg(xv + v), f);
+          const Piece<T> q(__ldg(xv + v));
+          if (q.max() >= bound) {
 #pragma unroll
-          for (int i = 0; i < V; ++i) offer(f[i], head + v * V + i);
+            for (int i = 0; i < V; ++i) offer(q.f[i], head + v * V + i);
+          }
         }
       }
       if (tid < edge) {
@@ -282,15 +356,22 @@ __global__ void __launch_bounds__(NT) token_logprobs_kernel(const LogprobParams 
     if (rank == 0) {
       // the slices' statistics, in order, and their entries ranked together
       int at = 0;
+      float top_m = -INFINITY;
+      for (int q = 0; q < C; ++q) top_m = fmaxf(top_m, cluster.map_shared_rank(&s_part, q)->stat.m);
+      Stat sum = {top_m, 0.f, 0.f};
       for (int q = 0; q < C; ++q) {
         const Partial* o = cluster.map_shared_rank(&s_part, q);
-        if (q > 0) a = merge(a, o->stat, c);
+        Stat b = o->stat;
+        rebase(b, top_m, c);
+        sum.s += b.s;
+        sum.u += b.u;
         if (TOP) {
-          const int m = o->n;
-          for (int i = tid; i < m; i += NT) s_cand[at + i] = o->best[i];
-          at += m;
+          const int k = o->n;
+          for (int i = tid; i < k; i += NT) s_cand[at + i] = o->best[i];
+          at += k;
         }
       }
+      a = sum;
       __syncthreads();
       if (TOP) {
         have = min(p.top, at);
@@ -311,21 +392,23 @@ __global__ void __launch_bounds__(NT) token_logprobs_kernel(const LogprobParams 
   }
   if (rank != 0) return;
   const float nan = __int_as_float(0x7fc00000);
-  const bool none = !(a.s > 0.f) || a.m == INFINITY;     // no logit above -inf, or NaN / +inf among them
-  const float lz2 = log2f(a.s), base = a.base();
-  if (tid == 0) {
+  // no logit above -inf, or NaN / +inf among them.  (Only warp 0 holds the sums.)
+  if (warp > 0) return;
+  const bool none = !(a.s > 0.f) || a.m == INFINITY;
+  const float lz2 = log2f(a.s);
+  const float lz = lz2 * kLn2;
+  auto logp = [&](float v) { return fmaf(v - a.m, p.inv_t, -lz); };
+  if (lane == 0) {
     float lp = nan;
     if (tgt == p.ignore) lp = 0.f;
-    else if (scored && !none) lp = fmaf(x_tgt - base, p.inv_t, -kLn2 * lz2);
+    else if (scored && !none) lp = logp(x_tgt);
     p.logprobs[r] = lp;
     p.entropy[r] = none ? nan : (lz2 - a.u / a.s) * kLn2;
   }
-  if (TOP) {
-    for (int i = tid; i < p.top; i += NT) {
-      const uint64_t e = i < have ? mine_best[i] : 0;
-      p.top_id[r * p.top + i] = i < have ? entry_index(e) : -1;
-      p.top_lp[r * p.top + i] = i < have && !none ? fmaf(key_value((uint32_t)(e >> 32)) - base, p.inv_t, -kLn2 * lz2) : nan;
-    }
+  if (TOP && lane < p.top) {   // top <= 32
+    const uint64_t e = lane < have ? mine_best[lane] : 0;
+    p.top_id[r * p.top + lane] = lane < have ? entry_index(e) : -1;
+    p.top_lp[r * p.top + lane] = lane < have && !none ? logp(key_value((uint32_t)(e >> 32))) : nan;
   }
 }
 
