@@ -133,19 +133,17 @@ template <> struct Piece<__half> {
   __device__ float max() const { return fmaxf(__low2float(top), __high2float(top)); }
 };
 
-// Adds a value, or a piece's values (mx: their maximum, NaN left out), to the statistics.  -inf (and anything far below)
-// counts as 2^-200 = 0 times a finite distance; NaN and +inf stay NaN.
+// Adds a value, or a piece's values, to the statistics.  -inf (and anything far below) counts as 2^-200 = 0 times a finite
+// distance; NaN and +inf stay NaN.
 __device__ __forceinline__ void take1(Stat& a, float v, float c) {
   if (v > a.m) rebase(a, v, c);
   const float t = max_nan((v - base_of(a.m)) * c, -200.f), e = ex2f(t);
   a.s += e;
   a.u = fmaf(t, e, a.u);
 }
+// (a.m is at least their maximum, NaN left out)
 template <int N>
-__device__ __forceinline__ void take(Stat& a, const float (&f)[N], float mx, float c) {
-  if (mx > a.m) rebase(a, mx, c);
-  const float nb = -base_of(a.m);
-  const F2 nb2(nb, nb), c2(c, c);
+__device__ __forceinline__ void add(Stat& a, const float (&f)[N], F2 nb2, F2 c2) {
   F2 s(a.s, 0.f), u(a.u, 0.f);
 #pragma unroll
   for (int i = 0; i < N; i += 2) {
@@ -199,16 +197,33 @@ __global__ void __launch_bounds__(NT) token_logprobs_kernel(const LogprobParams 
   const uint4* xv = reinterpret_cast<const uint4*>(x + head);
   auto edge_at = [&](int i) { return i < head ? i : pieces * V + i; };   // i-th value outside the pieces -> its column
   Stat a = {-INFINITY, 0.f, 0.f};
-  for (int v0 = tid; v0 < pieces; v0 += NT * kUnroll) {
+  const F2 c2(c, c);
+  int v0 = tid;
+  for (; v0 + (kUnroll - 1) * NT < pieces; v0 += kUnroll * NT) {   // four pieces, one look at their maximum
     uint4 raw[kUnroll];
 #pragma unroll
-    for (int k = 0; k < kUnroll; ++k)
+    for (int k = 0; k < kUnroll; ++k) raw[k] = __ldg(xv + v0 + k * NT);
+    float mx = Piece<T>(raw[0]).max();
+#pragma unroll
+    for (int k = 1; k < kUnroll; ++k) mx = fmaxf(mx, Piece<T>(raw[k]).max());
+    if (mx > a.m) rebase(a, mx, c);
+    const F2 nb2(-base_of(a.m), -base_of(a.m));
+#pragma unroll
+    for (int k = 0; k < kUnroll; ++k) add(a, Piece<T>(raw[k]).f, nb2, c2);
+  }
+  {
+    uint4 raw[kUnroll - 1];
+#pragma unroll
+    for (int k = 0; k < kUnroll - 1; ++k)
       if (v0 + k * NT < pieces) raw[k] = __ldg(xv + v0 + k * NT);
 #pragma unroll
-    for (int k = 0; k < kUnroll; ++k)
+    for (int k = 0; k < kUnroll - 1; ++k)
       if (v0 + k * NT < pieces) {
         const Piece<T> q(raw[k]);
-        take(a, q.f, q.max(), c);
+        const float mx = q.max();
+        if (mx > a.m) rebase(a, mx, c);
+        const F2 nb2(-base_of(a.m), -base_of(a.m));
+        add(a, q.f, nb2, c2);
       }
   }
   if (tid < edge) {   // fewer than 2 V <= NT of them
@@ -423,8 +438,10 @@ int launch(LogprobParams p, int64_t rows, cudaStream_t st) {
   int cluster = 1;
   while (cluster < 8 && rows * cluster * 2 <= 2 * 148 && p.cols / (cluster * 2) >= 4096) cluster *= 2;
   p.slice = ceil_div(ceil_div(p.cols, cluster), 64) * 64;
-  if (p.top > 0) return launch_as<T, 512, true>(p, rows, cluster, st);
-  return launch_as<T, 512, false>(p, rows, cluster, st);
+  // Many rows: CTAs of 256 threads, whose fixed work per row (joining the statistics, the bound) is half as much and whose
+  // rows overlap six to an SM; few: 512 threads get a row's bytes under way sooner.
+  if (rows * cluster > 2 * 148) return p.top > 0 ? launch_as<T, 256, true>(p, rows, cluster, st) : launch_as<T, 256, false>(p, rows, cluster, st);
+  return p.top > 0 ? launch_as<T, 512, true>(p, rows, cluster, st) : launch_as<T, 512, false>(p, rows, cluster, st);
 }
 
 }  // namespace

@@ -23,7 +23,7 @@ namespace {
 
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr int kMaxBatch = 4096;
-constexpr int kMinTiles = 4;    // least share of a warp: below this the join's traffic outweighs the parallelism
+constexpr int kMinTiles = 2;    // least share of a warp: below this the join's traffic outweighs the parallelism
 
 struct PagedParams {
   const void *q, *kc, *vc;
@@ -36,7 +36,8 @@ struct PagedParams {
   int64_t q_sb, q_sh, k_sh, v_sh, table_ld;     // elements
   int32_t k_sp, k_sr, v_sp, v_sr;               // bytes: page and row of a page
   int B, Hq, Hkv, hd, group, q_tiles, rows, page_size, width, num_pages, workers;
-  float scale_log2;  // scale * log2(e)
+  float scale_log2;  // |scale| log2(e)
+  uint32_t q_sign;   // flips the signs of a pair of query values where the scale is negative
 };
 
 // A warp's tile: 8 KB of K and V (16 KB of heads of 256, 4 KB of small ones); its ring keeps 16 KB in flight, a CTA 128 KB.
@@ -120,8 +121,9 @@ struct Cursor {
   bool poison;
 };
 
-// NQ: columns of eight query heads (group <= 8: 1).
-template <typename T, int HD, int NQ>
+// NQ: columns of eight query heads (group <= 8: 1).  P16: the page size is a multiple of 16, so that 16 tokens side by side
+// share a page: one look into the table for them.
+template <typename T, int HD, int NQ, bool P16>
 __global__ void __launch_bounds__(warps_of(HD) * 32, 1) paged_attention_kernel(const PagedParams p) {
   constexpr int NW = warps_of(HD), TT = tile_tokens(HD), CH = HD / 8, ST = stages_of(HD);
   constexpr int ROWB = HD * 2, KBYTES = TT * ROWB, STAGE = 2 * KBYTES;
@@ -214,45 +216,66 @@ __global__ void __launch_bounds__(warps_of(HD) * 32, 1) paged_attention_kernel(c
     __syncwarp();
   }
 
-  // ---- producer: four lanes (two of heads of 16) copy a row, every lane looks up the pages of its own R rows; that is done
-  // one tile before their copies are issued
+  // ---- producer: four lanes (two of heads of 16) copy a row; the pages are looked up one tile before the copies are issued
+  constexpr int L = P16 ? MT : R;             // looks per tile: of 16 tokens each, or of each of the lane's rows
   Cursor pc = cur;
   int to_look = left, to_issue = left;
-  int page0 = (int)(((int64_t)pc.t * TT) / p.page_size), off0 = (int)((int64_t)pc.t * TT - (int64_t)page0 * p.page_size);
-  const int32_t* trow = p.table + (int64_t)pc.b * p.table_ld;
-  const char *kb = nullptr, *vb = nullptr;    // the head's rows, of the tile that was looked up
-  int page[R], row[R];
-  bool bad_seen = false;            // a page outside the cache, in the tile that was looked up
-  uint32_t bad_bits = 0;            // the same per ring slot
+  const int unit = P16 ? p.page_size / 16 : p.page_size;      // looks per page
+  int page0, off0;                            // of the tile's first token: place in the table row, units into the page
+  {
+    const int64_t at = (int64_t)pc.t * (P16 ? MT : TT);
+    page0 = (int)(at / unit);
+    off0 = (int)(at - (int64_t)page0 * unit);
+  }
   const int prow = lane / LPR, pch = lane % LPR;
-  uint32_t dst[2];                  // of the lane's even and odd copies of a row
+  const int32_t* trow = nullptr;
+  const char *kb = nullptr, *vb = nullptr;    // the head's rows in page 0, from this lane's chunk on
+  auto head_of = [&]() {
+    const int kvh = p.q_tiles == 1 ? pc.h : pc.h / p.q_tiles;
+    trow = p.table + (int64_t)pc.b * p.table_ld;
+    kb = static_cast<const char*>(p.kc) + (int64_t)kvh * p.k_sh * 2 + pch * 16 + (P16 ? (int64_t)prow * p.k_sr : 0);
+    vb = static_cast<const char*>(p.vc) + (int64_t)kvh * p.v_sh * 2 + pch * 16 + (P16 ? (int64_t)prow * p.v_sr : 0);
+  };
+  head_of();
+  const char *kt = kb, *vt = vb;              // the same of the tile that was looked up
+  int page[L], off[L], rows_there = 0;        // its pages (-1: none), places in them, tokens
+  bool bad_seen = false;                      // a page outside the cache
+  uint32_t bad_bits = 0;                      // the same per ring slot
+  uint32_t dst[2];                            // of the lane's even and odd copies of a row
 #pragma unroll
   for (int i = 0; i < 2; ++i) dst[i] = ring_u + prow * ROWB + (((pch + (CI > 1 ? LPR * i : 0)) ^ swizzle<CH>(prow)) & (CH >= 8 ? 7 : CH - 1)) * 16;
   auto look = [&]() {
     if (to_look > 0) {
       --to_look;
-      const int kvh = p.q_tiles == 1 ? pc.h : pc.h / p.q_tiles;
-      kb = static_cast<const char*>(p.kc) + (int64_t)kvh * p.k_sh * 2 + pch * 16;
-      vb = static_cast<const char*>(p.vc) + (int64_t)kvh * p.v_sh * 2 + pch * 16;
+      kt = kb;
+      vt = vb;
       bool bad = pc.poison;
-      const int rows_in = pc.len - pc.t * TT;         // > 0
+      rows_there = pc.len - pc.t * TT;        // > 0
+      if constexpr (P16) {
 #pragma unroll
-      for (int j = 0; j < R; ++j) {
-        const int r = prow + j * RPI;
-        int pi = page0, o = off0 + r;
-        if (p.page_size >= TT) {                      // at most one page ends inside the tile
-          if (o >= p.page_size) { o -= p.page_size; ++pi; }
-        } else {
-          const int k = o / p.page_size;
-          pi += k;
-          o -= k * p.page_size;
+        for (int i = 0; i < MT; ++i) {
+          const bool in = i == 0 || i * 16 < rows_there;
+          page[i] = in ? __ldg(trow + page0) : 0;
+          bad |= (unsigned)page[i] >= (unsigned)p.num_pages;
+          off[i] = off0;
+          if (++off0 == unit) { off0 = 0; ++page0; }
         }
-        const bool in = r < rows_in;
-        const int id = in ? __ldg(trow + pi) : -1;
-        const bool ok = (unsigned)id < (unsigned)p.num_pages;
-        bad |= in && !ok;
-        page[j] = ok ? id : -1;
-        row[j] = o;
+      } else {
+#pragma unroll
+        for (int j = 0; j < R; ++j) {
+          const int r = prow + j * RPI;
+          int pi = page0, o = off0 + r;
+          const int k = o / unit;
+          pi += k;
+          o -= k * unit;
+          page[j] = r < rows_there ? __ldg(trow + pi) : 0;
+          bad |= (unsigned)page[j] >= (unsigned)p.num_pages;
+          off[j] = o;
+        }
+        off0 += TT;
+        const int k = off0 / unit;
+        page0 += k;
+        off0 -= k * unit;
       }
       bad_seen = bad;
       if (to_look > 0) {
@@ -260,29 +283,25 @@ __global__ void __launch_bounds__(warps_of(HD) * 32, 1) paged_attention_kernel(c
         advance(pc);
         if (pc.b != b || pc.h != h) {
           page0 = off0 = 0;
-          trow = p.table + (int64_t)pc.b * p.table_ld;
-        } else if (p.page_size >= TT) {
-          off0 += TT;
-          if (off0 >= p.page_size) { off0 -= p.page_size; ++page0; }
-        } else {
-          page0 = (int)(((unsigned)pc.t * TT) / (unsigned)p.page_size);
-          off0 = pc.t * TT - page0 * p.page_size;
+          head_of();
         }
       }
     }
   };
+  const int64_t k_next = (int64_t)RPI * p.k_sr, v_next = (int64_t)RPI * p.v_sr;
   auto issue = [&](int slot) {
     if (to_issue > 0) {
       --to_issue;
       const uint32_t so = slot * STAGE;
 #pragma unroll
       for (int j = 0; j < R; ++j) {
-        const bool there = page[j] >= 0;
-        const char *ks = kb, *vs = vb;
-        if (there) {
-          ks += (int64_t)page[j] * p.k_sp + (int64_t)row[j] * p.k_sr;
-          vs += (int64_t)page[j] * p.v_sp + (int64_t)row[j] * p.v_sr;
-        }
+        const int l = P16 ? j * RPI / 16 : j;
+        const bool ok = (unsigned)page[l] < (unsigned)p.num_pages;
+        const bool there = ok && prow + j * RPI < rows_there;
+        const int pg = ok ? page[l] : 0;
+        const char* ks = kt + (int64_t)pg * p.k_sp + (int64_t)(P16 ? off[l] * 16 : off[l]) * p.k_sr;
+        const char* vs = vt + (int64_t)pg * p.v_sp + (int64_t)(P16 ? off[l] * 16 : off[l]) * p.v_sr;
+        if (P16 && j * RPI % 16 != 0) { ks += k_next; vs += v_next; }
 #pragma unroll
         for (int i = 0; i < CI; ++i) {
           if (p.hd == HD || (pch + LPR * i) * 8 < p.hd) {
@@ -292,7 +311,7 @@ __global__ void __launch_bounds__(warps_of(HD) * 32, 1) paged_attention_kernel(c
           }
         }
       }
-      const bool any_bad = __any_sync(0xffffffffu, bad_seen);
+      const bool any_bad = P16 ? bad_seen : __any_sync(0xffffffffu, bad_seen);   // P16: the same in every lane
       bad_bits = any_bad ? bad_bits | (1u << slot) : bad_bits & ~(1u << slot);
     }
     cp_async_commit();
@@ -312,7 +331,8 @@ __global__ void __launch_bounds__(warps_of(HD) * 32, 1) paged_attention_kernel(c
     vofs[i] = KBYTES + ((mi >> 1) * 8 + mr) * ROWB + (((2 * i + (mi & 1)) ^ swizzle<CH>(mr)) & mask) * 16;
   }
   uint32_t qf[KS][NQ][2];
-  float o[KS][NQ][4], m[NQ][2], l[NQ][2];
+  float o[KS][NQ][4], m[NQ][2], l[NQ][2];   // m: the largest score; base: m scale log2(e), rounded once (0 while m is -inf)
+  float base[NQ][2];
   bool poison = false, fresh = true;
   int first_tile = cur.t, rows_here = 0, head0 = 0, slot = 0;
   while (left > 0) {
@@ -332,10 +352,10 @@ __global__ void __launch_bounds__(warps_of(HD) * 32, 1) paged_attention_kernel(c
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             const int d = ks * 16 + i * 8;
-            qf[ks][n][i] = (r < rows_here && d < p.hd) ? __ldg(reinterpret_cast<const uint32_t*>(qr + d)) : 0u;
+            qf[ks][n][i] = (r < rows_here && d < p.hd) ? __ldg(reinterpret_cast<const uint32_t*>(qr + d)) ^ p.q_sign : 0u;
           }
         m[n][0] = m[n][1] = -INFINITY;
-        l[n][0] = l[n][1] = 0.f;
+        l[n][0] = l[n][1] = base[n][0] = base[n][1] = 0.f;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) o[ks][n][0] = o[ks][n][1] = o[ks][n][2] = o[ks][n][3] = 0.f;
       }
@@ -344,7 +364,7 @@ __global__ void __launch_bounds__(warps_of(HD) * 32, 1) paged_attention_kernel(c
     cp_async_wait<ST - 2>();
     __syncwarp();
     poison |= (bad_bits >> slot) & 1u;
-    const uint32_t base = ring_u + slot * STAGE;
+    const uint32_t tile = ring_u + slot * STAGE;
 
     // scores
     float s[MT][NQ][4];
@@ -357,36 +377,34 @@ __global__ void __launch_bounds__(warps_of(HD) * 32, 1) paged_attention_kernel(c
 #pragma unroll
       for (int i = 0; i < MT; ++i) {
         uint32_t a[4];
-        ldsm_x4(a, base + kofs[ks & (NO - 1)] + (ks / 4) * 128 + i * 16 * ROWB);
+        ldsm_x4(a, tile + kofs[ks & (NO - 1)] + (ks / 4) * 128 + i * 16 * ROWB);
 #pragma unroll
         for (int n = 0; n < NQ; ++n) mma16816<T>(s[i][n], a[0], a[1], a[2], a[3], qf[ks][n][0], qf[ks][n][1]);
       }
 
     // running maximum and sum, in powers of two
     const int rows_in = cur.len - cur.t * TT;
-    // (the maximum is taken of the scaled scores: a negative scale turns their order)
     float mx[NQ][2];
     bool more = false;
+    if (rows_in < TT) {
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) {
+          if (i * 16 + g >= rows_in) s[i][n][0] = s[i][n][1] = -INFINITY;
+          if (i * 16 + g + 8 >= rows_in) s[i][n][2] = s[i][n][3] = -INFINITY;
+        }
+    }
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        float v = -INFINITY;
+        float v = m[n][e];
 #pragma unroll
-        for (int i = 0; i < MT; ++i) {
-          if (rows_in < TT) {
-            s[i][n][e] = i * 16 + g >= rows_in ? -INFINITY : s[i][n][e] * p.scale_log2;
-            s[i][n][2 + e] = i * 16 + g + 8 >= rows_in ? -INFINITY : s[i][n][2 + e] * p.scale_log2;
-          } else {
-            s[i][n][e] *= p.scale_log2;
-            s[i][n][2 + e] *= p.scale_log2;
-          }
-          v = fmaxf(v, fmaxf(s[i][n][e], s[i][n][2 + e]));
-        }
+        for (int i = 0; i < MT; ++i) v = fmaxf(v, fmaxf(s[i][n][e], s[i][n][2 + e]));
         v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
         v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
-        v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
-        mx[n][e] = fmaxf(v, m[n][e]);
+        mx[n][e] = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
         more |= mx[n][e] > m[n][e];
       }
     }
@@ -396,8 +414,11 @@ __global__ void __launch_bounds__(warps_of(HD) * 32, 1) paged_attention_kernel(c
         float f[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          f[e] = m[n][e] == mx[n][e] ? 1.f : ex2(m[n][e] - mx[n][e]);
+          const float to = mx[n][e] == -INFINITY ? 0.f : mx[n][e] * p.scale_log2;   // every score -inf so far: weights 0
+          f[e] = m[n][e] == mx[n][e] ? 1.f : ex2(base[n][e] - to);
+          if (m[n][e] == -INFINITY) f[e] = 0.f;
           m[n][e] = mx[n][e];
+          base[n][e] = to;
           l[n][e] *= f[e];
         }
 #pragma unroll
@@ -412,9 +433,8 @@ __global__ void __launch_bounds__(warps_of(HD) * 32, 1) paged_attention_kernel(c
       for (int n = 0; n < NQ; ++n) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const float b = m[n][e] == -INFINITY ? 0.f : m[n][e];   // every score -inf so far: weights 0
-          s[i][n][e] = ex2(s[i][n][e] - b);
-          s[i][n][2 + e] = ex2(s[i][n][2 + e] - b);
+          s[i][n][e] = ex2(fmaf(s[i][n][e], p.scale_log2, -base[n][e]));
+          s[i][n][2 + e] = ex2(fmaf(s[i][n][2 + e], p.scale_log2, -base[n][e]));
           l[n][e] += s[i][n][e] + s[i][n][2 + e];
         }
         split2<T>(s[i][n][0], s[i][n][1], hi[n][0], lo[n][0]);
@@ -428,7 +448,7 @@ __global__ void __launch_bounds__(warps_of(HD) * 32, 1) paged_attention_kernel(c
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
         uint32_t a[4];
-        ldsm_x4_trans(a, base + vofs[ks & (NO - 1)] + (ks / 4) * 128 + i * 16 * ROWB);
+        ldsm_x4_trans(a, tile + vofs[ks & (NO - 1)] + (ks / 4) * 128 + i * 16 * ROWB);
 #pragma unroll
         for (int n = 0; n < NQ; ++n) {
           mma16816<T>(o[ks][n], a[0], a[1], a[2], a[3], hi[n][0], hi[n][1]);
@@ -472,8 +492,8 @@ __global__ void __launch_bounds__(warps_of(HD) * 32, 1) paged_attention_kernel(c
                 }
               }
             if (g == 0) {
-              if (!whole) *reinterpret_cast<float2*>(pm + r * 2) = make_float2(m[n][e], sum);
-              else if (p.lse) p.lse[(int64_t)cur.b * p.Hq + head0 + r] = (m[n][e] + log2f(sum)) * kLn2;
+              if (!whole) *reinterpret_cast<float2*>(pm + r * 2) = make_float2(m[n][e] == -INFINITY ? -INFINITY : base[n][e], sum);
+              else if (p.lse) p.lse[(int64_t)cur.b * p.Hq + head0 + r] = (base[n][e] + log2f(sum)) * kLn2;
             }
           }
         }
@@ -484,23 +504,29 @@ __global__ void __launch_bounds__(warps_of(HD) * 32, 1) paged_attention_kernel(c
   cp_async_wait<0>();
 }
 
-// One CTA per (request, query head): nothing where one share held the whole pair, zeros for an empty request, else the
-// parts' weighted sum.  Thread d holds column d (and d + 128); parts in the order of their shares.
-template <typename T>
-__global__ void __launch_bounds__(128) paged_join_kernel(const PagedParams p) {
-  extern __shared__ float s_w[];    // [parts]
-  __shared__ float s_red[8];
-  const int b = blockIdx.x / p.Hq, hq = blockIdx.x - b * p.Hq;
+// WPR warps per (request, query head): nothing where one share held the whole pair, zeros for an empty request, else the
+// parts' weighted sum.  A warp takes every WPR-th part, its statistics one per lane, its values four side by side per lane.
+template <typename T, int WPR>
+__global__ void __launch_bounds__(256) paged_join_kernel(const PagedParams p) {
+  constexpr int RPC = 8 / WPR;                  // rows per CTA
+  __shared__ __align__(16) float s_o[WPR > 1 ? WPR : 1][256];
+  __shared__ float s_m[WPR], s_l[WPR];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, wi = warp % WPR;
+  const int64_t rw = (int64_t)blockIdx.x * RPC + warp / WPR;   // WPR > 1: the same for the whole CTA
+  const bool live = rw < (int64_t)p.B * p.Hq;
+  const int b = live ? (int)(rw / p.Hq) : 0, hq = live ? (int)(rw - (int64_t)b * p.Hq) : 0;
   const int kvh = hq / p.group, in_group = hq - kvh * p.group, qt = in_group / 16, r = in_group & 15;
-  const int H = p.Hkv * p.q_tiles, tid = threadIdx.x;
-  T* ob = static_cast<T*>(p.out) + (int64_t)blockIdx.x * p.hd;
+  const int H = p.Hkv * p.q_tiles;
+  T* ob = static_cast<T*>(p.out) + rw * p.hd;
   chain_wait();
+  if (!live) return;                            // (only with WPR = 1, where no barrier follows)
   const int c0 = __ldcg(p.cum + b), c1 = __ldcg(p.cum + b + 1), call = __ldcg(p.cum + p.B);
   const int n = c1 - c0;
   if (n == 0) {   // an empty request; one with a length but no table at all is NaN like any that outgrew its table
+    if (wi > 0) return;
     const bool wrong = p.lens[b] > 0;
-    for (int d = tid; d < p.hd; d += 128) ob[d] = Cvt<T>::from_f(wrong ? __int_as_float(0x7fc00000) : 0.f);
-    if (p.lse && tid == 0) p.lse[blockIdx.x] = wrong ? __int_as_float(0x7fc00000) : -INFINITY;
+    for (int d = lane; d < p.hd; d += 32) ob[d] = Cvt<T>::from_f(wrong ? __int_as_float(0x7fc00000) : 0.f);
+    if (p.lse && lane == 0) p.lse[rw] = wrong ? __int_as_float(0x7fc00000) : -INFINITY;
     return;
   }
   const int64_t total = (int64_t)call * H;
@@ -510,35 +536,69 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const PagedParams p) {
   if (w0 == w1) return;
   const int parts = w1 - w0 + 1;
   const int64_t first = (int64_t)w0 * 2 + (t0 == (int64_t)w0 * share ? 0 : 1);
-  auto slot = [&](int i) { return i == 0 ? first : (int64_t)(w0 + i) * 2; };
-  float m = -INFINITY;
-  for (int i = tid; i < parts; i += 128) m = fmaxf(m, __ldcg(p.part_ml + (slot(i) * p.rows + r) * 2));
+  auto at = [&](int i) { return ((i == 0 ? first : (int64_t)(w0 + i) * 2) * p.rows + r); };
+  const int d0 = lane * 4, d1 = d0 + 128;
+  float4 a = make_float4(0.f, 0.f, 0.f, 0.f), c = a;
+  float m = -INFINITY, l = 0.f;
+  auto scaled = [](float4 x, float f, float4 y) { return make_float4(fmaf(x.x, f, y.x), fmaf(x.y, f, y.y), fmaf(x.z, f, y.z), fmaf(x.w, f, y.w)); };
+  const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i0 = wi; i0 < parts; i0 += 32 * WPR) {
+    const int mine = i0 + lane * WPR;           // this lane's part
+    const float2 ml = mine < parts ? __ldcg(reinterpret_cast<const float2*>(p.part_ml + at(mine) * 2)) : make_float2(-INFINITY, 0.f);
+    float mx = ml.x;
 #pragma unroll
-  for (int s = 16; s > 0; s >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, s));
-  if ((tid & 31) == 0) s_red[tid >> 5] = m;
-  __syncthreads();
-  m = fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3]));
-  const float base = m == -INFINITY ? 0.f : m;
-  float l = 0.f;
-  for (int i = tid; i < parts; i += 128) {
-    const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.part_ml + (slot(i) * p.rows + r) * 2));
-    const float wgt = ex2(ml.x - base);
-    s_w[i] = wgt;
-    l += wgt * ml.y;
-  }
+    for (int s = 16; s > 0; s >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, s));
+    mx = fmaxf(mx, m);
+    const float base = mx == -INFINITY ? 0.f : mx, w = ex2(ml.x - base);
+    float sum = w * ml.y;
 #pragma unroll
-  for (int s = 16; s > 0; s >>= 1) l += __shfl_xor_sync(0xffffffffu, l, s);
-  if ((tid & 31) == 0) s_red[4 + (tid >> 5)] = l;
-  __syncthreads();
-  l = (s_red[4] + s_red[5]) + (s_red[6] + s_red[7]);
-  const float inv = 1.f / l;
-  for (int d = tid; d < p.hd; d += 128) {
-    float acc = 0.f;
-#pragma unroll 8
-    for (int i = 0; i < parts; ++i) acc += s_w[i] * __ldcg(p.part_o + (slot(i) * p.rows + r) * p.hd + d);
-    ob[d] = Cvt<T>::from_f(acc * inv);
+    for (int s = 16; s > 0; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
+    const float f = m == -INFINITY ? 0.f : ex2(m - base);
+    l = fmaf(l, f, sum);
+    m = mx;
+    a = scaled(a, f, zero);
+    c = scaled(c, f, zero);
+    const int here = min(32, (parts - i0 + WPR - 1) / WPR);
+#pragma unroll 4
+    for (int k = 0; k < here; ++k) {
+      const float f = __shfl_sync(0xffffffffu, w, k);
+      const float* o = p.part_o + at(i0 + k * WPR) * p.hd;
+      if (d0 < p.hd) a = scaled(__ldcg(reinterpret_cast<const float4*>(o + d0)), f, a);
+      if (d1 < p.hd) c = scaled(__ldcg(reinterpret_cast<const float4*>(o + d1)), f, c);
+    }
   }
-  if (p.lse && tid == 0) p.lse[blockIdx.x] = (m + log2f(l)) * kLn2;
+  if constexpr (WPR > 1) {
+    if (lane == 0) { s_m[wi] = m; s_l[wi] = l; }
+    __syncthreads();
+    float all = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < WPR; ++w) all = fmaxf(all, s_m[w]);
+    const float base = all == -INFINITY ? 0.f : all;
+    const float f = ex2(m - base);
+    reinterpret_cast<float4*>(s_o[wi])[lane] = scaled(a, f, zero);
+    if (p.hd > 128) reinterpret_cast<float4*>(s_o[wi])[lane + 32] = scaled(c, f, zero);
+    l = 0.f;
+#pragma unroll
+    for (int w = 0; w < WPR; ++w) l = fmaf(s_l[w], ex2(s_m[w] - base), l);
+    m = all;
+    __syncthreads();
+    const int d = threadIdx.x;
+    if (d < p.hd) {
+      float acc = 0.f;
+#pragma unroll
+      for (int w = 0; w < WPR; ++w) acc += s_o[w][d];
+      ob[d] = Cvt<T>::from_f(acc / l);
+    }
+  } else {
+    const float inv = 1.f / l;
+    auto put = [&](int d, float4 v) {           // hd is a multiple of 8
+      T four[4] = {Cvt<T>::from_f(v.x * inv), Cvt<T>::from_f(v.y * inv), Cvt<T>::from_f(v.z * inv), Cvt<T>::from_f(v.w * inv)};
+      *reinterpret_cast<uint2*>(ob + d) = *reinterpret_cast<const uint2*>(four);
+    };
+    if (d0 < p.hd) put(d0, a);
+    if (d1 < p.hd) put(d1, c);
+  }
+  if (p.lse && wi == 0 && lane == 0) p.lse[rw] = (m + log2f(l)) * kLn2;
 }
 
 int sm_count(int* out) {
@@ -562,9 +622,13 @@ template <typename T, int HD, int NQ>
 int launch(const PagedParams& p, int sms, cudaStream_t st) {
   constexpr int NW = warps_of(HD);
   const size_t smem = (size_t)NW * stages_of(HD) * 2 * tile_tokens(HD) * HD * 2 + (size_t)(2 * p.B + 1) * 4;
-  HB_PROPAGATE(ensure_dynamic_smem((const void*)paged_attention_kernel<T, HD, NQ>, smem));
-  HB_PROPAGATE(launch_chained(paged_attention_kernel<T, HD, NQ>, dim3((unsigned)sms), dim3(NW * 32), smem, st, false, 1, p));
-  return launch_chained(paged_join_kernel<T>, dim3((unsigned)(p.B * p.Hq)), dim3(128), (size_t)p.workers * 4, st, true, 1, p);
+  auto kern = p.page_size % 16 == 0 ? paged_attention_kernel<T, HD, NQ, true> : paged_attention_kernel<T, HD, NQ, false>;
+  HB_PROPAGATE(ensure_dynamic_smem((const void*)kern, smem));
+  HB_PROPAGATE(launch_chained(kern, dim3((unsigned)sms), dim3(NW * 32), smem, st, false, 1, p));
+  // a warp per row, or eight where a row has many parts (few requests)
+  const int64_t rows = (int64_t)p.B * p.Hq;
+  if ((int64_t)p.B * p.Hkv * p.q_tiles * 8 <= p.workers) return launch_chained(paged_join_kernel<T, 8>, dim3((unsigned)rows), dim3(256), 0, st, true, 1, p);
+  return launch_chained(paged_join_kernel<T, 1>, dim3((unsigned)ceil_div64(rows, 8)), dim3(256), 0, st, true, 1, p);
 }
 
 template <typename T, int NQ>
@@ -645,7 +709,10 @@ extern "C" int hb200_paged_decode_attention(const hb200_paged_cache* c, const vo
   p.rows = group < 16 ? group : 16;
   p.page_size = c->page_size; p.width = table_width; p.num_pages = c->num_pages;
   p.workers = sms * warps_of(padded_hd(c->head_dim));
-  p.scale_log2 = (float)((double)scale * 1.4426950408889634);
+  // (a scale of zero: near enough to it, so that the -inf of masked tokens stays -inf in the product)
+  const double magnitude = scale < 0.f ? -(double)scale : (double)scale;
+  p.scale_log2 = magnitude < 1e-30 ? 1e-30f : (float)(magnitude * 1.4426950408889634);
+  p.q_sign = scale < 0.f ? 0x80008000u : 0u;
   const size_t slots = (size_t)p.workers * 2;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   p.part_o = reinterpret_cast<float*>(ws);

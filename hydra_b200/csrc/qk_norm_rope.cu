@@ -4,12 +4,14 @@
 //   y = x * rsqrt(c * sum x^2 + eps) * w * s      (c = 1/hd: rms; c = 1: l2; no norm: y = x * s)
 //   pairs (i, i + rot/2) or (2i, 2i + 1) of the first rot values:  (y1 cos - y2 sin, y1 sin + y2 cos)
 //
-// Bound: HBM (each head row read once, written once; 32 bits from the load to the one rounding at the store).  A group of
-// lanes holds one head row, 8 values per lane through 16-byte accesses (or value by value where sizes, strides or
-// pointers are no multiples of 16 bytes).  A lane keeps the same place in the row for all heads of its token, so the
-// token's cosines and sines are loaded once into registers; the weights sit in shared memory.  Four head rows per group are
-// in flight while four are computed.  The half layout fetches the partner value from its lane where rot / 2 is a multiple of
-// 8 values, else through shared memory (padded by one word in eight: no bank conflicts), which works for every rot.
+// Bound: HBM (each head row read once, written once; 32 bits from the load to the one rounding at the store).  A warp takes
+// one token's queries, keys or values (or a part of them where there are few tokens).  A group of lanes holds one head row,
+// 8 values per lane through 16-byte accesses (or value by value where sizes, strides or pointers are no multiples of 16
+// bytes).  A lane keeps the same place in the row for all heads, so the products of the token's cosines and sines with the
+// weights sit in its registers, and a head row costs two packed products and a fused one per pair of values; the norm's factor is
+// the same for the whole row and comes last.  Four head rows per group are in flight while four are computed.  The half layout
+// fetches the partner value from its lane where rot / 2 is a multiple of 8 values, else through shared memory (padded by one
+// word in eight: no bank conflicts), which works for every rot.
 #include "common.cuh"
 
 namespace hb200 {
@@ -27,7 +29,7 @@ struct RopeParams {
   int64_t qo_s[3], ko_s[3];
   int64_t kc_s[3], vc_s[3];              // page, head, row
   int64_t tokens, pos_sb, table_ld, table_rows, capacity;
-  int S, Hq, Hkv, hd, rot, page_size, group_lanes, parts, pos64;
+  int S, Hq, Hkv, hd, rot, page_size, group_lanes, q_parts, kv_parts, pos64;
   float norm_c, eps, q_scale, k_scale;
   int norm;
 };
@@ -84,14 +86,30 @@ __device__ __forceinline__ void store8(T* p, int n, const float (&f)[8]) {
   r.copy(p, n);
 }
 
+// Two 32-bit values in one operation.
+struct F2 {
+  uint64_t v;
+  __device__ F2() {}
+  __device__ F2(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b)); }
+  __device__ void get(float& a, float& b) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+};
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+
 // VEC: rows by 16-byte accesses.  TAB: tables by 16-byte loads, a lane's values all turned or all kept, partners in one lane.
 // HALF: pairs (i, i + rot/2); else (2i, 2i + 1).  CACHE: k and v rows go to their slots, else k rows to k_out.
 template <typename T, bool VEC, bool TAB, bool HALF, bool CACHE>
 __global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(const RopeParams p) {
   constexpr int U = sizeof(T) == 4 ? 2 : 4;                // rows in flight per group, and as many in computation
-  constexpr int NC = HALF || !TAB ? 8 : 4;                 // cosines per lane
   extern __shared__ float s_rows[];
-  __shared__ __align__(16) float s_w[2][256];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int LG = p.group_lanes, groups = 32 / LG;          // lanes per head row (a power of two), rows per warp
   const int gl = lane & (LG - 1), grp = lane / LG;
@@ -99,34 +117,32 @@ __global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(const RopeParams
   const int mine = p.hd - e0 < 8 ? (p.hd - e0 > 0 ? p.hd - e0 : 0) : 8;
   const int half = p.rot >> 1;
   float* row = s_rows + (warp * groups + grp) * (LG * 9);
-  const int rows = p.Hq + p.Hkv + (CACHE ? p.Hkv : 0);
-  const int step = groups * p.parts;
-  for (int i = threadIdx.x; i < 256; i += kThreads) {
-    s_w[0][i] = p.q_scale * (p.wq && i < p.hd ? __ldg(p.wq + i) : 1.f);
-    s_w[1][i] = p.k_scale * (p.wk && i < p.hd ? __ldg(p.wk + i) : 1.f);
-  }
-  __syncthreads();
+  const int parts = p.q_parts + p.kv_parts * (CACHE ? 2 : 1);
+  const bool turn = e0 < p.rot;                            // TAB: of all the lane's values
+  const int partner = !turn ? lane : (e0 < half ? lane + (half >> 3) : lane - (half >> 3));
 
-  const int64_t items = p.tokens * p.parts, stride = (int64_t)gridDim.x * (kThreads / 32);
+  const int64_t items = p.tokens * parts, stride = (int64_t)gridDim.x * (kThreads / 32);
   for (int64_t item = (int64_t)blockIdx.x * (kThreads / 32) + warp; item < items; item += stride) {
-    const int64_t tok = p.parts == 1 ? item : item / p.parts;
-    const int part = (int)(item - tok * p.parts);          // which share of the token's heads
+    const int64_t tok = item / parts;
+    int part = (int)(item - tok * parts);                  // which share of the token's heads
+    const int kind = part < p.q_parts ? 0 : (part < p.q_parts + p.kv_parts ? 1 : 2);
+    part -= kind == 0 ? 0 : (kind == 1 ? p.q_parts : p.q_parts + p.kv_parts);
+    const int rows = kind == 0 ? p.Hq : p.Hkv, step = groups * (kind == 0 ? p.q_parts : p.kv_parts);
     const int64_t b = tok < p.S ? 0 : tok / p.S, s = tok - b * p.S;
-    const T* qb = static_cast<const T*>(p.q) + b * p.q_s[0] + s * p.q_s[1] + e0;
-    const T* kb = static_cast<const T*>(p.k) + b * p.k_s[0] + s * p.k_s[1] + e0;
-    const T* vb = CACHE ? static_cast<const T*>(p.v) + b * p.v_s[0] + s * p.v_s[1] + e0 : nullptr;
+    const int64_t* in_s = kind == 0 ? p.q_s : (kind == 1 ? p.k_s : p.v_s);
+    int r = part * groups + grp;                           // this lane's head row
+    const T* src = static_cast<const T*>(kind == 0 ? p.q : (kind == 1 ? p.k : p.v)) + b * in_s[0] + s * in_s[1] + r * in_s[2] + e0;
+    const int64_t in_step = in_s[2] * step;
     Raw<T, VEC> raw[U], next[U];
-    auto fetch = [&](Raw<T, VEC> (&x)[U], int r0) {
+    auto fetch = [&](Raw<T, VEC> (&x)[U], int r) {         // rows r, r + step, ... (src: row r)
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int r = r0 + u * step + grp;
-        const T* src = r < p.Hq ? qb + (int64_t)r * p.q_s[2]
-                                : (!CACHE || r < p.Hq + p.Hkv ? kb + (int64_t)(r - p.Hq) * p.k_s[2] : vb + (int64_t)(r - p.Hq - p.Hkv) * p.v_s[2]);
-        if (r < rows && mine > 0) x[u].load(src, mine);
+        if (r + u * step < rows && mine > 0) x[u].load(src + u * in_step, mine);
         else x[u].clear();
       }
+      src += U * in_step;
     };
-    fetch(raw, part * groups);
+    fetch(raw, r);
 
     int64_t pos = s;
     if (p.positions)
@@ -137,32 +153,76 @@ __global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(const RopeParams
     const bool pad = pos < 0;                              // a row of padding: zeros out, nothing into the cache
     bool wrong = pos >= p.table_rows;                      // no angle for it: NaN, not a silent clamp
     if constexpr (CACHE) wrong |= slot >= p.capacity;
-    const int64_t tr = pad || pos >= p.table_rows ? 0 : pos;
+    T* dst;
+    int64_t out_step;
+    if (CACHE && kind > 0) {
+      if (pad || slot < 0 || slot >= p.capacity) continue;
+      const int64_t page = slot / p.page_size, off = slot - page * p.page_size;
+      const int64_t* out_s = kind == 1 ? p.kc_s : p.vc_s;
+      dst = static_cast<T*>(kind == 1 ? p.kc : p.vc) + page * out_s[0] + r * out_s[1] + off * out_s[2] + e0;
+      out_step = out_s[1] * step;
+    } else {
+      const int64_t* out_s = kind == 0 ? p.qo_s : p.ko_s;
+      dst = static_cast<T*>(kind == 0 ? p.q_out : p.k_out) + b * out_s[0] + s * out_s[1] + r * out_s[2] + e0;
+      out_step = out_s[2] * step;
+    }
+    if ((CACHE && kind == 2) || pad) {                     // values go as they are; padding as zeros
+      for (int r0 = part * groups; r0 < rows; r0 += step * U, r += step * U) {   // uniform over the warp
+        if (r0 + step * U < rows) fetch(next, r + step * U);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          if (pad) raw[u].clear();
+          if (r + u * step < rows && mine > 0) raw[u].copy(dst + u * out_step, mine);
+          raw[u] = next[u];
+        }
+        dst += U * out_step;
+      }
+      continue;
+    }
 
-    // cosines and (signed) sines of the lane's values
-    float c[NC], n[NC];
+    // cw, nw: z_i = (x_i cw_i + x_partner nw_i) * factor of the norm
+    const int64_t tr = wrong ? 0 : pos;
     const float* ct = p.cos_t + tr * p.table_ld;
     const float* st = p.sin_t + tr * p.table_ld;
-    const bool turn = e0 < p.rot;                          // TAB: of all the lane's values
-    if constexpr (TAB) {
+    const float* wt = kind == 0 ? p.wq : p.wk;
+    const float scale = kind == 0 ? p.q_scale : p.k_scale;
+    float c[8], n[8], w[8];
 #pragma unroll
-      for (int i = 0; i < NC; ++i) c[i] = n[i] = 0.f;
+    for (int i = 0; i < 8; ++i) { c[i] = 1.f; n[i] = 0.f; w[i] = scale; }
+    if (wt) {
+      if (VEC && (reinterpret_cast<uintptr_t>(wt) & 15) == 0) {
+        if (mine > 0) {
+          const float4 a = __ldg(reinterpret_cast<const float4*>(wt + e0)), d = __ldg(reinterpret_cast<const float4*>(wt + e0) + 1);
+          w[0] *= a.x; w[1] *= a.y; w[2] *= a.z; w[3] *= a.w;
+          w[4] *= d.x; w[5] *= d.y; w[6] *= d.z; w[7] *= d.w;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (i < mine) w[i] *= __ldg(wt + e0 + i);
+      }
+    }
+    if constexpr (TAB) {
       if (turn) {
+        constexpr int NC = HALF ? 8 : 4;                   // table entries of the lane's values
         const int at = HALF ? (e0 < half ? e0 : e0 - half) : e0 >> 1;
-        const float sign = HALF && e0 < half ? -1.f : 1.f;
+        float a[NC], d[NC];
 #pragma unroll
         for (int i = 0; i < NC; i += 4) {
-          const float4 a = __ldg(reinterpret_cast<const float4*>(ct + at + i)), d = __ldg(reinterpret_cast<const float4*>(st + at + i));
-          c[i] = a.x; c[i + 1] = a.y; c[i + 2] = a.z; c[i + 3] = a.w;
-          n[i] = sign * d.x; n[i + 1] = sign * d.y; n[i + 2] = sign * d.z; n[i + 3] = sign * d.w;
+          const float4 x = __ldg(reinterpret_cast<const float4*>(ct + at + i)), y = __ldg(reinterpret_cast<const float4*>(st + at + i));
+          a[i] = x.x; a[i + 1] = x.y; a[i + 2] = x.z; a[i + 3] = x.w;
+          d[i] = y.x; d[i + 1] = y.y; d[i + 2] = y.z; d[i + 3] = y.w;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          c[i] = a[HALF ? i : i / 2];
+          n[i] = (HALF ? e0 < half : (i & 1) == 0) ? -d[HALF ? i : i / 2] : d[HALF ? i : i / 2];
         }
       }
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const int e = e0 + i;
-        c[i] = 1.f;
-        n[i] = 0.f;
         if (e < p.rot) {
           const int at = HALF ? (e < half ? e : e - half) : e >> 1;
           const bool first = HALF ? e < half : (e & 1) == 0;
@@ -171,90 +231,90 @@ __global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(const RopeParams
         }
       }
     }
-
-    T* qo = static_cast<T*>(p.q_out) + b * p.qo_s[0] + s * p.qo_s[1] + e0;
-    T *ko = nullptr, *vo = nullptr;
-    int64_t ko_h, vo_h = 0;
-    const bool into_cache = CACHE && !pad && slot >= 0 && slot < p.capacity;
-    if constexpr (CACHE) {
-      const int64_t page = into_cache ? slot / p.page_size : 0, off = into_cache ? slot - page * p.page_size : 0;
-      ko = static_cast<T*>(p.kc) + page * p.kc_s[0] + off * p.kc_s[2] + e0;
-      vo = static_cast<T*>(p.vc) + page * p.vc_s[0] + off * p.vc_s[2] + e0;
-      ko_h = p.kc_s[1];
-      vo_h = p.vc_s[1];
-    } else {
-      ko = static_cast<T*>(p.k_out) + b * p.ko_s[0] + s * p.ko_s[1] + e0;
-      ko_h = p.ko_s[2];
+    F2 cw[4], nw[4];
+    {
+      float wp[8];              // the partner's weight
+      if constexpr (HALF && TAB) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) wp[i] = __shfl_sync(0xffffffffu, w[i], partner);
+      } else if constexpr (HALF) {
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) row[gl * 9 + i] = w[i];
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int e = e0 + i, other = e < half ? e + half : e - half;
+          wp[i] = e < p.rot ? row[(other >> 3) * 9 + (other & 7)] : 0.f;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) wp[i] = w[i ^ 1];
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        cw[i] = F2(c[2 * i] * w[2 * i], c[2 * i + 1] * w[2 * i + 1]);
+        nw[i] = F2(n[2 * i] * wp[2 * i], n[2 * i + 1] * wp[2 * i + 1]);
+      }
     }
-
-    for (int r0 = part * groups; r0 < rows; r0 += step * U) {   // uniform over the warp
-      if (r0 + step * U < rows) fetch(next, r0 + step * U);
+    const float eps = wrong ? __int_as_float(0x7fc00000) : p.eps;
+    const bool partial = p.rot < p.hd;                     // some values are kept: not even touched by a partner's inf or NaN
+    for (int r0 = part * groups; r0 < rows; r0 += step * U, r += step * U) {   // uniform over the warp
+      if (r0 + step * U < rows) fetch(next, r + step * U);
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         if (r0 + u * step >= rows) break;                  // uniform over the warp
-        const int r = r0 + u * step + grp;
-        const bool is_q = r < p.Hq, is_v = CACHE && r >= p.Hq + p.Hkv;
-        float y[8], z[8];
-        raw[u].get(y);
-        float inv = 1.f;
-        if (p.norm) {
-          float ss = 0.f;
+        float x[8], y[8];
+        raw[u].get(x);
+        F2 x2[4];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) ss = fmaf(y[i], y[i], ss);
+        for (int i = 0; i < 4; ++i) x2[i] = F2(x[2 * i], x[2 * i + 1]);
+        float inv = wrong ? eps : 1.f;
+        if (p.norm) {
+          F2 ss = mul2(x2[0], x2[0]);
+#pragma unroll
+          for (int i = 1; i < 4; ++i) ss = fma2(x2[i], x2[i], ss);
+          float sa, sb;
+          ss.get(sa, sb);
+          sa += sb;
 #pragma unroll
           for (int o = 16; o > 0; o >>= 1)
-            if (o < LG) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-          inv = rsqrtf(ss * p.norm_c + p.eps);
+            if (o < LG) sa += __shfl_xor_sync(0xffffffffu, sa, o);
+          inv = rsqrtf(fmaf(sa, p.norm_c, eps));
         }
-        if (wrong) inv = __int_as_float(0x7fc00000);
-        const float4* w4 = reinterpret_cast<const float4*>(s_w[is_q ? 0 : 1] + e0);
-        const float4 wa = w4[0], wb = w4[1];
-        const float w[8] = {wa.x, wa.y, wa.z, wa.w, wb.x, wb.y, wb.z, wb.w};
-#pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] *= inv * w[i];
         if constexpr (HALF && TAB) {
-          const int away = half >> 3;                      // lanes between partners
-          const int partner = turn ? (e0 < half ? lane + away : lane - away) : lane;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float other = __shfl_sync(0xffffffffu, y[i], partner);
-            z[i] = turn ? fmaf(y[i], c[i], other * n[i]) : y[i];
-          }
+          for (int i = 0; i < 8; ++i) y[i] = __shfl_sync(0xffffffffu, x[i], partner);
         } else if constexpr (HALF) {
           __syncwarp();                                    // the row before this one has been read
 #pragma unroll
-          for (int i = 0; i < 8; ++i) row[gl * 9 + i] = y[i];
+          for (int i = 0; i < 8; ++i) row[gl * 9 + i] = x[i];
           __syncwarp();
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            const int e = e0 + i;
-            const int other = e < half ? e + half : e - half;
-            z[i] = e < p.rot ? fmaf(y[i], c[i], row[(other >> 3) * 9 + (other & 7)] * n[i]) : y[i];
+            const int e = e0 + i, other = e < half ? e + half : e - half;
+            y[i] = e < p.rot ? row[(other >> 3) * 9 + (other & 7)] : 0.f;
           }
         } else {
 #pragma unroll
-          for (int i = 0; i < 8; i += 2) {
-            const float cc = TAB ? c[i / 2] : c[i], first = TAB ? -n[i / 2] : n[i], second = TAB ? n[i / 2] : n[i + 1];
-            const bool in = TAB ? turn : e0 + i < p.rot;   // rot is even: a pair is turned or kept as a whole
-            z[i] = in ? fmaf(y[i], cc, y[i + 1] * first) : y[i];
-            z[i + 1] = in ? fmaf(y[i + 1], cc, y[i] * second) : y[i + 1];
-          }
+          for (int i = 0; i < 8; ++i) y[i] = x[i ^ 1];
         }
-        if (r < rows && mine > 0) {
-          if (pad) {
+        const F2 inv2(inv, inv);
+        float z[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) z[i] = 0.f;
-          }
-          if (is_q) {
-            store8<T, VEC>(qo + (int64_t)r * p.qo_s[2], mine, z);
-          } else if (!CACHE) {
-            store8<T, VEC>(ko + (int64_t)(r - p.Hq) * ko_h, mine, z);
-          } else if (into_cache) {
-            if (is_v) raw[u].copy(vo + (int64_t)(r - p.Hq - p.Hkv) * vo_h, mine);
-            else store8<T, VEC>(ko + (int64_t)(r - p.Hq) * ko_h, mine, z);
+        for (int i = 0; i < 4; ++i) {
+          const F2 a = mul2(x2[i], cw[i]);
+          mul2(fma2(F2(y[2 * i], y[2 * i + 1]), nw[i], a), inv2).get(z[2 * i], z[2 * i + 1]);
+          if (partial) {
+            float k0, k1;
+            mul2(a, inv2).get(k0, k1);
+            if (TAB ? !turn : e0 + 2 * i >= p.rot) z[2 * i] = k0;
+            if (TAB ? !turn : e0 + 2 * i + 1 >= p.rot) z[2 * i + 1] = k1;
           }
         }
+        if (r + u * step < rows && mine > 0) store8<T, VEC>(dst + u * out_step, mine, z);
       }
+      dst += U * out_step;
 #pragma unroll
       for (int u = 0; u < U; ++u) raw[u] = next[u];
     }
@@ -266,7 +326,7 @@ int launch_as(const RopeParams& p, cudaStream_t st) {
   int dev = 0, sms = 0;
   HB_CUDA(cudaGetDevice(&dev));
   HB_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
-  int64_t grid = ceil_div64(p.tokens * p.parts, kThreads / 32);
+  int64_t grid = ceil_div64(p.tokens * (p.q_parts + p.kv_parts * (CACHE ? 2 : 1)), kThreads / 32);
   if (grid > (int64_t)sms * 16) grid = (int64_t)sms * 16;
   qk_norm_rope_kernel<T, VEC, TAB, HALF, CACHE><<<(unsigned)grid, kThreads, HALF && !TAB ? kThreads * 9 * 4 : 0, st>>>(p);
   HB_LAUNCH_CHECK();
@@ -344,10 +404,18 @@ extern "C" int hb200_qk_norm_rope(const hb200_qk_norm_rope_args* a, const hb200_
   }
   p.group_lanes = 1;
   while (p.group_lanes * 8 < p.hd) p.group_lanes <<= 1;
-  // a token's head rows are shared out over `parts` warps until about 16 warps per SM have work
-  const int rows = a->Hq + a->Hkv * (c ? 2 : 1), groups = 32 / p.group_lanes;
-  p.parts = 1;
-  while (tokens * p.parts < 148 * 16 && p.parts * groups < rows) p.parts <<= 1;
+  // a token's head rows are shared out over more warps until about 16 warps per SM have work
+  const int groups = 32 / p.group_lanes, kinds = c ? 2 : 1;
+  p.q_parts = a->Hq ? 1 : 0;
+  p.kv_parts = a->Hkv ? 1 : 0;
+  for (bool more = true; more && tokens * (p.q_parts + kinds * p.kv_parts) < 148 * 16;) {
+    const bool q_first = p.q_parts * groups < a->Hq && (int64_t)p.kv_parts * a->Hq >= (int64_t)p.q_parts * a->Hkv;
+    more = true;
+    if (q_first) p.q_parts *= 2;
+    else if (p.kv_parts * groups < a->Hkv) p.kv_parts *= 2;
+    else if (p.q_parts * groups < a->Hq) p.q_parts *= 2;
+    else more = false;
+  }
   const bool tab = a->rot % (a->layout == HB200_ROPE_HALF ? 16 : 8) == 0 && a->table_ld % 4 == 0 && aligned16(a->cos) && aligned16(a->sin);
   cudaStream_t st = (cudaStream_t)stream;
   const bool half = a->layout == HB200_ROPE_HALF;
