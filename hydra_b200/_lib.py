@@ -63,7 +63,7 @@ class PagedCache(C.Structure):
 
 class QkNormRopeArgs(C.Structure):
     _fields_ = [(n, c_vp) for n in ("q", "k", "v", "q_out", "k_out", "slots", "positions", "cos", "sin", "q_weight", "k_weight")] + [
-        (n, c_i64 * 3) for n in ("q_stride", "k_stride", "v_stride", "q_out_stride", "k_out_stride")] + [
+        (f"{t}_stride_{d}", c_i64) for t in ("q", "k", "v", "q_out", "k_out") for d in ("batch", "token", "head")] + [   # int64 [3] each
         (n, c_i64) for n in ("positions_stride", "table_rows", "table_ld")] + [
         (n, C.c_int32) for n in ("positions_64", "B", "S", "Hq", "Hkv", "hd", "rot", "layout", "norm", "dtype")] + [
         (n, c_f32) for n in ("eps", "q_scale", "k_scale")]

@@ -4,8 +4,8 @@
 //   y = x * rsqrt(c * sum x^2 + eps) * w * s      (c = 1/hd: rms; c = 1: l2; no norm: y = x * s)
 //   pairs (i, i + rot/2) or (2i, 2i + 1) of the first rot values:  (y1 cos - y2 sin, y1 sin + y2 cos)
 //
-// Bound: HBM (each head row read once, written once; 32 bits from the load to the one rounding at the store).  A warp takes
-// one token's queries, keys or values (or a part of them where there are few tokens).  A group of lanes holds one head row,
+// Bound: HBM (each head row read once, written once; 32 bits from the load to the one rounding at the store).  A group of
+// lanes takes one token's queries, keys or values (or a part of them where there are few tokens), head row after head row,
 // 8 values per lane through 16-byte accesses (or value by value where sizes, strides or pointers are no multiples of 16
 // bytes).  A lane keeps the same place in the row for all heads, so the products of the token's cosines and sines with the
 // weights sit in its registers, and a head row costs two packed products and a fused one per pair of values; the norm's factor is
@@ -29,6 +29,7 @@ struct RopeParams {
   int64_t qo_s[3], ko_s[3];
   int64_t kc_s[3], vc_s[3];              // page, head, row
   int64_t tokens, pos_sb, table_ld, table_rows, capacity;
+  int64_t q_warps, kv_warps;             // warps' worth of query items, of key (and of value) items
   int S, Hq, Hkv, hd, rot, page_size, group_lanes, q_parts, kv_parts, pos64;
   float norm_c, eps, q_scale, k_scale;
   int norm;
@@ -51,6 +52,11 @@ struct Raw {
 #pragma unroll
     for (int i = 0; i < 8; ++i) f[i] = Cvt<T>::to_f(e[i]);
   }
+  __device__ __forceinline__ void set(const float (&f)[8]) {
+    T* e = reinterpret_cast<T*>(v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) e[i] = Cvt<T>::from_f(f[i]);
+  }
   __device__ __forceinline__ void copy(T* p, int) const {
 #pragma unroll
     for (int j = 0; j < (int)sizeof(T) / 2; ++j) reinterpret_cast<uint4*>(p)[j] = v[j];
@@ -71,21 +77,16 @@ struct Raw<T, false> {
 #pragma unroll
     for (int i = 0; i < 8; ++i) f[i] = Cvt<T>::to_f(v[i]);
   }
+  __device__ __forceinline__ void set(const float (&f)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = Cvt<T>::from_f(f[i]);
+  }
   __device__ __forceinline__ void copy(T* p, int n) const {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
       if (i < n) p[i] = v[i];
   }
 };
-template <typename T, bool VEC>
-__device__ __forceinline__ void store8(T* p, int n, const float (&f)[8]) {
-  Raw<T, VEC> r;
-  T* e = reinterpret_cast<T*>(r.v);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) e[i] = Cvt<T>::from_f(f[i]);
-  r.copy(p, n);
-}
-
 // Two 32-bit values in one operation.
 struct F2 {
   uint64_t v;
@@ -117,27 +118,30 @@ __global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(const RopeParams
   const int mine = p.hd - e0 < 8 ? (p.hd - e0 > 0 ? p.hd - e0 : 0) : 8;
   const int half = p.rot >> 1;
   float* row = s_rows + (warp * groups + grp) * (LG * 9);
-  const int parts = p.q_parts + p.kv_parts * (CACHE ? 2 : 1);
   const bool turn = e0 < p.rot;                            // TAB: of all the lane's values
   const int partner = !turn ? lane : (e0 < half ? lane + (half >> 3) : lane - (half >> 3));
 
-  const int64_t items = p.tokens * parts, stride = (int64_t)gridDim.x * (kThreads / 32);
-  for (int64_t item = (int64_t)blockIdx.x * (kThreads / 32) + warp; item < items; item += stride) {
-    const int64_t tok = item / parts;
-    int part = (int)(item - tok * parts);                  // which share of the token's heads
-    const int kind = part < p.q_parts ? 0 : (part < p.q_parts + p.kv_parts ? 1 : 2);
-    part -= kind == 0 ? 0 : (kind == 1 ? p.q_parts : p.q_parts + p.kv_parts);
-    const int rows = kind == 0 ? p.Hq : p.Hkv, step = groups * (kind == 0 ? p.q_parts : p.kv_parts);
+  // items: first all tokens' queries, then keys, then values; a warp's groups take neighbouring tokens and one kind
+  const int64_t warps = p.q_warps + p.kv_warps * (CACHE ? 2 : 1), stride = (int64_t)gridDim.x * (kThreads / 32);
+  for (int64_t wi = (int64_t)blockIdx.x * (kThreads / 32) + warp; wi < warps; wi += stride) {
+    const int kind = wi < p.q_warps ? 0 : (wi < p.q_warps + p.kv_warps ? 1 : 2);
+    const int step = kind == 0 ? p.q_parts : p.kv_parts;   // parts of a token's heads: a group takes every step-th row
+    const int64_t item = (wi - (kind == 0 ? 0 : (kind == 1 ? p.q_warps : p.q_warps + p.kv_warps))) * groups + grp;
+    int64_t tok = step == 1 ? item : item / step;
+    int r = (int)(item - tok * step);                      // this group's next head row
+    int rows = kind == 0 ? p.Hq : p.Hkv;
+    const int rounds = (rows + step - 1) / step;           // head rows per group, uniform over the warp
+    if (tok >= p.tokens) { tok = 0; rows = 0; }            // behind the last item: a group without rows
+    if (mine == 0) rows = 0;                               // a lane behind the head's end
     const int64_t b = tok < p.S ? 0 : tok / p.S, s = tok - b * p.S;
     const int64_t* in_s = kind == 0 ? p.q_s : (kind == 1 ? p.k_s : p.v_s);
-    int r = part * groups + grp;                           // this lane's head row
     const T* src = static_cast<const T*>(kind == 0 ? p.q : (kind == 1 ? p.k : p.v)) + b * in_s[0] + s * in_s[1] + r * in_s[2] + e0;
     const int64_t in_step = in_s[2] * step;
     Raw<T, VEC> raw[U], next[U];
     auto fetch = [&](Raw<T, VEC> (&x)[U], int r) {         // rows r, r + step, ... (src: row r)
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        if (r + u * step < rows && mine > 0) x[u].load(src + u * in_step, mine);
+        if (r + u * step < rows) x[u].load(src + u * in_step, mine);
         else x[u].clear();
       }
       src += U * in_step;
@@ -156,8 +160,9 @@ __global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(const RopeParams
     T* dst;
     int64_t out_step;
     if (CACHE && kind > 0) {
-      if (pad || slot < 0 || slot >= p.capacity) continue;
-      const int64_t page = slot / p.page_size, off = slot - page * p.page_size;
+      const bool there = !pad && slot >= 0 && slot < p.capacity;
+      if (!there) rows = 0;
+      const int64_t page = there ? slot / p.page_size : 0, off = there ? slot - page * p.page_size : 0;
       const int64_t* out_s = kind == 1 ? p.kc_s : p.vc_s;
       dst = static_cast<T*>(kind == 1 ? p.kc : p.vc) + page * out_s[0] + r * out_s[1] + off * out_s[2] + e0;
       out_step = out_s[1] * step;
@@ -166,13 +171,12 @@ __global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(const RopeParams
       dst = static_cast<T*>(kind == 0 ? p.q_out : p.k_out) + b * out_s[0] + s * out_s[1] + r * out_s[2] + e0;
       out_step = out_s[2] * step;
     }
-    if ((CACHE && kind == 2) || pad) {                     // values go as they are; padding as zeros
-      for (int r0 = part * groups; r0 < rows; r0 += step * U, r += step * U) {   // uniform over the warp
-        if (r0 + step * U < rows) fetch(next, r + step * U);
+    if (CACHE && kind == 2) {                              // values go as they are
+      for (int i0 = 0; i0 < rounds; i0 += U, r += step * U) {
+        if (i0 + U < rounds) fetch(next, r + step * U);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-          if (pad) raw[u].clear();
-          if (r + u * step < rows && mine > 0) raw[u].copy(dst + u * out_step, mine);
+          if (r + u * step < rows) raw[u].copy(dst + u * out_step, mine);
           raw[u] = next[u];
         }
         dst += U * out_step;
@@ -181,7 +185,7 @@ __global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(const RopeParams
     }
 
     // cw, nw: z_i = (x_i cw_i + x_partner nw_i) * factor of the norm
-    const int64_t tr = wrong ? 0 : pos;
+    const int64_t tr = wrong || pad ? 0 : pos;
     const float* ct = p.cos_t + tr * p.table_ld;
     const float* st = p.sin_t + tr * p.table_ld;
     const float* wt = kind == 0 ? p.wq : p.wk;
@@ -259,11 +263,11 @@ __global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(const RopeParams
     }
     const float eps = wrong ? __int_as_float(0x7fc00000) : p.eps;
     const bool partial = p.rot < p.hd;                     // some values are kept: not even touched by a partner's inf or NaN
-    for (int r0 = part * groups; r0 < rows; r0 += step * U, r += step * U) {   // uniform over the warp
-      if (r0 + step * U < rows) fetch(next, r + step * U);
+    for (int i0 = 0; i0 < rounds; i0 += U, r += step * U) {
+      if (i0 + U < rounds) fetch(next, r + step * U);
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        if (r0 + u * step >= rows) break;                  // uniform over the warp
+        if (i0 + u >= rounds) break;
         float x[8], y[8];
         raw[u].get(x);
         F2 x2[4];
@@ -312,7 +316,12 @@ __global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(const RopeParams
             if (TAB ? !turn : e0 + 2 * i + 1 >= p.rot) z[2 * i + 1] = k1;
           }
         }
-        if (r + u * step < rows && mine > 0) store8<T, VEC>(dst + u * out_step, mine, z);
+        if (r + u * step < rows) {
+          Raw<T, VEC> packed;
+          packed.set(z);
+          if (pad) packed.clear();
+          packed.copy(dst + u * out_step, mine);
+        }
       }
       dst += U * out_step;
 #pragma unroll
@@ -326,7 +335,7 @@ int launch_as(const RopeParams& p, cudaStream_t st) {
   int dev = 0, sms = 0;
   HB_CUDA(cudaGetDevice(&dev));
   HB_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
-  int64_t grid = ceil_div64(p.tokens * (p.q_parts + p.kv_parts * (CACHE ? 2 : 1)), kThreads / 32);
+  int64_t grid = ceil_div64(p.q_warps + p.kv_warps * (CACHE ? 2 : 1), kThreads / 32);
   if (grid > (int64_t)sms * 16) grid = (int64_t)sms * 16;
   qk_norm_rope_kernel<T, VEC, TAB, HALF, CACHE><<<(unsigned)grid, kThreads, HALF && !TAB ? kThreads * 9 * 4 : 0, st>>>(p);
   HB_LAUNCH_CHECK();
@@ -359,7 +368,7 @@ extern "C" int hb200_qk_norm_rope(const hb200_qk_norm_rope_args* a, const hb200_
              "qk_norm_rope: %d rotated values of a head of %d (an even number within the head)", a->rot, a->hd);
   HB_REQUIRE(a->layout == HB200_ROPE_INTERLEAVED || a->layout == HB200_ROPE_HALF, HB200_ERR_INVALID, "qk_norm_rope: unknown layout %d", a->layout);
   HB_REQUIRE(a->norm >= HB200_NORM_NONE && a->norm <= HB200_NORM_L2, HB200_ERR_INVALID, "qk_norm_rope: unknown norm %d", a->norm);
-  HB_REQUIRE(a->table_rows >= 0 && a->table_ld >= a->rot / 2, HB200_ERR_INVALID, "qk_norm_rope: bad table shape");
+  HB_REQUIRE(a->table_rows >= (a->rot > 0 ? 1 : 0) && a->table_ld >= a->rot / 2, HB200_ERR_INVALID, "qk_norm_rope: bad table shape");
   HB_REQUIRE(a->positions || a->S <= a->table_rows, HB200_ERR_INVALID, "qk_norm_rope: tables of %lld rows for %d positions",
              (long long)a->table_rows, a->S);
   const int64_t tokens = (int64_t)a->B * a->S;
@@ -404,17 +413,17 @@ extern "C" int hb200_qk_norm_rope(const hb200_qk_norm_rope_args* a, const hb200_
   }
   p.group_lanes = 1;
   while (p.group_lanes * 8 < p.hd) p.group_lanes <<= 1;
-  // a token's head rows are shared out over more warps until about 16 warps per SM have work
+  // a token's head rows are shared out over more groups of lanes until about 16 warps per SM have work
   const int groups = 32 / p.group_lanes, kinds = c ? 2 : 1;
-  p.q_parts = a->Hq ? 1 : 0;
-  p.kv_parts = a->Hkv ? 1 : 0;
-  for (bool more = true; more && tokens * (p.q_parts + kinds * p.kv_parts) < 148 * 16;) {
-    const bool q_first = p.q_parts * groups < a->Hq && (int64_t)p.kv_parts * a->Hq >= (int64_t)p.q_parts * a->Hkv;
-    more = true;
-    if (q_first) p.q_parts *= 2;
-    else if (p.kv_parts * groups < a->Hkv) p.kv_parts *= 2;
-    else if (p.q_parts * groups < a->Hq) p.q_parts *= 2;
-    else more = false;
+  p.q_parts = p.kv_parts = 1;
+  auto count = [&]() {
+    p.q_warps = a->Hq ? ceil_div64(tokens * p.q_parts, groups) : 0;
+    p.kv_warps = a->Hkv ? ceil_div64(tokens * p.kv_parts, groups) : 0;
+    return p.q_warps + kinds * p.kv_warps;
+  };
+  while (count() < 148 * 16 && (p.q_parts < a->Hq || p.kv_parts < a->Hkv)) {
+    const bool q_more = p.q_parts < a->Hq && (p.kv_parts >= a->Hkv || (int64_t)p.kv_parts * a->Hq >= (int64_t)p.q_parts * a->Hkv);
+    (q_more ? p.q_parts : p.kv_parts) *= 2;
   }
   const bool tab = a->rot % (a->layout == HB200_ROPE_HALF ? 16 : 8) == 0 && a->table_ld % 4 == 0 && aligned16(a->cos) && aligned16(a->sin);
   cudaStream_t st = (cudaStream_t)stream;

@@ -14,7 +14,6 @@ a CUDA device (a CPU tensor raises instead of silently taking a PyTorch path), t
 """
 from __future__ import annotations
 
-import ctypes as C
 from contextlib import nullcontext
 from typing import Optional, Tuple
 
@@ -49,10 +48,10 @@ def _dtype_code(t: Tensor) -> int:
 def _require_cuda(*ts: Tensor) -> torch.device:
     dev = ts[0].device
     for t in ts:
-        if not t.is_cuda:
-            raise RuntimeError("hydra_b200 kernels run on CUDA tensors only (there is no CPU fallback); "
-                               f"got a tensor on {t.device}")
-        if t.device != dev:
+        if t.device != dev or not t.is_cuda:
+            if not t.is_cuda:
+                raise RuntimeError("hydra_b200 kernels run on CUDA tensors only (there is no CPU fallback); "
+                                   f"got a tensor on {t.device}")
             raise RuntimeError(f"hydra_b200: tensors on different devices ({dev} and {t.device})")
     return dev
 
@@ -63,7 +62,9 @@ def _on(dev: torch.device):
 
 
 def _stream(dev: torch.device) -> int:
-    return torch.cuda.current_stream(dev).cuda_stream
+    """The device's current stream as the handle that the C entries take (its raw form: building the torch.cuda.Stream
+    object around it costs 2 us a call)."""
+    return torch._C._cuda_getCurrentRawStream(dev.index)
 
 
 # ----------------------------------------------------------------------------- custom ops
@@ -217,9 +218,6 @@ def _fp32(what: str, t: Optional[Tensor], n: int, dev: torch.device) -> Optional
     return t if t.dtype == torch.float32 and t.is_contiguous() else t.float().contiguous()
 
 
-_Strides = C.c_int64 * 3
-
-
 def _qk_norm_rope(what: str, dev: torch.device, q: Tensor, k: Tensor, cos: Tensor, sin: Tensor, positions: Optional[Tensor],
                   q_weight: Optional[Tensor], k_weight: Optional[Tensor], norm: Optional[str], eps: float, q_scale: float,
                   k_scale: float, layout: str, v: Optional[Tensor] = None, slots: Optional[Tensor] = None, cache=None):
@@ -229,51 +227,56 @@ def _qk_norm_rope(what: str, dev: torch.device, q: Tensor, k: Tensor, cos: Tenso
         raise ValueError(f"{what}: norm must be 'rms', 'l2' or None, got {norm!r}")
     if layout not in _lib.ROPE_LAYOUTS:
         raise ValueError(f"{what}: layout must be 'interleaved' or 'half', got {layout!r}")
-    hd = q.shape[-1]
+    dtype, shape = _dtype_code(q), q.shape
+    hd = shape[-1]
     if cos.dim() == 4:
         cos, sin = cos[0, 0], sin[0, 0]
     if cos.dim() != 2 or sin.shape != cos.shape or 2 * cos.shape[1] > hd:
         raise ValueError(f"{what}: cos and sin must be [rows, rotated / 2] with rotated <= {hd}, got {tuple(cos.shape)} and {tuple(sin.shape)}")
-    if cos.dtype != torch.float32 or sin.dtype != torch.float32 or cos.stride() != sin.stride() or cos.stride(1) != 1 or cos.stride(0) < cos.shape[1]:
+    table_rows, half = cos.shape
+    table_ld, unit = cos.stride()
+    if cos.dtype != torch.float32 or sin.dtype != torch.float32 or sin.stride() != (table_ld, unit) or unit != 1 or table_ld < half:
         cos, sin = cos.float().contiguous(), sin.float().contiguous()
-    q = q if q.stride(-1) == 1 else q.contiguous()
-    k = k if k.stride(-1) == 1 else k.contiguous()
-    if q.dim() == 3:
-        B, S = 1, q.shape[0]
-        strides = lambda t: _Strides(0, t.stride(0), t.stride(1))   # noqa: E731
-    else:
-        B, S = q.shape[0], q.shape[2]
-        strides = lambda t: _Strides(t.stride(0), t.stride(2), t.stride(1))   # noqa: E731
+        table_ld = half
+    qs, ks, vs = q.stride(), k.stride(), (0, 0, 0, 1) if v is None else v.stride()
+    if qs[-1] != 1 or ks[-1] != 1 or vs[-1] != 1:
+        q, k, v = q.contiguous(), k.contiguous(), None if v is None else v.contiguous()
+        qs, ks, vs = q.stride(), k.stride(), (0, 0, 0, 1) if v is None else v.stride()
+    q_out = torch.empty(shape, dtype=q.dtype, device=dev)
+    k_out = torch.empty(k.shape, dtype=q.dtype, device=dev) if cache is None else None
+    qos, kos = q_out.stride(), (0, 0, 0, 1) if k_out is None else k_out.stride()
+    if len(shape) == 3:                       # tokens, heads -> batch, tokens, heads
+        B, S, Hq, Hkv = 1, shape[0], shape[1], k.shape[1]
+        strides = (0, qs[0], qs[1], 0, ks[0], ks[1], 0, vs[0], vs[1], 0, qos[0], qos[1], 0, kos[0], kos[1])
+    else:                                     # batch, heads, tokens
+        B, Hq, S, _ = shape
+        Hkv = k.shape[1]
+        strides = (qs[0], qs[2], qs[1], ks[0], ks[2], ks[1], 0, 0, 0, qos[0], qos[2], qos[1], kos[0], kos[2], kos[1])
+    where, where_64, where_stride = None, 0, 0
     if positions is not None:
         if positions.dtype not in (torch.int32, torch.int64):
             raise TypeError(f"{what}: positions must be int32 or int64, got {positions.dtype}")
         if positions.shape != (S,) and positions.shape != (B, S):
             raise ValueError(f"{what}: positions {tuple(positions.shape)} for {B} x {S} tokens")
-        positions = positions if S < 2 or positions.stride(-1) == 1 else positions.contiguous()
-    elif cos.shape[0] < S:
+        if S > 1 and positions.stride(-1) != 1:
+            positions = positions.contiguous()
+        where, where_64 = positions.data_ptr(), int(positions.dtype == torch.int64)
+        where_stride = positions.stride(0) if positions.dim() == 2 else 0
+    elif table_rows < S:
         raise ValueError(f"{what}: tables {tuple(cos.shape)} do not cover {S} positions")
-    q_weight = _fp32(f"{what}: q_weight", q_weight, hd, dev)
-    k_weight = _fp32(f"{what}: k_weight", k_weight, hd, dev)
-    q_out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    k_out = torch.empty(k.shape, dtype=k.dtype, device=dev) if cache is None else None
-    if q.numel() + k.numel() == 0:
+    if q_weight is not None:
+        q_weight = _fp32(f"{what}: q_weight", q_weight, hd, dev)
+    if k_weight is not None:
+        k_weight = _fp32(f"{what}: k_weight", k_weight, hd, dev)
+    if (Hq + Hkv) * B * S * hd == 0:
         return q_out, k_out
-    if v is not None and v.stride(-1) != 1:
-        v = v.contiguous()
-    args = _lib.QkNormRopeArgs(
-        q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr() if v is not None else None, q_out=q_out.data_ptr(),
-        k_out=k_out.data_ptr() if k_out is not None else None, slots=slots.data_ptr() if slots is not None else None,
-        positions=positions.data_ptr() if positions is not None else None, cos=cos.data_ptr(), sin=sin.data_ptr(),
-        q_weight=q_weight.data_ptr() if q_weight is not None else None, k_weight=k_weight.data_ptr() if k_weight is not None else None,
-        q_stride=strides(q), k_stride=strides(k), v_stride=strides(v) if v is not None else _Strides(),
-        q_out_stride=strides(q_out), k_out_stride=strides(k_out) if k_out is not None else _Strides(),
-        positions_stride=positions.stride(0) if positions is not None and positions.dim() == 2 else 0,
-        table_rows=cos.shape[0], table_ld=cos.stride(0) if cos.shape[0] > 1 else cos.shape[1],
-        positions_64=int(positions is not None and positions.dtype == torch.int64), B=B, S=S, Hq=q.shape[1], Hkv=k.shape[1],
-        hd=hd, rot=2 * cos.shape[1], layout=_lib.ROPE_LAYOUTS[layout], norm=_lib.QK_NORMS[norm], dtype=_dtype_code(q),
-        eps=float(eps), q_scale=float(q_scale), k_scale=float(k_scale))
+    args = _lib.QkNormRopeArgs(                # in the order of the struct
+        q.data_ptr(), k.data_ptr(), None if v is None else v.data_ptr(), q_out.data_ptr(), None if k_out is None else k_out.data_ptr(),
+        None if slots is None else slots.data_ptr(), where, cos.data_ptr(), sin.data_ptr(), None if q_weight is None else q_weight.data_ptr(),
+        None if k_weight is None else k_weight.data_ptr(), *strides, where_stride, table_rows, table_ld, where_64, B, S, Hq, Hkv, hd,
+        2 * half, _lib.ROPE_LAYOUTS[layout], _lib.QK_NORMS[norm], dtype, eps, q_scale, k_scale)
     with _on(dev):
-        _lib.check(_lib.lib().hb200_qk_norm_rope(C.byref(args), C.byref(cache) if cache is not None else None, _stream(dev)), what)
+        _lib.check(_lib.lib().hb200_qk_norm_rope(args, cache, _stream(dev)), what)
     return q_out, k_out
 
 

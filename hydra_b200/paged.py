@@ -15,7 +15,6 @@ cache.  They are inference only and refuse tensors that autograd would record.
 """
 from __future__ import annotations
 
-import ctypes as C
 import math
 from typing import NamedTuple, Optional, Tuple, Union
 
@@ -78,9 +77,11 @@ def paged_plan(context_lens: Tensor, new_lens: Tensor, block_tables: Tensor, fre
     if free_start is not None:
         if free_start.device != dev or free_start.dtype != torch.int32 or free_start.numel() != 1:
             raise ValueError("paged_plan: free_start must be one int32 on the tables' device")
-    i32 = dict(dtype=torch.int32, device=dev)
-    plan = PagedPlan(torch.empty(B, **i32), torch.empty(B + 1, **i32), torch.empty(room, **i32),
-                     torch.empty(room, dtype=torch.int64, device=dev), torch.empty(1, **i32), torch.empty(1, **i32))
+    # one allocation for the five small arrays: positions first (16-byte aligned, as the kernel stores them)
+    head = (room + 3) // 4 * 4
+    positions, kv_lens, cu_new, start_out, status = torch.empty(head + 2 * B + 3, dtype=torch.int32, device=dev).split([head, B, B + 1, 1, 1])
+    plan = PagedPlan(kv_lens, cu_new, positions if head == room else positions[:room], torch.empty(room, dtype=torch.int64, device=dev), start_out,
+                     status)
     with kernels._on(dev):
         _lib.check(_lib.lib().hb200_paged_plan(
             context_lens.data_ptr(), new_lens.data_ptr(), B, block_tables.data_ptr(), block_tables.stride(0) if B > 1 else width, width,
@@ -100,9 +101,8 @@ def _cache(what: str, k_cache: Tensor, v_cache: Tensor) -> _lib.PagedCache:
         raise ValueError(f"{what}: a head's row in the cache must be contiguous")
     if k_cache.numel() == 0:
         raise ValueError(f"{what}: an empty cache {tuple(k_cache.shape)}")
-    return _lib.PagedCache(k=k_cache.data_ptr(), v=v_cache.data_ptr(), k_stride_page=ks[0], k_stride_head=ks[1], k_stride_row=ks[2],
-                           v_stride_page=vs[0], v_stride_head=vs[1], v_stride_row=vs[2], num_pages=pages, page_size=rows,
-                           n_kv_heads=heads, head_dim=hd, dtype=kernels._dtype_code(k_cache))
+    return _lib.PagedCache(k_cache.data_ptr(), v_cache.data_ptr(), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], pages, rows, heads, hd,
+                           kernels._dtype_code(k_cache))   # in the order of the struct
 
 
 def paged_append(q: Tensor, k: Tensor, v: Tensor, k_cache: Tensor, v_cache: Tensor, slots: Tensor, cos: Tensor, sin: Tensor,
@@ -161,7 +161,8 @@ def paged_decode_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_ta
     block_tables = _ints("paged_decode_attention: block_tables", block_tables, torch.int32, 2)
     if kv_lens.shape[0] != B or block_tables.shape[0] != B:
         raise ValueError(f"paged_decode_attention: {B} queries, {kv_lens.shape[0]} lengths, {block_tables.shape[0]} table rows")
-    if any(s % 8 for s in (*k_cache.stride()[:3], *v_cache.stride()[:3])) or k_cache.data_ptr() % 16 or v_cache.data_ptr() % 16:
+    if (cache.k_stride_page | cache.k_stride_head | cache.k_stride_row | cache.v_stride_page | cache.v_stride_head | cache.v_stride_row) % 8 \
+            or (cache.k | cache.v) % 16:
         raise ValueError("paged_decode_attention: the rows of the caches must begin on 16-byte boundaries")
     scale = hd ** -0.5 if scale is None else float(scale)
     if not math.isfinite(scale):
@@ -180,7 +181,7 @@ def paged_decode_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_ta
             n = L.hb200_paged_attention_workspace_bytes(B, Hq, k_cache.shape[1], hd)
             ws = torch.empty(max(n, 16), dtype=torch.uint8, device=dev)
             _lib.check(L.hb200_paged_decode_attention(
-                C.byref(cache), q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), lse.data_ptr() if return_lse else None,
+                cache, q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), lse.data_ptr() if return_lse else None,
                 block_tables.data_ptr(), block_tables.shape[1], block_tables.shape[1], kv_lens.data_ptr(), B, Hq, scale,
                 ws.data_ptr(), n, kernels._stream(dev)), "paged_decode_attention")
     return (out, lse) if return_lse else out

@@ -56,9 +56,8 @@ def test_paged_attention_without_requests_is_nothing():
 
 
 def _rope(cache=None, **kw):
-    s = (C.c_int64 * 3)(0, 512, 64)
-    d = dict(q=P, k=P, v=P, q_out=P, k_out=P, slots=P, positions=P, cos=P, sin=P, q_stride=s, k_stride=s, v_stride=s, q_out_stride=s,
-             k_out_stride=s, table_rows=128, table_ld=32, B=1, S=4, Hq=8, Hkv=4, hd=64, rot=64, norm=1, dtype=_lib.HB200_BF16, eps=1e-6,
+    s = {f"{t}_stride_{d}": n for t in ("q", "k", "v", "q_out", "k_out") for d, n in (("batch", 0), ("token", 512), ("head", 64))}
+    d = dict(q=P, k=P, v=P, q_out=P, k_out=P, slots=P, positions=P, cos=P, sin=P, **s, table_rows=128, table_ld=32, B=1, S=4, Hq=8, Hkv=4, hd=64, rot=64, norm=1, dtype=_lib.HB200_BF16, eps=1e-6,
              q_scale=1.0, k_scale=1.0)
     a = _lib.QkNormRopeArgs(**{**d, **kw})
     return _lib.lib().hb200_qk_norm_rope(C.byref(a), C.byref(cache) if cache is not None else None, None)
@@ -66,7 +65,7 @@ def _rope(cache=None, **kw):
 
 @pytest.mark.parametrize("bad, status, text", [
     (dict(S=-1), -1, "bad shape"), (dict(hd=0), -1, "bad shape"), (dict(hd=257, rot=64), -4, "256"), (dict(rot=66), -1, "rotated"),
-    (dict(rot=33), -1, "rotated"), (dict(layout=2), -1, "layout"), (dict(norm=3), -1, "norm"), (dict(table_ld=31), -1, "table"),
+    (dict(rot=33), -1, "rotated"), (dict(layout=2), -1, "layout"), (dict(norm=3), -1, "norm"), (dict(table_ld=31), -1, "table"), (dict(table_rows=0), -1, "table"),
     (dict(positions=None, S=129), -1, "129"), (dict(q=None), -1, "null"), (dict(k_out=None), -1, "null"), (dict(cos=None), -1, "null"),
     (dict(dtype=7), -4, "dtype"), (dict(cache=_cache(), slots=None), -1, "null"), (dict(cache=_cache(n_kv_heads=2)), -1, "cache"),
     (dict(cache=_cache(head_dim=32)), -1, "cache"), (dict(cache=_cache(dtype=_lib.HB200_F16)), -1, "cache"),
