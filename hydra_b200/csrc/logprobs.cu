@@ -133,34 +133,46 @@ template <> struct Piece<__half> {
   __device__ float max() const { return fmaxf(__low2float(top), __high2float(top)); }
 };
 
-// Adds a value, or a piece's values, to the statistics.  -inf (and anything far below) counts as 2^-200 = 0 times a finite
-// distance; NaN and +inf stay NaN.
-__device__ __forceinline__ void take1(Stat& a, float v, float c) {
-  if (v > a.m) rebase(a, v, c);
-  const float t = max_nan((v - base_of(a.m)) * c, -200.f), e = ex2f(t);
-  a.s += e;
-  a.u = fmaf(t, e, a.u);
-}
-// (a.m is at least their maximum, NaN left out)
-template <int N>
-__device__ __forceinline__ void add(Stat& a, const float (&f)[N], F2 nb2, F2 c2) {
-  F2 s(a.s, 0.f), u(a.u, 0.f);
-#pragma unroll
-  for (int i = 0; i < N; i += 2) {
-    float t0, t1;
-    mul2(add2(F2(f[i], f[i + 1]), nb2), c2).get(t0, t1);
-    t0 = max_nan(t0, -200.f);
-    t1 = max_nan(t1, -200.f);
-    const F2 e(ex2f(t0), ex2f(t1));
-    s = add2(s, e);
-    u = fma2(F2(t0, t1), e, u);
+// What a thread keeps while it reads: its maximum and the sums of its even and of its odd columns.  -inf (and anything far
+// below) counts as 2^-200 = 0 times a finite distance; NaN and +inf stay NaN.
+struct Running {
+  float m;
+  F2 s, u;
+  __device__ Running() : m(-INFINITY), s(0.f, 0.f), u(0.f, 0.f) {}
+  __device__ __forceinline__ void raise(float to, float c) {   // the maximum (a NaN is none)
+    if (to > m) {
+      const float d = fmaxf((base_of(m) - base_of(to)) * c, -200.f), f = ex2f(d);
+      const F2 f2(f, f);
+      u = mul2(fma2(F2(d, d), s, u), f2);
+      s = mul2(s, f2);
+      m = to;
+    }
   }
-  float x, y;
-  s.get(x, y);
-  a.s = x + y;
-  u.get(x, y);
-  a.u = x + y;
-}
+  template <int N>
+  __device__ __forceinline__ void add(const float (&f)[N], F2 c2) {
+    const F2 nb2(-base_of(m), -base_of(m));
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+      float t0, t1;
+      mul2(add2(F2(f[i], f[i + 1]), nb2), c2).get(t0, t1);
+      t0 = max_nan(t0, -200.f);
+      t1 = max_nan(t1, -200.f);
+      const F2 e(ex2f(t0), ex2f(t1));
+      s = add2(s, e);
+      u = fma2(F2(t0, t1), e, u);
+    }
+  }
+  __device__ __forceinline__ Stat stat() const {
+    Stat r;
+    float x, y;
+    s.get(x, y);
+    r.s = x + y;
+    u.get(x, y);
+    r.u = x + y;
+    r.m = m;
+    return r;
+  }
+};
 
 // What a CTA of a cluster leaves for the first one.
 struct Partial {
@@ -196,8 +208,8 @@ __global__ void __launch_bounds__(NT) token_logprobs_kernel(const LogprobParams 
   const int head = min(n, to_boundary), pieces = (n - head) / V, edge = head + (n - head - pieces * V);
   const uint4* xv = reinterpret_cast<const uint4*>(x + head);
   auto edge_at = [&](int i) { return i < head ? i : pieces * V + i; };   // i-th value outside the pieces -> its column
-  Stat a = {-INFINITY, 0.f, 0.f};
   const F2 c2(c, c);
+  Running own;
   int v0 = tid;
   for (; v0 + (kUnroll - 1) * NT < pieces; v0 += kUnroll * NT) {   // four pieces, one look at their maximum
     uint4 raw[kUnroll];
@@ -206,10 +218,9 @@ __global__ void __launch_bounds__(NT) token_logprobs_kernel(const LogprobParams 
     float mx = Piece<T>(raw[0]).max();
 #pragma unroll
     for (int k = 1; k < kUnroll; ++k) mx = fmaxf(mx, Piece<T>(raw[k]).max());
-    if (mx > a.m) rebase(a, mx, c);
-    const F2 nb2(-base_of(a.m), -base_of(a.m));
+    own.raise(mx, c);
 #pragma unroll
-    for (int k = 0; k < kUnroll; ++k) add(a, Piece<T>(raw[k]).f, nb2, c2);
+    for (int k = 0; k < kUnroll; ++k) own.add(Piece<T>(raw[k]).f, c2);
   }
   {
     uint4 raw[kUnroll - 1];
@@ -220,15 +231,16 @@ __global__ void __launch_bounds__(NT) token_logprobs_kernel(const LogprobParams 
     for (int k = 0; k < kUnroll - 1; ++k)
       if (v0 + k * NT < pieces) {
         const Piece<T> q(raw[k]);
-        const float mx = q.max();
-        if (mx > a.m) rebase(a, mx, c);
-        const F2 nb2(-base_of(a.m), -base_of(a.m));
-        add(a, q.f, nb2, c2);
+        own.raise(q.max(), c);
+        own.add(q.f, c2);
       }
   }
   if (tid < edge) {   // fewer than 2 V <= NT of them
-    take1(a, Cvt<T>::to_f(x[edge_at(tid)]), c);
+    const float f = Cvt<T>::to_f(x[edge_at(tid)]), two[2] = {f, -INFINITY};
+    own.raise(f, c);
+    own.add(two, c2);
   }
+  Stat a = own.stat();
   const float own_max = a.m;
 
   // the slice's maximum (on the way those of the 64 groups of threads), then its sums relative to it

@@ -362,7 +362,9 @@ __global__ void __launch_bounds__(warps_of(HD) * 32, 1) paged_attention_kernel(c
       poison = false;
     }
     cp_async_wait<ST - 2>();
-    __syncwarp();
+    __syncwarp();                       // the tile has come for every lane, and every lane is done with the slot before it
+    issue(slot == 0 ? ST - 1 : slot - 1);
+    look();
     poison |= (bad_bits >> slot) & 1u;
     const uint32_t tile = ring_u + slot * STAGE;
 
@@ -456,9 +458,6 @@ __global__ void __launch_bounds__(warps_of(HD) * 32, 1) paged_attention_kernel(c
         }
       }
     }
-    __syncwarp();                       // every lane has read the slot before it is filled again
-    issue(slot == 0 ? ST - 1 : slot - 1);
-    look();
     slot = slot + 1 == ST ? 0 : slot + 1;
     --left;
 
@@ -507,8 +506,8 @@ __global__ void __launch_bounds__(warps_of(HD) * 32, 1) paged_attention_kernel(c
 // WPR warps per (request, query head): nothing where one share held the whole pair, zeros for an empty request, else the
 // parts' weighted sum.  A warp takes every WPR-th part, its statistics one per lane, its values four side by side per lane.
 template <typename T, int WPR>
-__global__ void __launch_bounds__(256) paged_join_kernel(const PagedParams p) {
-  constexpr int RPC = 8 / WPR;                  // rows per CTA
+__global__ void __launch_bounds__(WPR > 8 ? WPR * 32 : 256) paged_join_kernel(const PagedParams p) {
+  constexpr int RPC = WPR > 8 ? 1 : 8 / WPR;    // rows per CTA
   __shared__ __align__(16) float s_o[WPR > 1 ? WPR : 1][256];
   __shared__ float s_m[WPR], s_l[WPR];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, wi = warp % WPR;
@@ -559,7 +558,7 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedParams p) {
     a = scaled(a, f, zero);
     c = scaled(c, f, zero);
     const int here = min(32, (parts - i0 + WPR - 1) / WPR);
-#pragma unroll 4
+#pragma unroll 8
     for (int k = 0; k < here; ++k) {
       const float f = __shfl_sync(0xffffffffu, w, k);
       const float* o = p.part_o + at(i0 + k * WPR) * p.hd;
@@ -625,9 +624,9 @@ int launch(const PagedParams& p, int sms, cudaStream_t st) {
   auto kern = p.page_size % 16 == 0 ? paged_attention_kernel<T, HD, NQ, true> : paged_attention_kernel<T, HD, NQ, false>;
   HB_PROPAGATE(ensure_dynamic_smem((const void*)kern, smem));
   HB_PROPAGATE(launch_chained(kern, dim3((unsigned)sms), dim3(NW * 32), smem, st, false, 1, p));
-  // a warp per row, or eight where a row has many parts (few requests)
+  // a warp per row, or sixteen where a row has many parts (few requests)
   const int64_t rows = (int64_t)p.B * p.Hq;
-  if ((int64_t)p.B * p.Hkv * p.q_tiles * 8 <= p.workers) return launch_chained(paged_join_kernel<T, 8>, dim3((unsigned)rows), dim3(256), 0, st, true, 1, p);
+  if ((int64_t)p.B * p.Hkv * p.q_tiles * 8 <= p.workers) return launch_chained(paged_join_kernel<T, 16>, dim3((unsigned)rows), dim3(512), 0, st, true, 1, p);
   return launch_chained(paged_join_kernel<T, 1>, dim3((unsigned)ceil_div64(rows, 8)), dim3(256), 0, st, true, 1, p);
 }
 

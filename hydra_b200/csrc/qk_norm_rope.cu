@@ -35,6 +35,15 @@ struct RopeParams {
   int norm;
 };
 
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) { return pack_bf16x2_rn(a, b); }
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
 // Eight values of a row as they come from memory.
 template <typename T, bool VEC>
 struct Raw {
@@ -53,9 +62,14 @@ struct Raw {
     for (int i = 0; i < 8; ++i) f[i] = Cvt<T>::to_f(e[i]);
   }
   __device__ __forceinline__ void set(const float (&f)[8]) {
-    T* e = reinterpret_cast<T*>(v);
+    uint32_t* w = reinterpret_cast<uint32_t*>(v);
+    if constexpr (sizeof(T) == 4) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) e[i] = Cvt<T>::from_f(f[i]);
+      for (int i = 0; i < 8; ++i) w[i] = __float_as_uint(f[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = pack2<T>(f[2 * i], f[2 * i + 1]);
+    }
   }
   __device__ __forceinline__ void copy(T* p, int) const {
 #pragma unroll
