@@ -6,18 +6,19 @@
 //
 // Bound: HBM (each head row read once, written once; 32 bits from the load to the one rounding at the store).  A group of
 // lanes takes one token's queries, keys or values (or a part of them where there are few tokens), head row after head row,
-// 8 values per lane through 16-byte accesses (or value by value where sizes, strides or pointers are no multiples of 16
-// bytes).  A lane keeps the same place in the row for all heads, so the products of the token's cosines and sines with the
+// 8 values per lane through 16- or 8-byte accesses (or value by value where sizes, strides or pointers are no multiples of
+// 16 bytes).  A lane keeps the same place in the row for all heads, so the products of the token's cosines and sines with the
 // weights sit in its registers, and a head row costs two packed products and a fused one per pair of values; the norm's factor is
-// the same for the whole row and comes last.  Four head rows per group are in flight while four are computed.  The half layout
-// fetches the partner value from its lane where rot / 2 is a multiple of 8 values, else through shared memory (padded by one
-// word in eight: no bank conflicts), which works for every rot.
+// the same for the whole row and comes last.  Four head rows per group are in flight while four are computed.  In the half
+// layout a lane holds four values and their four partners where rot is a multiple of 8; else partners meet in shared memory.
 #include "common.cuh"
 
 namespace hb200 {
 namespace {
 
-constexpr int kThreads = 128;
+// A warp per CTA: nothing is shared between warps, and a finished one makes room at once (32768 tokens of 48 heads of 128: 133 us;
+// 64 threads: 142, 128: 144, 256: 163).
+constexpr int kThreads = 32;
 
 struct RopeParams {
   const void *q, *k, *v;
@@ -44,25 +45,32 @@ __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
   const __half2 h = __floats2half2_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
-// Eight values of a row as they come from memory.
-template <typename T, bool VEC>
+// Eight values of a row as they come from memory: one after another, or (SPLIT) four and four, `gap` apart.
+template <typename T, bool VEC, bool SPLIT>
 struct Raw {
-  uint4 v[sizeof(T) / 2];
-  __device__ __forceinline__ void load(const T* p, int) {
+  uint32_t w[2 * sizeof(T)];
+  __device__ __forceinline__ void load(const T* p, int gap, int) {
+    if constexpr (sizeof(T) == 4 || !SPLIT) {
 #pragma unroll
-    for (int j = 0; j < (int)sizeof(T) / 2; ++j) v[j] = __ldg(reinterpret_cast<const uint4*>(p) + j);
+      for (int j = 0; j < (int)sizeof(T) / 2; ++j) {
+        const uint4 v = __ldg(reinterpret_cast<const uint4*>(SPLIT && j ? p + gap : p) + (SPLIT ? 0 : j));
+        w[4 * j] = v.x; w[4 * j + 1] = v.y; w[4 * j + 2] = v.z; w[4 * j + 3] = v.w;
+      }
+    } else {
+      const uint2 a = __ldg(reinterpret_cast<const uint2*>(p)), b = __ldg(reinterpret_cast<const uint2*>(p + gap));
+      w[0] = a.x; w[1] = a.y; w[2] = b.x; w[3] = b.y;
+    }
   }
   __device__ __forceinline__ void clear() {
 #pragma unroll
-    for (int j = 0; j < (int)sizeof(T) / 2; ++j) v[j] = make_uint4(0, 0, 0, 0);
+    for (int j = 0; j < 2 * (int)sizeof(T); ++j) w[j] = 0;
   }
   __device__ __forceinline__ void get(float (&f)[8]) const {
-    const T* e = reinterpret_cast<const T*>(v);
+    const T* e = reinterpret_cast<const T*>(w);
 #pragma unroll
     for (int i = 0; i < 8; ++i) f[i] = Cvt<T>::to_f(e[i]);
   }
   __device__ __forceinline__ void set(const float (&f)[8]) {
-    uint32_t* w = reinterpret_cast<uint32_t*>(v);
     if constexpr (sizeof(T) == 4) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) w[i] = __float_as_uint(f[i]);
@@ -71,15 +79,21 @@ struct Raw {
       for (int i = 0; i < 4; ++i) w[i] = pack2<T>(f[2 * i], f[2 * i + 1]);
     }
   }
-  __device__ __forceinline__ void copy(T* p, int) const {
+  __device__ __forceinline__ void copy(T* p, int gap, int) const {
+    if constexpr (sizeof(T) == 4 || !SPLIT) {
 #pragma unroll
-    for (int j = 0; j < (int)sizeof(T) / 2; ++j) reinterpret_cast<uint4*>(p)[j] = v[j];
+      for (int j = 0; j < (int)sizeof(T) / 2; ++j)
+        *(reinterpret_cast<uint4*>(SPLIT && j ? p + gap : p) + (SPLIT ? 0 : j)) = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+    } else {
+      *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+      *reinterpret_cast<uint2*>(p + gap) = make_uint2(w[2], w[3]);
+    }
   }
 };
 template <typename T>
-struct Raw<T, false> {
+struct Raw<T, false, false> {
   T v[8];
-  __device__ __forceinline__ void load(const T* p, int n) {
+  __device__ __forceinline__ void load(const T* p, int, int n) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = i < n ? p[i] : Cvt<T>::from_f(0.f);
   }
@@ -95,12 +109,13 @@ struct Raw<T, false> {
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = Cvt<T>::from_f(f[i]);
   }
-  __device__ __forceinline__ void copy(T* p, int n) const {
+  __device__ __forceinline__ void copy(T* p, int, int n) const {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
       if (i < n) p[i] = v[i];
   }
 };
+
 // Two 32-bit values in one operation.
 struct F2 {
   uint64_t v;
@@ -119,122 +134,128 @@ __device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
   return r;
 }
 
-// VEC: rows by 16-byte accesses.  TAB: tables by 16-byte loads, a lane's values all turned or all kept, partners in one lane.
-// HALF: pairs (i, i + rot/2); else (2i, 2i + 1).  CACHE: k and v rows go to their slots, else k rows to k_out.
-template <typename T, bool VEC, bool TAB, bool HALF, bool CACHE>
+// VEC: rows by 16-byte (8-byte) accesses.  FAST: a lane's values are all turned or all kept and it holds their partners, its
+// angles come by 16-byte loads; else value by value, partners through shared memory.  HALF: pairs (i, i + rot/2); else
+// (2i, 2i + 1).  CACHE: k and v rows go to their slots, else k rows to k_out.
+template <typename T, bool VEC, bool FAST, bool HALF, bool CACHE>
 __global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(const RopeParams p) {
-  constexpr int U = sizeof(T) == 4 ? 2 : 4;                // rows in flight per group, and as many in computation
-  extern __shared__ float s_rows[];
+  constexpr int U = sizeof(T) == 4 ? 2 : 4;                // head rows in flight per group, and as many in computation
+  constexpr bool SPLIT = HALF && FAST;                     // four values of the first half and their partners
+  using R = Raw<T, VEC, SPLIT>;
+  extern __shared__ __align__(16) float s_rows[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int LG = p.group_lanes, groups = 32 / LG;          // lanes per head row (a power of two), rows per warp
   const int gl = lane & (LG - 1), grp = lane / LG;
-  const int e0 = gl * 8;                                    // first value of this lane
-  const int mine = p.hd - e0 < 8 ? (p.hd - e0 > 0 ? p.hd - e0 : 0) : 8;
+  const bool in_head = gl * 8 < p.hd;                      // (else a lane behind the head's end: it reads what lane 0 reads)
   const int half = p.rot >> 1;
+  // first value of this lane, and how far from it its second four lie
+  int e0 = in_head ? gl * 8 : 0, gap = 4;
+  bool turn = e0 < p.rot;                                  // FAST: of all the lane's values
+  if constexpr (SPLIT) {
+    const int g = in_head ? gl : 0;
+    turn = g * 4 < half;
+    if (turn) { e0 = g * 4; gap = half; }                  // (else what is kept: rot is a multiple of 8)
+  }
+  const int mine = p.hd - e0 < 8 ? p.hd - e0 : 8;
   float* row = s_rows + (warp * groups + grp) * (LG * 9);
-  const bool turn = e0 < p.rot;                            // TAB: of all the lane's values
-  const int partner = !turn ? lane : (e0 < half ? lane + (half >> 3) : lane - (half >> 3));
+
+  // x of the lane's partners (what comes where a value has none is not used)
+  auto partners = [&](const float (&x)[8], float (&y)[8]) {
+    if constexpr (SPLIT) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] = x[i ^ 4];
+    } else if constexpr (!HALF) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] = x[i ^ 1];
+    } else {                                               // one word of padding in eight: no bank conflicts
+      __syncwarp();                                        // the row before this one has been read
+#pragma unroll
+      for (int i = 0; i < 8; ++i) row[gl * 9 + i] = x[i];
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int e = e0 + i, other = e < half ? e + half : (e < p.rot ? e - half : e);
+        y[i] = row[(other >> 3) * 9 + (other & 7)];
+      }
+    }
+  };
 
   // items: first all tokens' queries, then keys, then values; a warp's groups take neighbouring tokens and one kind
-  const int64_t warps = p.q_warps + p.kv_warps * (CACHE ? 2 : 1), stride = (int64_t)gridDim.x * (kThreads / 32);
-  for (int64_t wi = (int64_t)blockIdx.x * (kThreads / 32) + warp; wi < warps; wi += stride) {
-    const int kind = wi < p.q_warps ? 0 : (wi < p.q_warps + p.kv_warps ? 1 : 2);
-    const int step = kind == 0 ? p.q_parts : p.kv_parts;   // parts of a token's heads: a group takes every step-th row
-    const int64_t item = (wi - (kind == 0 ? 0 : (kind == 1 ? p.q_warps : p.q_warps + p.kv_warps))) * groups + grp;
-    int64_t tok = step == 1 ? item : item / step;
-    int r = (int)(item - tok * step);                      // this group's next head row
-    int rows = kind == 0 ? p.Hq : p.Hkv;
-    const int rounds = (rows + step - 1) / step;           // head rows per group, uniform over the warp
-    if (tok >= p.tokens) { tok = 0; rows = 0; }            // behind the last item: a group without rows
-    if (mine == 0) rows = 0;                               // a lane behind the head's end
-    const int64_t b = tok < p.S ? 0 : tok / p.S, s = tok - b * p.S;
-    const int64_t* in_s = kind == 0 ? p.q_s : (kind == 1 ? p.k_s : p.v_s);
-    const T* src = static_cast<const T*>(kind == 0 ? p.q : (kind == 1 ? p.k : p.v)) + b * in_s[0] + s * in_s[1] + r * in_s[2] + e0;
-    const int64_t in_step = in_s[2] * step;
-    Raw<T, VEC> raw[U], next[U];
-    auto fetch = [&](Raw<T, VEC> (&x)[U], int r) {         // rows r, r + step, ... (src: row r)
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (r + u * step < rows) x[u].load(src + u * in_step, mine);
-        else x[u].clear();
-      }
-      src += U * in_step;
-    };
-    fetch(raw, r);
+  // (a warp takes one item: a grid that fits the GPU once and walks over them was slower)
+  const int64_t wi = (int64_t)blockIdx.x * (kThreads / 32) + warp;
+  if (wi >= p.q_warps + p.kv_warps * (CACHE ? 2 : 1)) return;
+  const int kind = wi < p.q_warps ? 0 : (wi < p.q_warps + p.kv_warps ? 1 : 2);
+  const int step = kind == 0 ? p.q_parts : p.kv_parts;   // parts of a token's heads: a group takes every step-th row
+  const int rows = kind == 0 ? p.Hq : p.Hkv;
+  const int64_t item = (wi - (kind == 0 ? 0 : (kind == 1 ? p.q_warps : p.q_warps + p.kv_warps))) * groups + grp;
+  int64_t tok = step == 1 ? item : item / step;
+  const int first = (int)(item - tok * step);            // this group's first head row
+  bool put = in_head && tok < p.tokens;                  // whether this lane stores anything
+  if (tok >= p.tokens) tok = p.tokens - 1;               // (a group behind the last item reads the last token)
+  const int64_t b = tok < p.S ? 0 : tok / p.S, s = tok - b * p.S;
 
-    int64_t pos = s;
-    if (p.positions)
-      pos = p.pos64 ? __ldg(static_cast<const long long*>(p.positions) + b * p.pos_sb + s)
-                    : (int64_t)__ldg(static_cast<const int32_t*>(p.positions) + b * p.pos_sb + s);
-    int64_t slot = -1;
-    if constexpr (CACHE) slot = __ldg(reinterpret_cast<const long long*>(p.slots) + tok);
-    const bool pad = pos < 0;                              // a row of padding: zeros out, nothing into the cache
-    bool wrong = pos >= p.table_rows;                      // no angle for it: NaN, not a silent clamp
-    if constexpr (CACHE) wrong |= slot >= p.capacity;
-    T* dst;
-    int64_t out_step;
-    if (CACHE && kind > 0) {
-      const bool there = !pad && slot >= 0 && slot < p.capacity;
-      if (!there) rows = 0;
-      const int64_t page = there ? slot / p.page_size : 0, off = there ? slot - page * p.page_size : 0;
-      const int64_t* out_s = kind == 1 ? p.kc_s : p.vc_s;
-      dst = static_cast<T*>(kind == 1 ? p.kc : p.vc) + page * out_s[0] + r * out_s[1] + off * out_s[2] + e0;
-      out_step = out_s[1] * step;
-    } else {
-      const int64_t* out_s = kind == 0 ? p.qo_s : p.ko_s;
-      dst = static_cast<T*>(kind == 0 ? p.q_out : p.k_out) + b * out_s[0] + s * out_s[1] + r * out_s[2] + e0;
-      out_step = out_s[2] * step;
-    }
-    if (CACHE && kind == 2) {                              // values go as they are
-      for (int i0 = 0; i0 < rounds; i0 += U, r += step * U) {
-        if (i0 + U < rounds) fetch(next, r + step * U);
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          if (r + u * step < rows) raw[u].copy(dst + u * out_step, mine);
-          raw[u] = next[u];
-        }
-        dst += U * out_step;
-      }
-      continue;
-    }
+  int64_t pos = s;
+  if (p.positions)
+    pos = p.pos64 ? __ldg(static_cast<const long long*>(p.positions) + b * p.pos_sb + s)
+                  : (int64_t)__ldg(static_cast<const int32_t*>(p.positions) + b * p.pos_sb + s);
+  int64_t slot = -1;
+  if constexpr (CACHE) slot = __ldg(reinterpret_cast<const long long*>(p.slots) + tok);
 
-    // cw, nw: z_i = (x_i cw_i + x_partner nw_i) * factor of the norm
+  const int64_t* in_s = kind == 0 ? p.q_s : (kind == 1 ? p.k_s : p.v_s);
+  const T* src = static_cast<const T*>(kind == 0 ? p.q : (kind == 1 ? p.k : p.v)) + b * in_s[0] + s * in_s[1] + first * in_s[2] + e0;
+  const int64_t in_step = in_s[2] * step;
+  R raw[U];
+  const int full = rows / step / U * U;                  // rows that every group has, in whole batches
+  if (full > 0) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) raw[u].load(src + u * in_step, gap, mine);
+  } else {
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (first + u * step < rows) raw[u].load(src + u * in_step, gap, mine);
+      else raw[u].clear();
+  }
+
+  const bool pad = pos < 0;                              // a row of padding: zeros out, nothing into the cache
+  bool wrong = pos >= p.table_rows;                      // no angle for it: NaN, not a silent clamp
+  if constexpr (CACHE) wrong |= slot >= p.capacity;
+  T* dst;
+  int64_t out_step;
+  if (CACHE && kind > 0) {
+    const bool there = !pad && slot >= 0 && slot < p.capacity;
+    put &= there;
+    const int64_t page = there ? slot / p.page_size : 0, off = there ? slot - page * p.page_size : 0;
+    const int64_t* out_s = kind == 1 ? p.kc_s : p.vc_s;
+    dst = static_cast<T*>(kind == 1 ? p.kc : p.vc) + page * out_s[0] + first * out_s[1] + off * out_s[2] + e0;
+    out_step = out_s[1] * step;
+  } else {
+    const int64_t* out_s = kind == 0 ? p.qo_s : p.ko_s;
+    dst = static_cast<T*>(kind == 0 ? p.q_out : p.k_out) + b * out_s[0] + s * out_s[1] + first * out_s[2] + e0;
+    out_step = out_s[2] * step;
+  }
+
+  // cw, nw: z_i = (x_i cw_i + x_partner nw_i) * factor of the norm
+  F2 cw[4], nw[4];
+  if (!CACHE || kind < 2) {
     const int64_t tr = wrong || pad ? 0 : pos;
     const float* ct = p.cos_t + tr * p.table_ld;
     const float* st = p.sin_t + tr * p.table_ld;
     const float* wt = kind == 0 ? p.wq : p.wk;
     const float scale = kind == 0 ? p.q_scale : p.k_scale;
-    float c[8], n[8], w[8];
+    float c[8], n[8], w[8], wp[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) { c[i] = 1.f; n[i] = 0.f; w[i] = scale; }
-    if (wt) {
-      if (VEC && (reinterpret_cast<uintptr_t>(wt) & 15) == 0) {
-        if (mine > 0) {
-          const float4 a = __ldg(reinterpret_cast<const float4*>(wt + e0)), d = __ldg(reinterpret_cast<const float4*>(wt + e0) + 1);
-          w[0] *= a.x; w[1] *= a.y; w[2] *= a.z; w[3] *= a.w;
-          w[4] *= d.x; w[5] *= d.y; w[6] *= d.z; w[7] *= d.w;
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (i < mine) w[i] *= __ldg(wt + e0 + i);
-      }
-    }
-    if constexpr (TAB) {
+    if constexpr (FAST) {
       if (turn) {
-        constexpr int NC = HALF ? 8 : 4;                   // table entries of the lane's values
-        const int at = HALF ? (e0 < half ? e0 : e0 - half) : e0 >> 1;
-        float a[NC], d[NC];
+        const int at = HALF ? e0 : e0 >> 1;
+        const float4 x = __ldg(reinterpret_cast<const float4*>(ct + at)), y = __ldg(reinterpret_cast<const float4*>(st + at));
+        const float a[4] = {x.x, x.y, x.z, x.w}, d[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
-        for (int i = 0; i < NC; i += 4) {
-          const float4 x = __ldg(reinterpret_cast<const float4*>(ct + at + i)), y = __ldg(reinterpret_cast<const float4*>(st + at + i));
-          a[i] = x.x; a[i + 1] = x.y; a[i + 2] = x.z; a[i + 3] = x.w;
-          d[i] = y.x; d[i + 1] = y.y; d[i + 2] = y.z; d[i + 3] = y.w;
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          c[i] = a[HALF ? i : i / 2];
-          n[i] = (HALF ? e0 < half : (i & 1) == 0) ? -d[HALF ? i : i / 2] : d[HALF ? i : i / 2];
+        for (int i = 0; i < 4; ++i) {
+          const int lower = HALF ? i : 2 * i, upper = HALF ? i + 4 : 2 * i + 1;
+          c[lower] = c[upper] = a[i];
+          n[lower] = -d[i];
+          n[upper] = d[i];
         }
       }
     } else {
@@ -243,129 +264,132 @@ __global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(const RopeParams
         const int e = e0 + i;
         if (e < p.rot) {
           const int at = HALF ? (e < half ? e : e - half) : e >> 1;
-          const bool first = HALF ? e < half : (e & 1) == 0;
+          const bool lower = HALF ? e < half : (e & 1) == 0;
           c[i] = __ldg(ct + at);
-          n[i] = first ? -__ldg(st + at) : __ldg(st + at);
+          n[i] = lower ? -__ldg(st + at) : __ldg(st + at);
         }
       }
     }
-    F2 cw[4], nw[4];
-    {
-      float wp[8];              // the partner's weight
-      if constexpr (HALF && TAB) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) wp[i] = __shfl_sync(0xffffffffu, w[i], partner);
-      } else if constexpr (HALF) {
-        __syncwarp();
-#pragma unroll
-        for (int i = 0; i < 8; ++i) row[gl * 9 + i] = w[i];
-        __syncwarp();
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int e = e0 + i, other = e < half ? e + half : e - half;
-          wp[i] = e < p.rot ? row[(other >> 3) * 9 + (other & 7)] : 0.f;
-        }
+    if (wt) {
+      if (VEC && (reinterpret_cast<uintptr_t>(wt) & 15) == 0) {
+        const float4 a = __ldg(reinterpret_cast<const float4*>(wt + e0)), d = __ldg(reinterpret_cast<const float4*>(wt + e0 + gap));
+        w[0] *= a.x; w[1] *= a.y; w[2] *= a.z; w[3] *= a.w;
+        w[4] *= d.x; w[5] *= d.y; w[6] *= d.z; w[7] *= d.w;
       } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) wp[i] = w[i ^ 1];
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        cw[i] = F2(c[2 * i] * w[2 * i], c[2 * i + 1] * w[2 * i + 1]);
-        nw[i] = F2(n[2 * i] * wp[2 * i], n[2 * i + 1] * wp[2 * i + 1]);
+        for (int i = 0; i < 8; ++i)
+          if (i < mine || SPLIT) w[i] *= __ldg(wt + e0 + (i < 4 ? i : gap + i - 4));
       }
     }
-    const float eps = wrong ? __int_as_float(0x7fc00000) : p.eps;
-    const bool partial = p.rot < p.hd;                     // some values are kept: not even touched by a partner's inf or NaN
-    for (int i0 = 0; i0 < rounds; i0 += U, r += step * U) {
-      if (i0 + U < rounds) fetch(next, r + step * U);
+    partners(w, wp);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      cw[i] = F2(c[2 * i] * w[2 * i], c[2 * i + 1] * w[2 * i + 1]);
+      nw[i] = F2(n[2 * i] * wp[2 * i], n[2 * i + 1] * wp[2 * i + 1]);
+    }
+  }
+  const float eps = wrong ? __int_as_float(0x7fc00000) : p.eps;
+  const bool partial = p.rot < p.hd;                     // some values are kept: not even touched by a partner's inf or NaN
+  // The first `left` of U head rows in place (the same number for all lanes).  First the sums of squares of all of them, whose
+  // shuffles then run side by side.
+  auto work = [&](R (&v)[U], int left) {
+    float inv[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) inv[u] = wrong ? eps : 1.f;
+    if (p.norm) {
+      float ss[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        if (i0 + u >= rounds) break;
-        float x[8], y[8];
-        raw[u].get(x);
-        F2 x2[4];
+        ss[u] = 0.f;
+        if (u >= left) break;
+        float x[8], sa, sb;
+        v[u].get(x);
+        F2 s2 = mul2(F2(x[0], x[1]), F2(x[0], x[1]));
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x2[i] = F2(x[2 * i], x[2 * i + 1]);
-        float inv = wrong ? eps : 1.f;
-        if (p.norm) {
-          F2 ss = mul2(x2[0], x2[0]);
+        for (int i = 1; i < 4; ++i) s2 = fma2(F2(x[2 * i], x[2 * i + 1]), F2(x[2 * i], x[2 * i + 1]), s2);
+        s2.get(sa, sb);
+        ss[u] = in_head ? sa + sb : 0.f;
+      }
 #pragma unroll
-          for (int i = 1; i < 4; ++i) ss = fma2(x2[i], x2[i], ss);
-          float sa, sb;
-          ss.get(sa, sb);
-          sa += sb;
+      for (int o = 16; o > 0; o >>= 1)
+        if (o < LG) {
 #pragma unroll
-          for (int o = 16; o > 0; o >>= 1)
-            if (o < LG) sa += __shfl_xor_sync(0xffffffffu, sa, o);
-          inv = rsqrtf(fmaf(sa, p.norm_c, eps));
+          for (int u = 0; u < U; ++u) ss[u] += __shfl_xor_sync(0xffffffffu, ss[u], o);
         }
-        if constexpr (HALF && TAB) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) y[i] = __shfl_sync(0xffffffffu, x[i], partner);
-        } else if constexpr (HALF) {
-          __syncwarp();                                    // the row before this one has been read
+      for (int u = 0; u < U; ++u) inv[u] = rsqrtf(fmaf(ss[u], p.norm_c, eps));
+    }
 #pragma unroll
-          for (int i = 0; i < 8; ++i) row[gl * 9 + i] = x[i];
-          __syncwarp();
+    for (int u = 0; u < U; ++u) {
+      if (u >= left) break;
+      float x[8], y[8], z[8];
+      v[u].get(x);
+      partners(x, y);
+      const F2 inv2(inv[u], inv[u]);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int e = e0 + i, other = e < half ? e + half : e - half;
-            y[i] = e < p.rot ? row[(other >> 3) * 9 + (other & 7)] : 0.f;
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) y[i] = x[i ^ 1];
-        }
-        const F2 inv2(inv, inv);
-        float z[8];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const F2 a = mul2(x2[i], cw[i]);
-          mul2(fma2(F2(y[2 * i], y[2 * i + 1]), nw[i], a), inv2).get(z[2 * i], z[2 * i + 1]);
-          if (partial) {
-            float k0, k1;
-            mul2(a, inv2).get(k0, k1);
-            if (TAB ? !turn : e0 + 2 * i >= p.rot) z[2 * i] = k0;
-            if (TAB ? !turn : e0 + 2 * i + 1 >= p.rot) z[2 * i + 1] = k1;
-          }
-        }
-        if (r + u * step < rows) {
-          Raw<T, VEC> packed;
-          packed.set(z);
-          if (pad) packed.clear();
-          packed.copy(dst + u * out_step, mine);
+      for (int i = 0; i < 4; ++i) {
+        const F2 a = mul2(F2(x[2 * i], x[2 * i + 1]), cw[i]);
+        mul2(fma2(F2(y[2 * i], y[2 * i + 1]), nw[i], a), inv2).get(z[2 * i], z[2 * i + 1]);
+        if (partial) {
+          float k0, k1;
+          mul2(a, inv2).get(k0, k1);
+          if (FAST ? !turn : e0 + 2 * i >= p.rot) z[2 * i] = k0;
+          if (FAST ? !turn : e0 + 2 * i + 1 >= p.rot) z[2 * i + 1] = k1;
         }
       }
-      dst += U * out_step;
-#pragma unroll
-      for (int u = 0; u < U; ++u) raw[u] = next[u];
+      v[u].set(z);
+      if (pad) v[u].clear();
     }
+  };
+  // whole batches first, without a look at the bounds; the next batch's loads are under way while one is computed
+  int i = 0;
+  for (; i < full; i += U) {
+    R next[U];
+    src += U * in_step;
+    if (i + U < full) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) next[u].load(src + u * in_step, gap, mine);
+    } else {
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (first + (i + U + u) * step < rows) next[u].load(src + u * in_step, gap, mine);
+        else next[u].clear();
+    }
+    if (!CACHE || kind < 2) work(raw, U);                // (values go as they are)
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (put) raw[u].copy(dst + u * out_step, gap, mine);
+      raw[u] = next[u];
+    }
+    dst += U * out_step;
+  }
+  if (i * step >= rows) return;                          // uniform over the warp
+  if (!CACHE || kind < 2) work(raw, (rows - i * step + step - 1) / step);
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    if (put && first + (i + u) * step < rows) raw[u].copy(dst + u * out_step, gap, mine);
   }
 }
 
-template <typename T, bool VEC, bool TAB, bool HALF, bool CACHE>
+template <typename T, bool VEC, bool FAST, bool HALF, bool CACHE>
 int launch_as(const RopeParams& p, cudaStream_t st) {
-  int dev = 0, sms = 0;
-  HB_CUDA(cudaGetDevice(&dev));
-  HB_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
-  int64_t grid = ceil_div64(p.q_warps + p.kv_warps * (CACHE ? 2 : 1), kThreads / 32);
-  if (grid > (int64_t)sms * 16) grid = (int64_t)sms * 16;
-  qk_norm_rope_kernel<T, VEC, TAB, HALF, CACHE><<<(unsigned)grid, kThreads, HALF && !TAB ? kThreads * 9 * 4 : 0, st>>>(p);
+  const int64_t grid = ceil_div64(p.q_warps + p.kv_warps * (CACHE ? 2 : 1), kThreads / 32);
+  HB_REQUIRE(grid <= 0x7fffffff, HB200_ERR_UNSUPPORTED, "qk_norm_rope: too many tokens");
+  qk_norm_rope_kernel<T, VEC, FAST, HALF, CACHE><<<(unsigned)grid, kThreads, HALF && !FAST ? kThreads * 9 * 4 : 0, st>>>(p);
   HB_LAUNCH_CHECK();
   return 0;
 }
 
 template <typename T, bool HALF, bool CACHE>
-int launch_mode(const RopeParams& p, bool vec, bool tab, cudaStream_t st) {
+int launch_mode(const RopeParams& p, bool vec, bool fast, cudaStream_t st) {
   if (!vec) return launch_as<T, false, false, HALF, CACHE>(p, st);
-  return tab ? launch_as<T, true, true, HALF, CACHE>(p, st) : launch_as<T, true, false, HALF, CACHE>(p, st);
+  return fast ? launch_as<T, true, true, HALF, CACHE>(p, st) : launch_as<T, true, false, HALF, CACHE>(p, st);
 }
 
 template <typename T>
-int launch(const RopeParams& p, bool vec, bool tab, bool half, bool cache, cudaStream_t st) {
-  if (half) return cache ? launch_mode<T, true, true>(p, vec, tab, st) : launch_mode<T, true, false>(p, vec, tab, st);
-  return cache ? launch_mode<T, false, true>(p, vec, tab, st) : launch_mode<T, false, false>(p, vec, tab, st);
+int launch(const RopeParams& p, bool vec, bool fast, bool half, bool cache, cudaStream_t st) {
+  if (half) return cache ? launch_mode<T, true, true>(p, vec, fast, st) : launch_mode<T, true, false>(p, vec, fast, st);
+  return cache ? launch_mode<T, false, true>(p, vec, fast, st) : launch_mode<T, false, false>(p, vec, fast, st);
 }
 
 }  // namespace
@@ -427,7 +451,7 @@ extern "C" int hb200_qk_norm_rope(const hb200_qk_norm_rope_args* a, const hb200_
   }
   p.group_lanes = 1;
   while (p.group_lanes * 8 < p.hd) p.group_lanes <<= 1;
-  // a token's head rows are shared out over more groups of lanes until about 16 warps per SM have work
+  // a token's head rows are shared out over more groups of lanes until about 8 warps per SM have work
   const int groups = 32 / p.group_lanes, kinds = c ? 2 : 1;
   p.q_parts = p.kv_parts = 1;
   auto count = [&]() {
@@ -435,16 +459,16 @@ extern "C" int hb200_qk_norm_rope(const hb200_qk_norm_rope_args* a, const hb200_
     p.kv_warps = a->Hkv ? ceil_div64(tokens * p.kv_parts, groups) : 0;
     return p.q_warps + kinds * p.kv_warps;
   };
-  while (count() < 148 * 16 && (p.q_parts < a->Hq || p.kv_parts < a->Hkv)) {
+  while (count() < 148 * 8 && (p.q_parts < a->Hq || p.kv_parts < a->Hkv)) {
     const bool q_more = p.q_parts < a->Hq && (p.kv_parts >= a->Hkv || (int64_t)p.kv_parts * a->Hq >= (int64_t)p.q_parts * a->Hkv);
     (q_more ? p.q_parts : p.kv_parts) *= 2;
   }
-  const bool tab = a->rot % (a->layout == HB200_ROPE_HALF ? 16 : 8) == 0 && a->table_ld % 4 == 0 && aligned16(a->cos) && aligned16(a->sin);
+  const bool fast = a->rot % 8 == 0 && a->table_ld % 4 == 0 && aligned16(a->cos) && aligned16(a->sin);
   cudaStream_t st = (cudaStream_t)stream;
   const bool half = a->layout == HB200_ROPE_HALF;
-  if (a->dtype == HB200_F32) return launch<float>(p, vec, tab, half, c != nullptr, st);
-  if (a->dtype == HB200_BF16) return launch<__nv_bfloat16>(p, vec, tab, half, c != nullptr, st);
-  if (a->dtype == HB200_F16) return launch<__half>(p, vec, tab, half, c != nullptr, st);
+  if (a->dtype == HB200_F32) return launch<float>(p, vec, fast, half, c != nullptr, st);
+  if (a->dtype == HB200_BF16) return launch<__nv_bfloat16>(p, vec, fast, half, c != nullptr, st);
+  if (a->dtype == HB200_F16) return launch<__half>(p, vec, fast, half, c != nullptr, st);
   set_error("qk_norm_rope: unsupported dtype %d", a->dtype);
   return HB200_ERR_UNSUPPORTED;
 }
