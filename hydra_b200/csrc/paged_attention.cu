@@ -11,10 +11,11 @@
 // Work split: the tiles of all (request, kv head) pairs are laid end to end and dealt out in equal contiguous shares to
 // the warps of a grid that fits the GPU once (one CTA per SM), whatever the lengths are: a batch of one long and many
 // short requests keeps every SM busy to the end.  The lengths live on the device; each CTA scans them itself.  A warp
-// streams its share through a private cp.async ring that runs on across the ends of requests, so no barrier is met after
-// the scan.  A pair that lies within one share is finished by its warp; of the others each share leaves (max, sum,
-// unnormalised output) in 32 bits in the workspace and the join kernel adds them up in a fixed order (no atomics:
-// the same inputs give the same bits).
+// streams its share through a private cp.async ring that runs on across the ends of requests, so no barrier is met between
+// the scan and the share's end.  A pair that lies within one share is finished by its warp.  Of the others each warp leaves
+// (max, sum, unnormalised output) in 32 bits; the CTA, whose warps' shares are neighbours, adds up those of one pair, and
+// what then still spans CTAs goes through the workspace to the join kernel.  All sums run in a fixed order without
+// atomics: the same inputs give the same bits.
 #include "common.cuh"
 #include "mma.cuh"
 
@@ -22,20 +23,22 @@ namespace hb200 {
 namespace {
 
 constexpr float kLn2 = 0.6931471805599453f;
+
+__device__ __forceinline__ int64_t div_up(int64_t a, int b) {   // (a 64-bit division only where it takes one)
+  return a <= 0x7fffffff - b ? (int64_t)(((unsigned)a + (unsigned)b - 1) / (unsigned)b) : (a + b - 1) / b;
+}
 constexpr int kMaxBatch = 4096;
-constexpr int kMinTiles = 2;    // least share of a warp: below this the join's traffic outweighs the parallelism
 
 struct PagedParams {
   const void *q, *kc, *vc;
   void* out;
   float* lse;
   const int32_t *table, *lens;
-  float* part_o;     // [workers][2][rows][hd]
-  float* part_ml;    // [workers][2][rows][2]
+  float* part;       // [CTAs][2] parts, then [warps] of the warps' own: each [rows][hd] outputs, [rows][2] of max and sum
   int32_t* cum;      // [B + 1] tiles of the requests before each one
   int64_t q_sb, q_sh, k_sh, v_sh, table_ld;     // elements
   int32_t k_sp, k_sr, v_sp, v_sr;               // bytes: page and row of a page
-  int B, Hq, Hkv, hd, group, q_tiles, rows, page_size, width, num_pages, workers;
+  int B, Hq, Hkv, hd, group, q_tiles, q_tile, tile, warps, rows, part_floats, page_size, width, num_pages, ctas;
   float scale_log2;  // |scale| log2(e)
   uint32_t q_sign;   // flips the signs of a pair of query values where the scale is negative
 };
@@ -43,6 +46,8 @@ struct PagedParams {
 // A warp's tile: 8 KB of K and V (16 KB of heads of 256, 4 KB of small ones); its ring keeps 16 KB in flight, a CTA 128 KB.
 __host__ __device__ constexpr int tile_tokens(int HD) { return HD >= 128 ? 16 : (HD == 16 ? 64 : 32); }
 __host__ __device__ constexpr int warps_of(int HD) { return HD >= 256 ? 4 : 8; }
+// Query heads that are worked on together: their outputs and queries stay in a warp's registers.
+__host__ __device__ constexpr int q_tile_of(int HD) { return HD >= 256 ? 8 : 16; }
 __host__ __device__ constexpr int stages_of(int HD) { return HD <= 32 ? 5 : 3; }
 
 // Cache length of request b as the kernel reads it: what lies outside [0, width * page_size] is marked (`poison`).
@@ -173,12 +178,14 @@ __global__ void __launch_bounds__(warps_of(HD) * 32, 1) paged_attention_kernel(c
   }
   const int H = p.Hkv * p.q_tiles;
   const int64_t total = (int64_t)s_cum[p.B] * H;
-  const int64_t share = max((total + p.workers - 1) / p.workers, (int64_t)kMinTiles);
-  const int w = warp * gridDim.x + blockIdx.x;       // few shares: one per SM before any SM has two
-  const int64_t begin = (int64_t)w * share;
-  if (begin >= total) return;
-  const int64_t end = begin + share < total ? begin + share : total;
+  const int64_t share = div_up(total, p.ctas * NW);
+  const int w = blockIdx.x * NW + warp;
+  const int64_t begin = min((int64_t)w * share, total), end = min(begin + share, total);
   int left = (int)(end - begin);                     // tiles to compute
+  __shared__ int s_pair[2 * NW];                     // of the warps' first and last parts: request * H + head tile, or -1
+  __shared__ int s_ends[2 * NW];                     // 1: holds the pair's first tile; 2: its last
+  __shared__ const float* s_part[2 * NW];
+  if (lane < 2) s_pair[2 * warp + lane] = -1;
 
   auto enter = [&](Cursor& c) {   // request c.b's length and tiles
     c.n = s_cum[c.b + 1] - s_cum[c.b];
@@ -195,8 +202,8 @@ __global__ void __launch_bounds__(warps_of(HD) * 32, 1) paged_attention_kernel(c
       }
     }
   };
-  Cursor cur;
-  {
+  Cursor cur = {};
+  if (left > 0) {
     int lo = 0, hi = p.B;   // s_cum[lo] * H <= begin < s_cum[hi] * H
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
@@ -223,9 +230,9 @@ __global__ void __launch_bounds__(warps_of(HD) * 32, 1) paged_attention_kernel(c
   const int unit = P16 ? p.page_size / 16 : p.page_size;      // looks per page
   int page0, off0;                            // of the tile's first token: place in the table row, units into the page
   {
-    const int64_t at = (int64_t)pc.t * (P16 ? MT : TT);
-    page0 = (int)(at / unit);
-    off0 = (int)(at - (int64_t)page0 * unit);
+    const unsigned at = (unsigned)pc.t * (P16 ? MT : TT);
+    page0 = (int)(at / (unsigned)unit);
+    off0 = (int)(at - (unsigned)page0 * (unsigned)unit);
   }
   const int prow = lane / LPR, pch = lane % LPR;
   const int32_t* trow = nullptr;
@@ -339,9 +346,9 @@ __global__ void __launch_bounds__(warps_of(HD) * 32, 1) paged_attention_kernel(c
     if (fresh) {   // a new (request, head tile): its queries, empty statistics
       fresh = false;
       first_tile = cur.t;
-      const int kvh = cur.h / p.q_tiles, qt = cur.h - kvh * p.q_tiles;
-      head0 = kvh * p.group + qt * 16;
-      rows_here = min(16, p.group - qt * 16);
+      const int kvh = p.q_tiles == 1 ? cur.h : cur.h / p.q_tiles, qt = cur.h - kvh * p.q_tiles;
+      head0 = kvh * p.group + qt * q_tile_of(HD);
+      rows_here = min(q_tile_of(HD), p.group - qt * q_tile_of(HD));
       const T* qb = static_cast<const T*>(p.q) + (int64_t)cur.b * p.q_sb + (int64_t)head0 * p.q_sh;
 #pragma unroll
       for (int n = 0; n < NQ; ++n) {
@@ -463,10 +470,20 @@ __global__ void __launch_bounds__(warps_of(HD) * 32, 1) paged_attention_kernel(c
 
     if (cur.t + 1 == cur.n || left == 0) {   // the pair's end, or the share's
       const bool whole = first_tile == 0 && cur.t + 1 == cur.n;
-      // slot 0 of the share: the pair that its first tile belongs to; slot 1: the pair that begins inside and goes on
-      const int ps = (cur.t - first_tile + 1 == (int)(end - begin) - left) ? 0 : 1;
-      float* po = p.part_o + ((int64_t)w * 2 + ps) * p.rows * p.hd;
-      float* pm = p.part_ml + ((int64_t)w * 2 + ps) * p.rows * 2;
+      // a part that ends with the share stays in shared memory (the ring is done), one before it goes to the workspace
+      float* po = p.part + ((int64_t)p.ctas * 2 + w) * p.part_floats;
+      if (left == 0) {
+        cp_async_wait<0>();
+        __syncwarp();
+        po = reinterpret_cast<float*>(ring);
+      }
+      if (!whole && lane == 0) {
+        const int k = 2 * warp + (left == 0 ? 1 : 0);
+        s_pair[k] = cur.b * H + cur.h;
+        s_ends[k] = (first_tile == 0 ? 1 : 0) | (cur.t + 1 == cur.n ? 2 : 0);
+        s_part[k] = po;
+      }
+      float* pm = po + p.rows * p.hd;
       T* ob = static_cast<T*>(p.out) + ((int64_t)cur.b * p.Hq + head0) * p.hd;
 #pragma unroll
       for (int n = 0; n < NQ; ++n)
@@ -500,7 +517,51 @@ __global__ void __launch_bounds__(warps_of(HD) * 32, 1) paged_attention_kernel(c
     }
     if (left > 0) advance(cur);
   }
-  cp_async_wait<0>();
+  __syncthreads();
+
+  // the parts of one pair, neighbours in the order of the warps' shares: a thread has four values of one row
+  const int quads = p.hd / 4;
+  for (int k0 = 0; k0 < 2 * NW;) {
+    const int pair = s_pair[k0];
+    if (pair < 0) { ++k0; continue; }
+    int k1 = k0 + 1, ends = s_ends[k0], last = k0;
+    for (; k1 < 2 * NW && (s_pair[k1] < 0 || s_pair[k1] == pair); ++k1)
+      if (s_pair[k1] == pair) { ends |= s_ends[k1]; last = k1; }
+    const int b = pair / H, h = pair - b * H;
+    const int kvh = p.q_tiles == 1 ? h : h / p.q_tiles, qt = h - kvh * p.q_tiles;
+    const int head = kvh * p.group + qt * q_tile_of(HD), rows = min(q_tile_of(HD), p.group - qt * q_tile_of(HD));
+    // (the CTA's first tile belongs to its first part's pair: the join finds that one in place 0, one that begins later in 1)
+    const int64_t t0 = (int64_t)s_cum[b] * H + (int64_t)h * (s_cum[b + 1] - s_cum[b]);
+    float* po = p.part + ((int64_t)blockIdx.x * 2 + (t0 <= (int64_t)blockIdx.x * NW * share ? 0 : 1)) * p.part_floats;
+    for (int i = threadIdx.x; i < rows * quads; i += NW * 32) {
+      const int r = i / quads, d = (i - r * quads) * 4;
+      float m = -INFINITY;
+      for (int k = k0; k <= last; ++k)
+        if (s_pair[k] >= 0) m = fmaxf(m, s_part[k][p.rows * p.hd + 2 * r]);
+      const float base = m == -INFINITY ? 0.f : m;
+      float l = 0.f;
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int k = k0; k <= last; ++k)
+        if (s_pair[k] >= 0) {
+          const float* o = s_part[k];
+          const float f = ex2(o[p.rows * p.hd + 2 * r] - base);
+          const float4 v = *reinterpret_cast<const float4*>(o + r * p.hd + d);
+          l = fmaf(f, o[p.rows * p.hd + 2 * r + 1], l);
+          acc.x = fmaf(f, v.x, acc.x); acc.y = fmaf(f, v.y, acc.y); acc.z = fmaf(f, v.z, acc.z); acc.w = fmaf(f, v.w, acc.w);
+        }
+      if (ends == 3) {
+        const float inv = 1.f / l;
+        const int64_t at = (int64_t)b * p.Hq + head + r;
+        T four[4] = {Cvt<T>::from_f(acc.x * inv), Cvt<T>::from_f(acc.y * inv), Cvt<T>::from_f(acc.z * inv), Cvt<T>::from_f(acc.w * inv)};
+        *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + at * p.hd + d) = *reinterpret_cast<const uint2*>(four);
+        if (d == 0 && p.lse) p.lse[at] = (base + log2f(l)) * kLn2;
+      } else {
+        *reinterpret_cast<float4*>(po + r * p.hd + d) = acc;
+        if (d == 0) *reinterpret_cast<float2*>(po + p.rows * p.hd + 2 * r) = make_float2(m, l);
+      }
+    }
+    k0 = last + 1;
+  }
 }
 
 // WPR warps per (request, query head): nothing where one share held the whole pair, zeros for an empty request, else the
@@ -514,13 +575,45 @@ __global__ void __launch_bounds__(WPR > 8 ? WPR * 32 : 256) paged_join_kernel(co
   const int64_t rw = (int64_t)blockIdx.x * RPC + warp / WPR;   // WPR > 1: the same for the whole CTA
   const bool live = rw < (int64_t)p.B * p.Hq;
   const int b = live ? (int)(rw / p.Hq) : 0, hq = live ? (int)(rw - (int64_t)b * p.Hq) : 0;
-  const int kvh = hq / p.group, in_group = hq - kvh * p.group, qt = in_group / 16, r = in_group & 15;
+  const int kvh = hq / p.group, in_group = hq - kvh * p.group, qt = in_group / p.q_tile, r = in_group - qt * p.q_tile;
   const int H = p.Hkv * p.q_tiles;
   T* ob = static_cast<T*>(p.out) + rw * p.hd;
-  chain_wait();
+  // The lengths are inputs, which the attention kernel's own start has waited for: a small batch is scanned before its end.
+  const bool early = p.B <= 256;
+  int before = 0, all = 0, n = 0;
+  if (early) {
+    const int64_t cap = (int64_t)p.width * p.page_size;
+    for (int a = lane; a < p.B; a += 32) {
+      bool poison;
+      const int t = (clamp_len(__ldg(p.lens + a), cap, poison) + p.tile - 1) / p.tile;
+      all += t;
+      before += a < b ? t : 0;
+      n += a == b ? t : 0;
+    }
+#pragma unroll
+    for (int s = 16; s > 0; s >>= 1) {
+      all += __shfl_xor_sync(0xffffffffu, all, s);
+      before += __shfl_xor_sync(0xffffffffu, before, s);
+      n += __shfl_xor_sync(0xffffffffu, n, s);
+    }
+  } else {
+    chain_wait();
+    before = __ldcg(p.cum + b);
+    n = __ldcg(p.cum + b + 1) - before;
+    all = __ldcg(p.cum + p.B);
+  }
+  const int64_t total = (int64_t)all * H;
+  const int64_t share = div_up(total, p.ctas * p.warps) * p.warps;             // of a CTA
+  const int64_t t0 = (int64_t)before * H + (int64_t)(kvh * p.q_tiles + qt) * n, t1 = t0 + n;
+  int w0 = 0, w1 = 0;
+  if (n > 0) {
+    w0 = total <= 0x7fffffff ? (int)((unsigned)t0 / (unsigned)share) : (int)(t0 / share);
+    w1 = total <= 0x7fffffff ? (int)((unsigned)(t1 - 1) / (unsigned)share) : (int)((t1 - 1) / share);
+  }
+  const int64_t first = (int64_t)w0 * 2 + (t0 == (int64_t)w0 * share ? 0 : 1);
+  const int parts = w1 - w0 + 1;
+  if (early) chain_wait();
   if (!live) return;                            // (only with WPR = 1, where no barrier follows)
-  const int c0 = __ldcg(p.cum + b), c1 = __ldcg(p.cum + b + 1), call = __ldcg(p.cum + p.B);
-  const int n = c1 - c0;
   if (n == 0) {   // an empty request; one with a length but no table at all is NaN like any that outgrew its table
     if (wi > 0) return;
     const bool wrong = p.lens[b] > 0;
@@ -528,14 +621,8 @@ __global__ void __launch_bounds__(WPR > 8 ? WPR * 32 : 256) paged_join_kernel(co
     if (p.lse && lane == 0) p.lse[rw] = wrong ? __int_as_float(0x7fc00000) : -INFINITY;
     return;
   }
-  const int64_t total = (int64_t)call * H;
-  const int64_t share = max((total + p.workers - 1) / p.workers, (int64_t)kMinTiles);
-  const int64_t t0 = (int64_t)c0 * H + (int64_t)(kvh * p.q_tiles + qt) * n, t1 = t0 + n;
-  const int w0 = (int)(t0 / share), w1 = (int)((t1 - 1) / share);
-  if (w0 == w1) return;
-  const int parts = w1 - w0 + 1;
-  const int64_t first = (int64_t)w0 * 2 + (t0 == (int64_t)w0 * share ? 0 : 1);
-  auto at = [&](int i) { return ((i == 0 ? first : (int64_t)(w0 + i) * 2) * p.rows + r); };
+  if (parts == 1) return;
+  auto at = [&](int i) { return p.part + (i == 0 ? first : (int64_t)(w0 + i) * 2) * p.part_floats; };
   const int d0 = lane * 4, d1 = d0 + 128;
   float4 a = make_float4(0.f, 0.f, 0.f, 0.f), c = a;
   float m = -INFINITY, l = 0.f;
@@ -543,7 +630,7 @@ __global__ void __launch_bounds__(WPR > 8 ? WPR * 32 : 256) paged_join_kernel(co
   const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int i0 = wi; i0 < parts; i0 += 32 * WPR) {
     const int mine = i0 + lane * WPR;           // this lane's part
-    const float2 ml = mine < parts ? __ldcg(reinterpret_cast<const float2*>(p.part_ml + at(mine) * 2)) : make_float2(-INFINITY, 0.f);
+    const float2 ml = mine < parts ? __ldcg(reinterpret_cast<const float2*>(at(mine) + p.rows * p.hd + 2 * r)) : make_float2(-INFINITY, 0.f);
     float mx = ml.x;
 #pragma unroll
     for (int s = 16; s > 0; s >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, s));
@@ -561,7 +648,7 @@ __global__ void __launch_bounds__(WPR > 8 ? WPR * 32 : 256) paged_join_kernel(co
 #pragma unroll 8
     for (int k = 0; k < here; ++k) {
       const float f = __shfl_sync(0xffffffffu, w, k);
-      const float* o = p.part_o + at(i0 + k * WPR) * p.hd;
+      const float* o = at(i0 + k * WPR) + r * p.hd;
       if (d0 < p.hd) a = scaled(__ldcg(reinterpret_cast<const float4*>(o + d0)), f, a);
       if (d1 < p.hd) c = scaled(__ldcg(reinterpret_cast<const float4*>(o + d1)), f, c);
     }
@@ -611,10 +698,11 @@ int padded_hd(int hd) { return hd <= 16 ? 16 : (hd <= 32 ? 32 : (hd <= 64 ? 64 :
 
 size_t round256(size_t n) { return (n + 255) & ~(size_t)255; }
 
+int part_floats_of(int rows, int hd) { return ceil_div(rows * (hd + 2), 4) * 4; }   // 16-byte aligned parts
+
 size_t workspace_for(int B, int Hq, int Hkv, int hd, int sms) {
-  const int group = Hq / Hkv, rows = group < 16 ? group : 16;
-  const size_t slots = (size_t)sms * warps_of(padded_hd(hd)) * 2;
-  return round256(slots * rows * hd * 4) + round256(slots * rows * 8) + round256(((size_t)B + 1) * 4);
+  const int group = Hq / Hkv, HD = padded_hd(hd), rows = group < q_tile_of(HD) ? group : q_tile_of(HD);
+  return round256((size_t)sms * (2 + warps_of(HD)) * part_floats_of(rows, hd) * 4) + round256(((size_t)B + 1) * 4);
 }
 
 template <typename T, int HD, int NQ>
@@ -624,9 +712,9 @@ int launch(const PagedParams& p, int sms, cudaStream_t st) {
   auto kern = p.page_size % 16 == 0 ? paged_attention_kernel<T, HD, NQ, true> : paged_attention_kernel<T, HD, NQ, false>;
   HB_PROPAGATE(ensure_dynamic_smem((const void*)kern, smem));
   HB_PROPAGATE(launch_chained(kern, dim3((unsigned)sms), dim3(NW * 32), smem, st, false, 1, p));
-  // a warp per row, or sixteen where a row has many parts (few requests)
+  // a warp per row, or eight where a row has many parts (few pairs for the CTAs)
   const int64_t rows = (int64_t)p.B * p.Hq;
-  if ((int64_t)p.B * p.Hkv * p.q_tiles * 8 <= p.workers) return launch_chained(paged_join_kernel<T, 16>, dim3((unsigned)rows), dim3(512), 0, st, true, 1, p);
+  if ((int64_t)p.B * p.Hkv * p.q_tiles * 4 <= sms) return launch_chained(paged_join_kernel<T, 8>, dim3((unsigned)rows), dim3(256), 0, st, true, 1, p);
   return launch_chained(paged_join_kernel<T, 1>, dim3((unsigned)ceil_div64(rows, 8)), dim3(256), 0, st, true, 1, p);
 }
 
@@ -637,13 +725,13 @@ int launch_hd(const PagedParams& p, int sms, cudaStream_t st) {
     case 32: return launch<T, 32, NQ>(p, sms, st);
     case 64: return launch<T, 64, NQ>(p, sms, st);
     case 128: return launch<T, 128, NQ>(p, sms, st);
-    default: return launch<T, 256, NQ>(p, sms, st);
+    default: return launch<T, 256, 1>(p, sms, st);
   }
 }
 
 template <typename T>
 int launch_group(const PagedParams& p, int sms, cudaStream_t st) {
-  return p.group <= 8 ? launch_hd<T, 1>(p, sms, st) : launch_hd<T, 2>(p, sms, st);
+  return p.rows <= 8 ? launch_hd<T, 1>(p, sms, st) : launch_hd<T, 2>(p, sms, st);
 }
 
 int check_heads(const char* what, int64_t B, int Hq, int Hkv, int hd) {
@@ -704,21 +792,22 @@ extern "C" int hb200_paged_decode_attention(const hb200_paged_cache* c, const vo
   p.k_sp = (int32_t)in_bytes[0]; p.k_sr = (int32_t)in_bytes[1]; p.v_sp = (int32_t)in_bytes[2]; p.v_sr = (int32_t)in_bytes[3];
   p.table_ld = table_ld;
   p.B = B; p.Hq = Hq; p.Hkv = c->n_kv_heads; p.hd = c->head_dim; p.group = group;
-  p.q_tiles = (group + 15) / 16;
-  p.rows = group < 16 ? group : 16;
+  const int HD = padded_hd(c->head_dim);
+  p.q_tile = q_tile_of(HD);
+  p.q_tiles = ceil_div(group, p.q_tile);
+  p.rows = group < p.q_tile ? group : p.q_tile;
+  p.part_floats = part_floats_of(p.rows, p.hd);
+  p.tile = tile_tokens(HD);
+  p.warps = warps_of(HD);
   p.page_size = c->page_size; p.width = table_width; p.num_pages = c->num_pages;
-  p.workers = sms * warps_of(padded_hd(c->head_dim));
+  p.ctas = sms;
   // (a scale of zero: near enough to it, so that the -inf of masked tokens stays -inf in the product)
   const double magnitude = scale < 0.f ? -(double)scale : (double)scale;
   p.scale_log2 = magnitude < 1e-30 ? 1e-30f : (float)(magnitude * 1.4426950408889634);
   p.q_sign = scale < 0.f ? 0x80008000u : 0u;
-  const size_t slots = (size_t)p.workers * 2;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
-  p.part_o = reinterpret_cast<float*>(ws);
-  ws += round256(slots * p.rows * p.hd * 4);
-  p.part_ml = reinterpret_cast<float*>(ws);
-  ws += round256(slots * p.rows * 8);
-  p.cum = reinterpret_cast<int32_t*>(ws);
+  p.part = reinterpret_cast<float*>(ws);
+  p.cum = reinterpret_cast<int32_t*>(ws + round256((size_t)sms * (2 + p.warps) * p.part_floats * 4));
   cudaStream_t st = (cudaStream_t)stream;
   if (c->dtype == HB200_BF16) return launch_group<__nv_bfloat16>(p, sms, st);
   if (c->dtype == HB200_F16) return launch_group<__half>(p, sms, st);

@@ -136,6 +136,9 @@ def paged_append(q: Tensor, k: Tensor, v: Tensor, k_cache: Tensor, v_cache: Tens
     return q_out
 
 
+_workspace_bytes: dict = {}     # (device, requests, query heads, kv heads, head size) -> bytes
+
+
 def paged_decode_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_tables: Tensor, kv_lens: Tensor, *,
                            scale: Optional[float] = None, return_lse: bool = False,
                            out: Optional[Tensor] = None) -> Union[Tensor, Tuple[Tensor, Tensor]]:
@@ -178,8 +181,11 @@ def paged_decode_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_ta
     if B > 0:
         with kernels._on(dev):
             L = _lib.lib()
-            n = L.hb200_paged_attention_workspace_bytes(B, Hq, k_cache.shape[1], hd)
-            ws = torch.empty(max(n, 16), dtype=torch.uint8, device=dev)
+            key = (dev.index, B, Hq, cache.n_kv_heads, hd)
+            n = _workspace_bytes.get(key)
+            if n is None:
+                n = _workspace_bytes[key] = L.hb200_paged_attention_workspace_bytes(B, Hq, cache.n_kv_heads, hd)
+            ws = torch.empty(n, dtype=torch.uint8, device=dev)
             _lib.check(L.hb200_paged_decode_attention(
                 cache, q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), lse.data_ptr() if return_lse else None,
                 block_tables.data_ptr(), block_tables.shape[1], block_tables.shape[1], kv_lens.data_ptr(), B, Hq, scale,
