@@ -106,6 +106,7 @@ __device__ __forceinline__ void split2<__half>(float a, float b, uint32_t& hi, u
   lo = *reinterpret_cast<const uint32_t*>(&l);
 }
 
+__device__ __forceinline__ void prefetch(const void* p) { asm volatile("prefetch.global.L1 [%0];" ::"l"(p)); }
 // Transposes an 8x8 matrix of 16-bit values held as in a fragment (thread 4r + c/2 holds (r, c..c+1)).
 __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t a) {
   uint32_t r;
@@ -184,7 +185,6 @@ __global__ void __launch_bounds__(warps_of(HD) * 32, 1) paged_attention_kernel(c
   int left = (int)(end - begin);                     // tiles to compute
   __shared__ int s_pair[2 * NW];                     // of the warps' first and last parts: request * H + head tile, or -1
   __shared__ int s_ends[2 * NW];                     // 1: holds the pair's first tile; 2: its last
-  __shared__ const float* s_part[2 * NW];
   if (lane < 2) s_pair[2 * warp + lane] = -1;
 
   auto enter = [&](Cursor& c) {   // request c.b's length and tiles
@@ -291,6 +291,12 @@ __global__ void __launch_bounds__(warps_of(HD) * 32, 1) paged_attention_kernel(c
         if (pc.b != b || pc.h != h) {
           page0 = off0 = 0;
           head_of();
+          // the next pair's queries (128 bytes a lane) come near before they are asked for
+          const int qt = p.q_tiles == 1 ? 0 : pc.h % p.q_tiles, h0 = (p.q_tiles == 1 ? pc.h : pc.h / p.q_tiles) * p.group + qt * q_tile_of(HD);
+          constexpr int LPQ = (HD * 2 + 127) / 128;         // lanes per query head
+          const int r = lane / LPQ;
+          if (r < min(q_tile_of(HD), p.group - qt * q_tile_of(HD)) && lane % LPQ * 64 < p.hd)
+            prefetch(static_cast<const T*>(p.q) + (int64_t)pc.b * p.q_sb + (int64_t)(h0 + r) * p.q_sh + lane % LPQ * 64);
         }
       }
     }
@@ -469,22 +475,15 @@ __global__ void __launch_bounds__(warps_of(HD) * 32, 1) paged_attention_kernel(c
     --left;
 
     if (cur.t + 1 == cur.n || left == 0) {   // the pair's end, or the share's
-      const bool whole = first_tile == 0 && cur.t + 1 == cur.n;
-      // a part that ends with the share stays in shared memory (the ring is done), one before it goes to the workspace
-      float* po = p.part + ((int64_t)p.ctas * 2 + w) * p.part_floats;
-      if (left == 0) {
-        cp_async_wait<0>();
-        __syncwarp();
-        po = reinterpret_cast<float*>(ring);
-      }
-      if (!whole && lane == 0) {
-        const int k = 2 * warp + (left == 0 ? 1 : 0);
-        s_pair[k] = cur.b * H + cur.h;
-        s_ends[k] = (first_tile == 0 ? 1 : 0) | (cur.t + 1 == cur.n ? 2 : 0);
-        s_part[k] = po;
-      }
-      float* pm = po + p.rows * p.hd;
-      T* ob = static_cast<T*>(p.out) + ((int64_t)cur.b * p.Hq + head0) * p.hd;
+      // It goes through shared memory into rows: at the share's end to the ring's start, where it stays as a part for the CTA
+      // to add up, else through the slot just read (which is not filled again before the next tile) to the workspace or,
+      // if the share held the whole pair, to the output.
+      const bool whole = first_tile == 0 && cur.t + 1 == cur.n, stay = left == 0 && !whole;
+      if (left == 0) cp_async_wait<0>();
+      __syncwarp();
+      float* so = reinterpret_cast<float*>(left == 0 ? ring : ring + (slot == 0 ? ST - 1 : slot - 1) * STAGE);
+      const int ld = stay || NQ > 1 ? p.hd : p.hd + 4;      // (four more words per row: no bank conflicts)
+      float* sm = so + p.rows * p.hd;                       // of a part that stays
 #pragma unroll
       for (int n = 0; n < NQ; ++n)
 #pragma unroll
@@ -493,74 +492,124 @@ __global__ void __launch_bounds__(warps_of(HD) * 32, 1) paged_attention_kernel(c
           sum += __shfl_xor_sync(0xffffffffu, sum, 4);
           sum += __shfl_xor_sync(0xffffffffu, sum, 8);
           sum += __shfl_xor_sync(0xffffffffu, sum, 16);
-          if (poison) sum = __int_as_float(0x7fc00000);
+          l[n][e] = poison ? __int_as_float(0x7fc00000) : sum;
           const int r = n * 8 + t4 * 2 + e;
           if (r < rows_here) {
-            const float inv = 1.f / sum;
+            const float f = whole ? 1.f / l[n][e] : 1.f;
+            float* to = so + r * ld + g;
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-              for (int i = 0; i < 2; ++i) {
-                const int d = ks * 16 + i * 8 + g;
-                if (d < p.hd) {
-                  if (whole) ob[r * p.hd + d] = Cvt<T>::from_f(o[ks][n][i * 2 + e] * inv);
-                  else po[r * p.hd + d] = o[ks][n][i * 2 + e];
-                }
-              }
-            if (g == 0) {
-              if (!whole) *reinterpret_cast<float2*>(pm + r * 2) = make_float2(m[n][e] == -INFINITY ? -INFINITY : base[n][e], sum);
-              else if (p.lse) p.lse[(int64_t)cur.b * p.Hq + head0 + r] = (base[n][e] + log2f(sum)) * kLn2;
-            }
+              for (int i = 0; i < 2; ++i)
+                if (p.hd == HD || ks * 16 + i * 8 < p.hd) to[ks * 16 + i * 8] = o[ks][n][i * 2 + e] * f;
           }
         }
+      __syncwarp();
+      float* pg = p.part + ((int64_t)p.ctas * 2 + w) * p.part_floats;
+      if (!stay) {
+        if (whole) {
+          T* ob = static_cast<T*>(p.out) + ((int64_t)cur.b * p.Hq + head0) * p.hd;
+          const int per = p.hd / 8;
+          for (int u = lane; u < rows_here * per; u += 32) {
+            const int r = u / per, d = (u - r * per) * 8;
+            const float4 x = *reinterpret_cast<const float4*>(so + r * ld + d), y = *reinterpret_cast<const float4*>(so + r * ld + d + 4);
+            T eight[8] = {Cvt<T>::from_f(x.x), Cvt<T>::from_f(x.y), Cvt<T>::from_f(x.z), Cvt<T>::from_f(x.w),
+                          Cvt<T>::from_f(y.x), Cvt<T>::from_f(y.y), Cvt<T>::from_f(y.z), Cvt<T>::from_f(y.w)};
+            *reinterpret_cast<uint4*>(ob + r * p.hd + d) = *reinterpret_cast<const uint4*>(eight);
+          }
+        } else {
+          const int per = p.hd / 4;
+          for (int u = lane; u < rows_here * per; u += 32) {
+            const int r = u / per, d = (u - r * per) * 4;
+            *reinterpret_cast<float4*>(pg + r * p.hd + d) = *reinterpret_cast<const float4*>(so + r * ld + d);
+          }
+          sm = pg + p.rows * p.hd;
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < NQ; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int r = n * 8 + t4 * 2 + e;
+          if (g == 0 && r < rows_here) {
+            if (!whole) *reinterpret_cast<float2*>(sm + r * 2) = make_float2(m[n][e] == -INFINITY ? -INFINITY : base[n][e], l[n][e]);
+            else if (p.lse) p.lse[(int64_t)cur.b * p.Hq + head0 + r] = (base[n][e] + log2f(l[n][e])) * kLn2;
+          }
+        }
+      if (!whole && lane == 0) {
+        const int k = 2 * warp + (left == 0 ? 1 : 0);
+        s_pair[k] = cur.b * H + cur.h;
+        s_ends[k] = (first_tile == 0 ? 1 : 0) | (cur.t + 1 == cur.n ? 2 : 0);
+      }
+      __syncwarp();
+      if (p.hd < HD && left > 0) {                          // the slot's padding chunks back to zero
+        for (int u = lane; u < STAGE / 16; u += 32) reinterpret_cast<uint4*>(so)[u] = make_uint4(0, 0, 0, 0);
+        __syncwarp();
+      }
       fresh = true;
     }
     if (left > 0) advance(cur);
   }
   __syncthreads();
 
-  // the parts of one pair, neighbours in the order of the warps' shares: a thread has four values of one row
+  // The parts of one pair, neighbours in the order of the warps' shares (place 2 w: warp w's first, in the workspace; 2 w + 1: its
+  // last, in shared memory).  A thread has four values of one row, all parts' values on their way at once.
+  const int my_pair = lane < 2 * NW ? s_pair[lane] : -1;
+  const unsigned same = __match_any_sync(0xffffffffu, my_pair);
   const int quads = p.hd / 4;
-  for (int k0 = 0; k0 < 2 * NW;) {
-    const int pair = s_pair[k0];
-    if (pair < 0) { ++k0; continue; }
-    int k1 = k0 + 1, ends = s_ends[k0], last = k0;
-    for (; k1 < 2 * NW && (s_pair[k1] < 0 || s_pair[k1] == pair); ++k1)
-      if (s_pair[k1] == pair) { ends |= s_ends[k1]; last = k1; }
+  for (unsigned todo = __ballot_sync(0xffffffffu, my_pair >= 0); todo;) {
+    const int k0 = __ffs(todo) - 1;
+    const unsigned mask = __shfl_sync(0xffffffffu, same, k0);
+    const int pair = __shfl_sync(0xffffffffu, my_pair, k0), ends = s_ends[k0] | s_ends[31 - __clz(mask)];
+    todo &= ~mask;
     const int b = pair / H, h = pair - b * H;
     const int kvh = p.q_tiles == 1 ? h : h / p.q_tiles, qt = h - kvh * p.q_tiles;
     const int head = kvh * p.group + qt * q_tile_of(HD), rows = min(q_tile_of(HD), p.group - qt * q_tile_of(HD));
     // (the CTA's first tile belongs to its first part's pair: the join finds that one in place 0, one that begins later in 1)
     const int64_t t0 = (int64_t)s_cum[b] * H + (int64_t)h * (s_cum[b + 1] - s_cum[b]);
     float* po = p.part + ((int64_t)blockIdx.x * 2 + (t0 <= (int64_t)blockIdx.x * NW * share ? 0 : 1)) * p.part_floats;
+    const float* in_ws = p.part + ((int64_t)p.ctas * 2 + blockIdx.x * NW) * p.part_floats;
     for (int i = threadIdx.x; i < rows * quads; i += NW * 32) {
       const int r = i / quads, d = (i - r * quads) * 4;
-      float m = -INFINITY;
-      for (int k = k0; k <= last; ++k)
-        if (s_pair[k] >= 0) m = fmaxf(m, s_part[k][p.rows * p.hd + 2 * r]);
-      const float base = m == -INFINITY ? 0.f : m;
-      float l = 0.f;
+      float m = -INFINITY, l = 0.f;
       float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int k = k0; k <= last; ++k)
-        if (s_pair[k] >= 0) {
-          const float* o = s_part[k];
-          const float f = ex2(o[p.rows * p.hd + 2 * r] - base);
-          const float4 v = *reinterpret_cast<const float4*>(o + r * p.hd + d);
-          l = fmaf(f, o[p.rows * p.hd + 2 * r + 1], l);
-          acc.x = fmaf(f, v.x, acc.x); acc.y = fmaf(f, v.y, acc.y); acc.z = fmaf(f, v.z, acc.z); acc.w = fmaf(f, v.w, acc.w);
+#pragma unroll
+      for (int k8 = 0; k8 < 2 * NW; k8 += 8) {          // eight places at a time
+        if (((mask >> k8) & 0xff) == 0) continue;
+        float2 ml[8];
+        float4 v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const float* part = (k & 1) ? reinterpret_cast<const float*>(smem + ((k8 + k) / 2) * ST * STAGE) : in_ws + ((k8 + k) / 2) * p.part_floats;
+          const bool there = (mask >> (k8 + k)) & 1;
+          ml[k] = there ? *reinterpret_cast<const float2*>(part + p.rows * p.hd + 2 * r) : make_float2(-INFINITY, 0.f);
+          v[k] = there ? *reinterpret_cast<const float4*>(part + r * p.hd + d) : make_float4(0.f, 0.f, 0.f, 0.f);
         }
+        float to = m;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) to = fmaxf(to, ml[k].x);
+        const float base = to == -INFINITY ? 0.f : to, f = ex2(m - base);
+        l *= f;
+        acc.x *= f; acc.y *= f; acc.z *= f; acc.w *= f;
+        m = to;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const float f = ex2(ml[k].x - base);
+          l = fmaf(f, ml[k].y, l);
+          acc.x = fmaf(f, v[k].x, acc.x); acc.y = fmaf(f, v[k].y, acc.y); acc.z = fmaf(f, v[k].z, acc.z); acc.w = fmaf(f, v[k].w, acc.w);
+        }
+      }
       if (ends == 3) {
         const float inv = 1.f / l;
         const int64_t at = (int64_t)b * p.Hq + head + r;
         T four[4] = {Cvt<T>::from_f(acc.x * inv), Cvt<T>::from_f(acc.y * inv), Cvt<T>::from_f(acc.z * inv), Cvt<T>::from_f(acc.w * inv)};
         *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + at * p.hd + d) = *reinterpret_cast<const uint2*>(four);
-        if (d == 0 && p.lse) p.lse[at] = (base + log2f(l)) * kLn2;
+        if (d == 0 && p.lse) p.lse[at] = ((m == -INFINITY ? 0.f : m) + log2f(l)) * kLn2;
       } else {
         *reinterpret_cast<float4*>(po + r * p.hd + d) = acc;
         if (d == 0) *reinterpret_cast<float2*>(po + p.rows * p.hd + 2 * r) = make_float2(m, l);
       }
     }
-    k0 = last + 1;
   }
 }
 
