@@ -10,7 +10,9 @@
 //
 // Work split: the tiles of all (request, kv head) pairs are laid end to end and dealt out in equal contiguous shares to
 // the warps of a grid that fits the GPU once (one CTA per SM), whatever the lengths are: a batch of one long and many
-// short requests keeps every SM busy to the end.  The lengths live on the device; each CTA scans them itself.  A warp
+// short requests keeps every SM busy to the end.  Starting and finishing a pair costs a warp about as much as a tile, so each
+// pair is that much longer when the shares are cut (without it 256 requests of 1 to 300 tokens took 69 us, their warps'
+// loops between 28 and 60).  The lengths live on the device; each CTA scans them itself.  A warp
 // streams its share through a private cp.async ring that runs on across the ends of requests, so no barrier is met between
 // the scan and the share's end.  A pair that lies within one share is finished by its warp.  Of the others each warp leaves
 // (max, sum, unnormalised output) in 32 bits; the CTA, whose warps' shares are neighbours, adds up those of one pair, and
@@ -38,17 +40,21 @@ struct PagedParams {
   int32_t* cum;      // [B + 1] tiles of the requests before each one
   int64_t q_sb, q_sh, k_sh, v_sh, table_ld;     // elements
   int32_t k_sp, k_sr, v_sp, v_sr;               // bytes: page and row of a page
-  int B, Hq, Hkv, hd, group, q_tiles, q_tile, tile, warps, rows, part_floats, page_size, width, num_pages, ctas;
+  int B, Hq, Hkv, hd, group, q_tiles, q_tile, tile, pair_cost, warps, rows, part_floats, page_size, width, num_pages, ctas;
   float scale_log2;  // |scale| log2(e)
   uint32_t q_sign;   // flips the signs of a pair of query values where the scale is negative
 };
 
-// A warp's tile: 8 KB of K and V (16 KB of heads of 256, 4 KB of small ones); its ring keeps 16 KB in flight, a CTA 128 KB.
+// A warp's tile: 8 KB of K and V (16 KB of heads of 256, 4 KB of small ones, whose tokens cost more arithmetic per byte and get
+// twice the warps: 64 requests up to 16384 tokens on 4 kv heads of 16 took 45 us with eight warps, 43 with sixteen); two
+// tiles of a warp are in flight while one is computed, 128 KB of a CTA.
 __host__ __device__ constexpr int tile_tokens(int HD) { return HD >= 128 ? 16 : (HD == 16 ? 64 : 32); }
-__host__ __device__ constexpr int warps_of(int HD) { return HD >= 256 ? 4 : 8; }
+__host__ __device__ constexpr int warps_of(int HD) { return HD >= 256 ? 4 : (HD <= 32 ? 16 : 8); }
 // Query heads that are worked on together: their outputs and queries stay in a warp's registers.
 __host__ __device__ constexpr int q_tile_of(int HD) { return HD >= 256 ? 8 : 16; }
-__host__ __device__ constexpr int stages_of(int HD) { return HD <= 32 ? 5 : 3; }
+// Places that a pair takes before its first tile when the shares are cut: what its start and end cost, in tiles.
+__host__ __device__ constexpr int pair_cost(int HD) { return HD <= 32 ? 2 : 1; }
+__host__ __device__ constexpr int stages_of(int) { return 3; }
 
 // Cache length of request b as the kernel reads it: what lies outside [0, width * page_size] is marked (`poison`).
 __device__ __forceinline__ int clamp_len(int len, int64_t cap, bool& poison) {
@@ -138,6 +144,7 @@ __global__ void __launch_bounds__(warps_of(HD) * 32, 1) paged_attention_kernel(c
   constexpr int LPR = CH >= 4 ? 4 : CH;              // copies: lanes per row (64 bytes side by side)
   constexpr int RPI = 32 / LPR, R = TT / RPI;        // rows per copy instruction, rows per lane
   constexpr int CI = CH / LPR;                       // copies per row and lane
+  constexpr int PC = pair_cost(HD);
   constexpr int NO = KS < 4 ? KS : 4;                // distinct swizzled offsets of the 16-value steps
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int scan_buf[33];
@@ -146,7 +153,7 @@ __global__ void __launch_bounds__(warps_of(HD) * 32, 1) paged_attention_kernel(c
   int32_t* s_len = s_cum + p.B + 1;                                      // [B]
   chain_release();   // the join kernel may take its place; it waits for this grid's end before it reads anything
 
-  // tiles before each request
+  // places before each request: of its tiles, and PC before those of each request that has any
   const int64_t cap = (int64_t)p.width * p.page_size;
   {
     const int per = (p.B + NW * 32 - 1) / (NW * 32);
@@ -159,7 +166,7 @@ __global__ void __launch_bounds__(warps_of(HD) * 32, 1) paged_attention_kernel(c
         bool poison;
         const int len = clamp_len(raw, cap, poison);
         s_len[b] = poison ? -1 - len : len;
-        mine += (len + TT - 1) / TT;
+        mine += len > 0 ? (len + TT - 1) / TT + PC : 0;
       }
     }
     int total;
@@ -169,7 +176,8 @@ __global__ void __launch_bounds__(warps_of(HD) * 32, 1) paged_attention_kernel(c
       if (b < p.B) {
         s_cum[b] = at;
         const int v = s_len[b];
-        at += ((v < 0 ? -1 - v : v) + TT - 1) / TT;
+        const int len = v < 0 ? -1 - v : v;
+        at += len > 0 ? (len + TT - 1) / TT + PC : 0;
       }
     }
     if (threadIdx.x == 0) s_cum[p.B] = total;
@@ -182,13 +190,42 @@ __global__ void __launch_bounds__(warps_of(HD) * 32, 1) paged_attention_kernel(c
   const int64_t share = div_up(total, p.ctas * NW);
   const int w = blockIdx.x * NW + warp;
   const int64_t begin = min((int64_t)w * share, total), end = min(begin + share, total);
-  int left = (int)(end - begin);                     // tiles to compute
+  // request b, head tile h and place `at` of place v < total, and the tiles before it
+  auto locate = [&](int64_t v, int& b, int& h, int& at) {
+    int lo = 0, hi = p.B;   // s_cum[lo] * H <= v < s_cum[hi] * H
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if ((int64_t)s_cum[mid] * H <= v) lo = mid; else hi = mid;
+    }
+    int some = 0;           // requests before it that have tiles
+    for (int a = lane; a < lo; a += 32) some += s_len[a] != 0;
+    some = __reduce_add_sync(0xffffffffu, some);
+    const unsigned r = (unsigned)(v - (int64_t)s_cum[lo] * H), width = s_cum[lo + 1] - s_cum[lo];
+    b = lo;
+    h = (int)(r / width);
+    at = (int)(r - h * width);
+    return v - (int64_t)PC * ((int64_t)some * H + h) - min(at, PC);
+  };
+  Cursor cur = {};
+  int left = 0;                                      // tiles to compute
+  if (begin < total) {
+    int64_t after = 0;
+#pragma unroll 1
+    for (int k = 0; k < 2; ++k) {                    // the share's last place, then its first
+      int at = 0;
+      const int64_t n = locate(k ? begin : end - 1, cur.b, cur.h, at);
+      if (k == 0) after = n + (at >= PC ? 1 : 0);
+      left = (int)(after - n);
+      cur.t = max(at - PC, 0);
+    }
+  }
   __shared__ int s_pair[2 * NW];                     // of the warps' first and last parts: request * H + head tile, or -1
   __shared__ int s_ends[2 * NW];                     // 1: holds the pair's first tile; 2: its last
   if (lane < 2) s_pair[2 * warp + lane] = -1;
 
   auto enter = [&](Cursor& c) {   // request c.b's length and tiles
     c.n = s_cum[c.b + 1] - s_cum[c.b];
+    c.n -= c.n > 0 ? PC : 0;
     const int v = s_len[c.b];
     c.poison = v < 0;
     c.len = v < 0 ? -1 - v : v;
@@ -202,19 +239,7 @@ __global__ void __launch_bounds__(warps_of(HD) * 32, 1) paged_attention_kernel(c
       }
     }
   };
-  Cursor cur = {};
-  if (left > 0) {
-    int lo = 0, hi = p.B;   // s_cum[lo] * H <= begin < s_cum[hi] * H
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if ((int64_t)s_cum[mid] * H <= begin) lo = mid; else hi = mid;
-    }
-    cur.b = lo;
-    enter(cur);
-    const int r = (int)(begin - (int64_t)s_cum[lo] * H);
-    cur.h = r / cur.n;
-    cur.t = r % cur.n;
-  }
+  if (left > 0) enter(cur);
 
   uint8_t* ring = smem + warp * ST * STAGE;
   const uint32_t ring_u = smem_u32(ring);
@@ -550,54 +575,50 @@ __global__ void __launch_bounds__(warps_of(HD) * 32, 1) paged_attention_kernel(c
     }
     if (left > 0) advance(cur);
   }
+  // (a first part in the workspace comes back near the SM before the CTA adds it up)
+  if (s_pair[2 * warp] >= 0)
+    for (int i = lane * 32; i < p.part_floats; i += 1024) prefetch(p.part + ((int64_t)p.ctas * 2 + w) * p.part_floats + i);
   __syncthreads();
 
   // The parts of one pair, neighbours in the order of the warps' shares (place 2 w: warp w's first, in the workspace; 2 w + 1: its
-  // last, in shared memory).  A thread has four values of one row, all parts' values on their way at once.
+  // last, in shared memory).  Several pairs are shared out over the warps.
   const int my_pair = lane < 2 * NW ? s_pair[lane] : -1;
   const unsigned same = __match_any_sync(0xffffffffu, my_pair);
-  const int quads = p.hd / 4;
-  for (unsigned todo = __ballot_sync(0xffffffffu, my_pair >= 0); todo;) {
-    const int k0 = __ffs(todo) - 1;
+  unsigned firsts = __ballot_sync(0xffffffffu, my_pair >= 0 && (same & ((1u << lane) - 1)) == 0);   // of each pair's parts
+  const int quads = p.hd / 4, pairs = __popc(firsts);
+  const int wpp = NW / max(1, min(pairs, NW));              // warps per pair
+  for (int n = 0; n < pairs; ++n) {
+    const int k0 = __ffs(firsts) - 1;
+    firsts &= firsts - 1;
     const unsigned mask = __shfl_sync(0xffffffffu, same, k0);
     const int pair = __shfl_sync(0xffffffffu, my_pair, k0), ends = s_ends[k0] | s_ends[31 - __clz(mask)];
-    todo &= ~mask;
+    if (n % (NW / wpp) != warp / wpp) continue;
     const int b = pair / H, h = pair - b * H;
     const int kvh = p.q_tiles == 1 ? h : h / p.q_tiles, qt = h - kvh * p.q_tiles;
     const int head = kvh * p.group + qt * q_tile_of(HD), rows = min(q_tile_of(HD), p.group - qt * q_tile_of(HD));
-    // (the CTA's first tile belongs to its first part's pair: the join finds that one in place 0, one that begins later in 1)
-    const int64_t t0 = (int64_t)s_cum[b] * H + (int64_t)h * (s_cum[b + 1] - s_cum[b]);
-    float* po = p.part + ((int64_t)blockIdx.x * 2 + (t0 <= (int64_t)blockIdx.x * NW * share ? 0 : 1)) * p.part_floats;
+    // (the join finds the part of a pair that began in a CTA before this one in place 0, of one that goes on in the next in 1)
+    const int64_t t0 = (int64_t)s_cum[b] * H + (int64_t)h * (s_cum[b + 1] - s_cum[b]) + PC;   // the pair's first tile
+    float* po = p.part + ((int64_t)blockIdx.x * 2 + (t0 < (int64_t)blockIdx.x * NW * share ? 0 : 1)) * p.part_floats;
     const float* in_ws = p.part + ((int64_t)p.ctas * 2 + blockIdx.x * NW) * p.part_floats;
-    for (int i = threadIdx.x; i < rows * quads; i += NW * 32) {
+    // (rolled up: this runs once, and what it costs is the way of its instructions to the SM)
+#pragma unroll 1
+    for (int i = (warp % wpp) * 32 + lane; i < rows * quads; i += wpp * 32) {
       const int r = i / quads, d = (i - r * quads) * 4;
       float m = -INFINITY, l = 0.f;
       float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-      for (int k8 = 0; k8 < 2 * NW; k8 += 8) {          // eight places at a time
-        if (((mask >> k8) & 0xff) == 0) continue;
-        float2 ml[8];
-        float4 v[8];
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const float* part = (k & 1) ? reinterpret_cast<const float*>(smem + ((k8 + k) / 2) * ST * STAGE) : in_ws + ((k8 + k) / 2) * p.part_floats;
-          const bool there = (mask >> (k8 + k)) & 1;
-          ml[k] = there ? *reinterpret_cast<const float2*>(part + p.rows * p.hd + 2 * r) : make_float2(-INFINITY, 0.f);
-          v[k] = there ? *reinterpret_cast<const float4*>(part + r * p.hd + d) : make_float4(0.f, 0.f, 0.f, 0.f);
-        }
-        float to = m;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) to = fmaxf(to, ml[k].x);
-        const float base = to == -INFINITY ? 0.f : to, f = ex2(m - base);
-        l *= f;
-        acc.x *= f; acc.y *= f; acc.z *= f; acc.w *= f;
+#pragma unroll 1
+      for (unsigned parts = mask; parts; parts &= parts - 1) {
+        const int k = __ffs(parts) - 1;
+        const float* part = (k & 1) ? reinterpret_cast<const float*>(smem + (k / 2) * ST * STAGE) : in_ws + (k / 2) * p.part_floats;
+        const float2 ml = *reinterpret_cast<const float2*>(part + p.rows * p.hd + 2 * r);
+        const float4 v = *reinterpret_cast<const float4*>(part + i * 4);
+        const float to = fmaxf(m, ml.x), base = to == -INFINITY ? 0.f : to, f = ex2(m - base), g = ex2(ml.x - base);
         m = to;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const float f = ex2(ml[k].x - base);
-          l = fmaf(f, ml[k].y, l);
-          acc.x = fmaf(f, v[k].x, acc.x); acc.y = fmaf(f, v[k].y, acc.y); acc.z = fmaf(f, v[k].z, acc.z); acc.w = fmaf(f, v[k].w, acc.w);
-        }
+        l = fmaf(l, f, g * ml.y);
+        acc.x = fmaf(acc.x, f, g * v.x);
+        acc.y = fmaf(acc.y, f, g * v.y);
+        acc.z = fmaf(acc.z, f, g * v.z);
+        acc.w = fmaf(acc.w, f, g * v.w);
       }
       if (ends == 3) {
         const float inv = 1.f / l;
@@ -606,7 +627,7 @@ __global__ void __launch_bounds__(warps_of(HD) * 32, 1) paged_attention_kernel(c
         *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + at * p.hd + d) = *reinterpret_cast<const uint2*>(four);
         if (d == 0 && p.lse) p.lse[at] = ((m == -INFINITY ? 0.f : m) + log2f(l)) * kLn2;
       } else {
-        *reinterpret_cast<float4*>(po + r * p.hd + d) = acc;
+        *reinterpret_cast<float4*>(po + i * 4) = acc;
         if (d == 0) *reinterpret_cast<float2*>(po + p.rows * p.hd + 2 * r) = make_float2(m, l);
       }
     }
@@ -634,7 +655,7 @@ __global__ void __launch_bounds__(WPR > 8 ? WPR * 32 : 256) paged_join_kernel(co
     const int64_t cap = (int64_t)p.width * p.page_size;
     for (int a = lane; a < p.B; a += 32) {
       bool poison;
-      const int t = (clamp_len(__ldg(p.lens + a), cap, poison) + p.tile - 1) / p.tile;
+      const int len = clamp_len(__ldg(p.lens + a), cap, poison), t = len > 0 ? (len + p.tile - 1) / p.tile + p.pair_cost : 0;
       all += t;
       before += a < b ? t : 0;
       n += a == b ? t : 0;
@@ -653,13 +674,13 @@ __global__ void __launch_bounds__(WPR > 8 ? WPR * 32 : 256) paged_join_kernel(co
   }
   const int64_t total = (int64_t)all * H;
   const int64_t share = div_up(total, p.ctas * p.warps) * p.warps;             // of a CTA
-  const int64_t t0 = (int64_t)before * H + (int64_t)(kvh * p.q_tiles + qt) * n, t1 = t0 + n;
+  const int64_t t0 = (int64_t)before * H + (int64_t)(kvh * p.q_tiles + qt) * n + p.pair_cost, t1 = t0 + n - p.pair_cost;   // its tiles
   int w0 = 0, w1 = 0;
   if (n > 0) {
     w0 = total <= 0x7fffffff ? (int)((unsigned)t0 / (unsigned)share) : (int)(t0 / share);
     w1 = total <= 0x7fffffff ? (int)((unsigned)(t1 - 1) / (unsigned)share) : (int)((t1 - 1) / share);
   }
-  const int64_t first = (int64_t)w0 * 2 + (t0 == (int64_t)w0 * share ? 0 : 1);
+  const int64_t first = (int64_t)w0 * 2 + 1;     // (the part of the CTA that the pair begins in)
   const int parts = w1 - w0 + 1;
   if (early) chain_wait();
   if (!live) return;                            // (only with WPR = 1, where no barrier follows)
@@ -829,7 +850,7 @@ extern "C" int hb200_paged_decode_attention(const hb200_paged_cache* c, const vo
              workspace_for(B, Hq, c->n_kv_heads, c->head_dim, sms));
   // lengths are clamped to the table's reach, so this bounds every tile count in 32 bits
   const int64_t cap = (int64_t)table_width * c->page_size;
-  HB_REQUIRE(cap <= 0x7fffff00 && (int64_t)B * (cap / 16 + 1) <= 0x7fffffff, HB200_ERR_UNSUPPORTED,
+  HB_REQUIRE(cap <= 0x7fffff00 && (int64_t)B * (cap / 16 + 4) <= 0x7fffffff, HB200_ERR_UNSUPPORTED,
              "paged_decode_attention: tables of %d pages of %d tokens for %d requests reach too far", table_width, c->page_size, B);
   PagedParams p = {};
   p.q = q; p.kc = c->k; p.vc = c->v; p.out = out; p.lse = lse; p.table = block_tables; p.lens = kv_lens;
@@ -847,6 +868,7 @@ extern "C" int hb200_paged_decode_attention(const hb200_paged_cache* c, const vo
   p.rows = group < p.q_tile ? group : p.q_tile;
   p.part_floats = part_floats_of(p.rows, p.hd);
   p.tile = tile_tokens(HD);
+  p.pair_cost = pair_cost(HD);
   p.warps = warps_of(HD);
   p.page_size = c->page_size; p.width = table_width; p.num_pages = c->num_pages;
   p.ctas = sms;
