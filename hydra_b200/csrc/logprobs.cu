@@ -62,18 +62,22 @@ __device__ __forceinline__ float key_value(uint32_t k) {
 __device__ __forceinline__ uint64_t entry(float v, int i) { return ((uint64_t)order_key(v) << 32) | (uint32_t)~i; }
 __device__ __forceinline__ int entry_index(uint64_t e) { return (int)~(uint32_t)e; }
 
-// Running statistics of the logits a thread (a row) has seen: maximum m, and sum 2^t and sum t 2^t of t = (x - base) c, in
-// powers of two (c = log2(e) / T).  base is m kept finite: a thread may have seen nothing but -inf.  (x - base is formed before
-// the product: x c less a rounded m c would be off by 2^-24 of m c, whatever its size.)
+// Statistics of logits: maximum m, and sum 2^t and sum t 2^t with t = x c - ref(m) in powers of two, c = log2(e) / T.  ref is m c as
+// rounded to 32 bits: one fused multiply-add per logit, and exact, since all logits are off by the same off(m) = m c - ref(m),
+// which the results put right.  It is kept within kReach, where off is below one (a thread may have seen nothing but -inf);
+// a row whose maximum lies beyond (logits of millions, or a temperature near nothing) is summed up again from (x - m) c.
 struct Stat {
   float m, s, u;
 };
-__device__ __forceinline__ float base_of(float m) { return fmaxf(m, -3.402823466e38f); }
-__device__ __forceinline__ void rebase(Stat& a, float m, float c) {   // m >= a.m
-  const float d = fmaxf((base_of(a.m) - base_of(m)) * c, -200.f), f = ex2f(d);
+constexpr float kReach = 4e6f;
+__device__ __forceinline__ float ref_of(float m, float c) { return fminf(fmaxf(m * c, -kReach), kReach); }
+__device__ __forceinline__ bool beyond(float m, float c) { return fabsf(m * c) > kReach; }
+__device__ __forceinline__ float off_of(float m, float c) { return beyond(m, c) ? 0.f : fmaf(m, c, -(m * c)); }
+__device__ __forceinline__ void rebase(Stat& a, float d) {   // to a reference that is -d larger
+  d = fmaxf(d, -200.f);
+  const float f = ex2f(d);
   a.u = f * fmaf(d, a.s, a.u);
   a.s *= f;
-  a.m = m;
 }
 
 // Two 32-bit values in one operation.
@@ -99,68 +103,95 @@ __device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
   return r;
 }
 
-// One 16-byte piece.
+// A 16-byte piece's maximum (NaN left out), and its values.  kRaised: those far below the reach come raised to `low`, two at
+// a time in their own type (a bf16 reaches that far at every temperature), so that 2^t = 0 meets a finite t and no infinity.
 template <typename T> struct Piece;
 template <> struct Piece<float> {
-  float f[4];
-  __device__ explicit Piece(const uint4& r) {
+  static constexpr bool kRaised = false;
+  static __device__ __forceinline__ uint32_t low(float) { return 0; }
+  static __device__ __forceinline__ float max(const uint4& r) {
+    return fmaxf(fmaxf(__uint_as_float(r.x), __uint_as_float(r.y)), fmaxf(__uint_as_float(r.z), __uint_as_float(r.w)));
+  }
+  static __device__ __forceinline__ void values(const uint4& r, uint32_t, float (&f)[4]) {
     f[0] = __uint_as_float(r.x); f[1] = __uint_as_float(r.y); f[2] = __uint_as_float(r.z); f[3] = __uint_as_float(r.w);
   }
-  __device__ float max() const { return fmaxf(fmaxf(f[0], f[1]), fmaxf(f[2], f[3])); }
 };
 template <> struct Piece<__nv_bfloat16> {
-  float f[8];
-  __nv_bfloat162 top;
-  __device__ explicit Piece(const uint4& r) {
-    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
-    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(w);
-    top = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
-#pragma unroll
-    for (int i = 0; i < 4; ++i) { f[2 * i] = __uint_as_float(w[i] << 16); f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
+  static constexpr bool kRaised = true;
+  static __device__ __forceinline__ uint32_t low(float v) { return pack_bf16x2(v, v); }
+  static __device__ __forceinline__ __nv_bfloat162 as2(uint32_t w) { return *reinterpret_cast<__nv_bfloat162*>(&w); }
+  static __device__ __forceinline__ float max(const uint4& r) {
+    const __nv_bfloat162 t = __hmax2(__hmax2(as2(r.x), as2(r.y)), __hmax2(as2(r.z), as2(r.w)));
+    return fmaxf(__low2float(t), __high2float(t));
   }
-  __device__ float max() const { return fmaxf(__low2float(top), __high2float(top)); }
+  static __device__ __forceinline__ void values(const uint4& r, uint32_t low, float (&f)[8]) {
+    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __nv_bfloat162 h = __hmax2_nan(as2(w[i]), as2(low));
+      const uint32_t b = *reinterpret_cast<const uint32_t*>(&h);
+      f[2 * i] = __uint_as_float(b << 16);
+      f[2 * i + 1] = __uint_as_float(b & 0xffff0000u);
+    }
+  }
 };
 template <> struct Piece<__half> {
-  float f[8];
-  __half2 top;
-  __device__ explicit Piece(const uint4& r) {
-    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
-    const __half2* h = reinterpret_cast<const __half2*>(w);
-    top = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
-#pragma unroll
-    for (int i = 0; i < 4; ++i) { const float2 t = __half22float2(h[i]); f[2 * i] = t.x; f[2 * i + 1] = t.y; }
+  static constexpr bool kRaised = false;
+  static __device__ __forceinline__ uint32_t low(float) { return 0; }
+  static __device__ __forceinline__ __half2 as2(uint32_t w) { return *reinterpret_cast<__half2*>(&w); }
+  static __device__ __forceinline__ float max(const uint4& r) {
+    const __half2 t = __hmax2(__hmax2(as2(r.x), as2(r.y)), __hmax2(as2(r.z), as2(r.w)));
+    return fmaxf(__low2float(t), __high2float(t));
   }
-  __device__ float max() const { return fmaxf(__low2float(top), __high2float(top)); }
+  static __device__ __forceinline__ void values(const uint4& r, uint32_t, float (&f)[8]) {
+    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { const float2 t = __half22float2(as2(w[i])); f[2 * i] = t.x; f[2 * i + 1] = t.y; }
+  }
 };
 
 // What a thread keeps while it reads: its maximum and the sums of its even and of its odd columns.  -inf (and anything far
-// below) counts as 2^-200 = 0 times a finite distance; NaN and +inf stay NaN.
+// below) counts as 2^t = 0 times a finite distance; NaN stays NaN, +inf gives infinite sums.
+template <typename T>
 struct Running {
-  float m;
-  F2 s, u;
-  __device__ Running() : m(-INFINITY), s(0.f, 0.f), u(0.f, 0.f) {}
+  float m, ref;
+  uint32_t low;
+  F2 c2, s, u;
+  __device__ explicit Running(float c) : m(-INFINITY), ref(-kReach), low(Piece<T>::low(-2.5f * kReach / c)), c2(c, c), s(0.f, 0.f), u(0.f, 0.f) {}
   __device__ __forceinline__ void raise(float to, float c) {   // the maximum (a NaN is none)
     if (to > m) {
-      const float d = fmaxf((base_of(m) - base_of(to)) * c, -200.f), f = ex2f(d);
+      m = to;
+      const float next = ref_of(to, c), d = fmaxf(ref - next, -200.f), f = ex2f(d);
       const F2 f2(f, f);
       u = mul2(fma2(F2(d, d), s, u), f2);
       s = mul2(s, f2);
-      m = to;
+      ref = next;
     }
   }
-  template <int N>
-  __device__ __forceinline__ void add(const float (&f)[N], F2 c2) {
-    const F2 nb2(-base_of(m), -base_of(m));
+  __device__ __forceinline__ void add(const uint4& raw) {
+    constexpr int V = 16 / sizeof(T);
+    const F2 n2(-ref, -ref);
+    float f[V];
+    Piece<T>::values(raw, low, f);
 #pragma unroll
-    for (int i = 0; i < N; i += 2) {
+    for (int i = 0; i < V; i += 2) {
+      F2 t = fma2(F2(f[i], f[i + 1]), c2, n2);
       float t0, t1;
-      mul2(add2(F2(f[i], f[i + 1]), nb2), c2).get(t0, t1);
-      t0 = max_nan(t0, -200.f);
-      t1 = max_nan(t1, -200.f);
+      t.get(t0, t1);
+      if (!Piece<T>::kRaised) {
+        t0 = max_nan(t0, -200.f);
+        t1 = max_nan(t1, -200.f);
+        t = F2(t0, t1);
+      }
       const F2 e(ex2f(t0), ex2f(t1));
       s = add2(s, e);
-      u = fma2(F2(t0, t1), e, u);
+      u = fma2(t, e, u);
     }
+  }
+  __device__ __forceinline__ void add1(float f, float c) {
+    const float t = max_nan(fmaf(f, c, -ref), -200.f), e = ex2f(t);
+    s = add2(s, F2(e, 0.f));
+    u = fma2(F2(t, 0.f), F2(e, 0.f), u);
   }
   __device__ __forceinline__ Stat stat() const {
     Stat r;
@@ -200,27 +231,24 @@ __global__ void __launch_bounds__(NT) token_logprobs_kernel(const LogprobParams 
   const T* x = row + c0;
   const float c = p.inv_t * kLog2e;
   const int64_t tgt = rank == 0 ? p.tokens[r] : 0;
-  const bool scored = rank == 0 && tid == 0 && tgt >= 0 && tgt < p.cols;
-  const float x_tgt = scored ? Cvt<T>::to_f(row[tgt]) : 0.f;
 
   // values before the first 16-byte boundary, 16-byte pieces, values behind the last
   const int to_boundary = (int)(((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / sizeof(T));
   const int head = min(n, to_boundary), pieces = (n - head) / V, edge = head + (n - head - pieces * V);
   const uint4* xv = reinterpret_cast<const uint4*>(x + head);
   auto edge_at = [&](int i) { return i < head ? i : pieces * V + i; };   // i-th value outside the pieces -> its column
-  const F2 c2(c, c);
-  Running own;
+  Running<T> own(c);
   int v0 = tid;
   for (; v0 + (kUnroll - 1) * NT < pieces; v0 += kUnroll * NT) {   // four pieces, one look at their maximum
     uint4 raw[kUnroll];
 #pragma unroll
     for (int k = 0; k < kUnroll; ++k) raw[k] = __ldg(xv + v0 + k * NT);
-    float mx = Piece<T>(raw[0]).max();
+    float mx = Piece<T>::max(raw[0]);
 #pragma unroll
-    for (int k = 1; k < kUnroll; ++k) mx = fmaxf(mx, Piece<T>(raw[k]).max());
+    for (int k = 1; k < kUnroll; ++k) mx = fmaxf(mx, Piece<T>::max(raw[k]));
     own.raise(mx, c);
 #pragma unroll
-    for (int k = 0; k < kUnroll; ++k) own.add(Piece<T>(raw[k]).f, c2);
+    for (int k = 0; k < kUnroll; ++k) own.add(raw[k]);
   }
   {
     uint4 raw[kUnroll - 1];
@@ -230,16 +258,17 @@ __global__ void __launch_bounds__(NT) token_logprobs_kernel(const LogprobParams 
 #pragma unroll
     for (int k = 0; k < kUnroll - 1; ++k)
       if (v0 + k * NT < pieces) {
-        const Piece<T> q(raw[k]);
-        own.raise(q.max(), c);
-        own.add(q.f, c2);
+        own.raise(Piece<T>::max(raw[k]), c);
+        own.add(raw[k]);
       }
   }
   if (tid < edge) {   // fewer than 2 V <= NT of them
-    const float f = Cvt<T>::to_f(x[edge_at(tid)]), two[2] = {f, -INFINITY};
+    const float f = Cvt<T>::to_f(x[edge_at(tid)]);
     own.raise(f, c);
-    own.add(two, c2);
+    own.add1(f, c);
   }
+  const bool scored = rank == 0 && tid == 0 && tgt >= 0 && tgt < p.cols;
+  const float x_tgt = scored ? Cvt<T>::to_f(row[tgt]) : 0.f;
   Stat a = own.stat();
   const float own_max = a.m;
 
@@ -255,7 +284,16 @@ __global__ void __launch_bounds__(NT) token_logprobs_kernel(const LogprobParams 
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < NW; ++w) m = fmaxf(m, s_max[w]);
-  rebase(a, m, c);
+  if (beyond(m, c) && fabsf(m) < INFINITY) {     // the same for the whole CTA
+    a.s = a.u = 0.f;
+    for (int i = tid; i < n; i += NT) {
+      const float t = max_nan((Cvt<T>::to_f(x[i]) - m) * c, -200.f), e = ex2f(t);
+      a.s += e;
+      a.u = fmaf(t, e, a.u);
+    }
+  } else {
+    rebase(a, ref_of(a.m, c) - ref_of(m, c));
+  }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     a.s += __shfl_xor_sync(0xffffffffu, a.s, o);
@@ -302,10 +340,11 @@ __global__ void __launch_bounds__(NT) token_logprobs_kernel(const LogprobParams 
         const int l = __ffs(flagged) - 1;
         flagged &= flagged - 1;
         for (int v = warp * 32 + l + lane * NT; v < pieces; v += 32 * NT) {
-          const Piece<T> q(__ldg(xv + v));
-          if (q.max() >= bound) {
+          const uint4 raw = __ldg(xv + v);
+          if (Piece<T>::max(raw) >= bound) {
+            const T* e = reinterpret_cast<const T*>(&raw);
 #pragma unroll
-            for (int i = 0; i < V; ++i) offer(q.f[i], head + v * V + i);
+            for (int i = 0; i < V; ++i) offer(Cvt<T>::to_f(e[i]), head + v * V + i);
           }
         }
       }
@@ -381,37 +420,40 @@ __global__ void __launch_bounds__(NT) token_logprobs_kernel(const LogprobParams 
   if (C > 1) {
     cluster.sync();
     if (rank == 0) {
-      // the slices' statistics, in order, and their entries ranked together
-      int at = 0;
-      float top_m = -INFINITY;
-      for (int q = 0; q < C; ++q) top_m = fmaxf(top_m, cluster.map_shared_rank(&s_part, q)->stat.m);
-      Stat sum = {top_m, 0.f, 0.f};
-      for (int q = 0; q < C; ++q) {
-        const Partial* o = cluster.map_shared_rank(&s_part, q);
-        Stat b = o->stat;
-        rebase(b, top_m, c);
-        sum.s += b.s;
-        sum.u += b.u;
-        if (TOP) {
-          const int k = o->n;
-          for (int i = tid; i < k; i += NT) s_cand[at + i] = o->best[i];
-          at += k;
-        }
+      // The slices' statistics, a slice per lane of every warp, and their entries ranked together: each thread fetches one, all on
+      // their way at once (C <= 8 slices, kMaxTop places each, empty ones 0).
+      Stat b = {-INFINITY, 0.f, 0.f};
+      if (lane < C) b = cluster.map_shared_rank(&s_part, lane)->stat;
+      uint64_t e = 0;
+      if (TOP && tid < C * kMaxTop) {
+        const Partial* o = cluster.map_shared_rank(&s_part, tid / kMaxTop);
+        const int have_there = o->n;
+        e = o->best[tid % kMaxTop];
+        if (tid % kMaxTop >= have_there) e = 0;
       }
-      a = sum;
-      __syncthreads();
+      float top_m = b.m;
+#pragma unroll
+      for (int o = 4; o > 0; o >>= 1) top_m = fmaxf(top_m, __shfl_xor_sync(0xffffffffu, top_m, o));
+      top_m = __shfl_sync(0xffffffffu, top_m, 0);
+      rebase(b, (b.m - top_m) * c + (off_of(top_m, c) - off_of(b.m, c)));   // (-inf less -inf: a NaN that counts as -200)
+#pragma unroll
+      for (int o = 4; o > 0; o >>= 1) {
+        b.s += __shfl_xor_sync(0xffffffffu, b.s, o);
+        b.u += __shfl_xor_sync(0xffffffffu, b.u, o);
+      }
+      a = {top_m, __shfl_sync(0xffffffffu, b.s, 0), __shfl_sync(0xffffffffu, b.u, 0)};
       if (TOP) {
-        have = min(p.top, at);
-        uint64_t e = 0;
-        int rk = kMaxTop;
-        if (tid < at) {
-          e = s_cand[tid];
-          rk = 0;
-          for (int j = 0; j < at; ++j) rk += s_cand[j] > e ? 1 : 0;
-        }
+        if (tid < C * kMaxTop) s_cand[tid] = e;
         __syncthreads();
-        if (rk < have) s_cand[rk] = e;
-        mine_best = s_cand;
+        have = min(p.top, p.cols);
+        int rk = kMaxTop;
+        if (e != 0) {
+          rk = 0;
+          for (int q = 0; q < C; ++q)
+#pragma unroll 4
+            for (int j = 0; j < p.top; ++j) rk += s_cand[q * kMaxTop + j] > e ? 1 : 0;
+        }
+        if (rk < have) s_part.best[rk] = e;     // (its own entries have been fetched)
         __syncthreads();
       }
     }
@@ -423,7 +465,7 @@ __global__ void __launch_bounds__(NT) token_logprobs_kernel(const LogprobParams 
   if (warp > 0) return;
   const bool none = !(a.s > 0.f) || a.m == INFINITY;
   const float lz2 = log2f(a.s);
-  const float lz = lz2 * kLn2;
+  const float lz = (lz2 - off_of(a.m, c)) * kLn2;
   auto logp = [&](float v) { return fmaf(v - a.m, p.inv_t, -lz); };
   if (lane == 0) {
     float lp = nan;
