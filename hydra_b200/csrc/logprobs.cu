@@ -6,10 +6,11 @@
 // sums relative to it in 32 bits (new maxima are rare after the first pieces, so the rescaling hardly ever runs).
 //
 // Top alternatives without a second pass over the row: the maxima of the threads, taken over 64 groups of threads, give a
-// bound that at least `top` logits reach (the top-th largest group maximum); only threads whose own maximum reaches it
-// re-read their pieces (a warp together, out of L2), and the few logits found are ranked by (value, index).  Of
-// equal logits the lowest index comes first; ties at the bound beyond the candidate list's size are collected in index
-// order.  Rows that hold NaN or +inf, or more than kCand logits above the bound, take `top` exact selection rounds instead.
+// bound that at least `top` logits reach (the top-th largest group maximum).  Each thread has noted its maximum, or where many
+// alternatives are asked for those of eight stretches of its columns; only stretches that reach the bound are read again (out of L2, all of them at once), and the few
+// logits found are ranked by (value, index).  Of equal logits the lowest index comes first; ties at the bound beyond the
+// candidate list's size are collected in index order.  Rows that hold NaN, or more than kCand logits above the bound, take
+// `top` exact selection rounds instead.
 //
 // Few rows are split over a cluster of CTAs, whose partial results the first CTA merges through distributed shared memory.
 #include <cooperative_groups.h>
@@ -27,6 +28,7 @@ constexpr int kCand = 512;       // candidate list of a CTA
 constexpr int kMaxTop = 32;
 constexpr int kGroups = 64;
 constexpr int kUnroll = 4;
+constexpr int kList = 512;       // those that reach the bound
 
 struct LogprobParams {
   const void* x;
@@ -212,8 +214,10 @@ struct Partial {
   uint64_t best[kMaxTop];      // in order
 };
 
-template <typename T, int NT, bool TOP>
+// S: stretches of a thread's columns whose maxima are kept; 0: no alternatives are asked for.
+template <typename T, int NT, int S>
 __global__ void __launch_bounds__(NT) token_logprobs_kernel(const LogprobParams p) {
+  constexpr bool TOP = S > 0;
   constexpr int V = 16 / sizeof(T), NW = NT / 32, LPG = NT / kGroups;   // lanes per group of threads
   __shared__ Partial s_part;
   __shared__ float s_max[NW], s_sum[NW][2];
@@ -221,7 +225,9 @@ __global__ void __launch_bounds__(NT) token_logprobs_kernel(const LogprobParams 
   __shared__ uint64_t s_cand[kCand];
   __shared__ uint64_t s_best[NW];
   __shared__ float s_bound;
-  __shared__ int s_count, s_scan[NW];
+  __shared__ int s_count, s_listed, s_scan[NW];
+  __shared__ float s_stretch[S > 1 ? S * NT : 1];
+  __shared__ uint16_t s_list[S > 1 ? kList : 1];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   cg::cluster_group cluster = cg::this_cluster();
   const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
@@ -237,7 +243,11 @@ __global__ void __launch_bounds__(NT) token_logprobs_kernel(const LogprobParams 
   const int head = min(n, to_boundary), pieces = (n - head) / V, edge = head + (n - head - pieces * V);
   const uint4* xv = reinterpret_cast<const uint4*>(x + head);
   auto edge_at = [&](int i) { return i < head ? i : pieces * V + i; };   // i-th value outside the pieces -> its column
+  // a thread's j-th piece is tid + j NT; a stretch is kUnroll `length` of them
+  const int length = S > 1 ? (pieces + NT * kUnroll * S - 1) / (NT * kUnroll * (S > 0 ? S : 1)) : 0;
   Running<T> own(c);
+  float far = -INFINITY;       // the maximum of the stretch so far
+  int stretch = 0, batch = 0;
   int v0 = tid;
   for (; v0 + (kUnroll - 1) * NT < pieces; v0 += kUnroll * NT) {   // four pieces, one look at their maximum
     uint4 raw[kUnroll];
@@ -247,6 +257,14 @@ __global__ void __launch_bounds__(NT) token_logprobs_kernel(const LogprobParams 
 #pragma unroll
     for (int k = 1; k < kUnroll; ++k) mx = fmaxf(mx, Piece<T>::max(raw[k]));
     own.raise(mx, c);
+    if constexpr (S > 1) {
+      far = fmaxf(far, mx);
+      if (++batch == length) {
+        s_stretch[stretch++ * NT + tid] = far;
+        far = -INFINITY;
+        batch = 0;
+      }
+    }
 #pragma unroll
     for (int k = 0; k < kUnroll; ++k) own.add(raw[k]);
   }
@@ -258,9 +276,14 @@ __global__ void __launch_bounds__(NT) token_logprobs_kernel(const LogprobParams 
 #pragma unroll
     for (int k = 0; k < kUnroll - 1; ++k)
       if (v0 + k * NT < pieces) {
-        own.raise(Piece<T>::max(raw[k]), c);
+        const float mx = Piece<T>::max(raw[k]);
+        if (S > 1) far = fmaxf(far, mx);
+        own.raise(mx, c);
         own.add(raw[k]);
       }
+  }
+  if constexpr (S > 1) {
+    for (; stretch < S; ++stretch, far = -INFINITY) s_stretch[stretch * NT + tid] = far;   // (its last, and what it has not)
   }
   if (tid < edge) {   // fewer than 2 V <= NT of them
     const float f = Cvt<T>::to_f(x[edge_at(tid)]);
@@ -270,7 +293,6 @@ __global__ void __launch_bounds__(NT) token_logprobs_kernel(const LogprobParams 
   const bool scored = rank == 0 && tid == 0 && tgt >= 0 && tgt < p.cols;
   const float x_tgt = scored ? Cvt<T>::to_f(row[tgt]) : 0.f;
   Stat a = own.stat();
-  const float own_max = a.m;
 
   // the slice's maximum (on the way those of the 64 groups of threads), then its sums relative to it
   float m = a.m;
@@ -280,7 +302,7 @@ __global__ void __launch_bounds__(NT) token_logprobs_kernel(const LogprobParams 
     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
   }
   if (lane == 0) s_max[warp] = m;
-  if (tid == 0) s_count = 0;
+  if (tid == 0) s_count = s_listed = 0;
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < NW; ++w) m = fmaxf(m, s_max[w]);
@@ -335,17 +357,32 @@ __global__ void __launch_bounds__(NT) token_logprobs_kernel(const LogprobParams 
           if (at < kCand) s_cand[at] = entry(v, c0 + col);
         }
       };
-      unsigned flagged = __ballot_sync(0xffffffffu, own_max > bound || (equal && own_max == bound));
-      while (flagged) {                    // a thread's pieces, looked through by its whole warp
-        const int l = __ffs(flagged) - 1;
-        flagged &= flagged - 1;
-        for (int v = warp * 32 + l + lane * NT; v < pieces; v += 32 * NT) {
-          const uint4 raw = __ldg(xv + v);
-          if (Piece<T>::max(raw) >= bound) {
-            const T* e = reinterpret_cast<const T*>(&raw);
+      auto look_at = [&](int v) {
+        const uint4 raw = __ldg(xv + v);
+        if (Piece<T>::max(raw) >= bound) {
+          const T* u = reinterpret_cast<const T*>(&raw);
 #pragma unroll
-            for (int i = 0; i < V; ++i) offer(Cvt<T>::to_f(e[i]), head + v * V + i);
+          for (int i = 0; i < V; ++i) offer(Cvt<T>::to_f(u[i]), head + v * V + i);
+        }
+      };
+      if constexpr (S == 1) {              // a thread's pieces, by its whole warp
+        unsigned reach = __ballot_sync(0xffffffffu, own.m > bound || (equal && own.m == bound));
+        for (; reach; reach &= reach - 1)
+          for (int v = warp * 32 + __ffs(reach) - 1 + lane * NT; v < pieces; v += 32 * NT) look_at(v);
+      } else {                             // the stretches' pieces, by all threads
+        for (int e = 0; e < S; ++e) {
+          const float mx = s_stretch[e * NT + tid];
+          if (mx > bound || (equal && mx == bound)) {
+            const int at = atomicAdd(&s_listed, 1);
+            if (at < kList) s_list[at] = (uint16_t)(e * NT + tid);
           }
+        }
+        __syncthreads();
+        const int listed = s_listed, per = length * kUnroll;
+        if (listed > kList) return kCand + 1;
+        for (int i = tid; i < listed * per; i += NT) {
+          const int k = i / per, e = s_list[k] / NT, v = s_list[k] % NT + (e * per + i - k * per) * NT;
+          if (v < pieces) look_at(v);
         }
       }
       if (tid < edge) {
@@ -359,7 +396,7 @@ __global__ void __launch_bounds__(NT) token_logprobs_kernel(const LogprobParams 
     if (sane && bound > -INFINITY) found = collect(true);
     if (sane && found > kCand) {           // many ties at the bound: those above it, then the first that equal it
       __syncthreads();
-      if (tid == 0) s_count = 0;
+      if (tid == 0) s_count = s_listed = 0;
       __syncthreads();
       found = collect(false);
       if (found > kCand - kMaxTop) found = kCand + 1;
@@ -481,9 +518,18 @@ __global__ void __launch_bounds__(NT) token_logprobs_kernel(const LogprobParams 
   }
 }
 
-template <typename T, int NT, bool TOP>
+template <typename T, int NT, int S>
 int launch_as(const LogprobParams& p, int64_t rows, int cluster, cudaStream_t st) {
-  return launch_chained(token_logprobs_kernel<T, NT, TOP>, dim3((unsigned)(rows * cluster)), dim3(NT), 0, st, false, cluster, p);
+  return launch_chained(token_logprobs_kernel<T, NT, S>, dim3((unsigned)(rows * cluster)), dim3(NT), 0, st, false, cluster, p);
+}
+
+// One stretch per thread for a few alternatives, eight for more: a stretch that reaches the bound is read again (2048 rows of
+// 152064 bf16 columns, 20 alternatives: 115 us with eight, 150 with one), and noting eight costs registers (8192 rows of 50257,
+// one alternative: 140 us with one, 155 with eight).
+template <typename T, int NT>
+int launch_nt(const LogprobParams& p, int64_t rows, int cluster, cudaStream_t st) {
+  if (p.top == 0) return launch_as<T, NT, 0>(p, rows, cluster, st);
+  return p.top <= 4 ? launch_as<T, NT, 1>(p, rows, cluster, st) : launch_as<T, NT, 8>(p, rows, cluster, st);
 }
 
 template <typename T>
@@ -492,10 +538,12 @@ int launch(LogprobParams p, int64_t rows, cudaStream_t st) {
   int cluster = 1;
   while (cluster < 8 && rows * cluster * 2 <= 2 * 148 && p.cols / (cluster * 2) >= 4096) cluster *= 2;
   p.slice = ceil_div(ceil_div(p.cols, cluster), 64) * 64;
-  // Many rows: CTAs of 256 threads, whose fixed work per row (joining the statistics, the bound) is half as much and whose
-  // rows overlap six to an SM; few: 512 threads get a row's bytes under way sooner.
-  if (rows * cluster > 2 * 148) return p.top > 0 ? launch_as<T, 256, true>(p, rows, cluster, st) : launch_as<T, 256, false>(p, rows, cluster, st);
-  return p.top > 0 ? launch_as<T, 512, true>(p, rows, cluster, st) : launch_as<T, 512, false>(p, rows, cluster, st);
+  // Many rows: small CTAs, whose barriers hold up little and whose fixed work per row (joining the statistics, the bound) is
+  // small; few: 512 threads get a row's bytes under way sooner; between them, and for long rows of many alternatives, 256
+  // (600 rows of 50257: 19 us with 256 threads, 22 with 128; 8192 rows: 146 and 140 us).
+  if (rows * cluster <= 2 * 148) return launch_nt<T, 512>(p, rows, cluster, st);
+  if (rows < 6 * 148 || (p.top > 4 && p.cols > 65536)) return launch_nt<T, 256>(p, rows, cluster, st);
+  return launch_nt<T, 128>(p, rows, cluster, st);
 }
 
 }  // namespace
