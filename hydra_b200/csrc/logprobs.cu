@@ -520,7 +520,10 @@ __global__ void __launch_bounds__(NT) token_logprobs_kernel(const LogprobParams 
 
 template <typename T, int NT, int S>
 int launch_as(const LogprobParams& p, int64_t rows, int cluster, cudaStream_t st) {
-  return launch_chained(token_logprobs_kernel<T, NT, S>, dim3((unsigned)(rows * cluster)), dim3(NT), 0, st, false, cluster, p);
+  if (cluster > 1) return launch_chained(token_logprobs_kernel<T, NT, S>, dim3((unsigned)(rows * cluster)), dim3(NT), 0, st, false, cluster, p);
+  token_logprobs_kernel<T, NT, S><<<(unsigned)rows, NT, 0, st>>>(p);
+  HB_LAUNCH_CHECK();
+  return 0;
 }
 
 // One stretch per thread for a few alternatives, eight for more: a stretch that reaches the bound is read again (2048 rows of
@@ -563,6 +566,7 @@ extern "C" int hb200_token_logprobs(const void* logits, const int64_t* tokens, i
   if (rows == 0) return 0;
   HB_REQUIRE(logits && tokens && logprobs && entropy && (top == 0 || (top_logprobs && top_ids)), HB200_ERR_INVALID,
              "token_logprobs: null pointer");
+  HB_REQUIRE(cols <= 1 << 30, HB200_ERR_UNSUPPORTED, "token_logprobs: %d columns (up to 2^30 are built)", cols);
   HB_REQUIRE(rows <= 0x7fffffff / 8, HB200_ERR_UNSUPPORTED, "token_logprobs: too many rows");
   const size_t es = dtype == HB200_F32 ? 4 : 2;
   HB_REQUIRE(reinterpret_cast<uintptr_t>(logits) % es == 0, HB200_ERR_INVALID, "token_logprobs: misaligned logits");

@@ -781,7 +781,8 @@ int launch(const PagedParams& p, int sms, cudaStream_t st) {
   const size_t smem = (size_t)NW * stages_of(HD) * 2 * tile_tokens(HD) * HD * 2 + (size_t)(2 * p.B + 1) * 4;
   auto kern = p.page_size % 16 == 0 ? paged_attention_kernel<T, HD, NQ, true> : paged_attention_kernel<T, HD, NQ, false>;
   HB_PROPAGATE(ensure_dynamic_smem((const void*)kern, smem));
-  HB_PROPAGATE(launch_chained(kern, dim3((unsigned)sms), dim3(NW * 32), smem, st, false, 1, p));
+  kern<<<(unsigned)sms, NW * 32, smem, st>>>(p);
+  HB_LAUNCH_CHECK();
   // a warp per row, or eight where a row has many parts (few pairs for the CTAs)
   const int64_t rows = (int64_t)p.B * p.Hq;
   if ((int64_t)p.B * p.Hkv * p.q_tiles * 4 <= sms) return launch_chained(paged_join_kernel<T, 8>, dim3((unsigned)rows), dim3(256), 0, st, true, 1, p);
@@ -842,16 +843,18 @@ extern "C" int hb200_paged_decode_attention(const hb200_paged_cache* c, const vo
   for (int64_t s : strides)
     HB_REQUIRE(s % 8 == 0, HB200_ERR_INVALID, "paged_decode_attention: strides must be multiples of 8 elements");
   HB_REQUIRE(scale == scale, HB200_ERR_INVALID, "paged_decode_attention: scale is NaN");
+  // lengths are clamped to the table's reach, so this bounds every tile count in 32 bits
+  const int64_t cap = (int64_t)table_width * c->page_size;
+  HB_REQUIRE(cap <= 0x7fffff00 && (int64_t)B * (cap / 16 + 4) <= 0x7fffffff, HB200_ERR_UNSUPPORTED,
+             "paged_decode_attention: tables of %d pages of %d tokens for %d requests reach too far", table_width, c->page_size, B);
+  HB_REQUIRE((cap / 16 + 4) * Hq <= 0x7fffffff, HB200_ERR_UNSUPPORTED,
+             "paged_decode_attention: tables of %d pages of %d tokens for %d query heads reach too far", table_width, c->page_size, Hq);
   const int group = Hq / c->n_kv_heads;
   int sms = 0;
   HB_PROPAGATE(sm_count(&sms));
   HB_REQUIRE(workspace_bytes >= workspace_for(B, Hq, c->n_kv_heads, c->head_dim, sms), HB200_ERR_WORKSPACE,
              "paged_decode_attention: workspace of %zu bytes, needs %zu", workspace_bytes,
              workspace_for(B, Hq, c->n_kv_heads, c->head_dim, sms));
-  // lengths are clamped to the table's reach, so this bounds every tile count in 32 bits
-  const int64_t cap = (int64_t)table_width * c->page_size;
-  HB_REQUIRE(cap <= 0x7fffff00 && (int64_t)B * (cap / 16 + 4) <= 0x7fffffff, HB200_ERR_UNSUPPORTED,
-             "paged_decode_attention: tables of %d pages of %d tokens for %d requests reach too far", table_width, c->page_size, B);
   PagedParams p = {};
   p.q = q; p.kc = c->k; p.vc = c->v; p.out = out; p.lse = lse; p.table = block_tables; p.lens = kv_lens;
   p.q_sb = q_stride_b; p.q_sh = q_stride_h;

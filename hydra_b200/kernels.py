@@ -206,8 +206,10 @@ def fused_rms_norm(x: Tensor, weight: Tensor, eps: float = 1e-6) -> Tensor:
 
 
 def _refuse_autograd(what: str, *ts: Optional[Tensor]) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
-        raise RuntimeError(f"{what} is inference only: an input requires grad (wrap the call in torch.no_grad())")
+    if torch.is_grad_enabled():
+        for t in ts:
+            if t is not None and t.requires_grad:
+                raise RuntimeError(f"{what} is inference only: an input requires grad (wrap the call in torch.no_grad())")
 
 
 def _fp32(what: str, t: Optional[Tensor], n: int, dev: torch.device) -> Optional[Tensor]:
@@ -242,8 +244,8 @@ def _qk_norm_rope(what: str, dev: torch.device, q: Tensor, k: Tensor, cos: Tenso
     if qs[-1] != 1 or ks[-1] != 1 or vs[-1] != 1:
         q, k, v = q.contiguous(), k.contiguous(), None if v is None else v.contiguous()
         qs, ks, vs = q.stride(), k.stride(), (0, 0, 0, 1) if v is None else v.stride()
-    q_out = torch.empty(shape, dtype=q.dtype, device=dev)
-    k_out = torch.empty(k.shape, dtype=q.dtype, device=dev) if cache is None else None
+    q_out = torch.empty(*shape, dtype=q.dtype, device=dev)
+    k_out = torch.empty(*k.shape, dtype=q.dtype, device=dev) if cache is None else None
     qos, kos = q_out.stride(), (0, 0, 0, 1) if k_out is None else k_out.stride()
     if len(shape) == 3:                       # tokens, heads -> batch, tokens, heads
         B, S, Hq, Hkv = 1, shape[0], shape[1], k.shape[1]

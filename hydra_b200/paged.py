@@ -117,7 +117,7 @@ def paged_append(q: Tensor, k: Tensor, v: Tensor, k_cache: Tensor, v_cache: Tens
     contiguous rows (token-major pages: pass ``cache.transpose(1, 2)``).  Returns the normed and rotated queries
     [T, Hq, hd]; cache rows without a slot here stay as they are.  A row with a negative position is padding (zeros
     returned, nothing stored), one with a negative slot is computed but not stored; a position beyond the tables or a slot
-    beyond the cache gives NaN.  Two rows with the same slot: either may stay."""
+    beyond the cache gives NaN.  Of two rows with the same slot either's values may stay, or some of each's."""
     dev = kernels._require_cuda(q, k, v, k_cache, v_cache, slots, cos, sin, positions)
     if q.dim() != 3 or k.dim() != 3 or v.shape != k.shape or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2]:
         raise ValueError(f"paged_append: q [T, Hq, hd], k and v [T, Hkv, hd] are wanted, got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
@@ -174,10 +174,10 @@ def paged_decode_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_ta
         q = q.contiguous()
         q = q.clone() if q.data_ptr() % 16 else q
     if out is None:
-        out = torch.empty((B, Hq, hd), dtype=q.dtype, device=dev)
+        out = torch.empty(B, Hq, hd, dtype=q.dtype, device=dev)
     elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev or not out.is_contiguous() or out.data_ptr() % 16:
         raise ValueError("paged_decode_attention: out must be a contiguous, 16-byte aligned tensor of q's shape and dtype")
-    lse = torch.empty((B, Hq), dtype=torch.float32, device=dev) if return_lse else None
+    lse = torch.empty(B, Hq, dtype=torch.float32, device=dev) if return_lse else None
     if B > 0:
         with kernels._on(dev):
             L = _lib.lib()

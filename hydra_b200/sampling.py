@@ -74,9 +74,9 @@ def token_logprobs(logits: Tensor, tokens: Tensor, top: int = 0, temperature: fl
     if N > 1 and logits.stride(0) < V:
         logits = logits.contiguous()          # rows that overlap (an expanded row)
     tokens = tokens if tokens.is_contiguous() else tokens.contiguous()
-    f32 = dict(dtype=torch.float32, device=dev)
-    r = TokenLogprobs(torch.empty(N, **f32), torch.empty(N, **f32), torch.empty((N, top), **f32),
-                      torch.empty((N, top), dtype=torch.int64, device=dev))
+    f32 = torch.float32
+    r = TokenLogprobs(torch.empty(N, dtype=f32, device=dev), torch.empty(N, dtype=f32, device=dev),
+                      torch.empty(N, top, dtype=f32, device=dev), torch.empty(N, top, dtype=torch.int64, device=dev))
     if N > 0:
         with kernels._on(dev):
             _lib.check(_lib.lib().hb200_token_logprobs(

@@ -53,6 +53,41 @@ def test_against_64_bits(dtype, N, V, ld, top):
     check(x.cuda(), vocab=V, top=top, temperature=0.7 if N % 2 else 1.0)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("N,V,top", [(900, 3001, 4), (1000, 5000, 5), (900, 5003, 0), (2000, 300, 32), (890, 70001, 20), (400, 9000, 3), (400, 9000, 30)])
+def test_many_rows(dtype, N, V, top):
+    g = torch.Generator(device="cuda").manual_seed(V)
+    x = (torch.randn(N, V + 5, generator=g, device="cuda") * 3).to(dtype)
+    check(x[:, :V], top=top)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("temperature", [1e-6, 1e-3, 30.0, 1e6])
+@pytest.mark.parametrize("N,V", [(3, 700), (2, 40000)])
+def test_extreme_temperatures(dtype, temperature, N, V):
+    """Differences of logits over a temperature near nothing are far beyond what e^x holds, or one token takes all."""
+    g = torch.Generator().manual_seed(V)
+    x = (torch.randn(N, V, generator=g) * 4).to(dtype)
+    x[0, 5:90] = -INF
+    x[1] -= 20.0                                                          # a row of negative logits
+    check(x.cuda(), top=8, temperature=temperature)
+
+
+@pytest.mark.parametrize("scale", [1e5, 1e8, 1e30, -1e30])
+@pytest.mark.parametrize("N", [2, 300])
+def test_huge_logits(scale, N):
+    """The distances between logits stay small, or come out in whole steps of the type, whatever their size."""
+    g = torch.Generator().manual_seed(5)
+    for dtype in (torch.float32, torch.bfloat16):
+        x = (scale * (1 + 1e-6 * torch.randn(N, 9000, generator=g))).to(dtype)
+        check(x.cuda(), top=6)
+        x[:, ::2] = -INF
+        check(x.cuda(), top=6, tokens=torch.ones(N, dtype=torch.int64))
+    x = torch.full((N, 20000), -65504.0, dtype=torch.float16)             # half precision masked by its lowest value
+    x[:, 3::7] = -INF
+    check(x.cuda(), top=4, temperature=100.0, tokens=torch.zeros(N, dtype=torch.int64))
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("shift", [1, 3, 7])
 def test_rows_off_16_byte_boundaries(dtype, shift):

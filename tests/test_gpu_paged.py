@@ -190,7 +190,7 @@ def run(lens, hq, hkv, hd, page, dtype=torch.bfloat16, order="hnd", scale=None, 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("order", ["hnd", "nhd"])
 @pytest.mark.parametrize("hq,hkv,hd", [(4, 4, 128), (8, 2, 32), (32, 4, 16), (12, 3, 64), (2, 1, 256), (5, 1, 80), (16, 1, 8), (20, 1, 64), (40, 2, 128),
-                                       (33, 1, 24), (6, 2, 200), (3, 3, 40)])
+                                       (33, 1, 24), (6, 2, 200), (3, 3, 40), (20, 1, 256), (48, 2, 16), (9, 1, 32)])
 def test_heads_and_sizes(dtype, order, hq, hkv, hd):
     run([1, 17, 64, 0, 333, 2], hq, hkv, hd, 16, dtype, order)
 
@@ -202,9 +202,12 @@ def test_pages_that_end_inside_a_tile(page, hd):
 
 
 @pytest.mark.parametrize("lens", [[1], [4096], [3], [0, 0, 0], [0], [0, 5, 0, 0, 9, 0], [4000] + [1] * 63, [1] * 700, [50] * 300, [2500, 0, 7, 2500],
-                                  list(range(90))])
+                                  list(range(90)), [3000, 1] * 40 + [0] * 7 + [17] * 200, [6000, 5000, 1, 0, 2]])
 def test_lengths(lens):
     run(lens, 8, 2, 64, 16)
+    if len(lens) < 100:
+        run(lens, 4, 1, 128, 16)
+        run(lens, 20, 2, 32, 64)
 
 
 def test_large_batch_and_odd_scales():

@@ -43,7 +43,8 @@ def check(got, want, dtype, what=""):
 @pytest.mark.parametrize("T,hq,hkv,hd,rot,norm", [
     (1, 8, 2, 32, 32, "l2"), (7, 4, 4, 128, 128, "rms"), (33, 5, 1, 80, 40, "rms"), (3, 6, 2, 64, 16, None), (2, 3, 3, 256, 256, "rms"),
     (9, 1, 1, 8, 8, "rms"), (5, 2, 1, 6, 4, "rms"), (4, 3, 1, 17, 10, "l2"), (6, 4, 2, 96, 94, "rms"), (300, 32, 8, 64, 64, "rms"),
-    (2, 2, 1, 100, 0, "rms"), (3, 2, 2, 2, 2, None)])
+    (2, 2, 1, 100, 0, "rms"), (3, 2, 2, 2, 2, None),
+    (5000, 5, 3, 64, 32, "rms"), (2501, 9, 1, 24, 24, "l2"), (1300, 3, 3, 256, 64, "rms"), (4097, 1, 1, 16, 8, None)])
 def test_packed_tokens(dtype, layout, T, hq, hkv, hd, rot, norm):
     from hydra_b200.kernels import fused_qk_norm_rope
     g = torch.Generator().manual_seed(T * 1000 + hd)
