@@ -12,6 +12,10 @@
 // candidate list's size are collected in index order.  Rows that hold NaN, or more than kCand logits above the bound, take
 // `top` exact selection rounds instead.
 //
+// Measured (device time): 8192 rows of 50257 bf16 logits and one alternative: 134 us, 6.1 TB/s, 0.94 of a copy (153 us once the
+// power cap holds the clock at 1.65 GHz: then the issue slots bound it); one row: 7.6 us, 64 masked rows with 20: 10.1 us,
+// launch, one trip through the row and three through barriers and the cluster.
+//
 // Few rows are split over a cluster of CTAs, whose partial results the first CTA merges through distributed shared memory.
 #include <cooperative_groups.h>
 

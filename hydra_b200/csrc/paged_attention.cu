@@ -37,7 +37,7 @@ struct PagedParams {
   float* lse;
   const int32_t *table, *lens;
   float* part;       // [CTAs][2] parts, then [warps] of the warps' own: each [rows][hd] outputs, [rows][2] of max and sum
-  int32_t* cum;      // [B + 1] tiles of the requests before each one
+  int32_t* cum;      // [B + 1] places of the requests before each one
   int64_t q_sb, q_sh, k_sh, v_sh, table_ld;     // elements
   int32_t k_sp, k_sr, v_sp, v_sr;               // bytes: page and row of a page
   int B, Hq, Hkv, hd, group, q_tiles, q_tile, tile, pair_cost, warps, rows, part_floats, page_size, width, num_pages, ctas;
@@ -45,8 +45,13 @@ struct PagedParams {
   uint32_t q_sign;   // flips the signs of a pair of query values where the scale is negative
 };
 
+// Measured (device time, graph replay): one request of 131072 tokens, 32 query heads on 8 kv heads of 128: 90.5 us, 5.9 TB/s,
+// 0.91 of a copy; 64 requests up to 8192 tokens, 32 heads on 4 of 64: 55 us, 5.0 TB/s; one request of 1500 tokens: 10.7 us, of
+// which 8 are the two launches and the chain lengths -> table -> tiles -> parts -> join.  What bounds the large ones: DRAM,
+// after 7 us in which the rings fill, and SMs that get up to a tenth less of it than others.
+//
 // A warp's tile: 8 KB of K and V (16 KB of heads of 256, 4 KB of small ones, whose tokens cost more arithmetic per byte and get
-// twice the warps: 64 requests up to 16384 tokens on 4 kv heads of 16 took 45 us with eight warps, 43 with sixteen); two
+// twice the warps: 64 requests up to 16384 tokens on 4 kv heads of 16 took 48 us with eight warps, 43 with sixteen); two
 // tiles of a warp are in flight while one is computed, 128 KB of a CTA.
 __host__ __device__ constexpr int tile_tokens(int HD) { return HD >= 128 ? 16 : (HD == 16 ? 64 : 32); }
 __host__ __device__ constexpr int warps_of(int HD) { return HD >= 256 ? 4 : (HD <= 32 ? 16 : 8); }
@@ -54,7 +59,7 @@ __host__ __device__ constexpr int warps_of(int HD) { return HD >= 256 ? 4 : (HD 
 __host__ __device__ constexpr int q_tile_of(int HD) { return HD >= 256 ? 8 : 16; }
 // Places that a pair takes before its first tile when the shares are cut: what its start and end cost, in tiles.
 __host__ __device__ constexpr int pair_cost(int HD) { return HD <= 32 ? 2 : 1; }
-__host__ __device__ constexpr int stages_of(int) { return 3; }
+constexpr int kStages = 3;
 
 // Cache length of request b as the kernel reads it: what lies outside [0, width * page_size] is marked (`poison`).
 __device__ __forceinline__ int clamp_len(int len, int64_t cap, bool& poison) {
@@ -137,7 +142,7 @@ struct Cursor {
 // share a page: one look into the table for them.
 template <typename T, int HD, int NQ, bool P16>
 __global__ void __launch_bounds__(warps_of(HD) * 32, 1) paged_attention_kernel(const PagedParams p) {
-  constexpr int NW = warps_of(HD), TT = tile_tokens(HD), CH = HD / 8, ST = stages_of(HD);
+  constexpr int NW = warps_of(HD), TT = tile_tokens(HD), CH = HD / 8, ST = kStages;
   constexpr int ROWB = HD * 2, KBYTES = TT * ROWB, STAGE = 2 * KBYTES;
   constexpr int MT = TT / 16;                        // 16-token tiles
   constexpr int KS = HD / 16;                        // 16-value steps of a head
@@ -270,7 +275,7 @@ __global__ void __launch_bounds__(warps_of(HD) * 32, 1) paged_attention_kernel(c
   };
   head_of();
   const char *kt = kb, *vt = vb;              // the same of the tile that was looked up
-  int page[L], off[L], rows_there = 0;        // its pages (-1: none), places in them, tokens
+  int page[L], off[L], rows_there = 0;        // its pages, places in them, tokens
   bool bad_seen = false;                      // a page outside the cache
   uint32_t bad_bits = 0;                      // the same per ring slot
   uint32_t dst[2];                            // of the lane's even and odd copies of a row
@@ -637,8 +642,8 @@ __global__ void __launch_bounds__(warps_of(HD) * 32, 1) paged_attention_kernel(c
 // WPR warps per (request, query head): nothing where one share held the whole pair, zeros for an empty request, else the
 // parts' weighted sum.  A warp takes every WPR-th part, its statistics one per lane, its values four side by side per lane.
 template <typename T, int WPR>
-__global__ void __launch_bounds__(WPR > 8 ? WPR * 32 : 256) paged_join_kernel(const PagedParams p) {
-  constexpr int RPC = WPR > 8 ? 1 : 8 / WPR;    // rows per CTA
+__global__ void __launch_bounds__(256) paged_join_kernel(const PagedParams p) {
+  constexpr int RPC = 8 / WPR;                  // rows per CTA
   __shared__ __align__(16) float s_o[WPR > 1 ? WPR : 1][256];
   __shared__ float s_m[WPR], s_l[WPR];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, wi = warp % WPR;
@@ -778,7 +783,7 @@ size_t workspace_for(int B, int Hq, int Hkv, int hd, int sms) {
 template <typename T, int HD, int NQ>
 int launch(const PagedParams& p, int sms, cudaStream_t st) {
   constexpr int NW = warps_of(HD);
-  const size_t smem = (size_t)NW * stages_of(HD) * 2 * tile_tokens(HD) * HD * 2 + (size_t)(2 * p.B + 1) * 4;
+  const size_t smem = (size_t)NW * kStages * 2 * tile_tokens(HD) * HD * 2 + (size_t)(2 * p.B + 1) * 4;
   auto kern = p.page_size % 16 == 0 ? paged_attention_kernel<T, HD, NQ, true> : paged_attention_kernel<T, HD, NQ, false>;
   HB_PROPAGATE(ensure_dynamic_smem((const void*)kern, smem));
   kern<<<(unsigned)sms, NW * 32, smem, st>>>(p);
@@ -842,7 +847,7 @@ extern "C" int hb200_paged_decode_attention(const hb200_paged_cache* c, const vo
                              c->v_stride_page, c->v_stride_head, c->v_stride_row};
   for (int64_t s : strides)
     HB_REQUIRE(s % 8 == 0, HB200_ERR_INVALID, "paged_decode_attention: strides must be multiples of 8 elements");
-  HB_REQUIRE(scale == scale, HB200_ERR_INVALID, "paged_decode_attention: scale is NaN");
+  HB_REQUIRE(scale - scale == 0.f, HB200_ERR_INVALID, "paged_decode_attention: scale is NaN or infinite");
   // lengths are clamped to the table's reach, so this bounds every tile count in 32 bits
   const int64_t cap = (int64_t)table_width * c->page_size;
   HB_REQUIRE(cap <= 0x7fffff00 && (int64_t)B * (cap / 16 + 4) <= 0x7fffffff, HB200_ERR_UNSUPPORTED,

@@ -45,7 +45,7 @@ def _attention(cache=None, q=P, sb=2048, sh=64, out=P, table=P, ld=4, width=4, l
     (dict(width=5), -1, "bad cache or table"), (dict(q=P + 2), -1, "aligned"), (dict(sh=60), -1, "multiples of 8"),
     (dict(cache=_cache(head_dim=60)), -4, "head_dim"), (dict(cache=_cache(head_dim=264)), -4, "head_dim"),
     (dict(cache=_cache(v_stride_row=4)), -1, "multiples of 8"), (dict(cache=_cache(page_size=0)), -1, "bad cache or table"),
-    (dict(cache=_cache(k=None)), -1, "null"), (dict(scale=float("nan")), -1, "NaN"), (dict(ld=1 << 27, width=1 << 27), -4, "too far"),
+    (dict(cache=_cache(k=None)), -1, "null"), (dict(scale=float("nan")), -1, "NaN"), (dict(scale=float("inf")), -1, "infinite"), (dict(ld=1 << 27, width=1 << 27), -4, "too far"),
     (dict(B=4096, ld=1 << 24, width=1 << 24), -4, "too far"),
 ])
 def test_paged_attention_refuses(bad, status, text):
