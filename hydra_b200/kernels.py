@@ -46,14 +46,15 @@ def _dtype_code(t: Tensor) -> int:
 
 
 def _require_cuda(*ts: Tensor) -> torch.device:
-    dev = ts[0].device
+    index = ts[0].get_device()                # -1 on the CPU
     for t in ts:
-        if t.device != dev or not t.is_cuda:
-            if not t.is_cuda:
-                raise RuntimeError("hydra_b200 kernels run on CUDA tensors only (there is no CPU fallback); "
-                                   f"got a tensor on {t.device}")
-            raise RuntimeError(f"hydra_b200: tensors on different devices ({dev} and {t.device})")
-    return dev
+        if t.get_device() != index or index < 0:
+            for u in ts:
+                if not u.is_cuda:
+                    raise RuntimeError("hydra_b200 kernels run on CUDA tensors only (there is no CPU fallback); "
+                                       f"got a tensor on {u.device}")
+            raise RuntimeError(f"hydra_b200: tensors on different devices ({ts[0].device} and {t.device})")
+    return ts[0].device
 
 
 def _on(dev: torch.device):
@@ -215,7 +216,7 @@ def _refuse_autograd(what: str, *ts: Optional[Tensor]) -> None:
 def _fp32(what: str, t: Optional[Tensor], n: int, dev: torch.device) -> Optional[Tensor]:
     if t is None:
         return None
-    if t.device != dev or t.numel() != n:
+    if t.get_device() != dev.index or t.numel() != n:
         raise ValueError(f"{what} must have {n} elements on {dev}, got {tuple(t.shape)} on {t.device}")
     return t if t.dtype == torch.float32 and t.is_contiguous() else t.float().contiguous()
 
@@ -225,47 +226,53 @@ def _qk_norm_rope(what: str, dev: torch.device, q: Tensor, k: Tensor, cos: Tenso
                   k_scale: float, layout: str, v: Optional[Tensor] = None, slots: Optional[Tensor] = None, cache=None):
     """The call behind fused_qk_norm_rope and paged_append: q, k (v) [T, H, hd] or [B, H, S, hd]."""
     _refuse_autograd(what, q, k, v, q_weight, k_weight)
-    if norm not in _lib.QK_NORMS:
-        raise ValueError(f"{what}: norm must be 'rms', 'l2' or None, got {norm!r}")
-    if layout not in _lib.ROPE_LAYOUTS:
-        raise ValueError(f"{what}: layout must be 'interleaved' or 'half', got {layout!r}")
-    dtype, shape = _dtype_code(q), q.shape
+    try:
+        norm_code, layout_code = _lib.QK_NORMS[norm], _lib.ROPE_LAYOUTS[layout]
+    except KeyError:
+        raise ValueError(f"{what}: norm must be 'rms', 'l2' or None and layout 'interleaved' or 'half', got {norm!r} and {layout!r}") from None
+    dtype, torch_dtype, shape, k_shape = _dtype_code(q), q.dtype, q.shape, k.shape
     hd = shape[-1]
     if cos.dim() == 4:
         cos, sin = cos[0, 0], sin[0, 0]
-    if cos.dim() != 2 or sin.shape != cos.shape or 2 * cos.shape[1] > hd:
-        raise ValueError(f"{what}: cos and sin must be [rows, rotated / 2] with rotated <= {hd}, got {tuple(cos.shape)} and {tuple(sin.shape)}")
-    table_rows, half = cos.shape
+    table = cos.shape
+    if len(table) != 2 or sin.shape != table or 2 * table[1] > hd:
+        raise ValueError(f"{what}: cos and sin must be [rows, rotated / 2] with rotated <= {hd}, got {tuple(table)} and {tuple(sin.shape)}")
+    table_rows, half = table
     table_ld, unit = cos.stride()
-    if cos.dtype != torch.float32 or sin.dtype != torch.float32 or sin.stride() != (table_ld, unit) or unit != 1 or table_ld < half:
+    if unit != 1 or table_ld < half or cos.dtype != torch.float32 or sin.dtype != torch.float32 or sin.stride() != (table_ld, 1):
         cos, sin = cos.float().contiguous(), sin.float().contiguous()
         table_ld = half
-    qs, ks, vs = q.stride(), k.stride(), (0, 0, 0, 1) if v is None else v.stride()
+    qs, ks, vs = q.stride(), k.stride(), (0, 0, 1) if v is None else v.stride()
     if qs[-1] != 1 or ks[-1] != 1 or vs[-1] != 1:
         q, k, v = q.contiguous(), k.contiguous(), None if v is None else v.contiguous()
-        qs, ks, vs = q.stride(), k.stride(), (0, 0, 0, 1) if v is None else v.stride()
-    q_out = torch.empty(*shape, dtype=q.dtype, device=dev)
-    k_out = torch.empty(*k.shape, dtype=q.dtype, device=dev) if cache is None else None
-    qos, kos = q_out.stride(), (0, 0, 0, 1) if k_out is None else k_out.stride()
-    if len(shape) == 3:                       # tokens, heads -> batch, tokens, heads
-        B, S, Hq, Hkv = 1, shape[0], shape[1], k.shape[1]
-        strides = (0, qs[0], qs[1], 0, ks[0], ks[1], 0, vs[0], vs[1], 0, qos[0], qos[1], 0, kos[0], kos[1])
-    else:                                     # batch, heads, tokens
+        qs, ks, vs = q.stride(), k.stride(), (0, 0, 1) if v is None else v.stride()
+    q_out = torch.empty(*shape, dtype=torch_dtype, device=dev)
+    k_out = torch.empty(*k_shape, dtype=torch_dtype, device=dev) if cache is None else None
+    # strides of batch, token and head; the results are contiguous
+    if len(shape) == 3:
+        S, Hq, _ = shape
+        B, Hkv = 1, k_shape[1]
+        strides = (0, qs[0], qs[1], 0, ks[0], ks[1], 0, vs[0], vs[1], 0, Hq * hd, hd, 0, Hkv * hd, hd)
+    else:
         B, Hq, S, _ = shape
-        Hkv = k.shape[1]
-        strides = (qs[0], qs[2], qs[1], ks[0], ks[2], ks[1], 0, 0, 0, qos[0], qos[2], qos[1], kos[0], kos[2], kos[1])
+        Hkv = k_shape[1]
+        strides = (qs[0], qs[2], qs[1], ks[0], ks[2], ks[1], 0, 0, 0, Hq * S * hd, hd, S * hd, Hkv * S * hd, hd, S * hd)
     where, where_64, where_stride = None, 0, 0
     if positions is not None:
-        if positions.dtype not in (torch.int32, torch.int64):
+        if positions.dtype == torch.int64:
+            where_64 = 1
+        elif positions.dtype != torch.int32:
             raise TypeError(f"{what}: positions must be int32 or int64, got {positions.dtype}")
-        if positions.shape != (S,) and positions.shape != (B, S):
-            raise ValueError(f"{what}: positions {tuple(positions.shape)} for {B} x {S} tokens")
-        if S > 1 and positions.stride(-1) != 1:
+        where_shape = positions.shape
+        if where_shape != (S,) and where_shape != (B, S):
+            raise ValueError(f"{what}: positions {tuple(where_shape)} for {B} x {S} tokens")
+        where_strides = positions.stride()
+        if where_strides[-1] != 1 and S > 1:
             positions = positions.contiguous()
-        where, where_64 = positions.data_ptr(), int(positions.dtype == torch.int64)
-        where_stride = positions.stride(0) if positions.dim() == 2 else 0
+            where_strides = positions.stride()
+        where, where_stride = positions.data_ptr(), where_strides[0] if len(where_strides) == 2 else 0
     elif table_rows < S:
-        raise ValueError(f"{what}: tables {tuple(cos.shape)} do not cover {S} positions")
+        raise ValueError(f"{what}: tables {tuple(table)} do not cover {S} positions")
     if q_weight is not None:
         q_weight = _fp32(f"{what}: q_weight", q_weight, hd, dev)
     if k_weight is not None:
@@ -276,7 +283,7 @@ def _qk_norm_rope(what: str, dev: torch.device, q: Tensor, k: Tensor, cos: Tenso
         q.data_ptr(), k.data_ptr(), None if v is None else v.data_ptr(), q_out.data_ptr(), None if k_out is None else k_out.data_ptr(),
         None if slots is None else slots.data_ptr(), where, cos.data_ptr(), sin.data_ptr(), None if q_weight is None else q_weight.data_ptr(),
         None if k_weight is None else k_weight.data_ptr(), *strides, where_stride, table_rows, table_ld, where_64, B, S, Hq, Hkv, hd,
-        2 * half, _lib.ROPE_LAYOUTS[layout], _lib.QK_NORMS[norm], dtype, eps, q_scale, k_scale)
+        2 * half, layout_code, norm_code, dtype, eps, q_scale, k_scale)
     with _on(dev):
         _lib.check(_lib.lib().hb200_qk_norm_rope(args, cache, _stream(dev)), what)
     return q_out, k_out
@@ -297,8 +304,8 @@ def fused_qk_norm_rope(q: Tensor, k: Tensor, cos: Tensor, sin: Tensor, positions
     int32 or int64 [S], [B, S] or [T] are table rows (default 0 .. S - 1): a negative one marks padding (zeros), one beyond
     the tables gives NaN.  hd up to 256.  Returns contiguous q and k."""
     dev = _require_cuda(q, k, cos, sin, *(() if positions is None else (positions,)))
-    if q.dim() not in (3, 4) or k.dim() != q.dim() or q.dtype != k.dtype or q.shape[-1] != k.shape[-1] or q.shape[0] != k.shape[0] \
-            or (q.dim() == 4 and q.shape[2] != k.shape[2]):
+    a, b = q.shape, k.shape
+    if len(a) != len(b) or len(a) not in (3, 4) or a[-1] != b[-1] or a[0] != b[0] or (len(a) == 4 and a[2] != b[2]) or q.dtype != k.dtype:
         raise ValueError("fused_qk_norm_rope: q [B, Hq, S, hd] and k [B, Hkv, S, hd] (or [T, Hq, hd] and [T, Hkv, hd]) of one dtype "
                          f"are wanted, got {tuple(q.shape)} {q.dtype} and {tuple(k.shape)} {k.dtype}")
     return _qk_norm_rope("fused_qk_norm_rope", dev, q, k, cos, sin, positions, q_weight, k_weight, norm, eps, q_scale, k_scale, layout)

@@ -64,18 +64,18 @@ def paged_plan(context_lens: Tensor, new_lens: Tensor, block_tables: Tensor, fre
     context_lens = _ints("paged_plan: context_lens", context_lens, torch.int32, 1)
     new_lens = _ints("paged_plan: new_lens", new_lens, torch.int32, 1)
     free_pages = _ints("paged_plan: free_pages", free_pages, torch.int32, 1)
-    B = context_lens.shape[0]
-    if new_lens.shape[0] != B or block_tables.dim() != 2 or block_tables.shape[0] != B or block_tables.dtype != torch.int32:
+    B, shape = context_lens.shape[0], block_tables.shape
+    if new_lens.shape[0] != B or len(shape) != 2 or shape[0] != B or block_tables.dtype != torch.int32:
         raise ValueError(f"paged_plan: {B} context lengths, {new_lens.shape[0]} new lengths and int32 block tables [{B}, width] "
-                         f"are wanted, got {block_tables.dtype} {tuple(block_tables.shape)}")
-    width = block_tables.shape[1]
-    if (width > 1 and block_tables.stride(1) != 1) or (B > 1 and block_tables.stride(0) < width):
+                         f"are wanted, got {block_tables.dtype} {tuple(shape)}")
+    width, (ld, unit) = shape[1], block_tables.stride()
+    if (width > 1 and unit != 1) or (B > 1 and ld < width):
         raise ValueError("paged_plan: the rows of block_tables must be contiguous and apart (they are written in place)")
     page_size, room = int(page_size), int(max_new_tokens)
     if page_size < 1 or not 0 <= room <= 0x7fffffff:
         raise ValueError(f"paged_plan: page_size {page_size} and max_new_tokens {room} must be positive")
     if free_start is not None:
-        if free_start.device != dev or free_start.dtype != torch.int32 or free_start.numel() != 1:
+        if free_start.get_device() != dev.index or free_start.dtype != torch.int32 or free_start.numel() != 1:
             raise ValueError("paged_plan: free_start must be one int32 on the tables' device")
     # one allocation for the five small arrays: positions first (16-byte aligned, as the kernel stores them)
     head = (room + 3) // 4 * 4
@@ -84,23 +84,24 @@ def paged_plan(context_lens: Tensor, new_lens: Tensor, block_tables: Tensor, fre
                      status)
     with kernels._on(dev):
         _lib.check(_lib.lib().hb200_paged_plan(
-            context_lens.data_ptr(), new_lens.data_ptr(), B, block_tables.data_ptr(), block_tables.stride(0) if B > 1 else width, width,
+            context_lens.data_ptr(), new_lens.data_ptr(), B, block_tables.data_ptr(), ld if B > 1 else width, width,
             page_size, free_pages.data_ptr(), free_pages.shape[0], free_start.data_ptr() if free_start is not None else None,
-            plan.kv_lens.data_ptr(), plan.cu_new.data_ptr(), plan.positions.data_ptr(), plan.slots.data_ptr(), room,
-            plan.free_start.data_ptr(), plan.status.data_ptr(), kernels._stream(dev)), "paged_plan")
+            kv_lens.data_ptr(), cu_new.data_ptr(), positions.data_ptr(), plan.slots.data_ptr(), room, start_out.data_ptr(),
+            status.data_ptr(), kernels._stream(dev)), "paged_plan")
     return plan
 
 
 def _cache(what: str, k_cache: Tensor, v_cache: Tensor) -> _lib.PagedCache:
-    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape or k_cache.dtype != v_cache.dtype:
+    shape = k_cache.shape
+    if len(shape) != 4 or shape != v_cache.shape or k_cache.dtype != v_cache.dtype:
         raise ValueError(f"{what}: k_cache and v_cache must be [num_pages, kv_heads, page_size, head_dim] of one shape and dtype, "
-                         f"got {tuple(k_cache.shape)} {k_cache.dtype} and {tuple(v_cache.shape)} {v_cache.dtype}")
-    pages, heads, rows, hd = k_cache.shape
+                         f"got {tuple(shape)} {k_cache.dtype} and {tuple(v_cache.shape)} {v_cache.dtype}")
+    pages, heads, rows, hd = shape
     ks, vs = k_cache.stride(), v_cache.stride()
     if (ks[3] != 1 or vs[3] != 1) and hd > 1:
         raise ValueError(f"{what}: a head's row in the cache must be contiguous")
-    if k_cache.numel() == 0:
-        raise ValueError(f"{what}: an empty cache {tuple(k_cache.shape)}")
+    if pages * heads * rows * hd == 0:
+        raise ValueError(f"{what}: an empty cache {tuple(shape)}")
     return _lib.PagedCache(k_cache.data_ptr(), v_cache.data_ptr(), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], pages, rows, heads, hd,
                            kernels._dtype_code(k_cache))   # in the order of the struct
 
@@ -119,16 +120,17 @@ def paged_append(q: Tensor, k: Tensor, v: Tensor, k_cache: Tensor, v_cache: Tens
     returned, nothing stored), one with a negative slot is computed but not stored; a position beyond the tables or a slot
     beyond the cache gives NaN.  Of two rows with the same slot either's values may stay, or some of each's."""
     dev = kernels._require_cuda(q, k, v, k_cache, v_cache, slots, cos, sin, positions)
-    if q.dim() != 3 or k.dim() != 3 or v.shape != k.shape or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2]:
-        raise ValueError(f"paged_append: q [T, Hq, hd], k and v [T, Hkv, hd] are wanted, got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
+    a, b = q.shape, k.shape
+    if len(a) != 3 or len(b) != 3 or v.shape != b or a[0] != b[0] or a[2] != b[2]:
+        raise ValueError(f"paged_append: q [T, Hq, hd], k and v [T, Hkv, hd] are wanted, got {tuple(a)}, {tuple(b)}, {tuple(v.shape)}")
     if not (q.dtype == k.dtype == v.dtype == k_cache.dtype):
         raise ValueError("paged_append: q, k, v and the caches must share a dtype")
     cache = _cache("paged_append", k_cache, v_cache)
-    if k_cache.shape[1] != k.shape[1] or k_cache.shape[3] != k.shape[2]:
-        raise ValueError(f"paged_append: keys {tuple(k.shape)} do not fit the cache {tuple(k_cache.shape)}")
+    if cache.n_kv_heads != b[1] or cache.head_dim != b[2]:
+        raise ValueError(f"paged_append: keys {tuple(b)} do not fit the cache {tuple(k_cache.shape)}")
     slots = _ints("paged_append: slots", slots, torch.int64, 1)
-    if slots.shape[0] != q.shape[0]:
-        raise ValueError(f"paged_append: {slots.shape[0]} slots for {q.shape[0]} tokens")
+    if slots.shape[0] != a[0]:
+        raise ValueError(f"paged_append: {slots.shape[0]} slots for {a[0]} tokens")
     if k_cache.requires_grad or v_cache.requires_grad:
         raise RuntimeError("paged_append: the caches are written in place and cannot require grad")
     q_out, _ = kernels._qk_norm_rope("paged_append", dev, q, k, cos, sin, positions, q_weight, k_weight, norm, eps, q_scale, k_scale,
@@ -154,27 +156,31 @@ def paged_decode_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_ta
     its column.  Equal inputs give equal bits."""
     dev = kernels._require_cuda(q, k_cache, v_cache, block_tables, kv_lens)
     kernels._refuse_autograd("paged_decode_attention", q, k_cache, v_cache)
-    if q.dim() != 3 or q.dtype != k_cache.dtype or q.dtype not in (torch.bfloat16, torch.float16):
+    dtype = q.dtype
+    if q.dim() != 3 or dtype != k_cache.dtype or (dtype != torch.bfloat16 and dtype != torch.float16):
         raise ValueError(f"paged_decode_attention: q must be [B, Hq, hd] in the caches' dtype, bfloat16 or float16, got {tuple(q.shape)} {q.dtype}")
     cache = _cache("paged_decode_attention", k_cache, v_cache)
     B, Hq, hd = q.shape
-    if k_cache.shape[3] != hd or Hq < 1 or Hq % k_cache.shape[1]:
+    if cache.head_dim != hd or Hq < 1 or Hq % cache.n_kv_heads:
         raise ValueError(f"paged_decode_attention: queries {tuple(q.shape)} do not fit the cache {tuple(k_cache.shape)}")
     kv_lens = _ints("paged_decode_attention: kv_lens", kv_lens, torch.int32, 1)
     block_tables = _ints("paged_decode_attention: block_tables", block_tables, torch.int32, 2)
-    if kv_lens.shape[0] != B or block_tables.shape[0] != B:
-        raise ValueError(f"paged_decode_attention: {B} queries, {kv_lens.shape[0]} lengths, {block_tables.shape[0]} table rows")
+    rows, width = block_tables.shape
+    if kv_lens.shape[0] != B or rows != B:
+        raise ValueError(f"paged_decode_attention: {B} queries, {kv_lens.shape[0]} lengths, {rows} table rows")
     if (cache.k_stride_page | cache.k_stride_head | cache.k_stride_row | cache.v_stride_page | cache.v_stride_head | cache.v_stride_row) % 8 \
             or (cache.k | cache.v) % 16:
         raise ValueError("paged_decode_attention: the rows of the caches must begin on 16-byte boundaries")
     scale = hd ** -0.5 if scale is None else float(scale)
     if not math.isfinite(scale):
         raise ValueError(f"paged_decode_attention: scale {scale}")
-    if q.stride(2) != 1 or q.stride(0) % 8 or q.stride(1) % 8 or q.data_ptr() % 16:
+    sb, sh, unit = q.stride()
+    if unit != 1 or sb % 8 or sh % 8 or q.data_ptr() % 16:
         q = q.contiguous()
         q = q.clone() if q.data_ptr() % 16 else q
+        sb, sh, _ = q.stride()
     if out is None:
-        out = torch.empty(B, Hq, hd, dtype=q.dtype, device=dev)
+        out = torch.empty(B, Hq, hd, dtype=dtype, device=dev)
     elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev or not out.is_contiguous() or out.data_ptr() % 16:
         raise ValueError("paged_decode_attention: out must be a contiguous, 16-byte aligned tensor of q's shape and dtype")
     lse = torch.empty(B, Hq, dtype=torch.float32, device=dev) if return_lse else None
@@ -187,8 +193,8 @@ def paged_decode_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_ta
                 n = _workspace_bytes[key] = L.hb200_paged_attention_workspace_bytes(B, Hq, cache.n_kv_heads, hd)
             ws = torch.empty(n, dtype=torch.uint8, device=dev)
             _lib.check(L.hb200_paged_decode_attention(
-                cache, q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), lse.data_ptr() if return_lse else None,
-                block_tables.data_ptr(), block_tables.shape[1], block_tables.shape[1], kv_lens.data_ptr(), B, Hq, scale,
+                cache, q.data_ptr(), sb, sh, out.data_ptr(), lse.data_ptr() if return_lse else None,
+                block_tables.data_ptr(), width, width, kv_lens.data_ptr(), B, Hq, scale,
                 ws.data_ptr(), n, kernels._stream(dev)), "paged_decode_attention")
     return (out, lse) if return_lse else out
 

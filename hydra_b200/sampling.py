@@ -57,22 +57,26 @@ def token_logprobs(logits: Tensor, tokens: Tensor, top: int = 0, temperature: fl
     no part and come last; a row without any other, or with NaN or +inf, gives NaN."""
     dev = kernels._require_cuda(logits, tokens)
     kernels._refuse_autograd("token_logprobs", logits)
-    if logits.dim() != 2 or (logits.stride(1) != 1 and logits.shape[1] > 1):
+    shape, strides = logits.shape, logits.stride()
+    if len(shape) != 2 or (strides[1] != 1 and shape[1] > 1):
         raise ValueError("token_logprobs: logits must be [N, V] with unit column stride")
     dtype = kernels._dtype_code(logits)
-    N = logits.shape[0]
-    V = int(vocab) if vocab is not None else logits.shape[1]
+    N, columns = shape
+    V = int(vocab) if vocab is not None else columns
     top, temperature = int(top), float(temperature)
-    if not 1 <= V <= logits.shape[1]:
-        raise ValueError(f"token_logprobs: vocab {V} outside the row length {logits.shape[1]}")
+    if not 1 <= V <= columns:
+        raise ValueError(f"token_logprobs: vocab {V} outside the row length {columns}")
     if tokens.dtype != torch.int64 or tokens.numel() != N:
         raise ValueError(f"token_logprobs: one int64 token per row, got {tokens.dtype} {tuple(tokens.shape)} for {N} rows")
     if not 0 <= top <= min(32, V):
         raise ValueError(f"token_logprobs: top {top} (0 to 32, at most the vocabulary)")
     if not 1e-6 <= temperature <= 1e6:
         raise ValueError(f"token_logprobs: temperature {temperature} (1e-6 to 1e6)")
-    if N > 1 and logits.stride(0) < V:
-        logits = logits.contiguous()          # rows that overlap (an expanded row)
+    ld = strides[0]
+    if ld < V:
+        if N > 1:
+            logits = logits.contiguous()      # rows that overlap (an expanded row)
+        ld = columns
     tokens = tokens if tokens.is_contiguous() else tokens.contiguous()
     f32 = torch.float32
     r = TokenLogprobs(torch.empty(N, dtype=f32, device=dev), torch.empty(N, dtype=f32, device=dev),
@@ -80,8 +84,7 @@ def token_logprobs(logits: Tensor, tokens: Tensor, top: int = 0, temperature: fl
     if N > 0:
         with kernels._on(dev):
             _lib.check(_lib.lib().hb200_token_logprobs(
-                logits.data_ptr(), tokens.data_ptr(), N, V, logits.stride(0) if N > 1 else max(logits.stride(0), V), int(ignore_index),
-                temperature, top, r.logprobs.data_ptr(), r.entropy.data_ptr(), r.top_logprobs.data_ptr(), r.top_ids.data_ptr(),
+                logits.data_ptr(), tokens.data_ptr(), N, V, ld, ignore_index, temperature, top, r.logprobs.data_ptr(), r.entropy.data_ptr(), r.top_logprobs.data_ptr(), r.top_ids.data_ptr(),
                 dtype, kernels._stream(dev)), "token_logprobs")
     return r
 
