@@ -505,15 +505,16 @@ __global__ void __launch_bounds__(NT) token_logprobs_kernel(const LogprobParams 
   // no logit above -inf, or NaN / +inf among them.  (Only warp 0 holds the sums.)
   if (warp > 0) return;
   const bool none = !(a.s > 0.f) || a.m == INFINITY;
-  const float lz2 = log2f(a.s);
-  const float lz = (lz2 - off_of(a.m, c)) * kLn2;
-  auto logp = [&](float v) { return fmaf(v - a.m, p.inv_t, -lz); };
+  // The sum relative to the largest logit's own term, which is 2^off as the sum holds it: where one token is nearly certain, what
+  // is left is a sum of small terms next to a one, not to a power that was rounded.
+  const float off = off_of(a.m, c), lz2 = log2f(a.s / ex2f(off)), lz = lz2 * kLn2;
+  auto logp = [&](float v) { return fmaf(v - a.m, p.inv_t, -lz); };     // ln p of a logit
   if (lane == 0) {
     float lp = nan;
     if (tgt == p.ignore) lp = 0.f;
     else if (scored && !none) lp = logp(x_tgt);
     p.logprobs[r] = lp;
-    p.entropy[r] = none ? nan : (lz2 - a.u / a.s) * kLn2;
+    p.entropy[r] = none ? nan : (lz2 - (a.u / a.s - off)) * kLn2;
   }
   if (TOP && lane < p.top) {   // top <= 32
     const uint64_t e = lane < have ? mine_best[lane] : 0;

@@ -153,7 +153,7 @@ def paged_decode_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_ta
     and, if asked, the fp32 logarithm of each softmax's sum [B, Hq].  A request of length 0 gives zeros and -inf; one whose
     table names a page outside the cache, or whose length passes its table, gives NaN.  What lies behind a
     request's length in its last page is not looked at; an infinite value among the attended ones gives NaN or infinity in
-    its column.  Equal inputs give equal bits."""
+    its column.  Requests may share pages.  Equal inputs give equal bits."""
     dev = kernels._require_cuda(q, k_cache, v_cache, block_tables, kv_lens)
     kernels._refuse_autograd("paged_decode_attention", q, k_cache, v_cache)
     dtype = q.dtype

@@ -73,6 +73,29 @@ def test_extreme_temperatures(dtype, temperature, N, V):
     check(x.cuda(), top=8, temperature=temperature)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_nearly_certain_tokens(dtype):
+    """ln p and the entropy of rows in which one token takes all but a small part e of the mass are of the size of e, and right to
+    the roundings of the sum 1 + e.  Each of them is off by at most 2^-24 (half a step between one and two).  The sum that holds
+    the one is added to by its thread's other columns, in pairs (at most 15 of 30000 in four slices over 512 threads: 8
+    times), once by its second half, five times over the lanes, four over the warps and three over the slices: 21 roundings.
+    The terms' own are 2^-22 of e each and the product and the sum of the result a few 2^-24 of it: 2^-20 relative."""
+    g = torch.Generator().manual_seed(6)
+    for V in (1000, 30000):
+        x = torch.randn(40, V, generator=g)
+        x[:, 7] = torch.linspace(9.0, 30.0, 40)
+        x = x.to(dtype)
+        from hydra_b200.sampling import token_logprobs
+        t = torch.full((40,), 7)
+        r = token_logprobs(x.cuda(), t.cuda(), top=1)
+        lp, h, tl, ti = exact(x, t, 1, 1.0)
+        for got, want in ((r.logprobs, lp), (r.top_logprobs[:, 0], tl[:, 0])):
+            assert ((got.double().cpu() - want).abs() <= 21 * 2.0 ** -24 + 2.0 ** -20 * want.abs()).all()
+        # (an entropy's terms are e times distances of up to 34: their sum is rounded where e times 34 is, at less than 2^-24 of
+        # the entropy each; the one's roundings come in through ln Z and through the division)
+        assert ((r.entropy.double().cpu() - h).abs() <= 2 * 21 * 2.0 ** -24 + 2.0 ** -19 * h.abs()).all()
+
+
 @pytest.mark.parametrize("scale", [1e5, 1e8, 1e30, -1e30])
 @pytest.mark.parametrize("N", [2, 300])
 def test_huge_logits(scale, N):

@@ -309,6 +309,34 @@ def test_strided_queries_streams_out_and_refusals():
         paged_decode_attention(q.clone().requires_grad_(), kd, vd, tb, n)
 
 
+def test_shared_pages_and_two_streams_at_once():
+    """Requests that hold the same pages (a common prompt), and two calls that overlap on two streams, many times over."""
+    from hydra_b200.paged import paged_decode_attention
+    g = torch.Generator().manual_seed(9)
+    k, v, kd, vd, table = cache_of(g, [900], 2, 64, 16, torch.bfloat16)
+    lens = [900, 896, 1, 450, 900]
+    q = torch.randn(5, 8, 64, generator=g).to(torch.bfloat16)
+    tb = table.expand(5, -1).contiguous()
+    n = torch.tensor(lens, dtype=torch.int32).cuda()
+    out, lse = paged_decode_attention(q.cuda(), kd, vd, tb.cuda(), n, return_lse=True)
+    check(out, lse, *attend(q, k, v, tb, lens, 0.125), torch.bfloat16)
+    k2, v2, kd2, vd2, table2 = cache_of(g, [3000, 20, 777], 1, 128, 16, torch.float16)
+    q2, n2 = torch.randn(3, 4, 128, generator=g).half().cuda(), torch.tensor([3000, 20, 777], dtype=torch.int32).cuda()
+    want2 = paged_decode_attention(q2, kd2, vd2, table2.cuda(), n2)
+    qd, td, td2 = q.cuda(), tb.cuda(), table2.cuda()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for _ in range(30):
+        with torch.cuda.stream(streams[0]):
+            a = paged_decode_attention(qd, kd, vd, td, n)
+        with torch.cuda.stream(streams[1]):
+            b = paged_decode_attention(q2, kd2, vd2, td2, n2)
+        got.append((a, b))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, out) and torch.equal(b, want2) for a, b in got)
+
+
 # ------------------------------------------------------------------------------------------------------- whole steps
 def product(a, b):
     """a @ b in an order that is the same eagerly and in a graph."""
