@@ -13,10 +13,10 @@
 // `top` exact selection rounds instead.
 //
 // Measured (device time): 8192 rows of 50257 bf16 logits and one alternative: 134 us, 6.1 TB/s, 0.94 of a copy (153 us once the
-// power cap holds the clock at 1.65 GHz: then the issue slots bound it); one row: 7.6 us, 64 masked rows with 20: 10.1 us,
-// launch, one trip through the row and three through barriers and the cluster.
+// power cap holds the clock at 1.65 GHz: then the issue slots bound it); one row: 7.5 us, 64 masked rows with 20: 8.1 us,
+// launch, one trip through the row and three through barriers.
 //
-// Few rows are split over a cluster of CTAs, whose partial results the first CTA merges through distributed shared memory.
+// Few long rows are split over a cluster of CTAs, whose partial results the first CTA merges through distributed shared memory.
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -542,9 +542,11 @@ int launch_nt(const LogprobParams& p, int64_t rows, int cluster, cudaStream_t st
 
 template <typename T>
 int launch(LogprobParams p, int64_t rows, cudaStream_t st) {
-  // Few rows: up to eight CTAs per row, so that about two CTAs per SM have work and each still has 4096 columns.
+  // Few long rows: up to eight CTAs per row while there is an SM for each and each still has 64 KB: shorter slices cost more in
+  // the cluster's barriers and the merge than they save (one row of 152064 bf16 columns: 11.2 us in one CTA, 8.2 in four;
+  // 64 rows of 50257, 100 KB each: 8.1 in one, 10.1 in four).
   int cluster = 1;
-  while (cluster < 8 && rows * cluster * 2 <= 2 * 148 && p.cols / (cluster * 2) >= 4096) cluster *= 2;
+  while (cluster < 8 && rows * cluster * 2 <= 148 && (int64_t)p.cols * sizeof(T) / (cluster * 2) >= 65536) cluster *= 2;
   p.slice = ceil_div(ceil_div(p.cols, cluster), 64) * 64;
   // Many rows: small CTAs, whose barriers hold up little and whose fixed work per row (joining the statistics, the bound) is
   // small; few: 512 threads get a row's bytes under way sooner; between them, and for long rows of many alternatives, 256

@@ -451,7 +451,8 @@ extern "C" int hb200_qk_norm_rope(const hb200_qk_norm_rope_args* a, const hb200_
   }
   p.group_lanes = 1;
   while (p.group_lanes * 8 < p.hd) p.group_lanes <<= 1;
-  // a token's head rows are shared out over more groups of lanes until about 8 warps per SM have work
+  // a token's head rows are shared out over more groups of lanes until about 8 warps per SM have work (8192 tokens of ten heads of
+  // 32: 4.0 us; until 32 have: 6.1, each setting up its angles)
   const int groups = 32 / p.group_lanes, kinds = c ? 2 : 1;
   p.q_parts = p.kv_parts = 1;
   auto count = [&]() {
