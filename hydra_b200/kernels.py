@@ -57,9 +57,12 @@ def _require_cuda(*ts: Tensor) -> torch.device:
     return ts[0].device
 
 
+_HERE = nullcontext()
+
+
 def _on(dev: torch.device):
     """Context that makes `dev` the current CUDA device (kernels launch on the current device)."""
-    return nullcontext() if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+    return _HERE if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
 
 
 def _stream(dev: torch.device) -> int:
