@@ -51,15 +51,17 @@ struct PagedParams {
 //
 // A warp's tile: 8 KB of K and V (16 KB of heads of 256, 4 KB of small ones, whose tokens cost more arithmetic per byte and get
 // twice the warps: 64 requests up to 16384 tokens on 4 kv heads of 16 took 48 us with eight warps, 43 with sixteen); two
-// tiles of a warp are in flight while one is computed, 128 KB of a CTA.
+// tiles of a warp are in flight while one is computed, 128 KB of a CTA.  Heads of 64 do better with twelve warps and one tile
+// in flight each (64 requests up to 8192 tokens: 53.2 us instead of 54.7), heads of 128 no better and worse where there is
+// little to do (one request of 1500: 11.5 instead of 10.9).
 __host__ __device__ constexpr int tile_tokens(int HD) { return HD >= 128 ? 16 : (HD == 16 ? 64 : 32); }
-__host__ __device__ constexpr int warps_of(int HD) { return HD >= 256 ? 4 : (HD <= 32 ? 16 : 8); }
+__host__ __device__ constexpr int warps_of(int HD) { return HD >= 256 ? 4 : (HD == 128 ? 8 : (HD == 64 ? 12 : 16)); }
+__host__ __device__ constexpr int stages_of(int HD) { return HD == 64 ? 2 : 3; }
 // Query heads that are worked on together: their outputs and queries stay in a warp's registers.
 __host__ __device__ constexpr int q_tile_of(int HD) { return HD >= 256 ? 8 : 16; }
 // Places that a pair takes before its first tile when the shares are cut: what its start and end cost, in tiles.  (256 requests
 // of 1 to 300 tokens on 8 kv heads of 128: 54 us with one, 48 with two, 46 with three; all of 100 tokens: 36, 37 and 38.)
 __host__ __device__ constexpr int pair_cost(int HD) { return HD <= 32 ? 2 : 3; }
-constexpr int kStages = 3;
 
 // Cache length of request b as the kernel reads it: what lies outside [0, width * page_size] is marked (`poison`).
 __device__ __forceinline__ int clamp_len(int len, int64_t cap, bool& poison) {
@@ -142,7 +144,7 @@ struct Cursor {
 // share a page: one look into the table for them (64 requests, pages of 16: 55.3 us with it, 56.3 without).
 template <typename T, int HD, int NQ, bool P16>
 __global__ void __launch_bounds__(warps_of(HD) * 32, 1) paged_attention_kernel(const PagedParams p) {
-  constexpr int NW = warps_of(HD), TT = tile_tokens(HD), CH = HD / 8, ST = kStages;
+  constexpr int NW = warps_of(HD), TT = tile_tokens(HD), CH = HD / 8, ST = stages_of(HD);
   constexpr int ROWB = HD * 2, KBYTES = TT * ROWB, STAGE = 2 * KBYTES;
   constexpr int MT = TT / 16;                        // 16-token tiles
   constexpr int KS = HD / 16;                        // 16-value steps of a head
@@ -784,7 +786,7 @@ size_t workspace_for(int B, int Hq, int Hkv, int hd, int sms) {
 template <typename T, int HD, int NQ>
 int launch(const PagedParams& p, int sms, cudaStream_t st) {
   constexpr int NW = warps_of(HD);
-  const size_t smem = (size_t)NW * kStages * 2 * tile_tokens(HD) * HD * 2 + (size_t)(2 * p.B + 1) * 4;
+  const size_t smem = (size_t)NW * stages_of(HD) * 2 * tile_tokens(HD) * HD * 2 + (size_t)(2 * p.B + 1) * 4;
   auto kern = p.page_size % 16 == 0 ? paged_attention_kernel<T, HD, NQ, true> : paged_attention_kernel<T, HD, NQ, false>;
   HB_PROPAGATE(ensure_dynamic_smem((const void*)kern, smem));
   kern<<<(unsigned)sms, NW * 32, smem, st>>>(p);

@@ -437,6 +437,10 @@ extern "C" int hb200_qk_norm_rope(const hb200_qk_norm_rope_args* a, const hb200_
     HB_REQUIRE(a->slots && a->v && c->k && c->v, HB200_ERR_INVALID, "qk_norm_rope: null pointer (cache, slots or v)");
     HB_REQUIRE(c->n_kv_heads == a->Hkv && c->head_dim == a->hd && c->dtype == a->dtype && c->num_pages >= 0 && c->page_size >= 1,
                HB200_ERR_INVALID, "qk_norm_rope: the cache's heads or dtype are not those of k");
+    const int64_t apart[][2] = {{c->num_pages, c->k_stride_page}, {c->n_kv_heads, c->k_stride_head}, {c->page_size, c->k_stride_row},
+                                {c->num_pages, c->v_stride_page}, {c->n_kv_heads, c->v_stride_head}, {c->page_size, c->v_stride_row}};
+    for (const auto& d : apart)
+      HB_REQUIRE(d[0] <= 1 || d[1] != 0, HB200_ERR_INVALID, "qk_norm_rope: the cache's rows lie on top of one another");
     p.v = a->v; p.kc = c->k; p.vc = c->v; p.slots = a->slots;
     p.page_size = c->page_size;
     p.capacity = (int64_t)c->num_pages * c->page_size;

@@ -70,7 +70,7 @@ def _rope(cache=None, **kw):
     (dict(positions=None, S=129), -1, "129"), (dict(q=None), -1, "null"), (dict(k_out=None), -1, "null"), (dict(cos=None), -1, "null"),
     (dict(dtype=7), -4, "dtype"), (dict(cache=_cache(), slots=None), -1, "null"), (dict(cache=_cache(n_kv_heads=2)), -1, "cache"),
     (dict(cache=_cache(head_dim=32)), -1, "cache"), (dict(cache=_cache(dtype=_lib.HB200_F16)), -1, "cache"),
-    (dict(cache=_cache(v=None)), -1, "null"),
+    (dict(cache=_cache(v=None)), -1, "null"), (dict(cache=_cache(k_stride_page=0)), -1, "on top"), (dict(cache=_cache(v_stride_row=0)), -1, "on top"),
 ])
 def test_qk_norm_rope_refuses(bad, status, text):
     assert _rope(**bad) == status and text in _last()
