@@ -23,6 +23,12 @@ from . import _lib
 
 Tensor = torch.Tensor
 
+try:   # empty_strided on the current CUDA device by its shortest way: half the 1.5 us of torch.empty, several times a call
+    _empty_strided = torch._C._dynamo.guards._empty_strided_cuda   # (size, stride: plain tuples; dtype)
+except AttributeError:
+    def _empty_strided(size, stride, dtype):
+        return torch.empty_strided(size, stride, dtype=dtype, device="cuda")
+
 # Flags the reference exports.  No Triton is involved here; the names are kept so callers that read them
 # keep working, and they report whether the CUDA path is active.
 TRITON_AVAILABLE = False
@@ -216,11 +222,9 @@ def _refuse_autograd(what: str, *ts: Optional[Tensor]) -> None:
                 raise RuntimeError(f"{what} is inference only: an input requires grad (wrap the call in torch.no_grad())")
 
 
-def _fp32(what: str, t: Optional[Tensor], n: int, dev: torch.device) -> Optional[Tensor]:
-    if t is None:
-        return None
+def _fp32(what: str, t: Tensor, n: int, dev: torch.device) -> Tensor:
     if t.get_device() != dev.index or t.numel() != n:
-        raise ValueError(f"{what} must have {n} elements on {dev}, got {tuple(t.shape)} on {t.device}")
+        raise ValueError(f"{what}: q_weight and k_weight must have {n} elements on {dev}, got {tuple(t.shape)} on {t.device}")
     return t if t.dtype == torch.float32 and t.is_contiguous() else t.float().contiguous()
 
 
@@ -249,16 +253,16 @@ def _qk_norm_rope(what: str, dev: torch.device, q: Tensor, k: Tensor, cos: Tenso
     if qs[-1] != 1 or ks[-1] != 1 or vs[-1] != 1:
         q, k, v = q.contiguous(), k.contiguous(), None if v is None else v.contiguous()
         qs, ks, vs = q.stride(), k.stride(), (0, 0, 1) if v is None else v.stride()
-    q_out = torch.empty(*shape, dtype=torch_dtype, device=dev)
-    k_out = torch.empty(*k_shape, dtype=torch_dtype, device=dev) if cache is None else None
     # strides of batch, token and head; the results are contiguous
     if len(shape) == 3:
         S, Hq, _ = shape
         B, Hkv = 1, k_shape[1]
+        new = (S, Hq, hd), (Hq * hd, hd, 1), (S, Hkv, hd), (Hkv * hd, hd, 1)
         strides = (0, qs[0], qs[1], 0, ks[0], ks[1], 0, vs[0], vs[1], 0, Hq * hd, hd, 0, Hkv * hd, hd)
     else:
         B, Hq, S, _ = shape
         Hkv = k_shape[1]
+        new = (B, Hq, S, hd), (Hq * S * hd, S * hd, hd, 1), (B, Hkv, S, hd), (Hkv * S * hd, S * hd, hd, 1)
         strides = (qs[0], qs[2], qs[1], ks[0], ks[2], ks[1], 0, 0, 0, Hq * S * hd, hd, S * hd, Hkv * S * hd, hd, S * hd)
     where, where_64, where_stride = None, 0, 0
     if positions is not None:
@@ -277,18 +281,19 @@ def _qk_norm_rope(what: str, dev: torch.device, q: Tensor, k: Tensor, cos: Tenso
     elif table_rows < S:
         raise ValueError(f"{what}: tables {tuple(table)} do not cover {S} positions")
     if q_weight is not None:
-        q_weight = _fp32(f"{what}: q_weight", q_weight, hd, dev)
+        q_weight = _fp32(what, q_weight, hd, dev)
     if k_weight is not None:
-        k_weight = _fp32(f"{what}: k_weight", k_weight, hd, dev)
-    if (Hq + Hkv) * B * S * hd == 0:
-        return q_out, k_out
-    args = _lib.QkNormRopeArgs(                # in the order of the struct
-        q.data_ptr(), k.data_ptr(), None if v is None else v.data_ptr(), q_out.data_ptr(), None if k_out is None else k_out.data_ptr(),
-        None if slots is None else slots.data_ptr(), where, cos.data_ptr(), sin.data_ptr(), None if q_weight is None else q_weight.data_ptr(),
-        None if k_weight is None else k_weight.data_ptr(), *strides, where_stride, table_rows, table_ld, where_64, B, S, Hq, Hkv, hd,
-        2 * half, layout_code, norm_code, dtype, eps, q_scale, k_scale)
+        k_weight = _fp32(what, k_weight, hd, dev)
     with _on(dev):
-        _lib.check(_lib.lib().hb200_qk_norm_rope(args, cache, _stream(dev)), what)
+        q_out = _empty_strided(new[0], new[1], torch_dtype)
+        k_out = _empty_strided(new[2], new[3], torch_dtype) if cache is None else None
+        if (Hq + Hkv) * B * S * hd > 0:
+            args = _lib.QkNormRopeArgs(        # in the order of the struct
+                q.data_ptr(), k.data_ptr(), None if v is None else v.data_ptr(), q_out.data_ptr(), None if k_out is None else k_out.data_ptr(),
+                None if slots is None else slots.data_ptr(), where, cos.data_ptr(), sin.data_ptr(),
+                None if q_weight is None else q_weight.data_ptr(), None if k_weight is None else k_weight.data_ptr(), *strides, where_stride,
+                table_rows, table_ld, where_64, B, S, Hq, Hkv, hd, 2 * half, layout_code, norm_code, dtype, eps, q_scale, k_scale)
+            _lib.check(_lib.lib().hb200_qk_norm_rope(args, cache, _stream(dev)), what)
     return q_out, k_out
 
 

@@ -77,16 +77,16 @@ def paged_plan(context_lens: Tensor, new_lens: Tensor, block_tables: Tensor, fre
     if free_start is not None:
         if free_start.get_device() != dev.index or free_start.dtype != torch.int32 or free_start.numel() != 1:
             raise ValueError("paged_plan: free_start must be one int32 on the tables' device")
-    # one allocation for the five small arrays: positions first (16-byte aligned, as the kernel stores them)
-    head = (room + 3) // 4 * 4
-    positions, kv_lens, cu_new, start_out, status = torch.empty(head + 2 * B + 3, dtype=torch.int32, device=dev).split([head, B, B + 1, 1, 1])
-    plan = PagedPlan(kv_lens, cu_new, positions if head == room else positions[:room], torch.empty(room, dtype=torch.int64, device=dev), start_out,
-                     status)
+    i32, one = torch.int32, (1,)
     with kernels._on(dev):
+        new = kernels._empty_strided
+        plan = PagedPlan(new((B,), one, i32), new((B + 1,), one, i32), new((room,), one, i32), new((room,), one, torch.int64), new(one, one, i32),
+                         new(one, one, i32))
+        kv_lens, cu_new, positions, slots, start_out, status = plan
         _lib.check(_lib.lib().hb200_paged_plan(
             context_lens.data_ptr(), new_lens.data_ptr(), B, block_tables.data_ptr(), ld if B > 1 else width, width,
             page_size, free_pages.data_ptr(), free_pages.shape[0], free_start.data_ptr() if free_start is not None else None,
-            kv_lens.data_ptr(), cu_new.data_ptr(), positions.data_ptr(), plan.slots.data_ptr(), room, start_out.data_ptr(),
+            kv_lens.data_ptr(), cu_new.data_ptr(), positions.data_ptr(), slots.data_ptr(), room, start_out.data_ptr(),
             status.data_ptr(), kernels._stream(dev)), "paged_plan")
     return plan
 
@@ -179,19 +179,20 @@ def paged_decode_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_ta
         q = q.contiguous()
         q = q.clone() if q.data_ptr() % 16 else q
         sb, sh, _ = q.stride()
-    if out is None:
-        out = torch.empty(B, Hq, hd, dtype=dtype, device=dev)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev or not out.is_contiguous() or out.data_ptr() % 16:
+    if out is not None and (out.shape != q.shape or out.dtype != dtype or out.device != dev or not out.is_contiguous() or out.data_ptr() % 16):
         raise ValueError("paged_decode_attention: out must be a contiguous, 16-byte aligned tensor of q's shape and dtype")
-    lse = torch.empty(B, Hq, dtype=torch.float32, device=dev) if return_lse else None
-    if B > 0:
-        with kernels._on(dev):
+    with kernels._on(dev):
+        new = kernels._empty_strided
+        if out is None:
+            out = new((B, Hq, hd), (Hq * hd, hd, 1), dtype)
+        lse = new((B, Hq), (Hq, 1), torch.float32) if return_lse else None
+        if B > 0:
             L = _lib.lib()
             key = (dev.index, B, Hq, cache.n_kv_heads, hd)
             n = _workspace_bytes.get(key)
             if n is None:
                 n = _workspace_bytes[key] = L.hb200_paged_attention_workspace_bytes(B, Hq, cache.n_kv_heads, hd)
-            ws = torch.empty(n, dtype=torch.uint8, device=dev)
+            ws = new((n,), (1,), torch.uint8)
             _lib.check(L.hb200_paged_decode_attention(
                 cache, q.data_ptr(), sb, sh, out.data_ptr(), lse.data_ptr() if return_lse else None,
                 block_tables.data_ptr(), width, width, kv_lens.data_ptr(), B, Hq, scale,

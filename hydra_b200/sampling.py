@@ -78,14 +78,14 @@ def token_logprobs(logits: Tensor, tokens: Tensor, top: int = 0, temperature: fl
             logits = logits.contiguous()      # rows that overlap (an expanded row)
         ld = columns
     tokens = tokens if tokens.is_contiguous() else tokens.contiguous()
-    f32 = torch.float32
-    r = TokenLogprobs(torch.empty(N, dtype=f32, device=dev), torch.empty(N, dtype=f32, device=dev),
-                      torch.empty(N, top, dtype=f32, device=dev), torch.empty(N, top, dtype=torch.int64, device=dev))
-    if N > 0:
-        with kernels._on(dev):
+    with kernels._on(dev):
+        new, f32 = kernels._empty_strided, torch.float32
+        r = TokenLogprobs(new((N,), (1,), f32), new((N,), (1,), f32), new((N, top), (max(top, 1), 1), f32),
+                          new((N, top), (max(top, 1), 1), torch.int64))
+        if N > 0:
             _lib.check(_lib.lib().hb200_token_logprobs(
-                logits.data_ptr(), tokens.data_ptr(), N, V, ld, ignore_index, temperature, top, r.logprobs.data_ptr(), r.entropy.data_ptr(), r.top_logprobs.data_ptr(), r.top_ids.data_ptr(),
-                dtype, kernels._stream(dev)), "token_logprobs")
+                logits.data_ptr(), tokens.data_ptr(), N, V, ld, ignore_index, temperature, top, r.logprobs.data_ptr(),
+                r.entropy.data_ptr(), r.top_logprobs.data_ptr(), r.top_ids.data_ptr(), dtype, kernels._stream(dev)), "token_logprobs")
     return r
 
 
