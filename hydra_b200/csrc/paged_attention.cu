@@ -57,8 +57,11 @@ struct PagedParams {
 __host__ __device__ constexpr int tile_tokens(int HD) { return HD >= 128 ? 16 : (HD == 16 ? 64 : 32); }
 __host__ __device__ constexpr int warps_of(int HD) { return HD >= 256 ? 4 : (HD == 128 ? 8 : (HD == 64 ? 12 : 16)); }
 __host__ __device__ constexpr int stages_of(int HD) { return HD == 64 ? 2 : 3; }
-// Query heads that are worked on together: their outputs and queries stay in a warp's registers.
-__host__ __device__ constexpr int q_tile_of(int HD) { return HD >= 256 ? 8 : 16; }
+// Most query heads that are worked on together: their outputs and queries stay in a warp's registers.  Larger groups are cut
+// into tiles of one size, each of which reads the keys and values again.  (Groups of 20: 82 requests of 5115 tokens on heads of
+// 80 take 181 us in one tile and 240 in two of ten, 64 requests up to 32768 on heads of 16 59 and 73; where the second read
+// comes out of the L2, 32 requests up to 8192 on two kv heads of 128, 57 and 53.)
+__host__ __device__ constexpr int most_heads(int HD) { return HD >= 256 ? 8 : 24; }
 // Places that a pair takes before its first tile when the shares are cut: what its start and end cost, in tiles.  (256 requests
 // of 1 to 300 tokens on 8 kv heads of 128: 54 us with one, 48 with two, 46 with three; all of 100 tokens: 36, 37 and 38.)
 __host__ __device__ constexpr int pair_cost(int HD) { return HD <= 32 ? 2 : 3; }
@@ -140,7 +143,7 @@ struct Cursor {
   bool poison;
 };
 
-// NQ: columns of eight query heads (group <= 8: 1).  P16: the page size is a multiple of 16, so that 16 tokens side by side
+// NQ: columns of eight query heads (a tile of up to 8: 1).  P16: the page size is a multiple of 16, so that 16 tokens side by side
 // share a page: one look into the table for them (64 requests, pages of 16: 55.3 us with it, 56.3 without).
 template <typename T, int HD, int NQ, bool P16>
 __global__ void __launch_bounds__(warps_of(HD) * 32, 1) paged_attention_kernel(const PagedParams p) {
@@ -324,11 +327,14 @@ __global__ void __launch_bounds__(warps_of(HD) * 32, 1) paged_attention_kernel(c
           page0 = off0 = 0;
           head_of();
           // the next pair's queries (128 bytes a lane) come near before they are asked for
-          const int qt = p.q_tiles == 1 ? 0 : pc.h % p.q_tiles, h0 = (p.q_tiles == 1 ? pc.h : pc.h / p.q_tiles) * p.group + qt * q_tile_of(HD);
+          const int qt = p.q_tiles == 1 ? 0 : pc.h % p.q_tiles, h0 = (p.q_tiles == 1 ? pc.h : pc.h / p.q_tiles) * p.group + qt * p.q_tile;
           constexpr int LPQ = (HD * 2 + 127) / 128;         // lanes per query head
-          const int r = lane / LPQ;
-          if (r < min(q_tile_of(HD), p.group - qt * q_tile_of(HD)) && lane % LPQ * 64 < p.hd)
-            prefetch(static_cast<const T*>(p.q) + (int64_t)pc.b * p.q_sb + (int64_t)(h0 + r) * p.q_sh + lane % LPQ * 64);
+#pragma unroll
+          for (int i = 0; i < (NQ * 8 * LPQ + 31) / 32; ++i) {
+            const int u = i * 32 + lane, r = u / LPQ;
+            if (r < min(p.q_tile, p.group - qt * p.q_tile) && u % LPQ * 64 < p.hd)
+              prefetch(static_cast<const T*>(p.q) + (int64_t)pc.b * p.q_sb + (int64_t)(h0 + r) * p.q_sh + u % LPQ * 64);
+          }
         }
       }
     }
@@ -385,8 +391,8 @@ __global__ void __launch_bounds__(warps_of(HD) * 32, 1) paged_attention_kernel(c
       fresh = false;
       first_tile = cur.t;
       const int kvh = p.q_tiles == 1 ? cur.h : cur.h / p.q_tiles, qt = cur.h - kvh * p.q_tiles;
-      head0 = kvh * p.group + qt * q_tile_of(HD);
-      rows_here = min(q_tile_of(HD), p.group - qt * q_tile_of(HD));
+      head0 = kvh * p.group + qt * p.q_tile;
+      rows_here = min(p.q_tile, p.group - qt * p.q_tile);
       const T* qb = static_cast<const T*>(p.q) + (int64_t)cur.b * p.q_sb + (int64_t)head0 * p.q_sh;
 #pragma unroll
       for (int n = 0; n < NQ; ++n) {
@@ -507,17 +513,19 @@ __global__ void __launch_bounds__(warps_of(HD) * 32, 1) paged_attention_kernel(c
     --left;
 
     if (cur.t + 1 == cur.n || left == 0) {   // the pair's end, or the share's
-      // It goes through shared memory into rows: at the share's end to the ring's start, where it stays as a part for the CTA
-      // to add up, else through the slot just read (which is not filled again before the next tile) to the workspace or,
-      // if the share held the whole pair, to the output.
+      // It goes through shared memory into rows.  At the share's end to the ring's start, where it stays as a part for the CTA
+      // to add up; else, eight rows at a time, through the slot just read (which is not filled again before the next tile) to
+      // the workspace or, if the share held the whole pair, to the output.
       const bool whole = first_tile == 0 && cur.t + 1 == cur.n, stay = left == 0 && !whole;
       if (left == 0) cp_async_wait<0>();
       __syncwarp();
       float* so = reinterpret_cast<float*>(left == 0 ? ring : ring + (slot == 0 ? ST - 1 : slot - 1) * STAGE);
-      const int ld = stay || NQ > 1 ? p.hd : p.hd + 4;      // (four more words per row: no bank conflicts)
-      float* sm = so + p.rows * p.hd;                       // of a part that stays
+      float* po = stay ? so : p.part + ((int64_t)p.ctas * 2 + w) * p.part_floats;   // of a part
+      T* ob = static_cast<T*>(p.out) + ((int64_t)cur.b * p.Hq + head0) * p.hd;
+      const int ld = stay ? p.hd : p.hd + 4;                // (four more words per row: no bank conflicts)
 #pragma unroll
-      for (int n = 0; n < NQ; ++n)
+      for (int n = 0; n < NQ; ++n) {
+        float* rows_of = stay ? so + n * 8 * p.hd : so;
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           float sum = l[n][e];
@@ -528,46 +536,36 @@ __global__ void __launch_bounds__(warps_of(HD) * 32, 1) paged_attention_kernel(c
           const int r = n * 8 + t4 * 2 + e;
           if (r < rows_here) {
             const float f = whole ? 1.f / l[n][e] : 1.f;
-            float* to = so + r * ld + g;
+            float* to = rows_of + (t4 * 2 + e) * ld + g;
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
               for (int i = 0; i < 2; ++i)
                 if (p.hd == HD || ks * 16 + i * 8 < p.hd) to[ks * 16 + i * 8] = o[ks][n][i * 2 + e] * f;
+            if (g == 0) {
+              if (!whole) *reinterpret_cast<float2*>(po + p.rows * p.hd + r * 2) = make_float2(m[n][e] == -INFINITY ? -INFINITY : base[n][e], l[n][e]);
+              else if (p.lse) p.lse[(int64_t)cur.b * p.Hq + head0 + r] = (base[n][e] + log2f(l[n][e])) * kLn2;
+            }
           }
         }
-      __syncwarp();
-      float* pg = p.part + ((int64_t)p.ctas * 2 + w) * p.part_floats;
-      if (!stay) {
-        if (whole) {
-          T* ob = static_cast<T*>(p.out) + ((int64_t)cur.b * p.Hq + head0) * p.hd;
-          const int per = p.hd / 8;
-          for (int u = lane; u < rows_here * per; u += 32) {
-            const int r = u / per, d = (u - r * per) * 8;
+        if (stay) continue;
+        __syncwarp();
+        const int here = min(8, rows_here - n * 8), per = whole ? p.hd / 8 : p.hd / 4;
+        for (int u = lane; u < here * per; u += 32) {
+          const int r = u / per;
+          if (whole) {
+            const int d = (u - r * per) * 8;
             const float4 x = *reinterpret_cast<const float4*>(so + r * ld + d), y = *reinterpret_cast<const float4*>(so + r * ld + d + 4);
             T eight[8] = {Cvt<T>::from_f(x.x), Cvt<T>::from_f(x.y), Cvt<T>::from_f(x.z), Cvt<T>::from_f(x.w),
                           Cvt<T>::from_f(y.x), Cvt<T>::from_f(y.y), Cvt<T>::from_f(y.z), Cvt<T>::from_f(y.w)};
-            *reinterpret_cast<uint4*>(ob + r * p.hd + d) = *reinterpret_cast<const uint4*>(eight);
+            *reinterpret_cast<uint4*>(ob + (n * 8 + r) * p.hd + d) = *reinterpret_cast<const uint4*>(eight);
+          } else {
+            const int d = (u - r * per) * 4;
+            *reinterpret_cast<float4*>(po + (n * 8 + r) * p.hd + d) = *reinterpret_cast<const float4*>(so + r * ld + d);
           }
-        } else {
-          const int per = p.hd / 4;
-          for (int u = lane; u < rows_here * per; u += 32) {
-            const int r = u / per, d = (u - r * per) * 4;
-            *reinterpret_cast<float4*>(pg + r * p.hd + d) = *reinterpret_cast<const float4*>(so + r * ld + d);
-          }
-          sm = pg + p.rows * p.hd;
         }
+        __syncwarp();
       }
-#pragma unroll
-      for (int n = 0; n < NQ; ++n)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int r = n * 8 + t4 * 2 + e;
-          if (g == 0 && r < rows_here) {
-            if (!whole) *reinterpret_cast<float2*>(sm + r * 2) = make_float2(m[n][e] == -INFINITY ? -INFINITY : base[n][e], l[n][e]);
-            else if (p.lse) p.lse[(int64_t)cur.b * p.Hq + head0 + r] = (base[n][e] + log2f(l[n][e])) * kLn2;
-          }
-        }
       if (!whole && lane == 0) {
         const int k = 2 * warp + (left == 0 ? 1 : 0);
         s_pair[k] = cur.b * H + cur.h;
@@ -602,7 +600,7 @@ __global__ void __launch_bounds__(warps_of(HD) * 32, 1) paged_attention_kernel(c
     if (n % (NW / wpp) != warp / wpp) continue;
     const int b = pair / H, h = pair - b * H;
     const int kvh = p.q_tiles == 1 ? h : h / p.q_tiles, qt = h - kvh * p.q_tiles;
-    const int head = kvh * p.group + qt * q_tile_of(HD), rows = min(q_tile_of(HD), p.group - qt * q_tile_of(HD));
+    const int head = kvh * p.group + qt * p.q_tile, rows = min(p.q_tile, p.group - qt * p.q_tile);
     // (the join finds the part of a pair that began in a CTA before this one in place 0, of one that goes on in the next in 1)
     const int64_t t0 = (int64_t)s_cum[b] * H + (int64_t)h * (s_cum[b + 1] - s_cum[b]) + PC;   // the pair's first tile
     float* po = p.part + ((int64_t)blockIdx.x * 2 + (t0 < (int64_t)blockIdx.x * NW * share ? 0 : 1)) * p.part_floats;
@@ -776,10 +774,13 @@ int padded_hd(int hd) { return hd <= 16 ? 16 : (hd <= 32 ? 32 : (hd <= 64 ? 64 :
 
 size_t round256(size_t n) { return (n + 255) & ~(size_t)255; }
 
+// Heads per tile of a group: as few tiles as there can be, of one size.
+int q_tile_for(int group, int HD) { return ceil_div(group, ceil_div(group, most_heads(HD))); }
+
 int part_floats_of(int rows, int hd) { return ceil_div(rows * (hd + 2), 4) * 4; }   // 16-byte aligned parts
 
 size_t workspace_for(int B, int Hq, int Hkv, int hd, int sms) {
-  const int group = Hq / Hkv, HD = padded_hd(hd), rows = group < q_tile_of(HD) ? group : q_tile_of(HD);
+  const int HD = padded_hd(hd), rows = q_tile_for(Hq / Hkv, HD);
   return round256((size_t)sms * (2 + warps_of(HD)) * part_floats_of(rows, hd) * 4) + round256(((size_t)B + 1) * 4);
 }
 
@@ -811,7 +812,7 @@ int launch_hd(const PagedParams& p, int sms, cudaStream_t st) {
 
 template <typename T>
 int launch_group(const PagedParams& p, int sms, cudaStream_t st) {
-  return p.rows <= 8 ? launch_hd<T, 1>(p, sms, st) : launch_hd<T, 2>(p, sms, st);
+  return p.rows <= 8 ? launch_hd<T, 1>(p, sms, st) : (p.rows <= 16 ? launch_hd<T, 2>(p, sms, st) : launch_hd<T, 3>(p, sms, st));
 }
 
 int check_heads(const char* what, int64_t B, int Hq, int Hkv, int hd) {
@@ -875,9 +876,8 @@ extern "C" int hb200_paged_decode_attention(const hb200_paged_cache* c, const vo
   p.table_ld = table_ld;
   p.B = B; p.Hq = Hq; p.Hkv = c->n_kv_heads; p.hd = c->head_dim; p.group = group;
   const int HD = padded_hd(c->head_dim);
-  p.q_tile = q_tile_of(HD);
+  p.q_tile = p.rows = q_tile_for(group, HD);
   p.q_tiles = ceil_div(group, p.q_tile);
-  p.rows = group < p.q_tile ? group : p.q_tile;
   p.part_floats = part_floats_of(p.rows, p.hd);
   p.tile = tile_tokens(HD);
   p.pair_cost = pair_cost(HD);

@@ -190,7 +190,8 @@ def run(lens, hq, hkv, hd, page, dtype=torch.bfloat16, order="hnd", scale=None, 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("order", ["hnd", "nhd"])
 @pytest.mark.parametrize("hq,hkv,hd", [(4, 4, 128), (8, 2, 32), (32, 4, 16), (12, 3, 64), (2, 1, 256), (5, 1, 80), (16, 1, 8), (20, 1, 64), (40, 2, 128),
-                                       (33, 1, 24), (6, 2, 200), (3, 3, 40), (20, 1, 256), (48, 2, 16), (9, 1, 32)])
+                                       (33, 1, 24), (6, 2, 200), (3, 3, 40), (20, 1, 256), (48, 2, 16), (9, 1, 32), (26, 1, 64), (51, 1, 128),
+                                       (17, 1, 16), (64, 1, 32)])
 def test_heads_and_sizes(dtype, order, hq, hkv, hd):
     run([1, 17, 64, 0, 333, 2], hq, hkv, hd, 16, dtype, order)
 
