@@ -232,7 +232,7 @@ def _qk_norm_rope(what: str, dev: torch.device, q: Tensor, k: Tensor, cos: Tenso
                   q_weight: Optional[Tensor], k_weight: Optional[Tensor], norm: Optional[str], eps: float, q_scale: float,
                   k_scale: float, layout: str, v: Optional[Tensor] = None, slots: Optional[Tensor] = None, cache=None):
     """The call behind fused_qk_norm_rope and paged_append: q, k (v) [T, H, hd] or [B, H, S, hd]."""
-    _refuse_autograd(what, q, k, v, q_weight, k_weight)
+    _refuse_autograd(what, q, k, v, cos, sin, q_weight, k_weight)
     try:
         norm_code, layout_code = _lib.QK_NORMS[norm], _lib.ROPE_LAYOUTS[layout]
     except KeyError:

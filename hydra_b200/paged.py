@@ -149,13 +149,13 @@ def paged_decode_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_ta
     ``h // (Hq // Hkv)``), softmax of ``scale * q . k`` (default ``hd ** -0.5``).
 
     q [B, Hq, hd] bf16 or f16 (up to 4096 requests, 1024 heads; hd a multiple of 8 up to 256), caches as in
-    :func:`paged_append`, ``block_tables`` int32 [B, width], ``kv_lens`` int32 [B].  Returns [B, Hq, hd] (in ``out`` if given)
+    :func:`paged_append`, ``block_tables`` int32 [B, width], ``kv_lens`` int32 [B].  Returns [B, Hq, hd] (in ``out`` if given, which overlaps no input)
     and, if asked, the fp32 logarithm of each softmax's sum [B, Hq].  A request of length 0 gives zeros and -inf; one whose
     table names a page outside the cache, or whose length passes its table, gives NaN.  What lies behind a
     request's length in its last page is not looked at; an infinite value among the attended ones gives NaN or infinity in
     its column.  Requests may share pages.  Equal inputs give equal bits."""
     dev = kernels._require_cuda(q, k_cache, v_cache, block_tables, kv_lens)
-    kernels._refuse_autograd("paged_decode_attention", q, k_cache, v_cache)
+    kernels._refuse_autograd("paged_decode_attention", q, k_cache, v_cache, out)
     dtype = q.dtype
     if q.dim() != 3 or dtype != k_cache.dtype or (dtype != torch.bfloat16 and dtype != torch.float16):
         raise ValueError(f"paged_decode_attention: q must be [B, Hq, hd] in the caches' dtype, bfloat16 or float16, got {tuple(q.shape)} {q.dtype}")
@@ -179,8 +179,11 @@ def paged_decode_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_ta
         q = q.contiguous()
         q = q.clone() if q.data_ptr() % 16 else q
         sb, sh, _ = q.stride()
-    if out is not None and (out.shape != q.shape or out.dtype != dtype or out.device != dev or not out.is_contiguous() or out.data_ptr() % 16):
-        raise ValueError("paged_decode_attention: out must be a contiguous, 16-byte aligned tensor of q's shape and dtype")
+    if out is not None:
+        if out.shape != q.shape or out.dtype != dtype or out.device != dev or not out.is_contiguous() or out.data_ptr() % 16:
+            raise ValueError("paged_decode_attention: out must be a contiguous, 16-byte aligned tensor of q's shape and dtype")
+        if B > 0 and out.data_ptr() < q.data_ptr() + 2 * ((B - 1) * sb + (Hq - 1) * sh + hd) and q.data_ptr() < out.data_ptr() + 2 * B * Hq * hd:
+            raise ValueError("paged_decode_attention: out must not overlap q, which several blocks read")
     with kernels._on(dev):
         new = kernels._empty_strided
         if out is None:

@@ -468,3 +468,26 @@ def test_a_captured_step_replays_with_new_lengths_beside_another_graph():
         for s, p in ((a, got[0]), (b, want[0]), (other, graphs[1][1][0])):
             s.context.copy_(p.kv_lens)
             s.start.copy_(p.free_start)
+
+
+def test_outputs_that_overlap_queries_or_record_gradients_are_refused():
+    from hydra_b200.paged import paged_append, paged_decode_attention
+    g = torch.Generator().manual_seed(21)
+    lens = [40, 3]
+    k, v, kd, vd, table = cache_of(g, lens, 2, 64, 16, torch.bfloat16)
+    q = torch.randn(2, 8, 64, generator=g).to(torch.bfloat16).cuda()
+    tb, n = table.cuda(), torch.tensor(lens, dtype=torch.int32).cuda()
+    room = torch.cat([q, q, q])            # q lies at the end, an output at the beginning touches it or just does not
+    want = paged_decode_attention(q, kd, vd, tb, n)
+    for q_at, out_at in ((2, 2), (2, 3), (3, 2)):
+        with pytest.raises(ValueError, match="overlap"):
+            paged_decode_attention(room[q_at:q_at + 2], kd, vd, tb, n, out=room[out_at:out_at + 2])
+    assert torch.equal(room, torch.cat([q, q, q]))
+    assert torch.equal(paged_decode_attention(room[2:4], kd, vd, tb, n, out=room[:2]), want) and torch.equal(room[2:], torch.cat([q, q]))
+    assert torch.equal(paged_decode_attention(room[2:4], kd, vd, tb, n, out=room[4:]), want) and torch.equal(room[2:4], q)
+    with pytest.raises(RuntimeError, match="inference only"):
+        paged_decode_attention(q, kd, vd, tb, n, out=torch.empty_like(q).requires_grad_())
+    cos = torch.ones(8, 32, device="cuda", requires_grad=True)
+    where = torch.zeros(2, dtype=torch.int32, device="cuda")
+    with pytest.raises(RuntimeError, match="inference only"):
+        paged_append(q, q[:, :2], q[:, 2:4], kd, vd, where.long(), cos, cos, where)
