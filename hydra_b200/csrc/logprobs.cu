@@ -429,13 +429,13 @@ __global__ void __launch_bounds__(NT) token_logprobs_kernel(const LogprobParams 
         if (rk < want) s_part.best[rk] = mine;
       }
     } else {
-      // exact selection rounds: the largest entry below the last one
-      uint64_t last = ~0ull;
+      // exact selection rounds: the largest entry, then the largest below the last one (NaN in column 0 is the largest number there is)
+      uint64_t last = 0;
       for (int k = 0; k < want; ++k) {
         uint64_t best = 0;
         for (int i = tid; i < n; i += NT) {
           const uint64_t e = entry(Cvt<T>::to_f(x[i]), c0 + i);
-          if (e < last && e > best) best = e;
+          if ((k == 0 || e < last) && e > best) best = e;
         }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) {
