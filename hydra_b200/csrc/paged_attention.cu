@@ -89,6 +89,10 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// ln sum e^{scale s} from the largest score and the sum relative to it (0 where every score is -inf).
+__device__ __forceinline__ float log_sum(float m, float l, float scale_log2) {
+  return fmaf(m == -INFINITY ? 0.f : m, scale_log2, log2f(l)) * kLn2;
+}
 template <typename T>
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1);
@@ -382,8 +386,9 @@ __global__ void __launch_bounds__(warps_of(HD) * 32, 1) paged_attention_kernel(c
     vofs[i] = KBYTES + ((mi >> 1) * 8 + mr) * ROWB + (((2 * i + (mi & 1)) ^ swizzle<CH>(mr)) & mask) * 16;
   }
   uint32_t qf[KS][NQ][2];
-  float o[KS][NQ][4], m[NQ][2], l[NQ][2];   // m: the largest score; base: m scale log2(e), rounded once (0 while m is -inf)
-  float base[NQ][2];
+  // m: the largest score; base: the same, 0 while it is -inf.  A weight is 2^((s - base) scale log2(e)): the distance first, which is
+  // exact where it matters, so that scores of any size keep their weights (a product m scale log2(e) is off by 2^7 at 2^31)
+  float o[KS][NQ][4], m[NQ][2], l[NQ][2], base[NQ][2];
   bool poison = false, fresh = true;
   int first_tile = cur.t, rows_here = 0, head0 = 0, slot = 0;
   while (left > 0) {
@@ -467,8 +472,8 @@ __global__ void __launch_bounds__(warps_of(HD) * 32, 1) paged_attention_kernel(c
         float f[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const float to = mx[n][e] == -INFINITY ? 0.f : mx[n][e] * p.scale_log2;   // every score -inf so far: weights 0
-          f[e] = m[n][e] == mx[n][e] ? 1.f : ex2(base[n][e] - to);
+          const float to = mx[n][e] == -INFINITY ? 0.f : mx[n][e];   // every score -inf so far: weights 0
+          f[e] = m[n][e] == mx[n][e] ? 1.f : ex2((base[n][e] - to) * p.scale_log2);
           if (m[n][e] == -INFINITY) f[e] = 0.f;
           m[n][e] = mx[n][e];
           base[n][e] = to;
@@ -486,8 +491,8 @@ __global__ void __launch_bounds__(warps_of(HD) * 32, 1) paged_attention_kernel(c
       for (int n = 0; n < NQ; ++n) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          s[i][n][e] = ex2(fmaf(s[i][n][e], p.scale_log2, -base[n][e]));
-          s[i][n][2 + e] = ex2(fmaf(s[i][n][2 + e], p.scale_log2, -base[n][e]));
+          s[i][n][e] = ex2((s[i][n][e] - base[n][e]) * p.scale_log2);
+          s[i][n][2 + e] = ex2((s[i][n][2 + e] - base[n][e]) * p.scale_log2);
           l[n][e] += s[i][n][e] + s[i][n][2 + e];
         }
         split2<T>(s[i][n][0], s[i][n][1], hi[n][0], lo[n][0]);
@@ -543,8 +548,8 @@ __global__ void __launch_bounds__(warps_of(HD) * 32, 1) paged_attention_kernel(c
               for (int i = 0; i < 2; ++i)
                 if (p.hd == HD || ks * 16 + i * 8 < p.hd) to[ks * 16 + i * 8] = o[ks][n][i * 2 + e] * f;
             if (g == 0) {
-              if (!whole) *reinterpret_cast<float2*>(po + p.rows * p.hd + r * 2) = make_float2(m[n][e] == -INFINITY ? -INFINITY : base[n][e], l[n][e]);
-              else if (p.lse) p.lse[(int64_t)cur.b * p.Hq + head0 + r] = (base[n][e] + log2f(l[n][e])) * kLn2;
+              if (!whole) *reinterpret_cast<float2*>(po + p.rows * p.hd + r * 2) = make_float2(m[n][e], l[n][e]);
+              else if (p.lse) p.lse[(int64_t)cur.b * p.Hq + head0 + r] = log_sum(m[n][e], l[n][e], p.scale_log2);
             }
           }
         }
@@ -617,7 +622,7 @@ __global__ void __launch_bounds__(warps_of(HD) * 32, 1) paged_attention_kernel(c
         const float* part = (k & 1) ? reinterpret_cast<const float*>(smem + (k / 2) * ST * STAGE) : in_ws + (k / 2) * p.part_floats;
         const float2 ml = *reinterpret_cast<const float2*>(part + p.rows * p.hd + 2 * r);
         const float4 v = *reinterpret_cast<const float4*>(part + i * 4);
-        const float to = fmaxf(m, ml.x), base = to == -INFINITY ? 0.f : to, f = ex2(m - base), g = ex2(ml.x - base);
+        const float to = fmaxf(m, ml.x), base = to == -INFINITY ? 0.f : to, f = ex2((m - base) * p.scale_log2), g = ex2((ml.x - base) * p.scale_log2);
         m = to;
         l = fmaf(l, f, g * ml.y);
         acc.x = fmaf(acc.x, f, g * v.x);
@@ -630,7 +635,7 @@ __global__ void __launch_bounds__(warps_of(HD) * 32, 1) paged_attention_kernel(c
         const int64_t at = (int64_t)b * p.Hq + head + r;
         T four[4] = {Cvt<T>::from_f(acc.x * inv), Cvt<T>::from_f(acc.y * inv), Cvt<T>::from_f(acc.z * inv), Cvt<T>::from_f(acc.w * inv)};
         *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + at * p.hd + d) = *reinterpret_cast<const uint2*>(four);
-        if (d == 0 && p.lse) p.lse[at] = ((m == -INFINITY ? 0.f : m) + log2f(l)) * kLn2;
+        if (d == 0 && p.lse) p.lse[at] = log_sum(m, l, p.scale_log2);
       } else {
         *reinterpret_cast<float4*>(po + i * 4) = acc;
         if (d == 0) *reinterpret_cast<float2*>(po + p.rows * p.hd + 2 * r) = make_float2(m, l);
@@ -711,11 +716,11 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedParams p) {
 #pragma unroll
     for (int s = 16; s > 0; s >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, s));
     mx = fmaxf(mx, m);
-    const float base = mx == -INFINITY ? 0.f : mx, w = ex2(ml.x - base);
+    const float base = mx == -INFINITY ? 0.f : mx, w = ex2((ml.x - base) * p.scale_log2);
     float sum = w * ml.y;
 #pragma unroll
     for (int s = 16; s > 0; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
-    const float f = m == -INFINITY ? 0.f : ex2(m - base);
+    const float f = m == -INFINITY ? 0.f : ex2((m - base) * p.scale_log2);
     l = fmaf(l, f, sum);
     m = mx;
     a = scaled(a, f, zero);
@@ -736,12 +741,12 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedParams p) {
 #pragma unroll
     for (int w = 0; w < WPR; ++w) all = fmaxf(all, s_m[w]);
     const float base = all == -INFINITY ? 0.f : all;
-    const float f = ex2(m - base);
+    const float f = ex2((m - base) * p.scale_log2);
     reinterpret_cast<float4*>(s_o[wi])[lane] = scaled(a, f, zero);
     if (p.hd > 128) reinterpret_cast<float4*>(s_o[wi])[lane + 32] = scaled(c, f, zero);
     l = 0.f;
 #pragma unroll
-    for (int w = 0; w < WPR; ++w) l = fmaf(s_l[w], ex2(s_m[w] - base), l);
+    for (int w = 0; w < WPR; ++w) l = fmaf(s_l[w], ex2((s_m[w] - base) * p.scale_log2), l);
     m = all;
     __syncthreads();
     const int d = threadIdx.x;
@@ -760,7 +765,7 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedParams p) {
     if (d0 < p.hd) put(d0, a);
     if (d1 < p.hd) put(d1, c);
   }
-  if (p.lse && wi == 0 && lane == 0) p.lse[rw] = (m + log2f(l)) * kLn2;
+  if (p.lse && wi == 0 && lane == 0) p.lse[rw] = log_sum(m, l, p.scale_log2);
 }
 
 int sm_count(int* out) {

@@ -20,3 +20,55 @@ def test_nan_in_the_first_column_is_the_first_alternative(dtype, N, V, top):
     key = x.float().nan_to_num(nan=INF, posinf=3e38)
     assert torch.equal(r.top_ids.cpu(), torch.sort(key, dim=1, descending=True, stable=True).indices[:, :top])
     assert r.logprobs.isnan().all() and r.entropy.isnan().all() and r.top_logprobs.isnan().all()
+
+
+# ------------------------------------------------------------------------------------------------------------ attention
+def pages_of(k, v, page, seed=0):
+    """k, v [B, n, hkv, hd] -> caches [pages, hkv, page, hd] with the pages in any order, and the table"""
+    B, n, hkv, hd = k.shape
+    W = -(-n // page)
+    g = torch.Generator().manual_seed(seed)
+    ids = torch.randperm(B * W, generator=g).view(B, W)
+    kc, vc = (torch.zeros(B * W, hkv, page, hd, dtype=t.dtype) for t in (k, v))
+    for c, t in ((kc, k), (vc, v)):
+        full = torch.zeros(B, W * page, hkv, hd, dtype=t.dtype)
+        full[:, :n] = t
+        c[ids.flatten()] = full.view(B * W, page, hkv, hd).transpose(1, 2)
+    return kc.cuda(), vc.cuda(), ids.int().cuda()
+
+
+def attend(q, k, v, scale):
+    """One kv head.  -> out, lse and sum of weights times |v|, in 64 bits"""
+    s = torch.einsum("bhd,bnd->bhn", q.double(), k[:, :, 0].double()) * scale
+    p = torch.softmax(s, 2)
+    return torch.einsum("bhn,bnd->bhd", p, v[:, :, 0].double()), torch.logsumexp(s, 2), torch.einsum("bhn,bnd->bhd", p, v[:, :, 0].double().abs())
+
+
+@pytest.mark.parametrize("dtype,top", [(torch.bfloat16, 2.0 ** 20), (torch.bfloat16, 2.0 ** 40), (torch.float16, 2.0 ** 15), (torch.float16, 2.0 ** 10)])
+@pytest.mark.parametrize("heads,hd", [(1, 128), (8, 64), (20, 16), (3, 256)])
+@pytest.mark.parametrize("n", [70, 5000])
+def test_scores_of_any_size(dtype, top, heads, hd, n):
+    """Scores of up to 2^80 * scale: their distances decide, whatever the size.  Two keys share the largest one, all others lie below
+    by at least 2^-10 of it: the answer is the two values' mean (2^-22 of the weights' exponentials, one rounding)."""
+    from hydra_b200.paged import paged_decode_attention
+    scale = hd ** -0.5
+    g = torch.Generator().manual_seed(n + heads)
+    q, k = torch.zeros(2, heads, hd), torch.zeros(2, n, 1, hd)
+    q[:, :, :4] = top
+    k[..., :4] = (top * (0.25 + 0.5 * torch.rand(2, n, 1, 1, generator=g)))
+    k[1] = -k[1]                                                          # and a request of scores far below zero
+    k[0, 3, 0, :4] = k[0, n - 2, 0, :4] = top
+    k[1, 3, 0, :4] = k[1, n - 2, 0, :4] = -top / 8
+    v = torch.randn(2, n, 1, hd, generator=g)
+    q, k, v = q.to(dtype), k.to(dtype), v.to(dtype)
+    kc, vc, table = pages_of(k, v, 16)
+    out, l = (t.double().cpu() for t in paged_decode_attention(q.cuda(), kc, vc, table, torch.full((2,), n, dtype=torch.int32).cuda(), scale=scale,
+                                                               return_lse=True))
+    want, lse, mass = attend(q, k, v, scale)
+    half = torch.finfo(dtype).eps / 2
+    assert ((out - want).abs() <= half * want.abs() + 2.0 ** -16 * mass + 2.0 ** -25).all(), float((out - want).abs().max())
+    assert float(((l - lse).abs() / (1 + lse.abs())).max()) <= 1e-5
+    small = paged_decode_attention(q.cuda(), kc, vc, table, torch.full((2,), n, dtype=torch.int32).cuda(), scale=-scale).double().cpu()
+    want = attend(q, k, v, -scale)[0]
+    if n == 70:                                                           # (one share: the order turned round)
+        assert small.isfinite().all() and float((small - want).abs().max()) <= 2 * half * 8
