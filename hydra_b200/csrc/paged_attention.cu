@@ -89,10 +89,6 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// ln sum e^{scale s} from the largest score and the sum relative to it (0 where every score is -inf).
-__device__ __forceinline__ float log_sum(float m, float l, float scale_log2) {
-  return fmaf(m == -INFINITY ? 0.f : m, scale_log2, log2f(l)) * kLn2;
-}
 template <typename T>
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1);
@@ -109,7 +105,21 @@ __device__ __forceinline__ void mma16816<__half>(float (&d)[4], uint32_t a0, uin
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// Two weights in T and what the rounding left of them, in T again: together they carry 16 (bf16) or 22 (f16) bits.
+// Powers of two that every weight is raised by.  A bf16 holds 2^-126 as well as 1, but both f16 summands end in steps of 2^-24: with the
+// largest weight at 2^15, next to the largest f16, they reach 2^-40 of it instead of 2^-25 (a head that rests on one token
+// whose own values are zero keeps those that lie 20 nats below).  Sums and outputs are raised alike, so only the sum's
+// logarithm has to know.
+template <typename T> struct Raise { static constexpr float kBits = 0.f; };
+template <> struct Raise<__half> { static constexpr float kBits = 15.f; };
+
+// ln sum e^{scale s} from the largest score and the sum relative to it (0 where every score is -inf).
+template <typename T>
+__device__ __forceinline__ float log_sum(float m, float l, float scale_log2) {
+  return fmaf(m == -INFINITY ? 0.f : m, scale_log2, log2f(l) - Raise<T>::kBits) * kLn2;
+}
+
+// Two weights in T and what the rounding left of them, in T again: each is off by at most 2^-17 of itself in bf16, and in f16 by 2^-22
+// of itself or, where that is more, 2^-40 of the largest.
 template <typename T>
 __device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo);
 template <>
@@ -491,8 +501,8 @@ __global__ void __launch_bounds__(warps_of(HD) * 32, 1) paged_attention_kernel(c
       for (int n = 0; n < NQ; ++n) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          s[i][n][e] = ex2((s[i][n][e] - base[n][e]) * p.scale_log2);
-          s[i][n][2 + e] = ex2((s[i][n][2 + e] - base[n][e]) * p.scale_log2);
+          s[i][n][e] = ex2(fmaf(s[i][n][e] - base[n][e], p.scale_log2, Raise<T>::kBits));
+          s[i][n][2 + e] = ex2(fmaf(s[i][n][2 + e] - base[n][e], p.scale_log2, Raise<T>::kBits));
           l[n][e] += s[i][n][e] + s[i][n][2 + e];
         }
         split2<T>(s[i][n][0], s[i][n][1], hi[n][0], lo[n][0]);
@@ -549,7 +559,7 @@ __global__ void __launch_bounds__(warps_of(HD) * 32, 1) paged_attention_kernel(c
                 if (p.hd == HD || ks * 16 + i * 8 < p.hd) to[ks * 16 + i * 8] = o[ks][n][i * 2 + e] * f;
             if (g == 0) {
               if (!whole) *reinterpret_cast<float2*>(po + p.rows * p.hd + r * 2) = make_float2(m[n][e], l[n][e]);
-              else if (p.lse) p.lse[(int64_t)cur.b * p.Hq + head0 + r] = log_sum(m[n][e], l[n][e], p.scale_log2);
+              else if (p.lse) p.lse[(int64_t)cur.b * p.Hq + head0 + r] = log_sum<T>(m[n][e], l[n][e], p.scale_log2);
             }
           }
         }
@@ -635,7 +645,7 @@ __global__ void __launch_bounds__(warps_of(HD) * 32, 1) paged_attention_kernel(c
         const int64_t at = (int64_t)b * p.Hq + head + r;
         T four[4] = {Cvt<T>::from_f(acc.x * inv), Cvt<T>::from_f(acc.y * inv), Cvt<T>::from_f(acc.z * inv), Cvt<T>::from_f(acc.w * inv)};
         *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + at * p.hd + d) = *reinterpret_cast<const uint2*>(four);
-        if (d == 0 && p.lse) p.lse[at] = log_sum(m, l, p.scale_log2);
+        if (d == 0 && p.lse) p.lse[at] = log_sum<T>(m, l, p.scale_log2);
       } else {
         *reinterpret_cast<float4*>(po + i * 4) = acc;
         if (d == 0) *reinterpret_cast<float2*>(po + p.rows * p.hd + 2 * r) = make_float2(m, l);
@@ -765,7 +775,7 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedParams p) {
     if (d0 < p.hd) put(d0, a);
     if (d1 < p.hd) put(d1, c);
   }
-  if (p.lse && wi == 0 && lane == 0) p.lse[rw] = log_sum(m, l, p.scale_log2);
+  if (p.lse && wi == 0 && lane == 0) p.lse[rw] = log_sum<T>(m, l, p.scale_log2);
 }
 
 int sm_count(int* out) {

@@ -72,3 +72,33 @@ def test_scores_of_any_size(dtype, top, heads, hd, n):
     want = attend(q, k, v, -scale)[0]
     if n == 70:                                                           # (one share: the order turned round)
         assert small.isfinite().all() and float((small - want).abs().max()) <= 2 * half * 8
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("heads", [1, 8, 20])
+@pytest.mark.parametrize("B,n,at", [(64, 4096, 0), (64, 4096, 4095), (200, 1000, 500), (1, 4096, 0), (1, 60000, 7), (3, 20000, 19999)])
+def test_a_token_that_takes_nearly_all_and_gives_nothing(dtype, heads, B, n, at):
+    """One key 10 to 20 nats above thousands of equal others, its value row zero: the output is what the others leave.
+
+    Per value: half a step of the type (2^-25 in f16 below its normal range) for the rounding; the weights as two summands: f16
+    ones are held up to 2^15 in steps of 2^-24, so each is off by at most 2^-40 of the largest, or 2^-17 of itself (bf16; f16:
+    2^-22); exponentials 2^-22 and 2^-24 times an exponent of at most 2^6 (log2(e) 20 + 15) twice: 2^-17; the sums of n / 16
+    products 2^-24 each, at most twice (numerator and denominator): n 2^-27."""
+    from hydra_b200.paged import paged_decode_attention
+    hd, scale = 64, 0.125
+    g = torch.Generator().manual_seed(n)
+    q = torch.zeros(B, heads, hd)
+    q[:, :, 0] = 10.0 + (torch.arange(heads) % 9) * 1.25                  # scores: 8 q scale = 10 .. 20
+    k = torch.randn(B, n, 1, hd, generator=g)
+    k[..., 0] = 0.0
+    v = (0.5 + torch.rand(B, n, 1, hd, generator=g)) * 8
+    k[:, at, :, 0], v[:, at] = 8.0, 0.0
+    q, k, v = q.to(dtype), k.to(dtype), v.to(dtype)
+    want, lse, mass = attend(q, k, v, scale)
+    kc, vc, table = pages_of(k, v, 16)
+    out, l = paged_decode_attention(q.cuda(), kc, vc, table, torch.full((B,), n, dtype=torch.int32).cuda(), scale=scale, return_lse=True)
+    half = torch.finfo(dtype).eps / 2
+    off = (out.double().cpu() - want).abs()
+    tol = half * want.abs() + (2.0 ** -25 if dtype == torch.float16 else 0.0) + n * 2.0 ** -40 * 12 + (2.0 ** -16 + n * 2.0 ** -27) * mass
+    assert (off <= tol).all(), f"off by {float((off / tol).max()):.2f} tolerances, {float((off / want).max()):.2e} of the value"
+    assert float(((l.double().cpu() - lse).abs() / (1 + lse.abs())).max()) <= 1e-5
