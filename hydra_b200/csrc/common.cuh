@@ -9,6 +9,7 @@
 
 #include <cstdarg>
 #include <cstdio>
+#include <initializer_list>
 
 #include "../../include/hydra_b200.h"
 
@@ -100,6 +101,24 @@ inline int launch_chained(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t 
 // Raises a kernel's dynamic shared memory limit to at least `bytes` on the current device (the attribute is a
 // per-device property of the kernel; the sizes already set are remembered per (kernel, device)).  Defined in api.cu.
 int ensure_dynamic_smem(const void* kernel, size_t bytes);
+
+// The bytes [lo, hi) that rows of `row_bytes` reach over, laid out along axes of `n` entries `step` bytes apart; none where there is
+// no row.
+struct Axis {
+  int64_t n, step;
+};
+struct Reach {
+  int64_t lo, hi;
+};
+inline Reach reach_of(const void* p, int64_t row_bytes, std::initializer_list<Axis> axes = {}) {
+  Reach r = {(int64_t)reinterpret_cast<uintptr_t>(p), (int64_t)reinterpret_cast<uintptr_t>(p) + row_bytes};
+  for (const Axis& a : axes) {
+    if (a.n < 1) return {0, 0};
+    (a.step < 0 ? r.lo : r.hi) += (a.n - 1) * a.step;
+  }
+  return r;
+}
+inline bool overlap(const Reach& a, const Reach& b) { return a.lo < a.hi && b.lo < b.hi && a.lo < b.hi && b.lo < a.hi; }
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 inline int ceil_div(int a, int b) { return (a + b - 1) / b; }

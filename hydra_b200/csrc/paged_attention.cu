@@ -874,6 +874,16 @@ extern "C" int hb200_paged_decode_attention(const hb200_paged_cache* c, const vo
              "paged_decode_attention: tables of %d pages of %d tokens for %d requests reach too far", table_width, c->page_size, B);
   HB_REQUIRE((cap / 16 + 4) * Hq <= 0x7fffffff, HB200_ERR_UNSUPPORTED,
              "paged_decode_attention: tables of %d pages of %d tokens for %d query heads reach too far", table_width, c->page_size, Hq);
+  // Warps store what they have finished while others still read.
+  const Reach k_reach = reach_of(c->k, c->head_dim * 2, {{c->num_pages, c->k_stride_page * 2}, {c->n_kv_heads, c->k_stride_head * 2}, {c->page_size, c->k_stride_row * 2}});
+  const Reach v_reach = reach_of(c->v, c->head_dim * 2, {{c->num_pages, c->v_stride_page * 2}, {c->n_kv_heads, c->v_stride_head * 2}, {c->page_size, c->v_stride_row * 2}});
+  const Reach read[] = {reach_of(q, c->head_dim * 2, {{B, q_stride_b * 2}, {Hq, q_stride_h * 2}}), k_reach, v_reach,
+                        reach_of(block_tables, (int64_t)table_width * 4, {{B, table_ld * 4}}), reach_of(kv_lens, (int64_t)B * 4)};
+  const Reach written[] = {reach_of(out, (int64_t)B * Hq * c->head_dim * 2), reach_of(lse, lse ? (int64_t)B * Hq * 4 : 0)};
+  for (const Reach& w : written)
+    for (const Reach& r : read)
+      HB_REQUIRE(!overlap(w, r), HB200_ERR_INVALID, "paged_decode_attention: out and lse must not overlap what is read");
+  HB_REQUIRE(!overlap(written[0], written[1]), HB200_ERR_INVALID, "paged_decode_attention: out and lse must not overlap one another");
   const int group = Hq / c->n_kv_heads;
   int sms = 0;
   HB_PROPAGATE(sm_count(&sms));

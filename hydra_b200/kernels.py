@@ -215,6 +215,15 @@ def fused_rms_norm(x: Tensor, weight: Tensor, eps: float = 1e-6) -> Tensor:
     return _rms_norm_op(x, weight, float(eps))
 
 
+def _overlap(a: Tensor, b: Tensor) -> bool:
+    """Whether the memory that one tensor reaches over, from its first byte to its last, meets the other's."""
+    def reach(t):
+        lo = t.data_ptr()
+        return lo, lo + (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))) * t.element_size() if t.numel() else lo
+    (a0, a1), (b0, b1) = reach(a), reach(b)
+    return a0 < b1 and b0 < a1 and a0 < a1 and b0 < b1
+
+
 def _refuse_autograd(what: str, *ts: Optional[Tensor]) -> None:
     if torch.is_grad_enabled():
         for t in ts:

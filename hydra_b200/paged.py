@@ -149,7 +149,8 @@ def paged_decode_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_ta
     ``h // (Hq // Hkv)``), softmax of ``scale * q . k`` (default ``hd ** -0.5``).
 
     q [B, Hq, hd] bf16 or f16 (up to 4096 requests, 1024 heads; hd a multiple of 8 up to 256), caches as in
-    :func:`paged_append`, ``block_tables`` int32 [B, width], ``kv_lens`` int32 [B].  Returns [B, Hq, hd] (in ``out`` if given, which overlaps no input)
+    :func:`paged_append`, ``block_tables`` int32 [B, width], ``kv_lens`` int32 [B].  Returns [B, Hq, hd] (in ``out`` if given, which must not lie within
+    the memory that an input reaches over)
     and, if asked, the fp32 logarithm of each softmax's sum [B, Hq].  A request of length 0 gives zeros and -inf; one whose
     table names a page outside the cache, or whose length passes its table, gives NaN.  What lies behind a
     request's length in its last page is not looked at; an infinite value among the attended ones gives NaN or infinity in
@@ -182,8 +183,9 @@ def paged_decode_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_ta
     if out is not None:
         if out.shape != q.shape or out.dtype != dtype or out.device != dev or not out.is_contiguous() or out.data_ptr() % 16:
             raise ValueError("paged_decode_attention: out must be a contiguous, 16-byte aligned tensor of q's shape and dtype")
-        if B > 0 and out.data_ptr() < q.data_ptr() + 2 * ((B - 1) * sb + (Hq - 1) * sh + hd) and q.data_ptr() < out.data_ptr() + 2 * B * Hq * hd:
-            raise ValueError("paged_decode_attention: out must not overlap q, which several blocks read")
+        for name, t in (("q", q), ("k_cache", k_cache), ("v_cache", v_cache), ("block_tables", block_tables), ("kv_lens", kv_lens)):
+            if kernels._overlap(out, t):
+                raise ValueError(f"paged_decode_attention: out must not overlap {name}, which is read while results are stored")
     with kernels._on(dev):
         new = kernels._empty_strided
         if out is None:

@@ -459,8 +459,9 @@ typedef struct hb200_qk_norm_rope_args {
  * the tables, or a slot beyond the cache, gives NaN (nothing is written out of range).  head_dim up to 256. */
 int hb200_qk_norm_rope(const hb200_qk_norm_rope_args* args, const hb200_paged_cache* cache, void* stream);
 
-/* Attention of one new token per request over the paged cache: q [B, Hq, hd] by strides, out [B, Hq, hd] contiguous (apart from q) in
- * the cache's dtype (bf16 or f16), lse fp32 [B, Hq] (ln of the sum of exponentials) or NULL.  block_tables int32 [B,
+/* Attention of one new token per request over the paged cache: q [B, Hq, hd] by strides, out [B, Hq, hd] contiguous in the
+ * cache's dtype (bf16 or f16), lse fp32 [B, Hq] (ln of the sum of exponentials) or NULL; neither may lie within the reach of an
+ * input (from its first byte to its last) or of the other.  block_tables int32 [B,
  * table_width], kv_lens int32 [B]: request b attends to its first kv_lens[b] tokens.  An empty request gives zeros and -inf;
  * one whose table names a page outside the cache, or whose length passes its table, gives NaN.  head_dim a multiple of 8 up
  * to 256; Hq a multiple of the kv heads; up to 4096 requests.  Strides are multiples of 8 elements, pointers 16-byte

@@ -102,3 +102,19 @@ def test_a_token_that_takes_nearly_all_and_gives_nothing(dtype, heads, B, n, at)
     tol = half * want.abs() + (2.0 ** -25 if dtype == torch.float16 else 0.0) + n * 2.0 ** -40 * 12 + (2.0 ** -16 + n * 2.0 ** -27) * mass
     assert (off <= tol).all(), f"off by {float((off / tol).max()):.2f} tolerances, {float((off / want).max()):.2e} of the value"
     assert float(((l.double().cpu() - lse).abs() / (1 + lse.abs())).max()) <= 1e-5
+
+
+def test_out_within_what_is_read_is_refused():
+    from hydra_b200.paged import paged_decode_attention
+    arena = torch.zeros(3, 4, 2, 16, 64, dtype=torch.float16, device="cuda")
+    kc, vc, spare = arena.unbind(0)
+    q = torch.randn(2, 8, 64, device="cuda").half()
+    ints = torch.zeros(4096, dtype=torch.int32, device="cuda")
+    table, n = ints[:4].view(2, 2), ints[4:6].fill_(20)
+    as_out = lambda t: t.view(torch.float16).flatten()[:q.numel()].view(q.shape)   # noqa: E731
+    for name, out in (("k_cache", as_out(kc)), ("v_cache", as_out(vc[2])), ("block_tables", as_out(ints)), ("kv_lens", as_out(ints[4:]))):
+        with pytest.raises(ValueError, match=f"overlap {name}"):
+            paged_decode_attention(q, kc, vc, table, n, out=out)
+    assert (arena == 0).all() and (ints[:4] == 0).all()
+    want = paged_decode_attention(q, kc, vc, table, n)
+    assert torch.equal(paged_decode_attention(q, kc, vc, table, n, out=as_out(spare)), want)
