@@ -118,6 +118,24 @@ inline Reach reach_of(const void* p, int64_t row_bytes, std::initializer_list<Ax
   }
   return r;
 }
+// Whether all rows lie apart, shown by nesting: along each axis, from the smallest step on, an entry ends before the next begins.
+inline bool rows_apart(int64_t row_bytes, std::initializer_list<Axis> axes) {
+  Axis by_step[4];
+  int n = 0;
+  for (const Axis& a : axes) {
+    if (a.n < 2) continue;
+    Axis x = {a.n, a.step < 0 ? -a.step : a.step};
+    int i = n++;
+    for (; i > 0 && by_step[i - 1].step > x.step; --i) by_step[i] = by_step[i - 1];
+    by_step[i] = x;
+  }
+  int64_t entry = row_bytes;
+  for (int i = 0; i < n; ++i) {
+    if (by_step[i].step < entry) return false;
+    entry += (by_step[i].n - 1) * by_step[i].step;
+  }
+  return true;
+}
 inline bool overlap(const Reach& a, const Reach& b) { return a.lo < a.hi && b.lo < b.hi && a.lo < b.hi && b.lo < a.hi; }
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }

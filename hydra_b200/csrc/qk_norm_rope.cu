@@ -437,10 +437,32 @@ extern "C" int hb200_qk_norm_rope(const hb200_qk_norm_rope_args* a, const hb200_
     HB_REQUIRE(a->slots && a->v && c->k && c->v, HB200_ERR_INVALID, "qk_norm_rope: null pointer (cache, slots or v)");
     HB_REQUIRE(c->n_kv_heads == a->Hkv && c->head_dim == a->hd && c->dtype == a->dtype && c->num_pages >= 0 && c->page_size >= 1,
                HB200_ERR_INVALID, "qk_norm_rope: the cache's heads or dtype are not those of k");
-    const int64_t apart[][2] = {{c->num_pages, c->k_stride_page}, {c->n_kv_heads, c->k_stride_head}, {c->page_size, c->k_stride_row},
-                                {c->num_pages, c->v_stride_page}, {c->n_kv_heads, c->v_stride_head}, {c->page_size, c->v_stride_row}};
-    for (const auto& d : apart)
-      HB_REQUIRE(d[0] <= 1 || d[1] != 0, HB200_ERR_INVALID, "qk_norm_rope: the cache's rows lie on top of one another");
+    // Rows that share bytes, with one another or with what is read, would hold what came last.  (Keys and values may lie between
+    // one another, by the same strides.)
+    const int64_t size = (int64_t)es, row = a->hd * size;
+    const Axis kp = {c->num_pages, c->k_stride_page * size}, kh = {c->n_kv_heads, c->k_stride_head * size}, kr = {c->page_size, c->k_stride_row * size};
+    const Axis vp = {c->num_pages, c->v_stride_page * size}, vh = {c->n_kv_heads, c->v_stride_head * size}, vr = {c->page_size, c->v_stride_row * size};
+    const Reach stored[] = {reach_of(c->k, row, {kp, kh, kr}), reach_of(c->v, row, {vp, vh, vr})};
+    HB_REQUIRE(rows_apart(row, {kp, kh, kr}) && rows_apart(row, {vp, vh, vr}), HB200_ERR_INVALID,
+               "qk_norm_rope: the cache's rows lie on top of one another");
+    auto same = [](const Axis& x, const Axis& y) { return x.n < 2 || x.step == y.step; };
+    const int64_t from_k_to_v = (int64_t)reinterpret_cast<uintptr_t>(c->v) - (int64_t)reinterpret_cast<uintptr_t>(c->k);
+    HB_REQUIRE(!overlap(stored[0], stored[1]) ||
+                   (same(kp, vp) && same(kh, vh) && same(kr, vr) && rows_apart(row, {kp, kh, kr, {2, from_k_to_v}})),
+               HB200_ERR_INVALID, "qk_norm_rope: the caches of keys and values lie on top of one another");
+    auto heads = [&](const void* ptr, const int64_t (&s)[3], int n) {
+      return reach_of(ptr, row, {{a->B, s[0] * size}, {a->S, s[1] * size}, {n, s[2] * size}});
+    };
+    const int64_t angles = a->rot / 2 * 4;
+    const Reach others[] = {heads(a->q, a->q_stride, a->Hq), heads(a->k, a->k_stride, a->Hkv), heads(a->v, a->v_stride, a->Hkv),
+                            heads(a->q_out, a->q_out_stride, a->Hq), reach_of(a->slots, tokens * 8),
+                            reach_of(a->positions, a->positions ? (int64_t)a->S * (a->positions_64 ? 8 : 4) : 0,
+                                     {{a->B, a->positions_stride * (a->positions_64 ? 8 : 4)}}),
+                            reach_of(a->cos, angles, {{a->table_rows, a->table_ld * 4}}), reach_of(a->sin, angles, {{a->table_rows, a->table_ld * 4}}),
+                            reach_of(a->q_weight, a->q_weight ? a->hd * 4 : 0), reach_of(a->k_weight, a->k_weight ? a->hd * 4 : 0)};
+    for (const Reach& w : stored)
+      for (const Reach& r : others)
+        HB_REQUIRE(!overlap(w, r), HB200_ERR_INVALID, "qk_norm_rope: the caches overlap the queries, keys, values or tables that are read");
     p.v = a->v; p.kc = c->k; p.vc = c->v; p.slots = a->slots;
     p.page_size = c->page_size;
     p.capacity = (int64_t)c->num_pages * c->page_size;

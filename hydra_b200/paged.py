@@ -115,7 +115,8 @@ def paged_append(q: Tensor, k: Tensor, v: Tensor, k_cache: Tensor, v_cache: Tens
 
     q [T, Hq, hd], k and v [T, Hkv, hd] (views of one projection are read in place), ``slots`` int64 and ``positions`` int32 or
     int64 [T] as :func:`paged_plan` writes them, caches [num_pages, Hkv, page_size, hd] in q's dtype by any strides with
-    contiguous rows that do not overlap (token-major pages: pass ``cache.transpose(1, 2)``).  Returns the normed and rotated queries
+    contiguous rows (token-major pages: pass ``cache.transpose(1, 2)``) that do not overlap: not one another, k's not v's (they may
+    lie side by side in one tensor), and neither any other argument (which is refused).  Returns the normed and rotated queries
     [T, Hq, hd]; cache rows without a slot here stay as they are.  A row with a negative position is padding (zeros
     returned, nothing stored), one with a negative slot is computed but not stored; a position beyond the tables or a slot
     beyond the cache gives NaN.  Of two rows with the same slot either's values may stay, or some of each's."""

@@ -455,7 +455,7 @@ typedef struct hb200_qk_norm_rope_args {
 
 /* Per-head norm (times weight and scale) of q and k and rotation of the first `rot` values of each head, in one pass: 32 bits
  * inside, rounded once.  With `cache`, k and v rows go to their slots instead of k_out (v unchanged; other slots are left as
- * they are).  A row with a negative position is padding: zeros in q_out / k_out, nothing into the cache.  A position beyond
+ * they are); the cache's rows lie apart from one another and from everything else.  A row with a negative position is padding: zeros in q_out / k_out, nothing into the cache.  A position beyond
  * the tables, or a slot beyond the cache, gives NaN (nothing is written out of range).  head_dim up to 256. */
 int hb200_qk_norm_rope(const hb200_qk_norm_rope_args* args, const hb200_paged_cache* cache, void* stream);
 

@@ -6,9 +6,14 @@ import pytest
 import torch
 
 from hydra_b200 import _lib
-from tests.test_cpu_serving_ops import _cache, _last
+from tests.test_cpu_serving_ops import _cache as _cache_struct, _last
 
-M = 1 << 32   # addresses far from one another that no call below gets far enough to use
+M = 1 << 32   # addresses far from one another that no call below gets far enough to use: its type is none that is built, which is
+NONE = 7      # what a call that passes all checks is refused for, with or without a GPU
+
+
+def _cache(**kw):
+    return _cache_struct(**{"dtype": NONE, **kw})
 
 
 # ------------------------------------------------------------------------------------------------------ memory: C entries
@@ -26,6 +31,59 @@ def _attention(out=6 * M, lse=7 * M, q=M, table=4 * M, lens=5 * M, cache=None):
 ])
 def test_attention_refuses_results_among_its_inputs(bad):
     assert _attention(**bad) == -1 and "overlap" in _last()
+
+
+# 4 tokens of 8 query and 4 key heads of 64 into the same cache
+def _append(cache, **kw):
+    s = {f"{t}_stride_{d}": n for t in ("q", "k", "v", "q_out", "k_out") for d, n in (("batch", 0), ("token", 512), ("head", 64))}
+    d = dict(q=10 * M, k=11 * M, v=12 * M, q_out=13 * M, k_out=None, slots=14 * M, positions=15 * M, cos=16 * M, sin=17 * M, q_weight=18 * M,
+             k_weight=19 * M, **s, table_rows=128, table_ld=32, B=1, S=4, Hq=8, Hkv=4, hd=64, rot=64, layout=1, norm=1,
+             dtype=NONE, eps=1e-6, q_scale=1.0, k_scale=1.0)
+    a = _lib.QkNormRopeArgs(**{**d, **kw})
+    return _lib.lib().hb200_qk_norm_rope(C.byref(a), C.byref(cache), None)
+
+
+K = dict(k=2 * M, v=3 * M)
+
+
+@pytest.mark.parametrize("cache", [
+    dict(K, k_stride_row=32), dict(K, v_stride_head=960), dict(K, k_stride_page=4032), dict(K, k_stride_row=64, k_stride_head=64),
+    dict(K, v_stride_row=-63), dict(K, k_stride_page=64, k_stride_row=512 - 8),
+    dict(k=2 * M, v=2 * M), dict(k=2 * M, v=2 * M + 64), dict(k=2 * M, v=2 * M + 8192 * 7), dict(k=2 * M, v=2 * M - 4096),
+    dict(k=2 * M, v=2 * M + 128, v_stride_row=256, v_stride_head=64, v_stride_page=4096),
+])
+def test_append_refuses_caches_on_top_of_themselves_or_one_another(cache):
+    assert _append(_cache(**cache)) == -1 and "on top" in _last()
+
+
+@pytest.mark.parametrize("bad", [
+    dict(q=2 * M + 65536 - 128), dict(q=2 * M - 4096 + 2), dict(k=3 * M), dict(v=2 * M + 640), dict(q_out=3 * M - 2048), dict(slots=2 * M - 24),
+    dict(positions=3 * M + 65532), dict(cos=2 * M - 128 * 32 * 4 + 4), dict(sin=3 * M), dict(q_weight=2 * M + 256), dict(k_weight=3 * M - 252),
+])
+def test_append_refuses_inputs_in_the_cache(bad):
+    assert _append(_cache(**K), **bad) == -1 and "overlap" in _last()
+
+
+def _layouts():
+    """Ways to keep keys and values side by side: [2, pages, ...], [pages, 2, ...], heads or values of a row in turn, token-major."""
+    for shape, at in (((2, 8, 4, 16, 64), 0), ((8, 2, 4, 16, 64), 1), ((8, 4, 2, 16, 64), 2), ((8, 4, 16, 2, 64), 3)):
+        yield torch.empty(shape, dtype=torch.bfloat16).unbind(at)
+    yield torch.empty(8, 2, 16, 4, 64, dtype=torch.bfloat16).transpose(2, 3).unbind(1)
+    pool = torch.empty(16, 4, 16, 64, dtype=torch.bfloat16)
+    yield pool[:8], pool[8:]
+    yield pool[::2], pool[1::2]
+    yield pool[1::2], pool[::2]
+    yield torch.empty(8, 3, 2, 4, 16, 64, dtype=torch.bfloat16)[:, 1].unbind(1)      # one of three layers
+
+
+def test_caches_side_by_side_are_taken():
+    """Layouts whose rows lie apart byte by byte pass all checks; the same tensor for both does not."""
+    for k, v in _layouts():
+        for a, b, good in ((k, v, True), (k, k, False)):
+            strides = {f"{n}_stride_{d}": s for n, t in (("k", a), ("v", b)) for d, s in zip(("page", "head", "row"), t.stride())}
+            at = min(a.data_ptr(), b.data_ptr())
+            status = _append(_cache(k=2 * M + a.data_ptr() - at, v=2 * M + b.data_ptr() - at, **strides))
+            assert (status, "dtype" in _last()) == (-4, True) if good else (status, "on top" in _last()) == (-1, True), (k.stride(), _last())
 
 
 # -------------------------------------------------------------------------------------------------- memory: Python entries

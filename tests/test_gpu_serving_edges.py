@@ -118,3 +118,26 @@ def test_out_within_what_is_read_is_refused():
     assert (arena == 0).all() and (ints[:4] == 0).all()
     want = paged_decode_attention(q, kc, vc, table, n)
     assert torch.equal(paged_decode_attention(q, kc, vc, table, n, out=as_out(spare)), want)
+
+
+@pytest.mark.parametrize("at", [0, 1, 2, 3])
+def test_keys_and_values_in_one_tensor(at):
+    """Caches that lie between one another are filled like any others; one tensor for both, or rows that overlap, are refused."""
+    from hydra_b200.paged import paged_append
+    sizes = [6, 2, 8, 16]
+    room = torch.zeros(*sizes[:at], 2, *sizes[at:], device="cuda")
+    kc, vc = room.unbind(at)
+    apart = torch.zeros(6, 2, 8, 16, device="cuda"), torch.zeros(6, 2, 8, 16, device="cuda")
+    cos, sin = torch.ones(32, 8, device="cuda"), torch.zeros(32, 8, device="cuda")
+    x, y, z = torch.randn(3, 5, 2, 16, device="cuda")
+    slots, pos = torch.tensor([3, 47, 0, 16, 9]).cuda(), torch.arange(5).cuda()
+    q = paged_append(x, y, z, kc, vc, slots, cos, sin, pos)
+    assert torch.equal(q, paged_append(x, y, z, *apart, slots, cos, sin, pos)) and torch.equal(kc, apart[0]) and torch.equal(vc, apart[1])
+    before = room.clone()
+    for k, v in ((kc, kc), (kc, kc.as_strided(kc.shape, kc.stride())), (kc[:1].expand(6, -1, -1, -1), vc),
+                 (apart[0].as_strided((6, 2, 8, 16), (256, 128, 8, 1)), vc)):
+        with pytest.raises(RuntimeError, match="on top"):
+            paged_append(x, y, z, k, v, slots, cos, sin, pos)
+    with pytest.raises(RuntimeError, match="overlap"):
+        paged_append(kc[:5, :, 0], y, z, kc, vc, slots, cos, sin, pos)
+    assert torch.equal(room, before)
