@@ -187,6 +187,17 @@ extern "C" int hb200_paged_plan(const int32_t* context_lens, const int32_t* new_
                  (B == 0 || table_width == 0 || block_tables) && (n_free == 0 || free_pages) && (max_new == 0 || (positions && slots)),
              HB200_ERR_INVALID, "paged_plan: null pointer");
   HB_REQUIRE(aligned16(positions) && aligned16(slots), HB200_ERR_INVALID, "paged_plan: positions and slots must be 16-byte aligned");
+  // Every CTA reads all lengths while others store.
+  const int64_t each = (int64_t)B * 4;
+  const Reach read[] = {reach_of(context_lens, each), reach_of(new_lens, each), reach_of(free_pages, n_free * 4), reach_of(free_start, free_start ? 4 : 0)};
+  const Reach written[] = {reach_of(block_tables, (int64_t)table_width * 4, {{B, table_ld * 4}}), reach_of(kv_lens, each), reach_of(cu_new, each + 4),
+                           reach_of(positions, (int64_t)max_new * 4), reach_of(slots, (int64_t)max_new * 8), reach_of(free_start_out, 4), reach_of(status, 4)};
+  for (const Reach& w : written) {
+    for (const Reach& r : read)
+      HB_REQUIRE(!overlap(w, r), HB200_ERR_INVALID, "paged_plan: block_tables and the results must not overlap the lengths or the free list");
+    for (const Reach* other = written; other != &w; ++other)
+      HB_REQUIRE(!overlap(w, *other), HB200_ERR_INVALID, "paged_plan: block_tables and the results must not overlap one another");
+  }
   PlanParams p = {};
   p.context = context_lens; p.fresh = new_lens; p.free_pages = free_pages; p.free_start = free_start;
   p.table = block_tables; p.kv_lens = kv_lens; p.cu = cu_new; p.positions = positions; p.start_out = free_start_out;

@@ -54,7 +54,8 @@ def paged_plan(context_lens: Tensor, new_lens: Tensor, block_tables: Tensor, fre
     ``context_lens`` and ``new_lens`` int32 [B] (up to 4096 requests): tokens that request b has in the cache and tokens that it
     adds.  ``block_tables`` int32 [B, width]: its pages; the entries that it needs beyond ``ceil(context / page_size)`` are
     taken from ``free_pages`` int32 [F], request after request, from ``free_start`` int32 [1] on (default 0), and written in
-    place.  The other inputs are left as they are, so repeating a call repeats its result.  ``max_new_tokens``: rows of
+    place.  The other inputs are left as they are, so repeating a call repeats its result; none of them may lie between the
+    tables' first and last entry.  ``max_new_tokens``: rows of
     ``slots`` and ``positions`` (the new tokens of all requests, packed; a fixed number serves a captured graph).
 
     Where pages, table columns or rows run out the entries concerned are -1 and ``status`` says so (one int32 on the device:

@@ -86,6 +86,22 @@ def test_caches_side_by_side_are_taken():
             assert (status, "dtype" in _last()) == (-4, True) if good else (status, "on top" in _last()) == (-1, True), (k.stride(), _last())
 
 
+# two requests, tables of 4 in rows of 8, 8 free pages, 8 rows.
+def _plan(**kw):
+    a = dict(context=M, new=2 * M, table=3 * M, free=4 * M, start=5 * M, lens=6 * M, cu=7 * M, pos=8 * M, slots=9 * M, out=10 * M, status=11 * M)
+    a.update(kw)
+    return _lib.lib().hb200_paged_plan(a["context"], a["new"], 2, a["table"], 8, 4, 16, a["free"], 8, a["start"], a["lens"], a["cu"], a["pos"],
+                                       a["slots"], 8, a["out"], a["status"], None)
+
+
+@pytest.mark.parametrize("bad", [
+    dict(context=3 * M + 44), dict(new=3 * M - 4), dict(free=3 * M + 16), dict(start=3 * M), dict(lens=M + 4), dict(cu=2 * M - 8), dict(pos=4 * M + 16),
+    dict(slots=4 * M - 48), dict(out=5 * M), dict(status=M), dict(lens=3 * M + 40), dict(pos=9 * M + 48), dict(out=11 * M), dict(cu=6 * M + 4),
+])
+def test_plan_refuses_results_among_its_inputs(bad):
+    assert _plan(**bad) == -1 and "overlap" in _last()
+
+
 # -------------------------------------------------------------------------------------------------- memory: Python entries
 def test_reach_of_strided_tensors():
     from hydra_b200.kernels import _overlap

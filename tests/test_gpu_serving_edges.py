@@ -141,3 +141,14 @@ def test_keys_and_values_in_one_tensor(at):
     with pytest.raises(RuntimeError, match="overlap"):
         paged_append(kc[:5, :, 0], y, z, kc, vc, slots, cos, sin, pos)
     assert torch.equal(room, before)
+
+
+def test_plan_with_a_free_list_in_its_tables_is_refused():
+    from hydra_b200.paged import paged_plan
+    room = torch.arange(40, dtype=torch.int32, device="cuda")
+    n = torch.zeros(2, dtype=torch.int32, device="cuda")
+    with pytest.raises(RuntimeError, match="overlap"):
+        paged_plan(n, n + 5, room[:8].view(2, 4), room[6:20], 16, 16)
+    assert torch.equal(room, torch.arange(40, device="cuda").int())
+    plan = paged_plan(n, n + 5, room[:8].view(2, 4), room[8:20], 16, 16)
+    assert room[:8].tolist() == [8, 1, 2, 3, 9, 5, 6, 7] and int(plan.status) == 0
