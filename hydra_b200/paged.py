@@ -20,6 +20,8 @@ from typing import NamedTuple, Optional, Tuple, Union
 
 import torch
 
+from torch.autograd.graph import increment_version
+
 from . import _lib, kernels
 
 Tensor = torch.Tensor
@@ -89,6 +91,7 @@ def paged_plan(context_lens: Tensor, new_lens: Tensor, block_tables: Tensor, fre
             page_size, free_pages.data_ptr(), free_pages.shape[0], free_start.data_ptr() if free_start is not None else None,
             kv_lens.data_ptr(), cu_new.data_ptr(), positions.data_ptr(), slots.data_ptr(), room, start_out.data_ptr(),
             status.data_ptr(), kernels._stream(dev)), "paged_plan")
+    increment_version(block_tables)   # (written behind torch's back: a graph that kept the old entries has to know)
     return plan
 
 
@@ -137,6 +140,7 @@ def paged_append(q: Tensor, k: Tensor, v: Tensor, k_cache: Tensor, v_cache: Tens
         raise RuntimeError("paged_append: the caches are written in place and cannot require grad")
     q_out, _ = kernels._qk_norm_rope("paged_append", dev, q, k, cos, sin, positions, q_weight, k_weight, norm, eps, q_scale, k_scale,
                                      layout, v=v, slots=slots, cache=cache)
+    increment_version((k_cache, v_cache))
     return q_out
 
 
@@ -182,7 +186,8 @@ def paged_decode_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_ta
         q = q.contiguous()
         q = q.clone() if q.data_ptr() % 16 else q
         sb, sh, _ = q.stride()
-    if out is not None:
+    given = out is not None
+    if given:
         if out.shape != q.shape or out.dtype != dtype or out.device != dev or not out.is_contiguous() or out.data_ptr() % 16:
             raise ValueError("paged_decode_attention: out must be a contiguous, 16-byte aligned tensor of q's shape and dtype")
         for name, t in (("q", q), ("k_cache", k_cache), ("v_cache", v_cache), ("block_tables", block_tables), ("kv_lens", kv_lens)):
@@ -204,6 +209,8 @@ def paged_decode_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_ta
                 cache, q.data_ptr(), sb, sh, out.data_ptr(), lse.data_ptr() if return_lse else None,
                 block_tables.data_ptr(), width, width, kv_lens.data_ptr(), B, Hq, scale,
                 ws.data_ptr(), n, kernels._stream(dev)), "paged_decode_attention")
+    if given:
+        increment_version(out)
     return (out, lse) if return_lse else out
 
 

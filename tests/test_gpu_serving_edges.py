@@ -152,3 +152,37 @@ def test_plan_with_a_free_list_in_its_tables_is_refused():
     assert torch.equal(room, torch.arange(40, device="cuda").int())
     plan = paged_plan(n, n + 5, room[:8].view(2, 4), room[8:20], 16, 16)
     assert room[:8].tolist() == [8, 1, 2, 3, 9, 5, 6, 7] and int(plan.status) == 0
+
+
+# ------------------------------------------------------------------------------------------------------------- autograd
+def small_server():
+    i32 = dict(dtype=torch.int32, device="cuda")
+    kc, vc = torch.zeros(2, 6, 2, 8, 16, device="cuda").unbind(0)
+    cos, sin = torch.ones(32, 8, device="cuda"), torch.zeros(32, 8, device="cuda")
+    return i32, kc.clone(), vc.clone(), cos, sin
+
+
+def test_writes_in_place_are_seen_by_autograd():
+    """A tensor that a call writes counts as changed: a backward pass that needs its old contents says so."""
+    from hydra_b200.paged import paged_append, paged_decode_attention, paged_plan
+    i32, kc, vc, cos, sin = small_server()
+    w = torch.ones_like(kc, requires_grad=True)
+    table = torch.full((2, 3), -1, **i32)
+    kept = (w * kc).sum(), (w * vc).sum()
+    version = table._version
+    plan = paged_plan(torch.zeros(2, **i32), torch.tensor([3, 1], **i32), table, torch.arange(6, **i32), 8, 4)
+    assert table._version > version
+    x = torch.randn(4, 2, 16, device="cuda")
+    paged_append(x, x, x, kc, vc, plan.slots, cos, sin, plan.positions)
+    for y in kept:
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+    with torch.inference_mode():                                          # (inference tensors keep no versions)
+        a, b = torch.zeros_like(kc), torch.zeros_like(vc)
+        paged_append(x, x, x, a, b, plan.slots, cos, sin, plan.positions)
+        assert torch.equal(a, kc) and torch.equal(b, vc)
+    h = torch.randn(2, 2, 16, device="cuda").half()
+    out = torch.zeros_like(h)
+    version = out._version
+    paged_decode_attention(h, kc.half(), vc.half(), table, plan.kv_lens, out=out)
+    assert out._version > version
