@@ -138,6 +138,7 @@ def paged_append(q: Tensor, k: Tensor, v: Tensor, k_cache: Tensor, v_cache: Tens
         raise ValueError(f"paged_append: {slots.shape[0]} slots for {a[0]} tokens")
     if k_cache.requires_grad or v_cache.requires_grad:
         raise RuntimeError("paged_append: the caches are written in place and cannot require grad")
+    kernels._refuse_autograd("paged_append", k_cache, v_cache)
     q_out, _ = kernels._qk_norm_rope("paged_append", dev, q, k, cos, sin, positions, q_weight, k_weight, norm, eps, q_scale, k_scale,
                                      layout, v=v, slots=slots, cache=cache)
     increment_version((k_cache, v_cache))

@@ -186,3 +186,30 @@ def test_writes_in_place_are_seen_by_autograd():
     version = out._version
     paged_decode_attention(h, kc.half(), vc.half(), table, plan.kv_lens, out=out)
     assert out._version > version
+
+
+def test_forward_mode_tangents_are_refused():
+    """A derivative that would be dropped in silence is refused, in forward mode too, under no_grad too (which does not end it)."""
+    import torch.autograd.forward_ad as fwd
+    from hydra_b200.kernels import fused_qk_norm_rope
+    from hydra_b200.paged import paged_append, paged_decode_attention
+    from hydra_b200.sampling import token_logprobs
+    i32, kc, vc, cos, sin = small_server()
+    x = torch.randn(4, 2, 16, device="cuda")
+    where = torch.arange(4, **i32)
+    n = torch.tensor([1, 2, 3, 4], **i32)
+    table = torch.zeros(4, 1, **i32)
+    h, hk, hv = x.half(), kc.half(), vc.half()
+    with fwd.dual_level():
+        d = lambda t: fwd.make_dual(t, torch.ones_like(t))                # noqa: E731
+        for call in (lambda: fused_qk_norm_rope(d(x), x, cos, sin), lambda: fused_qk_norm_rope(x, x, d(cos), sin),
+                     lambda: fused_qk_norm_rope(x, x, cos, sin, q_weight=d(torch.ones(16, device="cuda"))),
+                     lambda: paged_append(x, x, d(x), kc, vc, where.long(), cos, sin, where),
+                     lambda: paged_append(x, x, x, d(kc), vc, where.long(), cos, sin, where),
+                     lambda: paged_decode_attention(d(h), hk, hv, table, n), lambda: paged_decode_attention(h, hk, d(hv), table, n),
+                     lambda: token_logprobs(d(x[0]), torch.zeros(2, dtype=torch.int64, device="cuda"))):
+            with pytest.raises(RuntimeError, match="inference only"):
+                call()
+            with torch.no_grad(), pytest.raises(RuntimeError, match="inference only"):
+                call()
+        fused_qk_norm_rope(x, x, cos, sin)                                # without tangents: as ever
