@@ -531,7 +531,7 @@ class HydraB200Model:
         B, S = ids.shape
         lg = self.forward(ids)
         padded = lg.as_strided((B * S, self.ld_logits), (self.ld_logits, 1))      # the rows with their padding columns
-        r = token_logprobs(padded, targets.to(self.device).reshape(-1), top, temperature, vocab=self.vocab_size,
+        r = token_logprobs(padded, targets.to(self.device, torch.int64).reshape(-1), top, temperature, vocab=self.vocab_size,
                            ignore_index=ignore_index)
         return TokenLogprobs(r.logprobs.view(B, S), r.entropy.view(B, S), r.top_logprobs.view(B, S, top), r.top_ids.view(B, S, top))
 

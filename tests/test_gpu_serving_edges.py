@@ -213,3 +213,16 @@ def test_forward_mode_tangents_are_refused():
             with torch.no_grad(), pytest.raises(RuntimeError, match="inference only"):
                 call()
         fused_qk_norm_rope(x, x, cos, sin)                                # without tangents: as ever
+
+
+# ---------------------------------------------------------------------------------------------------------------- model
+def test_model_scores_ids_of_any_integer_type():
+    """HydraB200Model.token_logprobs takes what forward and eval_loss take."""
+    from tests import golden_io as G
+    from tests.test_gpu_model import build
+    fx, cfg, w = G.model_fixture("model_hd32.npz")
+    m = build(w, cfg)
+    ids = torch.from_numpy(fx["ids"]).clamp(0, cfg.vocab_size - 1).cuda()
+    want = m.token_logprobs(ids, top=2)
+    for got in (m.token_logprobs(ids.int(), top=2), m.token_logprobs(ids[:, :-1].int(), ids[:, 1:].int(), top=2)):
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
