@@ -216,6 +216,12 @@ def fused_rms_norm(x: Tensor, weight: Tensor, eps: float = 1e-6) -> Tensor:
     return _rms_norm_op(x, weight, float(eps))
 
 
+def _fits_int32(what: str, *sizes: int) -> None:
+    """ctypes would cut a larger size to its low 32 bits."""
+    if max(sizes) > 0x7fffffff:
+        raise ValueError(f"{what}: a size of {max(sizes)} (up to 2^31 - 1)")
+
+
 def _overlap(a: Tensor, b: Tensor) -> bool:
     """Whether the memory that one tensor reaches over, from its first byte to its last, meets the other's."""
     def reach(t):
@@ -253,6 +259,7 @@ def _qk_norm_rope(what: str, dev: torch.device, q: Tensor, k: Tensor, cos: Tenso
         raise ValueError(f"{what}: norm must be 'rms', 'l2' or None and layout 'interleaved' or 'half', got {norm!r} and {layout!r}") from None
     dtype, torch_dtype, shape, k_shape = _dtype_code(q), q.dtype, q.shape, k.shape
     hd = shape[-1]
+    _fits_int32(what, *shape, *k_shape)
     if cos.dim() == 4:
         cos, sin = cos[0, 0], sin[0, 0]
     table = cos.shape

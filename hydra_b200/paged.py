@@ -75,8 +75,9 @@ def paged_plan(context_lens: Tensor, new_lens: Tensor, block_tables: Tensor, fre
     if (width > 1 and unit != 1) or (B > 1 and ld < width):
         raise ValueError("paged_plan: the rows of block_tables must be contiguous and apart (they are written in place)")
     page_size, room = int(page_size), int(max_new_tokens)
-    if page_size < 1 or not 0 <= room <= 0x7fffffff:
+    if page_size < 1 or room < 0:
         raise ValueError(f"paged_plan: page_size {page_size} and max_new_tokens {room} must be positive")
+    kernels._fits_int32("paged_plan", B, width, page_size, room)
     if free_start is not None:
         if free_start.get_device() != dev.index or free_start.dtype != torch.int32 or free_start.numel() != 1:
             raise ValueError("paged_plan: free_start must be one int32 on the tables' device")
@@ -101,6 +102,7 @@ def _cache(what: str, k_cache: Tensor, v_cache: Tensor) -> _lib.PagedCache:
         raise ValueError(f"{what}: k_cache and v_cache must be [num_pages, kv_heads, page_size, head_dim] of one shape and dtype, "
                          f"got {tuple(shape)} {k_cache.dtype} and {tuple(v_cache.shape)} {v_cache.dtype}")
     pages, heads, rows, hd = shape
+    kernels._fits_int32(what, *shape)
     ks, vs = k_cache.stride(), v_cache.stride()
     if (ks[3] != 1 or vs[3] != 1) and hd > 1:
         raise ValueError(f"{what}: a head's row in the cache must be contiguous")
@@ -169,6 +171,7 @@ def paged_decode_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_ta
         raise ValueError(f"paged_decode_attention: q must be [B, Hq, hd] in the caches' dtype, bfloat16 or float16, got {tuple(q.shape)} {q.dtype}")
     cache = _cache("paged_decode_attention", k_cache, v_cache)
     B, Hq, hd = q.shape
+    kernels._fits_int32("paged_decode_attention", B, Hq, *block_tables.shape)
     if cache.head_dim != hd or Hq < 1 or Hq % cache.n_kv_heads:
         raise ValueError(f"paged_decode_attention: queries {tuple(q.shape)} do not fit the cache {tuple(k_cache.shape)}")
     kv_lens = _ints("paged_decode_attention: kv_lens", kv_lens, torch.int32, 1)

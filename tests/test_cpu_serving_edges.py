@@ -110,3 +110,72 @@ def test_reach_of_strided_tensors():
     assert _overlap(room[::2, 10:20], room[1])                            # between its rows
     assert not _overlap(room[0, :0], room) and not _overlap(room[:, :10].t()[9:], room[0, :9])
     assert _overlap(room[:1].expand(3, 100), room[0, 99:]) and not _overlap(room[:1].expand(3, 100), room[1])
+
+
+# --------------------------------------------------------------------------------------------------------------- sizes
+class Taken(Exception):
+    pass
+
+
+@pytest.fixture
+def up_to_the_c_call(monkeypatch):
+    """The Python entries on tensors without memory, up to their C call."""
+    from contextlib import nullcontext
+    from hydra_b200 import kernels
+
+    class Lib:
+        def __getattr__(self, name):
+            def call(*args):
+                raise Taken(name)
+            return call
+    lib = Lib()
+    monkeypatch.setattr(_lib, "lib", lambda: lib)
+    monkeypatch.setattr(kernels, "_require_cuda", lambda *t: torch.device("meta"))
+    monkeypatch.setattr(kernels, "_on", lambda dev: nullcontext())
+    monkeypatch.setattr(kernels, "_stream", lambda dev: 0)
+    monkeypatch.setattr(torch.Tensor, "data_ptr", lambda t: M)
+    monkeypatch.setattr(kernels, "_empty_strided", lambda size, stride, dtype: torch.empty_strided(size, stride, dtype=dtype, device="meta"))
+
+
+def _meta(*shape, dtype=torch.bfloat16):
+    return torch.empty(shape, dtype=dtype, device="meta")
+
+
+def test_sizes_past_32_bits_are_refused(up_to_the_c_call):
+    """ctypes cuts an int to 32 bits: 2^32 + 16 rows of a page were 16."""
+    from hydra_b200.kernels import fused_qk_norm_rope
+    from hydra_b200.paged import paged_append, paged_decode_attention, paged_plan
+    from hydra_b200.sampling import token_logprobs
+    i32, i64, f32, big = dict(dtype=torch.int32), dict(dtype=torch.int64), dict(dtype=torch.float32), (1 << 32) + 4
+
+    def plan(B=2, width=4, page=16, room=8):
+        return paged_plan(_meta(B, **i32), _meta(B, **i32), _meta(B, width, **i32), _meta(9, **i32), page, room)
+
+    def rope(T=4, hq=4, hkv=2, hd=64, table=8):
+        return fused_qk_norm_rope(_meta(T, hq, hd), _meta(T, hkv, hd), _meta(table, 4, **f32), _meta(table, 4, **f32), _meta(T, **i32))
+
+    def rope4(B=1, S=4):
+        return fused_qk_norm_rope(_meta(B, 2, S, 8), _meta(B, 1, S, 8), _meta(S, 4, **f32), _meta(S, 4, **f32))
+
+    def append(T=4, pages=8, page=16):
+        x, c = _meta(T, 2, 16), _meta(pages, 2, page, 16)
+        return paged_append(x, x, x, c, c, _meta(T, **i64), _meta(8, 8, **f32), _meta(8, 8, **f32), _meta(T, **i32))
+
+    def attention(B=2, hq=4, pages=8, page=16, hd=16, width=4):
+        c = _meta(pages, 2, page, hd)
+        return paged_decode_attention(_meta(B, hq, hd), c, c, _meta(B, width, **i32), _meta(B, **i32))
+
+    def logprobs(N=2, V=64, vocab=None):
+        return token_logprobs(_meta(N, V), _meta(N, **i64), vocab=vocab)
+
+    for call, sizes in ((plan, ("B", "width", "page", "room")), (rope, ("T", "hq", "hkv", "hd")), (rope4, ("B", "S")), (append, ("T", "pages", "page")),
+                        (attention, ("B", "hq", "pages", "page", "hd", "width")), (logprobs, ("V",))):
+        with pytest.raises(Taken):
+            call()
+        for size in sizes:
+            with pytest.raises(ValueError):
+                call(**{size: big})
+    with pytest.raises(Taken):
+        logprobs(V=big, vocab=64)
+    with pytest.raises(Taken):
+        rope(table=big)
