@@ -260,11 +260,11 @@ def _qk_norm_rope(what: str, dev: torch.device, q: Tensor, k: Tensor, cos: Tenso
     dtype, torch_dtype, shape, k_shape = _dtype_code(q), q.dtype, q.shape, k.shape
     hd = shape[-1]
     _fits_int32(what, *shape, *k_shape)
-    if cos.dim() == 4:
+    if cos.dim() == 4 and cos.shape[:2] == (1, 1) and sin.shape == cos.shape:
         cos, sin = cos[0, 0], sin[0, 0]
     table = cos.shape
     if len(table) != 2 or sin.shape != table or 2 * table[1] > hd:
-        raise ValueError(f"{what}: cos and sin must be [rows, rotated / 2] with rotated <= {hd}, got {tuple(table)} and {tuple(sin.shape)}")
+        raise ValueError(f"{what}: cos and sin must be [rows, rotated / 2] or [1, 1, rows, rotated / 2] with rotated <= {hd}, got {tuple(table)} and {tuple(sin.shape)}")
     table_rows, half = table
     table_ld, unit = cos.stride()
     if unit != 1 or table_ld < half or cos.dtype != torch.float32 or sin.dtype != torch.float32 or sin.stride() != (table_ld, 1):

@@ -179,3 +179,17 @@ def test_sizes_past_32_bits_are_refused(up_to_the_c_call):
         logprobs(V=big, vocab=64)
     with pytest.raises(Taken):
         rope(table=big)
+
+
+def test_tables_of_several_sequences_are_refused(up_to_the_c_call):
+    """cos and sin [1, 1, rows, rot / 2] are one table; of a table per sequence or head the first one served for all."""
+    from hydra_b200.kernels import fused_qk_norm_rope
+    q, k = _meta(2, 4, 8, 16), _meta(2, 2, 8, 16)
+    t = lambda *s: _meta(*s, dtype=torch.float32)                         # noqa: E731
+    for cos, sin in ((t(8, 8), t(8, 8)), (t(1, 1, 8, 8), t(1, 1, 8, 8))):
+        with pytest.raises(Taken):
+            fused_qk_norm_rope(q, k, cos, sin)
+    for cos, sin in ((t(2, 1, 8, 8), t(2, 1, 8, 8)), (t(1, 4, 8, 8), t(1, 4, 8, 8)), (t(1, 1, 8, 8), t(2, 1, 8, 8)), (t(1, 1, 8, 8), t(8, 8)),
+                     (t(8, 8), t(1, 1, 8, 8)), (t(0, 1, 8, 8), t(0, 1, 8, 8))):
+        with pytest.raises(ValueError, match="rotated"):
+            fused_qk_norm_rope(q, k, cos, sin)
