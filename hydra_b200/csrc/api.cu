@@ -1,4 +1,5 @@
 // Version and thread-local error text of the C ABI; per-device kernel attribute bookkeeping.
+#include <atomic>
 #include <map>
 #include <mutex>
 #include <utility>
@@ -24,6 +25,18 @@ int ensure_dynamic_smem(const void* kernel, size_t bytes) {
   if (bytes > have) {
     HB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
     have = bytes;
+  }
+  return 0;
+}
+
+int device_sms(int* sms) {
+  static std::atomic<int> known[64];
+  int dev = 0;
+  HB_CUDA(cudaGetDevice(&dev));
+  *sms = dev < 64 ? known[dev].load(std::memory_order_relaxed) : 0;
+  if (*sms == 0) {
+    HB_CUDA(cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev));
+    if (dev < 64) known[dev].store(*sms, std::memory_order_relaxed);
   }
   return 0;
 }

@@ -138,6 +138,9 @@ inline bool rows_apart(int64_t row_bytes, std::initializer_list<Axis> axes) {
 }
 inline bool overlap(const Reach& a, const Reach& b) { return a.lo < a.hi && b.lo < b.hi && a.lo < b.hi && b.lo < a.hi; }
 
+// SMs of the current device (asked for once per device).  Defined in api.cu.
+int device_sms(int* sms);
+
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 inline int ceil_div(int a, int b) { return (a + b - 1) / b; }
 inline int64_t ceil_div64(int64_t a, int64_t b) { return (a + b - 1) / b; }

@@ -545,14 +545,15 @@ int launch(LogprobParams p, int64_t rows, cudaStream_t st) {
   // Few long rows: up to eight CTAs per row while there is an SM for each and each still has 64 KB: shorter slices cost more in
   // the cluster's barriers and the merge than they save (one row of 152064 bf16 columns: 11.2 us in one CTA, 8.2 in four;
   // 64 rows of 50257, 100 KB each: 8.1 in one, 10.1 in four).
-  int cluster = 1;
-  while (cluster < 8 && rows * cluster * 2 <= 148 && (int64_t)p.cols * sizeof(T) / (cluster * 2) >= 65536) cluster *= 2;
+  int cluster = 1, sms = 0;
+  HB_PROPAGATE(device_sms(&sms));
+  while (cluster < 8 && rows * cluster * 2 <= sms && (int64_t)p.cols * sizeof(T) / (cluster * 2) >= 65536) cluster *= 2;
   p.slice = ceil_div(ceil_div(p.cols, cluster), 64) * 64;
   // Many rows: small CTAs, whose barriers hold up little and whose fixed work per row (joining the statistics, the bound) is
   // small; few: 512 threads get a row's bytes under way sooner; between them, and for long rows of many alternatives, 256
   // (600 rows of 50257: 19 us with 256 threads, 22 with 128; 8192 rows: 146 and 140 us).
-  if (rows * cluster <= 2 * 148) return launch_nt<T, 512>(p, rows, cluster, st);
-  if (rows < 6 * 148 || (p.top > 4 && p.cols > 65536)) return launch_nt<T, 256>(p, rows, cluster, st);
+  if (rows * cluster <= 2 * sms) return launch_nt<T, 512>(p, rows, cluster, st);
+  if (rows < 6 * sms || (p.top > 4 && p.cols > 65536)) return launch_nt<T, 256>(p, rows, cluster, st);
   return launch_nt<T, 128>(p, rows, cluster, st);
 }
 

@@ -778,13 +778,6 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedParams p) {
   if (p.lse && wi == 0 && lane == 0) p.lse[rw] = log_sum<T>(m, l, p.scale_log2);
 }
 
-int sm_count(int* out) {
-  int dev = 0;
-  HB_CUDA(cudaGetDevice(&dev));
-  HB_CUDA(cudaDeviceGetAttribute(out, cudaDevAttrMultiProcessorCount, dev));
-  return 0;
-}
-
 int padded_hd(int hd) { return hd <= 16 ? 16 : (hd <= 32 ? 32 : (hd <= 64 ? 64 : (hd <= 128 ? 128 : 256))); }
 
 size_t round256(size_t n) { return (n + 255) & ~(size_t)255; }
@@ -847,7 +840,7 @@ using namespace hb200;
 
 extern "C" size_t hb200_paged_attention_workspace_bytes(int B, int Hq, int Hkv, int hd) {
   int sms = 0;
-  if (check_heads("paged_attention_workspace_bytes", B, Hq, Hkv, hd) != 0 || sm_count(&sms) != 0) return 0;
+  if (check_heads("paged_attention_workspace_bytes", B, Hq, Hkv, hd) != 0 || device_sms(&sms) != 0) return 0;
   return workspace_for(B, Hq, Hkv, hd, sms);
 }
 
@@ -886,7 +879,7 @@ extern "C" int hb200_paged_decode_attention(const hb200_paged_cache* c, const vo
   HB_REQUIRE(!overlap(written[0], written[1]), HB200_ERR_INVALID, "paged_decode_attention: out and lse must not overlap one another");
   const int group = Hq / c->n_kv_heads;
   int sms = 0;
-  HB_PROPAGATE(sm_count(&sms));
+  HB_PROPAGATE(device_sms(&sms));
   HB_REQUIRE(workspace_bytes >= workspace_for(B, Hq, c->n_kv_heads, c->head_dim, sms), HB200_ERR_WORKSPACE,
              "paged_decode_attention: workspace of %zu bytes, needs %zu", workspace_bytes,
              workspace_for(B, Hq, c->n_kv_heads, c->head_dim, sms));

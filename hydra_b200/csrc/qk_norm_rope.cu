@@ -475,6 +475,9 @@ extern "C" int hb200_qk_norm_rope(const hb200_qk_norm_rope_args* a, const hb200_
     HB_REQUIRE(a->k_out, HB200_ERR_INVALID, "qk_norm_rope: null pointer");
     fits(p.k_out, p.ko_s);
   }
+  HB_REQUIRE(a->dtype == HB200_F32 || a->dtype == HB200_BF16 || a->dtype == HB200_F16, HB200_ERR_UNSUPPORTED, "qk_norm_rope: unsupported dtype %d", a->dtype);
+  int sms = 0;
+  HB_PROPAGATE(device_sms(&sms));
   p.group_lanes = 1;
   while (p.group_lanes * 8 < p.hd) p.group_lanes <<= 1;
   // a token's head rows are shared out over more groups of lanes until about 8 warps per SM have work (8192 tokens of ten heads of
@@ -486,7 +489,7 @@ extern "C" int hb200_qk_norm_rope(const hb200_qk_norm_rope_args* a, const hb200_
     p.kv_warps = a->Hkv ? ceil_div64(tokens * p.kv_parts, groups) : 0;
     return p.q_warps + kinds * p.kv_warps;
   };
-  while (count() < 148 * 8 && (p.q_parts < a->Hq || p.kv_parts < a->Hkv)) {
+  while (count() < sms * 8 && (p.q_parts < a->Hq || p.kv_parts < a->Hkv)) {
     const bool q_more = p.q_parts < a->Hq && (p.kv_parts >= a->Hkv || (int64_t)p.kv_parts * a->Hq >= (int64_t)p.q_parts * a->Hkv);
     (q_more ? p.q_parts : p.kv_parts) *= 2;
   }
@@ -495,7 +498,5 @@ extern "C" int hb200_qk_norm_rope(const hb200_qk_norm_rope_args* a, const hb200_
   const bool half = a->layout == HB200_ROPE_HALF;
   if (a->dtype == HB200_F32) return launch<float>(p, vec, fast, half, c != nullptr, st);
   if (a->dtype == HB200_BF16) return launch<__nv_bfloat16>(p, vec, fast, half, c != nullptr, st);
-  if (a->dtype == HB200_F16) return launch<__half>(p, vec, fast, half, c != nullptr, st);
-  set_error("qk_norm_rope: unsupported dtype %d", a->dtype);
-  return HB200_ERR_UNSUPPORTED;
+  return launch<__half>(p, vec, fast, half, c != nullptr, st);
 }
