@@ -17,6 +17,8 @@
 // (max, sum, unnormalised output) in 32 bits; the CTA, whose warps' shares are neighbours, adds up those of one pair, and
 // what then still spans CTAs goes through the workspace to the join kernel.  All sums run in a fixed order without
 // atomics: the same inputs give the same bits.
+#include <cfloat>
+
 #include "common.cuh"
 #include "mma.cuh"
 
@@ -42,6 +44,7 @@ struct PagedParams {
   int B, Hq, Hkv, hd, group, q_tiles, q_tile, tile, pair_cost, warps, rows, part_floats, page_size, width, num_pages, ctas;
   float scale_log2;  // |scale| log2(e)
   uint32_t q_sign;   // flips the signs of a pair of query values where the scale is negative
+  uint32_t q_keep;   // all bits; none where the scale is zero: scores of exactly 0 (and a scale of one, for the -inf of masked tokens)
 };
 
 // Measured (device time, graph replay): one request of 131072 tokens, 32 query heads on 8 kv heads of 128: 90.5 us, 5.9 TB/s,
@@ -418,7 +421,7 @@ __global__ void __launch_bounds__(warps_of(HD) * 32, 1) paged_attention_kernel(c
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             const int d = ks * 16 + i * 8;
-            qf[ks][n][i] = (r < rows_here && d < p.hd) ? __ldg(reinterpret_cast<const uint32_t*>(qr + d)) ^ p.q_sign : 0u;
+            qf[ks][n][i] = (r < rows_here && d < p.hd) ? (__ldg(reinterpret_cast<const uint32_t*>(qr + d)) ^ p.q_sign) & p.q_keep : 0u;
           }
         m[n][0] = m[n][1] = -INFINITY;
         l[n][0] = l[n][1] = base[n][0] = base[n][1] = 0.f;
@@ -902,9 +905,10 @@ extern "C" int hb200_paged_decode_attention(const hb200_paged_cache* c, const vo
   p.warps = warps_of(HD);
   p.page_size = c->page_size; p.width = table_width; p.num_pages = c->num_pages;
   p.ctas = sms;
-  // (a scale of zero: near enough to it, so that the -inf of masked tokens stays -inf in the product)
-  const double magnitude = scale < 0.f ? -(double)scale : (double)scale;
-  p.scale_log2 = magnitude < 1e-30 ? 1e-30f : (float)(magnitude * 1.4426950408889634);
+  // (from the smallest scale to the largest it stays above zero and finite, for distances of zero and of infinity)
+  const double log2_scale = (scale < 0.f ? -(double)scale : (double)scale) * 1.4426950408889634;
+  p.scale_log2 = scale == 0.f ? 1.f : (log2_scale < FLT_MAX ? (float)log2_scale : FLT_MAX);
+  p.q_keep = scale == 0.f ? 0u : 0xffffffffu;
   p.q_sign = scale < 0.f ? 0x80008000u : 0u;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   p.part = reinterpret_cast<float*>(ws);

@@ -103,6 +103,25 @@ def test_a_token_that_takes_nearly_all_and_gives_nothing(dtype, heads, B, n, at)
     assert (off <= tol).all(), f"off by {float((off / tol).max()):.2f} tolerances, {float((off / want).max()):.2e} of the value"
     assert float(((l.double().cpu() - lse).abs() / (1 + lse.abs())).max()) <= 1e-5
 
+@pytest.mark.parametrize("heads,hd", [(4, 64), (20, 16)])
+@pytest.mark.parametrize("n", [1, 37, 3000])
+@pytest.mark.parametrize("power,scale", [(60, 2.0 ** -119), (60, -2.0 ** -119), (60, 0.0), (0, 0.0), (30, -0.0), (-70, 2.0 ** 126), (-70, -2.0 ** 127.5), (63, 2.0 ** -140)])
+def test_scales_of_any_size(heads, hd, n, power, scale):
+    """Scores near 2^(2 power) times a scale near its inverse: weights, mean values and sums as at ordinary sizes (2^-16 of the
+    weights' exponents, whose size is below 2^7; a scale of zero weighs all tokens alike)."""
+    from hydra_b200.paged import paged_decode_attention
+    g = torch.Generator().manual_seed(n + hd)
+    q, k, v = torch.zeros(2, heads, hd), torch.zeros(2, n, 1, hd), torch.randn(2, n, 1, hd, generator=g)
+    q[..., 0] = 2.0 ** power
+    k[..., 0] = (torch.randint(-64, 64, (2, n, 1), generator=g) / 32) * 2.0 ** power
+    q, k, v = (t.to(torch.bfloat16) for t in (q, k, v))
+    kc, vc, table = pages_of(k, v, 16)
+    out, l = (t.double().cpu() for t in paged_decode_attention(q.cuda(), kc, vc, table, torch.full((2,), n, dtype=torch.int32).cuda(), scale=scale,
+                                                               return_lse=True))
+    want, lse, mass = attend(q, k, v, torch.tensor(scale, dtype=torch.float32).item())
+    assert ((out - want).abs() <= 2.0 ** -8 * want.abs() + (2.0 ** -14 + n * 2.0 ** -27) * mass).all(), float((out - want).abs().max())
+    assert float(((l - lse).abs() / (1 + lse.abs())).max()) <= 1e-5
+
 
 def test_out_within_what_is_read_is_refused():
     from hydra_b200.paged import paged_decode_attention
