@@ -13,7 +13,7 @@
 // `top` exact selection rounds instead.
 //
 // Measured (device time): 8192 rows of 50257 bf16 logits and one alternative: 134 us, 6.1 TB/s, 0.94 of a copy (153 us once the
-// power cap holds the clock at 1.65 GHz: then the issue slots bound it); one row: 7.5 us, 64 masked rows with 20: 8.1 us,
+// power cap holds the clock at 1.65 GHz: then the issue slots bound it), in f16 137, 4096 rows in fp32 135; one row: 7.9 us, 64 masked rows with 20: 8.4 us,
 // launch, one trip through the row and three through barriers.
 //
 // Few long rows are split over a cluster of CTAs, whose partial results the first CTA merges through distributed shared memory.
@@ -532,8 +532,8 @@ int launch_as(const LogprobParams& p, int64_t rows, int cluster, cudaStream_t st
 }
 
 // One stretch per thread for a few alternatives, eight for more: a stretch that reaches the bound is read again (2048 rows of
-// 152064 bf16 columns, 20 alternatives: 115 us with eight, 150 with one), and noting eight costs registers (8192 rows of 50257,
-// one alternative: 140 us with one, 155 with eight).
+// 152064 bf16 columns, 20 alternatives: 113 us with eight, 151 with one), and noting eight costs registers (8192 rows of 50257,
+// one alternative: 134 us with one, 149 with eight).
 template <typename T, int NT>
 int launch_nt(const LogprobParams& p, int64_t rows, int cluster, cudaStream_t st) {
   if (p.top == 0) return launch_as<T, NT, 0>(p, rows, cluster, st);
@@ -543,15 +543,15 @@ int launch_nt(const LogprobParams& p, int64_t rows, int cluster, cudaStream_t st
 template <typename T>
 int launch(LogprobParams p, int64_t rows, cudaStream_t st) {
   // Few long rows: up to eight CTAs per row while there is an SM for each and each still has 64 KB: shorter slices cost more in
-  // the cluster's barriers and the merge than they save (one row of 152064 bf16 columns: 11.2 us in one CTA, 8.2 in four;
-  // 64 rows of 50257, 100 KB each: 8.1 in one, 10.1 in four).
+  // the cluster's barriers and the merge than they save (one row of 152064 bf16 columns: 11.4 us in one CTA, 8.4 in four;
+  // 64 rows of 50257, 100 KB each: 8.1 in one, 8.9 in two).
   int cluster = 1, sms = 0;
   HB_PROPAGATE(device_sms(&sms));
   while (cluster < 8 && rows * cluster * 2 <= sms && (int64_t)p.cols * sizeof(T) / (cluster * 2) >= 65536) cluster *= 2;
   p.slice = ceil_div(ceil_div(p.cols, cluster), 64) * 64;
   // Many rows: small CTAs, whose barriers hold up little and whose fixed work per row (joining the statistics, the bound) is
   // small; few: 512 threads get a row's bytes under way sooner; between them, and for long rows of many alternatives, 256
-  // (600 rows of 50257: 19 us with 256 threads, 22 with 128; 8192 rows: 146 and 140 us).
+  // (600 rows of 50257: 18 us with 256 threads, 19 with 128; 8192 rows: 139 and 134 us).
   if (rows * cluster <= 2 * sms) return launch_nt<T, 512>(p, rows, cluster, st);
   if (rows < 6 * sms || (p.top > 4 && p.cols > 65536)) return launch_nt<T, 256>(p, rows, cluster, st);
   return launch_nt<T, 128>(p, rows, cluster, st);

@@ -3,16 +3,16 @@
 //   s_j = scale * q . k_j  (j < len),   out = sum_j e^{s_j} v_j / sum_j e^{s_j},   lse = ln sum_j e^{s_j}
 //
 // Bound: HBM.  Every K and V row of the valid tokens is read once (4 * hd bytes per token and kv head) for 4 * hd * group
-// operations, so the tensor cores are needed only to keep the arithmetic out of the way.  tcgen05 would want 64 or 128 rows
-// on the accumulator's side and a TMEM round trip for the weights; with 1..16 query heads per kv head the warp-level m16n8k16
-// is used, transposed (scores^T = K Q^T, out^T = V^T P^T): the tokens and the head's values are the 16 rows and the query heads
-// the 8 columns, so a group of up to 8 heads costs half of what 16 padded query rows cost, in registers too.
+// operations, so for groups of up to 8 query heads the tensor cores are needed only to keep the arithmetic out of the way.  tcgen05
+// would want 64 or 128 rows on the accumulator's side and a TMEM round trip for the weights; the warp-level m16n8k16 is used,
+// transposed (scores^T = K Q^T, out^T = V^T P^T): the tokens and the head's values are the 16 rows and the query heads the 8
+// columns, so a group of up to 8 heads costs half of what 16 padded query rows cost, in registers too.  Groups of 9 to 24 take two
+// or three columns, and there it is the arithmetic that bounds: half of the issue slots, few of them waiting for memory.
 //
 // Work split: the tiles of all (request, kv head) pairs are laid end to end and dealt out in equal contiguous shares to
 // the warps of a grid that fits the GPU once (one CTA per SM), whatever the lengths are: a batch of one long and many
 // short requests keeps every SM busy to the end.  Starting and finishing a pair costs a warp as much as a few tiles, so each
-// pair is that much longer when the shares are cut (without it 256 requests of 1 to 300 tokens took 69 us, their warps'
-// loops between 28 and 60).  The lengths live on the device; each CTA scans them itself.  A warp streams its share through a private cp.async ring that runs on across the ends of requests, so no barrier is met between
+// pair is that much longer when the shares are cut.  The lengths live on the device; each CTA scans them itself.  A warp streams its share through a private cp.async ring that runs on across the ends of requests, so no barrier is met between
 // the scan and the share's end.  A pair that lies within one share is finished by its warp.  Of the others each warp leaves
 // (max, sum, unnormalised output) in 32 bits; the CTA, whose warps' shares are neighbours, adds up those of one pair, and
 // what then still spans CTAs goes through the workspace to the join kernel.  All sums run in a fixed order without
@@ -47,26 +47,27 @@ struct PagedParams {
   uint32_t q_keep;   // all bits; none where the scale is zero: scores of exactly 0 (and a scale of one, for the -inf of masked tokens)
 };
 
-// Measured (device time, graph replay): one request of 131072 tokens, 32 query heads on 8 kv heads of 128: 90.5 us, 5.9 TB/s,
-// 0.91 of a copy; 64 requests up to 8192 tokens, 32 heads on 4 of 64: 55 us, 5.0 TB/s; one request of 1500 tokens: 10.7 us, of
+// Measured (device time, graph replay): one request of 131072 tokens, 32 query heads on 8 kv heads of 128: 92.8 us, 5.8 TB/s,
+// 0.89 of a copy; 64 requests up to 8192 tokens, 32 heads on 4 of 64: 55.3 us, 4.9 TB/s; one request of 1500 tokens: 11.1 us, of
 // which 8 are the two launches and the chain lengths -> table -> tiles -> parts -> join.  What bounds the large ones: DRAM,
-// after 7 us in which the rings fill, and SMs that get up to a tenth less of it than others.
+// after 7 us in which the rings fill, and SMs that get up to a tenth less of it than others.  All figures in this file are
+// of one state of the code and one B200; those with another choice of a constant, of that code with the one constant changed.
 //
 // A warp's tile: 8 KB of K and V (16 KB of heads of 256, 4 KB of small ones, whose tokens cost more arithmetic per byte and get
-// twice the warps: 64 requests up to 16384 tokens on 4 kv heads of 16 took 48 us with eight warps, 43 with sixteen); two
-// tiles of a warp are in flight while one is computed, 128 KB of a CTA.  Heads of 64 do better with twelve warps and one tile
-// in flight each (64 requests up to 8192 tokens: 53.2 us instead of 54.7), heads of 128 no better and worse where there is
-// little to do (one request of 1500: 11.5 instead of 10.9).
+// twice the warps: 64 requests up to 16384 tokens, 32 heads on 4 of 16: 54.9 us with eight warps, 52.2 with sixteen).  Two tiles of a
+// warp are in flight while one is computed, 128 KB of a CTA; of heads of 64 one, 96 KB, which leaves room for twelve warps (64
+// requests up to 8192 tokens: 55.4 us, with eight warps and two tiles 56.2).  Heads of 128 gain nothing by that, and lose where
+// there is little to do (one request of 1500: 11.6 instead of 11.1).
 __host__ __device__ constexpr int tile_tokens(int HD) { return HD >= 128 ? 16 : (HD == 16 ? 64 : 32); }
 __host__ __device__ constexpr int warps_of(int HD) { return HD >= 256 ? 4 : (HD == 128 ? 8 : (HD == 64 ? 12 : 16)); }
 __host__ __device__ constexpr int stages_of(int HD) { return HD == 64 ? 2 : 3; }
 // Most query heads that are worked on together: their outputs and queries stay in a warp's registers.  Larger groups are cut
-// into tiles of one size, each of which reads the keys and values again.  (Groups of 20: 82 requests of 5115 tokens on heads of
-// 80 take 181 us in one tile and 240 in two of ten, 64 requests up to 32768 on heads of 16 59 and 73; where the second read
-// comes out of the L2, 32 requests up to 8192 on two kv heads of 128, 57 and 53.)
+// into tiles of one size, each of which reads the keys and values again.  (Groups of 20: 82 requests of 5115 tokens on 4 kv
+// heads of 80 take 175 us in one tile and 285 in two of ten, 64 requests up to 32768 on 4 of 16 145 and 228; where the second
+// read comes out of the L2, 32 requests up to 8192 on two of 128, 61 and 56.)
 __host__ __device__ constexpr int most_heads(int HD) { return HD >= 256 ? 8 : 24; }
 // Places that a pair takes before its first tile when the shares are cut: what its start and end cost, in tiles.  (256 requests
-// of 1 to 300 tokens on 8 kv heads of 128: 54 us with one, 48 with two, 46 with three; all of 100 tokens: 36, 37 and 38.)
+// of 1 to 300 tokens, 32 heads on 8 of 128: 56 us with one, 50 with two, 47 with three; all of 100 tokens: 37, 39 and 39.)
 __host__ __device__ constexpr int pair_cost(int HD) { return HD <= 32 ? 2 : 3; }
 
 // Cache length of request b as the kernel reads it: what lies outside [0, width * page_size] is marked (`poison`).
@@ -161,7 +162,8 @@ struct Cursor {
 };
 
 // NQ: columns of eight query heads (a tile of up to 8: 1).  P16: the page size is a multiple of 16, so that 16 tokens side by side
-// share a page: one look into the table for them (64 requests, pages of 16: 55.3 us with it, 56.3 without).
+// share a page: one look into the table for them (64 requests, pages of 16: 55.3 us with it, 55.6 without; one
+// of 131072, pages of 64: 93.3 and 93.8).
 template <typename T, int HD, int NQ, bool P16>
 __global__ void __launch_bounds__(warps_of(HD) * 32, 1) paged_attention_kernel(const PagedParams p) {
   constexpr int NW = warps_of(HD), TT = tile_tokens(HD), CH = HD / 8, ST = stages_of(HD);
@@ -803,8 +805,8 @@ int launch(const PagedParams& p, int sms, cudaStream_t st) {
   HB_PROPAGATE(ensure_dynamic_smem((const void*)kern, smem));
   kern<<<(unsigned)sms, NW * 32, smem, st>>>(p);
   HB_LAUNCH_CHECK();
-  // a warp per row, or eight where a row has many parts (few pairs for the CTAs): one request of 1500 tokens takes 10.9 us with
-  // eight and 13.6 with one, 64 requests 62 and 55
+  // a warp per row, or eight where a row has many parts (few pairs for the CTAs): one request of 1500 tokens takes 11.1 us with
+  // eight and 14.0 with one, 64 requests 61.6 and 55.3
   const int64_t rows = (int64_t)p.B * p.Hq;
   if ((int64_t)p.B * p.Hkv * p.q_tiles * 4 <= sms) return launch_chained(paged_join_kernel<T, 8>, dim3((unsigned)rows), dim3(256), 0, st, true, 1, p);
   return launch_chained(paged_join_kernel<T, 1>, dim3((unsigned)ceil_div64(rows, 8)), dim3(256), 0, st, true, 1, p);

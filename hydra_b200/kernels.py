@@ -216,10 +216,12 @@ def fused_rms_norm(x: Tensor, weight: Tensor, eps: float = 1e-6) -> Tensor:
     return _rms_norm_op(x, weight, float(eps))
 
 
-def _fits_int32(what: str, *sizes: int) -> None:
-    """ctypes would cut a larger size to its low 32 bits."""
-    if max(sizes) > 0x7fffffff:
-        raise ValueError(f"{what}: a size of {max(sizes)} (up to 2^31 - 1)")
+_INT32_MAX = 0x7fffffff
+
+
+def _past_int32(what: str, *sizes: int) -> ValueError:
+    """For sizes that the C entries take as 32 bits: ctypes would cut a larger one to its low 32."""
+    return ValueError(f"{what}: a size of {max(sizes)} (up to 2^31 - 1)")
 
 
 def _overlap(a: Tensor, b: Tensor) -> bool:
@@ -236,10 +238,15 @@ def _refuse_autograd(what: str, *ts: Optional[Tensor]) -> None:
         for t in ts:
             if t is not None and t.requires_grad:
                 raise RuntimeError(f"{what} is inference only: an input requires grad (wrap the call in torch.no_grad())")
-    if getattr(forward_ad, "_current_level", 0) >= 0:   # (within forward_ad.dual_level() only: 0.3 us a tensor)
-        for t in ts:
-            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
-                raise RuntimeError(f"{what} is inference only: an input carries a forward-mode tangent")
+    if forward_ad._current_level >= 0:
+        _refuse_tangents(what, *ts)
+
+
+def _refuse_tangents(what: str, *ts: Optional[Tensor]) -> None:
+    """(Called within forward_ad.dual_level() only: a look at a tensor costs 0.3 us.)"""
+    for t in ts:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError(f"{what} is inference only: an input carries a forward-mode tangent")
 
 
 def _fp32(what: str, t: Tensor, n: int, dev: torch.device) -> Tensor:
@@ -259,7 +266,9 @@ def _qk_norm_rope(what: str, dev: torch.device, q: Tensor, k: Tensor, cos: Tenso
         raise ValueError(f"{what}: norm must be 'rms', 'l2' or None and layout 'interleaved' or 'half', got {norm!r} and {layout!r}") from None
     dtype, torch_dtype, shape, k_shape = _dtype_code(q), q.dtype, q.shape, k.shape
     hd = shape[-1]
-    _fits_int32(what, *shape, *k_shape)
+    if q.numel() > _INT32_MAX or k.numel() > _INT32_MAX:
+        if max(*shape, *k_shape) > _INT32_MAX:
+            raise _past_int32(what, *shape, *k_shape)
     if cos.dim() == 4 and cos.shape[:2] == (1, 1) and sin.shape == cos.shape:
         cos, sin = cos[0, 0], sin[0, 0]
     table = cos.shape

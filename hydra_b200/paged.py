@@ -20,11 +20,13 @@ from typing import NamedTuple, Optional, Tuple, Union
 
 import torch
 
+from torch.autograd import forward_ad
 from torch.autograd.graph import increment_version
 
 from . import _lib, kernels
 
 Tensor = torch.Tensor
+_MAX = kernels._INT32_MAX
 
 
 class PagedPlan(NamedTuple):
@@ -77,7 +79,8 @@ def paged_plan(context_lens: Tensor, new_lens: Tensor, block_tables: Tensor, fre
     page_size, room = int(page_size), int(max_new_tokens)
     if page_size < 1 or room < 0:
         raise ValueError(f"paged_plan: page_size {page_size} and max_new_tokens {room} must be positive")
-    kernels._fits_int32("paged_plan", B, width, page_size, room)
+    if B > _MAX or width > _MAX or page_size > _MAX or room > _MAX:
+        raise kernels._past_int32("paged_plan", B, width, page_size, room)
     if free_start is not None:
         if free_start.get_device() != dev.index or free_start.dtype != torch.int32 or free_start.numel() != 1:
             raise ValueError("paged_plan: free_start must be one int32 on the tables' device")
@@ -102,7 +105,8 @@ def _cache(what: str, k_cache: Tensor, v_cache: Tensor) -> _lib.PagedCache:
         raise ValueError(f"{what}: k_cache and v_cache must be [num_pages, kv_heads, page_size, head_dim] of one shape and dtype, "
                          f"got {tuple(shape)} {k_cache.dtype} and {tuple(v_cache.shape)} {v_cache.dtype}")
     pages, heads, rows, hd = shape
-    kernels._fits_int32(what, *shape)
+    if pages > _MAX or heads > _MAX or rows > _MAX or hd > _MAX:
+        raise kernels._past_int32(what, *shape)
     ks, vs = k_cache.stride(), v_cache.stride()
     if (ks[3] != 1 or vs[3] != 1) and hd > 1:
         raise ValueError(f"{what}: a head's row in the cache must be contiguous")
@@ -140,7 +144,8 @@ def paged_append(q: Tensor, k: Tensor, v: Tensor, k_cache: Tensor, v_cache: Tens
         raise ValueError(f"paged_append: {slots.shape[0]} slots for {a[0]} tokens")
     if k_cache.requires_grad or v_cache.requires_grad:
         raise RuntimeError("paged_append: the caches are written in place and cannot require grad")
-    kernels._refuse_autograd("paged_append", k_cache, v_cache)
+    if forward_ad._current_level >= 0:
+        kernels._refuse_tangents("paged_append", k_cache, v_cache)
     q_out, _ = kernels._qk_norm_rope("paged_append", dev, q, k, cos, sin, positions, q_weight, k_weight, norm, eps, q_scale, k_scale,
                                      layout, v=v, slots=slots, cache=cache)
     increment_version((k_cache, v_cache))
@@ -171,12 +176,13 @@ def paged_decode_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_ta
         raise ValueError(f"paged_decode_attention: q must be [B, Hq, hd] in the caches' dtype, bfloat16 or float16, got {tuple(q.shape)} {q.dtype}")
     cache = _cache("paged_decode_attention", k_cache, v_cache)
     B, Hq, hd = q.shape
-    kernels._fits_int32("paged_decode_attention", B, Hq, *block_tables.shape)
     if cache.head_dim != hd or Hq < 1 or Hq % cache.n_kv_heads:
         raise ValueError(f"paged_decode_attention: queries {tuple(q.shape)} do not fit the cache {tuple(k_cache.shape)}")
     kv_lens = _ints("paged_decode_attention: kv_lens", kv_lens, torch.int32, 1)
     block_tables = _ints("paged_decode_attention: block_tables", block_tables, torch.int32, 2)
     rows, width = block_tables.shape
+    if B > _MAX or Hq > _MAX or width > _MAX:
+        raise kernels._past_int32("paged_decode_attention", B, Hq, width)
     if kv_lens.shape[0] != B or rows != B:
         raise ValueError(f"paged_decode_attention: {B} queries, {kv_lens.shape[0]} lengths, {rows} table rows")
     if (cache.k_stride_page | cache.k_stride_head | cache.k_stride_row | cache.v_stride_page | cache.v_stride_head | cache.v_stride_row) % 8 \

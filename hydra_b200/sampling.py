@@ -66,7 +66,8 @@ def token_logprobs(logits: Tensor, tokens: Tensor, top: int = 0, temperature: fl
     top, temperature = int(top), float(temperature)
     if not 1 <= V <= columns:
         raise ValueError(f"token_logprobs: vocab {V} outside the row length {columns}")
-    kernels._fits_int32("token_logprobs", V)
+    if V > kernels._INT32_MAX:
+        raise kernels._past_int32("token_logprobs", V)
     if tokens.dtype != torch.int64 or tokens.numel() != N:
         raise ValueError(f"token_logprobs: one int64 token per row, got {tokens.dtype} {tuple(tokens.shape)} for {N} rows")
     if not 0 <= top <= min(32, V):
