@@ -103,7 +103,7 @@ inline int launch_chained(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t 
 int ensure_dynamic_smem(const void* kernel, size_t bytes);
 
 // The bytes [lo, hi) that rows of `row_bytes` reach over, laid out along axes of `n` entries `step` bytes apart; none where there is
-// no row.
+// no row or nothing in it.
 struct Axis {
   int64_t n, step;
 };
@@ -112,6 +112,7 @@ struct Reach {
 };
 inline Reach reach_of(const void* p, int64_t row_bytes, std::initializer_list<Axis> axes = {}) {
   Reach r = {(int64_t)reinterpret_cast<uintptr_t>(p), (int64_t)reinterpret_cast<uintptr_t>(p) + row_bytes};
+  if (row_bytes < 1) return {0, 0};
   for (const Axis& a : axes) {
     if (a.n < 1) return {0, 0};
     (a.step < 0 ? r.lo : r.hi) += (a.n - 1) * a.step;

@@ -64,6 +64,12 @@ def test_append_refuses_inputs_in_the_cache(bad):
     assert _append(_cache(**K), **bad) == -1 and "overlap" in _last()
 
 
+def test_append_takes_what_it_does_not_read_from_anywhere():
+    for unread in (dict(rot=0, cos=2 * M, sin=3 * M), dict(positions=None, positions_stride=M // 2, B=2), dict(q_weight=None, k_weight=None),
+                   dict(Hq=0, q=2 * M, q_out=3 * M)):
+        assert _append(_cache(**K), **unread) == -4 and "dtype" in _last(), _last()
+
+
 def _layouts():
     """Ways to keep keys and values side by side: [2, pages, ...], [pages, 2, ...], heads or values of a row in turn, token-major."""
     for shape, at in (((2, 8, 4, 16, 64), 0), ((8, 2, 4, 16, 64), 1), ((8, 4, 2, 16, 64), 2), ((8, 4, 16, 2, 64), 3)):
