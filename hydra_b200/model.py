@@ -830,7 +830,7 @@ class DecodeSession:
 
     def token_logprobs(self, top: int = 0, temperature: float = 1.0) -> TokenLogprobs:
         """Log probabilities of the tokens that the latest ``prefill`` / ``step`` / ``resample`` chose, with the entropy and
-        the ``top`` alternatives of the distributions they were chosen from (rows of ``last_logits``)."""
+        the ``top`` alternatives, under ``softmax(last_logits / temperature)`` (not cut to a sampler's top-k or top-p)."""
         if self.pos < 1:
             raise RuntimeError("token_logprobs() needs a prefill first")
         return token_logprobs(self.last_logits, self.tokens, top, temperature, vocab=self.model.vocab_size)

@@ -11,7 +11,8 @@ the answer's tokens are ``hydra_b200.sampling.token_logprobs``.
 
 The reference has no cache (its generation helper re-runs the whole forward, diagnostics/eval_checkpoint.py:127-160), so
 nothing here has a counterpart in it.  The calls are plain functions, not registered torch ops: they write into the caller's
-cache.  They are inference only and refuse tensors that autograd would record.
+cache.  They are inference only: they refuse tensors that autograd would record, tensors that they write count as changed, and
+under ``torch.compile`` they break the graph.
 """
 from __future__ import annotations
 
@@ -126,7 +127,8 @@ def paged_append(q: Tensor, k: Tensor, v: Tensor, k_cache: Tensor, v_cache: Tens
     q [T, Hq, hd], k and v [T, Hkv, hd] (views of one projection are read in place), ``slots`` int64 and ``positions`` int32 or
     int64 [T] as :func:`paged_plan` writes them, caches [num_pages, Hkv, page_size, hd] in q's dtype by any strides with
     contiguous rows (token-major pages: pass ``cache.transpose(1, 2)``) that do not overlap: not one another, k's not v's (they may
-    lie side by side in one tensor), and neither any other argument (which is refused).  Returns the normed and rotated queries
+    lie side by side in one tensor), and neither any other argument (which is refused).  hd up to 256 in any of the three types;
+    :func:`paged_decode_attention` reads bf16 and f16 caches with hd a multiple of 8.  Returns the normed and rotated queries
     [T, Hq, hd]; cache rows without a slot here stay as they are.  A row with a negative position is padding (zeros
     returned, nothing stored), one with a negative slot is computed but not stored; a position beyond the tables or a slot
     beyond the cache gives NaN.  Of two rows with the same slot either's values may stay, or some of each's."""
@@ -163,9 +165,9 @@ def paged_decode_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_ta
     ``h // (Hq // Hkv)``), softmax of ``scale * q . k`` (default ``hd ** -0.5``).
 
     q [B, Hq, hd] bf16 or f16 (up to 4096 requests, 1024 heads; hd a multiple of 8 up to 256), caches as in
-    :func:`paged_append`, ``block_tables`` int32 [B, width], ``kv_lens`` int32 [B].  Returns [B, Hq, hd] (in ``out`` if given, which must not lie within
-    the memory that an input reaches over)
-    and, if asked, the fp32 logarithm of each softmax's sum [B, Hq].  A request of length 0 gives zeros and -inf; one whose
+    :func:`paged_append`, ``block_tables`` int32 [B, width], ``kv_lens`` int32 [B].  Returns [B, Hq, hd] (in ``out``
+    if given, which must not lie within the memory that an input reaches over) and, if asked, the fp32 logarithm of each softmax's
+    sum [B, Hq].  Scores and weights in 32 bits, for any finite scale.  A request of length 0 gives zeros and -inf; one whose
     table names a page outside the cache, or whose length passes its table, gives NaN.  What lies behind a
     request's length in its last page is not looked at; an infinite value among the attended ones gives NaN or infinity in
     its column.  Requests may share pages.  Equal inputs give equal bits."""
